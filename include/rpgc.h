@@ -45,9 +45,11 @@ extern "C" {
 #define RPGC_E_TIMEOUT (-6)      /* a bounded device wait gave up */
 #define RPGC_E_IO (-7)           /* GGUF file could not be read */
 
-/* ggml type ids (src/quant.h:22-38); the kernels take F32, Q8_0, Q4_K, Q6_K. */
+/* ggml type ids (src/quant.h:22-38); the kernels take F32, Q8_0, Q4_K, Q6_K,
+ * and the paged-cache calls F16 and BF16. */
 #define RPGC_F32 0u
 #define RPGC_F16 1u
+#define RPGC_BF16 30u
 #define RPGC_Q8_0 8u
 #define RPGC_Q4_K 12u
 #define RPGC_Q6_K 14u
@@ -350,6 +352,98 @@ RPGC_API int rpgc_matmul_noalloc(uint32_t type, const void* w, int64_t rows, int
  * src/kernels.h:42-52); *token_dev receives the id. */
 RPGC_API int rpgc_sample(const float* logits, int64_t n, float temperature, int32_t top_k,
                          float top_p, float u, int32_t* token_dev, void* stream);
+
+/* -------------------------------------------------- paged KV cache */
+/* A cache of one layer in 16 bits, cut into pages of a pool that many
+ * sequences share; no counterpart in the reference, whose KvCache
+ * (src/kv_cache.h:35-82) is one fp32 block per session sized for its longest
+ * use.  A block table names the pages of each sequence: position t of
+ * sequence s is slot t % page_size of page block_table[s][t / page_size].
+ * Sequences may name the same page (a shared prefix).  The caller owns every
+ * buffer, and says which pages belong to whom.
+ *
+ * All pointers below are device pointers on the current device, rows of
+ * head_dim values are contiguous, and every base address and stride is a
+ * multiple of 16 bytes (strides count elements).  head_dim is 64 or 128,
+ * page_size a power of two from 16 to 256, n_heads / n_kv_heads a whole
+ * number up to 16.  Lengths and tables are read on the device when the call
+ * runs, so no call waits for the GPU, and a captured graph follows their
+ * changes.  What they hold is bounded on the device: a page id outside
+ * [0, n_pages) or a position past max_pages is a position that is not there,
+ * left out of attention (a sequence whose early pages were given back may
+ * name them -1) and not written by append.
+ *
+ * The values of a sequence's slots past its length, and of pages no sequence
+ * names, are never used, whatever they are. */
+typedef struct rpgc_paged_kv {
+  void* k; /* slot (page, position, head) at page*stride[0] + position*stride[1] + head*stride[2] */
+  void* v;
+  int64_t k_stride[3], v_stride[3];
+  uint32_t type; /* RPGC_F16 or RPGC_BF16 */
+  int32_t n_pages, page_size, n_kv_heads, head_dim;
+} rpgc_paged_kv;
+
+typedef struct rpgc_paged_batch {
+  const int32_t* block_table; /* [n_seqs] rows of max_pages ids, table_stride apart */
+  int64_t table_stride;
+  int32_t max_pages;
+  int32_t n_seqs;
+  const int32_t* kv_lens; /* [n_seqs] cache lengths, this call's new tokens included */
+  const int32_t* cu_q;    /* [n_seqs + 1] sequence s's new tokens are rows [cu_q[s], cu_q[s+1]);
+                             NULL: one new token per sequence, row s */
+  int64_t n_tokens;       /* rows of q (and of k and v in append) */
+  int32_t* status;        /* optional: RPGC_PAGED_* bits are OR-ed into it on the device */
+} rpgc_paged_batch;
+#define RPGC_PAGED_DROPPED 1 /* append: a new token's position has no page or no rope row */
+#define RPGC_PAGED_TIMEOUT 2 /* a bounded wait inside a kernel gave up; the output is not valid */
+
+/* QK-norm, rotary positions and the cache write of new tokens
+ * (src/qwen3.cc:141-163, src/kv_cache.cc:5-33), from the rows the matmuls
+ * give: token i of sequence s has position kv_lens[s] - (its new tokens) + i.
+ * q, k and v are n_tokens rows of heads ({token, head} strides) in in_type
+ * (RPGC_F32, RPGC_F16 or RPGC_BF16); q_norm and k_norm are head_dim fp32 gains (both
+ * NULL: no norm), rope is rope_rows rows of head_dim/2 cosines, then
+ * head_dim/2 sines (NULL: no rotation).  q_out receives n_tokens rows of
+ * n_heads * head_dim values in the cache's type; q and q_out may both be NULL.
+ * Arithmetic is fp32; each output is rounded once.  Tokens whose position has
+ * no page or no rope row are dropped: nothing is written to the cache, their
+ * q_out rows are zeros, and RPGC_PAGED_DROPPED is set. */
+RPGC_API int rpgc_paged_append(const rpgc_paged_kv* kv, const rpgc_paged_batch* b, uint32_t in_type,
+                               const void* q, const int64_t* q_stride, int32_t n_heads, const void* k,
+                               const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                               const float* q_norm, const float* k_norm, float eps, const float* rope,
+                               int64_t rope_rows, void* q_out, void* stream);
+
+/* Attention of one new token per sequence over its pages: b->cu_q is NULL
+ * and n_tokens == n_seqs.  q has {token, head} strides and the cache's type;
+ * out is [n_seqs][n_heads][head_dim], contiguous, of the same type.  Query
+ * head h reads kv head h / (n_heads / n_kv_heads); scores are scale * (q.k),
+ * scale finite and > 0.  A sequence with no position to see gets zeros.
+ * Sequences are split over their length as far as the GPU has room: workspace holds
+ * the partial results (rpgc_paged_decode_workspace bytes, 16-byte aligned, filled
+ * with zeros before its first use; every call leaves it ready for the next).
+ * Calls that share a workspace must be ordered. */
+RPGC_API int64_t rpgc_paged_decode_workspace(const rpgc_paged_kv* kv, int32_t n_seqs, int32_t n_heads);
+RPGC_API int rpgc_paged_attention_decode(const rpgc_paged_kv* kv, const rpgc_paged_batch* b, const void* q,
+                                         const int64_t* q_stride, int32_t n_heads, float scale, void* out,
+                                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Causal attention of packed prompts whose K and V are in the pages: token i
+ * of sequence s sees positions 0 .. kv_lens[s] - (its new tokens) + i, so a
+ * prompt that continues a cached prefix sees the prefix too.  q, out and
+ * scale as above, with n_tokens rows; rows that no sequence holds are not written. */
+RPGC_API int rpgc_paged_attention_prompt(const rpgc_paged_kv* kv, const rpgc_paged_batch* b, const void* q,
+                                         const int64_t* q_stride, int32_t n_heads, float scale, void* out,
+                                         void* stream);
+
+/* The same for whole prompts whose K and V lie packed beside q: n_tokens
+ * rows of each, sequence s in rows [cu[s], cu[s+1]).  type is RPGC_F16 or
+ * RPGC_BF16; strides are {token, head}; status as in rpgc_paged_batch. */
+RPGC_API int rpgc_attention_prompt(uint32_t type, const void* q, const int64_t* q_stride, const void* k,
+                                   const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                                   const int32_t* cu, int32_t n_seqs, int64_t n_tokens, int32_t n_heads,
+                                   int32_t n_kv_heads, int32_t head_dim, float scale, void* out,
+                                   int32_t* status, void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -9,6 +9,8 @@ Python host mirror of the reference's token-level interface:
   dequantize_rows              DequantizeRow             (src/quant.h:65)
   matvec / matmul_batch        MatVec / MatMulBatch      (src/model.cc:23-69)
   sample_token                 SampleToken / ArgMax      (src/sampler.cc:96-112)
+  PagedKV, paged_* ,           a 16-bit KV cache in pages, its writer and its
+  attention_prompt             attention (paged.py; no counterpart)
 
 Every call goes through librpgc.so (include/rpgc.h).  There is no CPU
 fallback: without the built library, or without a CUDA device, calls fail.
@@ -27,7 +29,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librpgc.so")
 
 OK, E_ARG, E_CUDA, E_OOM, E_STATE, E_CONTEXT_FULL, E_TIMEOUT, E_IO = 0, -1, -2, -3, -4, -5, -6, -7
-F32, F16, Q8_0, Q4_K, Q6_K = 0, 1, 8, 12, 14
+F32, F16, Q8_0, Q4_K, Q6_K, BF16 = 0, 1, 8, 12, 14, 30
 MAX_STOP = 16
 
 
@@ -140,6 +142,11 @@ def lib() -> C.CDLL:
         "rpgc_matmul": ([u32, vp, i64, i64, vp, i64, vp, vp], C.c_int),
         "rpgc_sample": ([vp, i64, f32, i32, f32, f32, vp, vp], C.c_int),
         "rpgc_attention_decode": ([vp, vp, vp, i64, i32, i32, i32, i64, vp, vp], C.c_int),
+        "rpgc_paged_append": ([vp, vp, u32, vp, vp, i32, vp, vp, vp, vp, vp, vp, f32, vp, i64, vp, vp], C.c_int),
+        "rpgc_paged_decode_workspace": ([vp, i32, i32], i64),
+        "rpgc_paged_attention_decode": ([vp, vp, vp, vp, i32, f32, vp, vp, i64, vp], C.c_int),
+        "rpgc_paged_attention_prompt": ([vp, vp, vp, vp, i32, f32, vp, vp], C.c_int),
+        "rpgc_attention_prompt": ([u32, vp, vp, vp, vp, vp, vp, vp, i32, i64, i32, i32, i32, f32, vp, vp, vp], C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -500,3 +507,7 @@ class EngineSession:
             self.close()
         except Exception:
             pass
+
+
+from .paged import (PagedBatch, PagedKV, attention_prompt, paged_append, paged_attention_decode,  # noqa: E402
+                    paged_attention_prompt, rope_table)

@@ -330,4 +330,55 @@ cudaError_t state_set_launch(DecodeState* st, const DecodeState& v, cudaStream_t
 // Number of active sessions among states[0, n) into *out (batched decode's early end).
 cudaError_t count_active_launch(DecodeState* const* states, int32_t n, int32_t* out, cudaStream_t s);
 
+// ------------------------------------------------------- paged KV cache
+// One layer's cache in pages, or (table == nullptr) K and V rows packed like
+// q's.  Strides count elements.
+struct PagedView {
+  const void* k;
+  const void* v;
+  int64_t k_page, k_pos, k_head;
+  int64_t v_page, v_pos, v_head;
+  int32_t n_pages, page_shift;  // page_size = 1 << page_shift
+  int32_t n_kv, hd;
+  bool bf16;                    // else fp16
+};
+// The sequences of one call.  cu == nullptr: one new token per sequence.
+struct PagedSeqs {
+  const int32_t* table;  // [n_seqs] rows of max_pages ids; nullptr: packed K and V
+  int64_t table_stride;
+  int32_t max_pages;
+  int32_t n_seqs;
+  const int32_t* kv_lens;  // nullptr with packed K and V
+  const int32_t* cu;
+  int64_t n_tokens;
+  int32_t* status;
+};
+struct PagedAppendArgs {
+  PagedView kv;
+  PagedSeqs b;
+  uint32_t in_type;
+  const void *q, *k, *v;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;  // input strides
+  int32_t n_heads;  // 0: no q
+  const float *q_norm, *k_norm;
+  float eps;
+  const float* rope;
+  int64_t rope_rows;
+  void* q_out;
+};
+struct PagedAttnArgs {
+  PagedView kv;
+  PagedSeqs b;
+  const void* q;
+  int64_t q_tok, q_head;
+  int32_t n_heads;
+  float scale;
+  void* out;
+  void* workspace;
+};
+cudaError_t paged_append_launch(const PagedAppendArgs& a, cudaStream_t s);
+int64_t paged_decode_workspace(const PagedView& kv, int32_t n_seqs, int32_t n_heads);
+cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s);
+cudaError_t prompt_attn_launch(const PagedAttnArgs& a, cudaStream_t s);
+
 }  // namespace rpgc
