@@ -1,0 +1,742 @@
+// k_prompt.cu -- causal attention of packed prompts on the 5th-generation
+// tensor cores (tcgen05, TMEM), K and V packed beside q or in cache pages.
+//
+// Mathematics: out_i = sum_t p_t v_t / sum_t p_t with p_t = 2^(c s_t - m),
+// s_t = q_i . k_t, c = scale * log2(e), over the keys t that row i sees, one
+// pass over the keys with a running reference m.  m follows the running
+// maximum only when that has grown by more than kGrow: until then the
+// probabilities exceed 1 by at most 2^kGrow, which 16-bit floats hold, and the
+// sums need no rescaling (in fp32, so nothing is lost).  fp16 probabilities
+// carry another 2^kLift, so that small ones keep their 11 bits.
+//
+// Layout: the G query heads of a kv head share its keys, so a tile of 128 MMA
+// rows holds T = 128 / G tokens x G heads; a work unit is two such tiles (A,
+// B) of one sequence and kv head, one CTA per SM taking units from a list
+// sorted by cost, longest first.  Warps 0-3 / 4-7: softmax of tile A / B, one
+// row per thread; warp 8: issues the MMAs; warp 9: TMA; warp 10: finds the
+// next unit.  S = Q K^T goes to TMEM (128 fp32 columns per tile); the softmax
+// warps read their row, write P over it in 16 bits, and O += P V takes P from
+// TMEM and V as it lies in the cache (keys are its rows: an MN-major operand).
+// While the softmax of one tile runs, the tensor core works on the other.
+//
+// TMEM columns: S/P of A 0-127, of B 128-255, O of A 256-, of B 384-.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+#include "paged_dev.cuh"
+#include "tc_dev.cuh"
+
+namespace rpgc {
+namespace {
+
+using namespace paged;
+using namespace tc;
+
+constexpr int kRows = 128;  // MMA rows of a tile
+constexpr int kKeys = 128;  // keys of a tile
+constexpr int kPThreads = 384;
+constexpr int kUnits = 2;   // units in flight between the finder and the other warps
+constexpr float kGrow = 8.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Unit {
+  int32_t seq, kh;           // seq < 0: no more work
+  int32_t rows[2];           // tokens of tiles A and B
+  int32_t tiles[2];          // their key tiles
+  int32_t end[2];            // keys [0, end) are seen by some row
+  int32_t pos0;              // position of tile A's first token (negative: before the cache)
+  int32_t reach;             // positions that exist
+  int64_t row0;              // packed row of tile A's first token
+  int64_t key0;              // packed K/V: row of key 0
+};
+
+template <int HD>
+struct Shape {
+  static constexpr int kHalves = HD / 64;              // 64-column operand panels
+  static constexpr int kPanel = kRows * 128;           // bytes of one
+  static constexpr int kQBytes = 2 * kHalves * kPanel; // tiles A and B
+  static constexpr int kStage = kHalves * kPanel;      // a K or V tile
+  static constexpr int kStages = HD == 128 ? 5 : 10;
+  static constexpr int kBars = 1024;                   // barriers and units
+  static constexpr int kSmem = 1024 + kQBytes + kStages * kStage + kBars;
+};
+
+struct PromptParams {
+  PagedAttnArgs a;
+  int32_t T;       // tokens of a tile
+  int32_t G;       // heads per kv head
+  int32_t dual;    // two tiles per unit
+  int32_t box;     // K/V rows of one TMA copy
+};
+
+RPGC_DEV void tma_3d(void* dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+RPGC_DEV void tma_4d(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// V as the B operand of O += P V: rows are keys (the MMA's K), the 64 values
+// of a panel row are N.  128-byte swizzle; 1024 B between groups of 8 keys,
+// one panel between 64-column blocks.
+RPGC_DEV uint64_t vdesc(const void* p, uint32_t panel) {
+  const uint64_t a = smem_u32(p);
+  return ((a >> 4) & 0x3FFFull) | ((uint64_t)(panel >> 4) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// D += A B with A (16-bit) in TMEM.
+RPGC_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+RPGC_DEV void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// The registers pass through the wait, so that nothing uses them before it.
+RPGC_DEV void tmem_wait_ld32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+RPGC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+RPGC_DEV void tmem_st16_nowait(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+RPGC_DEV float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Bounded wait of one role (about two seconds); after the first that gives up,
+// the CTA's other waits end at once and the call's status says so.
+constexpr long long kWaitClocks = 4000000000ll;
+RPGC_DEV bool wait_for(uint64_t* bar, uint32_t parity, volatile int32_t* gave_up, int32_t* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    for (int i = 0; i < 16; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*gave_up) return false;
+    if (clock64() - t0 > kWaitClocks) break;
+  }
+  *gave_up = 1;
+  if (status) atomicOr(status, kStatusTimeout);
+  return false;
+}
+
+// ---------------------------------------------------------- the unit list
+// Token tiles sorted by cost, the number of key tiles their last row sees;
+// within one cost by sequence.  Every rank is found from the lengths alone, so
+// the list is never written down.
+struct SeqLens {
+  int32_t n, pre;  // new tokens, positions before them
+};
+RPGC_DEV SeqLens seq_lens(const PagedSeqs& b, int s) {
+  SeqLens q{0, 0};
+  if (s < b.n_seqs) {
+    q.n = max(0, (int32_t)(seq_row(b, s + 1) - seq_row(b, s)));
+    if (b.table) q.pre = max(0, __ldg(b.kv_lens + s)) - q.n;
+  }
+  return q;
+}
+// First tile of the sequence whose cost is at least c (all later ones cost more).
+RPGC_DEV int32_t first_tile(SeqLens q, int32_t U, int32_t c) {
+  const int32_t tiles = (q.n + U - 1) / U;
+  if (c <= 0) return 0;
+  const int32_t pre = min(q.pre, 1 << 30);
+  const int64_t x = (int64_t)kKeys * (c - 1) + 1;
+  if (pre + q.n < x) return tiles;
+  const int64_t d = x - pre;
+  return d <= 0 ? 0 : (int32_t)((d - 1) / U);
+}
+RPGC_DEV int32_t tiles_at_least(const PagedSeqs& b, SeqLens mine, int32_t U, int32_t c, int lane) {
+  int32_t n = (mine.n + U - 1) / U - first_tile(mine, U, c);
+  for (int s = lane + 32; s < b.n_seqs; s += 32) {
+    const SeqLens q = seq_lens(b, s);
+    n += (q.n + U - 1) / U - first_tile(q, U, c);
+  }
+  return __reduce_add_sync(0xffffffffu, n);
+}
+
+template <int HD, bool BF>
+__global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_constant__ CUtensorMap tm_q,
+                                                              const __grid_constant__ CUtensorMap tm_k,
+                                                              const __grid_constant__ CUtensorMap tm_v,
+                                                              const __grid_constant__ PromptParams p) {
+  using S = Shape<HD>;
+  constexpr int kHalves = S::kHalves, kPanel = S::kPanel, kStages = S::kStages;
+  constexpr uint32_t kFmt = BF ? 1u : 0u;
+  constexpr uint32_t kIdBase = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(kRows >> 4) << 24);
+  constexpr uint32_t kIdS = kIdBase | ((uint32_t)(kKeys >> 3) << 17);
+  constexpr uint32_t kIdO = kIdBase | ((uint32_t)(HD >> 3) << 17) | (1u << 16);
+  constexpr float kLift = BF ? 0.0f : 6.0f;
+
+  extern __shared__ uint8_t psm_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(psm_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* Qs = sm;
+  uint8_t* ring = sm + S::kQBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kStages * S::kStage);
+  uint64_t* full = bars;                   // [kStages] K/V tile landed
+  uint64_t* empty = full + kStages;        // [kStages] its MMAs done
+  uint64_t* q_full = empty + kStages;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;          // [2] S of tile A / B ready
+  uint64_t* p_full = s_full + 2;           // [2] P written, S read
+  uint64_t* o_full = p_full + 2;           // [2] last P V of the unit done
+  uint64_t* u_full = o_full + 2;           // [kUnits] unit described
+  uint64_t* u_empty = u_full + kUnits;     // [kUnits] read by every role
+  uint64_t* done = u_empty + kUnits;
+  Unit* units = reinterpret_cast<Unit*>(done + 1);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(units + kUnits);
+  volatile int32_t* gave_up = reinterpret_cast<volatile int32_t*>(tslot + 1);
+
+  const PagedAttnArgs& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const bool paged = a.b.table != nullptr;
+  int32_t* status = a.b.status;
+
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(s_full + g, 1);
+      mbar_init(p_full + g, 4);
+      mbar_init(o_full + g, 1);
+    }
+    for (int i = 0; i < kUnits; ++i) {
+      mbar_init(u_full + i, 1);
+      mbar_init(u_empty + i, 10);
+    }
+    mbar_init(done, 1);
+    *gave_up = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tslot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, status); };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  }
+
+  if (warp == 10) {
+    // ---------------------------------------------------- finds the units
+    const int32_t U = p.T * (p.dual ? 2 : 1);
+    const SeqLens mine = seq_lens(a.b, lane);
+    int32_t cmax = (max(0, min(mine.pre, 1 << 30) + mine.n) + kKeys - 1) / kKeys;
+    for (int s = lane + 32; s < a.b.n_seqs; s += 32) {
+      const SeqLens q = seq_lens(a.b, s);
+      cmax = max(cmax, (max(0, min(q.pre, 1 << 30) + q.n) + kKeys - 1) / kKeys);
+    }
+    cmax = __reduce_max_sync(0xffffffffu, cmax);
+    const int32_t total = tiles_at_least(a.b, mine, U, 0, lane);
+    const int64_t units_n = (int64_t)total * a.kv.n_kv;
+    int32_t hi = cmax;
+    for (int it = 0;; ++it) {
+      // there and back over the CTAs, so that nobody gets the longest of every round
+      const int64_t u = (int64_t)it * gridDim.x + ((it & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      if (it >= kUnits) wait(u_empty + it % kUnits, (uint32_t)((it / kUnits) - 1) & 1u);
+      Unit un;
+      un.seq = -1;
+      if (u < units_n) {
+        const int32_t k = (int32_t)(u / a.kv.n_kv);
+        int32_t lo = 0;  // largest c with more than k tiles of at least that cost
+        while (lo < hi) {
+          const int32_t mid = (lo + hi + 1) >> 1;
+          if (tiles_at_least(a.b, mine, U, mid, lane) > k) lo = mid;
+          else hi = mid - 1;
+        }
+        int32_t r = k - tiles_at_least(a.b, mine, U, lo + 1, lane);
+        for (int s0 = 0; s0 < a.b.n_seqs; s0 += 32) {
+          const SeqLens q = s0 ? seq_lens(a.b, s0 + lane) : mine;
+          const int32_t f = first_tile(q, U, lo), n = first_tile(q, U, lo + 1) - f;
+          int32_t sum = n;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+          }
+          const uint32_t in = __ballot_sync(0xffffffffu, r < sum);
+          if (in) {
+            const int src = __ffs(in) - 1;
+            const int32_t i = __shfl_sync(0xffffffffu, f + r - (sum - n), src);
+            const int32_t n_new = __shfl_sync(0xffffffffu, q.n, src), pre = __shfl_sync(0xffffffffu, q.pre, src);
+            const int32_t t0 = i * U;
+            un.seq = s0 + src;
+            un.kh = (int32_t)(u % a.kv.n_kv);
+            un.key0 = seq_row(a.b, un.seq);
+            un.row0 = un.key0 + t0;
+            un.pos0 = pre + t0;
+            const int64_t reach = paged ? table_reach(a.kv, a.b) : (int64_t)n_new;
+            un.reach = (int32_t)min(reach, (int64_t)0x7fffffff);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int32_t first = g * p.T;
+              un.rows[g] = (g == 0 || p.dual) ? max(0, min(p.T, n_new - t0 - first)) : 0;
+              un.end[g] = un.rows[g] ? (int32_t)max((int64_t)0, min((int64_t)un.pos0 + first + un.rows[g], reach)) : 0;
+              un.tiles[g] = (un.end[g] + kKeys - 1) / kKeys;
+            }
+            break;
+          }
+          r -= __shfl_sync(0xffffffffu, sum, 31);
+        }
+        hi = lo;
+      }
+      if (lane == 0) {
+        units[it % kUnits] = un;
+        mbar_arrive(u_full + it % kUnits);
+      }
+      __syncwarp();
+      if (un.seq < 0 || *gave_up) break;
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ loads
+    int st = 0;
+    uint32_t ph = 0;
+    int nq = 0;
+    const int per = kKeys / p.box;  // copies of a tile and panel
+    for (int it = 0;; ++it) {
+      wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
+      const Unit un = units[it % kUnits];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(u_empty + it % kUnits);
+      if (un.seq < 0 || *gave_up) break;
+      const int nt = max(un.tiles[0], un.tiles[1]);
+      if (!nt) continue;
+      if (nq) wait(q_empty, (uint32_t)(nq - 1) & 1u);
+      ++nq;
+      if (lane == 0) {
+        const uint32_t bytes = (uint32_t)(p.T * p.G * 128 * kHalves);
+        mbar_arrive_expect_tx(q_full, bytes * (un.rows[1] ? 2 : 1));
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (g == 0 || un.rows[1])
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            tma_3d(Qs + (g * kHalves + h) * kPanel, &tm_q, 64 * h, un.kh * p.G, (int)(un.row0 + g * p.T), q_full);
+      }
+      for (int j = 0; j < nt; ++j) {
+        // lane l: the page of copy l; a page that is not there becomes the one
+        // past the last, which TMA fills with zeros
+        int page = 0, at = 0;
+        if (paged) {
+          const int64_t t = (int64_t)j * kKeys + (int64_t)lane * p.box;
+          if (lane < per) page = page_of(a.kv, a.b, un.seq, t);
+          if (page < 0) page = a.kv.n_pages;
+          at = (int)(t & ((1 << a.kv.page_shift) - 1));
+        }
+        for (int v = 0; v < 2; ++v) {
+          wait(empty + st, ph ^ 1u);
+          uint8_t* dst = ring + st * S::kStage;
+          const CUtensorMap* m = v ? &tm_v : &tm_k;
+          if (lane == 0) mbar_arrive_expect_tx(full + st, S::kStage);
+          __syncwarp();
+          if (lane < per) {
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+              uint8_t* d = dst + h * kPanel + lane * p.box * 128;
+              if (paged) tma_4d(d, m, 64 * h, un.kh, at, page, full + st);
+              else tma_3d(d, m, 64 * h, un.kh, (int)un.key0 + j * kKeys, full + st);
+            }
+          }
+          if (++st == kStages) st = 0, ph ^= 1u;
+        }
+        if (*gave_up) break;
+      }
+    }
+    if (*gave_up) {  // copies in flight end before the CTA does
+      for (int i = 0; i < kStages; ++i)
+        for (int k = 0; k < 1 << 12; ++k)
+          if (mbar_try_wait(full + i, ph ^ (i < st ? 0u : 1u))) break;
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------- MMAs
+    int st = 0;
+    uint32_t ph = 0;
+    uint32_t pp[2] = {0u, 0u};  // parity of p_full
+    int nq = 0;
+    auto next = [&] {
+      if (++st == kStages) st = 0, ph ^= 1u;
+    };
+    for (int it = 0;; ++it) {
+      wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
+      const Unit un = units[it % kUnits];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(u_empty + it % kUnits);
+      if (un.seq < 0 || *gave_up) break;
+      const int nt = max(un.tiles[0], un.tiles[1]);
+      if (!nt) continue;
+      const int end = max(un.end[0], un.end[1]);
+      auto issue_s = [&](int g, int stage) {  // S of tile g over the K tile in `stage`
+        if (lane == 0) {
+          const uint8_t* q = Qs + g * kHalves * kPanel;
+          const uint8_t* k = ring + stage * S::kStage;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const int o = (kk >> 2) * kPanel + (kk & 3) * 32;
+            mma_f16(tmem + 128u * g, sdesc(q + o), sdesc(k + o), kIdS, kk > 0);
+          }
+          mma_commit(s_full + g);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (lane == 0) mma_commit(bar);
+        __syncwarp();
+      };
+      wait(q_full, (uint32_t)nq & 1u);
+      ++nq;
+      wait(full + st, ph);
+      tc_fence_after();
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (un.tiles[g] > 0) issue_s(g, st);
+      commit(empty + st);
+      if (nt == 1) commit(q_empty);
+      next();
+      for (int j = 0; j < nt; ++j) {
+        const int vst = st;
+        wait(full + st, ph);
+        next();
+        const int kst = st;
+        const uint32_t kph = ph;
+        const bool more = j + 1 < nt;
+        if (more) next();
+        uint8_t* v = ring + vst * S::kStage;
+        const int keys = min(kKeys, end - j * kKeys);
+        if (keys & 15) {  // the values past the last position of the last step of 16 become zeros
+          const int stop = (keys + 15) & ~15;
+          for (int i = lane; i < (stop - keys) * 8 * kHalves; i += 32) {
+            const int h = i / ((stop - keys) * 8), c = i % ((stop - keys) * 8);
+            *reinterpret_cast<uint4*>(v + h * kPanel + (keys + (c >> 3)) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        bool waited = false;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (j < un.tiles[g]) {
+            wait(p_full + g, pp[g]);
+            pp[g] ^= 1u;
+            tc_fence_after();
+            const int steps = (min(kKeys, un.end[g] - j * kKeys) + 15) >> 4;
+            if (lane == 0)
+              for (int kk = 0; kk < steps; ++kk)
+                mma_ts(tmem + 256u + 128u * g, tmem + 128u * g + 8u * kk, vdesc(v + kk * 2048, kPanel), kIdO, j > 0 || kk > 0);
+            __syncwarp();
+            if (j + 1 == un.tiles[g]) commit(o_full + g);
+          }
+          if (j + 1 < un.tiles[g]) {
+            if (!waited) {
+              wait(full + kst, kph);
+              tc_fence_after();
+              waited = true;
+            }
+            issue_s(g, kst);
+          }
+        }
+        commit(empty + vst);
+        if (more) {
+          commit(empty + kst);
+          if (j + 2 == nt) commit(q_empty);
+        }
+        if (*gave_up) break;
+      }
+      if (*gave_up) break;
+    }
+    if (lane == 0) mma_commit(done);
+    for (int k = 0; k < 1 << 14; ++k)
+      if (mbar_try_wait(done, 0)) break;
+  } else if (warp < 8) {
+    // ---------------------------------------------------------- softmax
+    const int g = warp >> 2, r = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + 128u * g, to = tmem + lanes + 256u + 128u * g;
+    const int tok = r / p.G, head = r - tok * p.G;
+    const float c = a.scale * kLog2e;
+    const int shift = paged ? min(a.kv.page_shift, 7) : 7, npg = paged ? (shift < 7 ? kKeys >> shift : 1) : 0;
+    uint32_t sp = 0, op = 0;
+    for (int it = 0;; ++it) {
+      wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
+      const Unit* up = units + it % kUnits;
+      const int seq = up->seq, rows = up->rows[g], tiles = up->tiles[g], first = up->pos0 + g * p.T, reach = up->reach;
+      const int h = up->kh * p.G + head;
+      const int64_t row = up->row0 + g * p.T + tok;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(u_empty + it % kUnits);
+      if (seq < 0 || *gave_up) break;
+      if (!rows) continue;
+      const bool live = tok < rows;  // (rows past T * G have tok >= T >= rows)
+      const int lim = live ? (int)max((int64_t)0, min((int64_t)first + tok + 1, (int64_t)reach)) : 0;
+      const int whole = max(0, min(first + 1, reach)) / kKeys;  // key tiles that every row sees whole
+      float m = -INFINITY, l = 0.0f;
+      const int32_t* tab = paged ? a.b.table + (int64_t)seq * a.b.table_stride : nullptr;
+      auto entry = [&](int j) {  // page of this lane's part of key tile j
+        const int64_t e = (((int64_t)j * kKeys) >> a.kv.page_shift) + lane;
+        return lane < npg && e < a.b.max_pages ? __ldg(tab + e) : 0;
+      };
+      int32_t pg = paged && tiles ? entry(0) : 0;
+      for (int j = 0; j < tiles; ++j) {
+        uint32_t gone = 0;  // this tile's pages that are not there
+        if (paged) {
+          gone = __ballot_sync(0xffffffffu, lane < npg && (uint32_t)pg >= (uint32_t)a.kv.n_pages);
+          if (j + 1 < tiles) pg = entry(j + 1);
+        }
+        wait(s_full + g, sp);
+        sp ^= 1u;
+        tc_fence_after();
+        // the row is read twice, 32 columns at a time: for its maximum, then for
+        // the probabilities; a column that the row does not see counts as -inf
+        const bool some = j >= whole || gone;
+        const int n = lim - j * kKeys;
+        auto masked = [&](uint32_t* s, int q) {
+          if (some) {
+            const int k = n - 32 * q;
+            uint32_t on = k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
+            if (gone >> ((32 * q) >> shift) & 1u) on &= 0xffff0000u;
+            if (gone >> ((32 * q + 16) >> shift) & 1u) on &= 0x0000ffffu;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(on >> i & 1u)) s[i] = 0xff800000u;
+          }
+        };
+        uint32_t s[2][32];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld32_nowait(ts, s[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          tmem_wait_ld32(s[q & 1]);
+          tmem_ld32_nowait(ts + 32u * ((q + 1) & 3), s[(q + 1) & 1]);
+          masked(s[q & 1], q);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[q & 1][i]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+        // (a row that has seen nothing has m = -inf and takes the new maximum)
+        if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top > m))) {
+          const float mn = fmaxf(m, top);
+          const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+          if (j > 0) {  // O's row: P(j-1) V(j-1) was done before S(j)
+            l *= f;
+#pragma unroll 1
+            for (int q = 0; q < HD / 32; ++q) {
+              float t[32];
+              tmem_ld32(to + 32u * q, t);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) t[i] *= f;
+              tmem_st32(to + 32u * q, t);
+            }
+          }
+          m = mn;
+        }
+        const float base = (m == -INFINITY ? 0.0f : m) - kLift;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          tmem_wait_ld32(s[q & 1]);
+          if (q < 3) tmem_ld32_nowait(ts + 32u * (q + 1), s[(q + 1) & 1]);
+          masked(s[q & 1], q);
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = exp2_fast(fmaf(__uint_as_float(s[q & 1][2 * i]), c, -base));
+            const float y = exp2_fast(fmaf(__uint_as_float(s[q & 1][2 * i + 1]), c, -base));
+            sum[i & 3] += x + y;
+            w[i] = pack2<BF>(x, y);
+          }
+          tmem_st16_nowait(ts + 16u * q, w);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + g);
+        if (*gave_up) break;
+      }
+      // ------------------------------------------------------- the rows out
+      uint16_t* out = static_cast<uint16_t*>(a.out) + (row * a.n_heads + h) * HD;
+      if (!tiles) {
+        if (live)
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      wait(o_full + g, op);
+      op ^= 1u;
+      tc_fence_after();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      float bad = 0.0f;
+#pragma unroll 1
+      for (int q = 0; q < HD / 32; ++q) {
+        float t[32];
+        tmem_ld32(to + 32u * q, t);
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          bad = fmaf(t[2 * i], 0.0f, fmaf(t[2 * i + 1], 0.0f, bad));  // NaN where one is not finite
+          w[i] = pack2<BF>(t[2 * i] * inv, t[2 * i + 1] * inv);
+        }
+        if (live)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            reinterpret_cast<uint4*>(out)[4 * q + i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      }
+      // 0 * x is NaN for an infinite or NaN x in a place that a row does not
+      // see: such rows are computed again from their visible keys alone
+      uint32_t again = __ballot_sync(0xffffffffu, live && bad != 0.0f);
+      tc_fence_before();
+      while (again) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1;
+        const int64_t rr = __shfl_sync(0xffffffffu, row, src);
+        const int hh = __shfl_sync(0xffffffffu, h, src);
+        attn_row<HD, BF>(a, seq, rr, hh, lane);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+// A map of 16-bit values: rows of hd values, `rank` - 1 strides in elements.
+bool make_map(CUtensorMap* m, const void* base, int rank, const int64_t* dims, const int64_t* strides, const int* box) {
+  auto enc = encoder();
+  if (!enc) return false;
+  cuuint64_t d[4], st[3];
+  cuuint32_t b[4], es[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    b[i] = (cuuint32_t)box[i];
+    if (i) st[i - 1] = (cuuint64_t)strides[i - 1] * 2;
+  }
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, b, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count(int dev) {
+  static int sms[64] = {0};
+  if (dev < 0 || dev >= 64) return 148;
+  if (!sms[dev]) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+  return sms[dev] > 0 ? sms[dev] : 148;
+}
+
+template <int HD, bool BF>
+cudaError_t prompt_go(const PagedAttnArgs& a, cudaStream_t s) {
+  PromptParams p{};
+  p.a = a;
+  p.G = a.n_heads / a.kv.n_kv;
+  p.T = kRows / p.G;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int sms = sm_count(dev);
+  const int64_t pairs = (a.b.n_tokens + 2 * p.T - 1) / (2 * p.T);
+  p.dual = pairs * a.kv.n_kv >= sms;
+  const int U = p.T * (p.dual ? 2 : 1);
+  p.box = a.b.table && a.kv.page_shift < 7 ? 1 << a.kv.page_shift : kKeys;
+  CUtensorMap mq, mk, mv;
+  {
+    const int64_t dims[3] = {HD, a.n_heads, a.b.n_tokens}, st[2] = {a.q_head, a.q_tok};
+    const int box[3] = {64, p.G, p.T};
+    if (!make_map(&mq, a.q, 3, dims, st, box)) return cudaErrorInvalidValue;
+  }
+  for (int v = 0; v < 2; ++v) {
+    const void* base = v ? a.kv.v : a.kv.k;
+    const int64_t pos = v ? a.kv.v_pos : a.kv.k_pos, head = v ? a.kv.v_head : a.kv.k_head, page = v ? a.kv.v_page : a.kv.k_page;
+    CUtensorMap* m = v ? &mv : &mk;
+    if (a.b.table) {
+      const int64_t dims[4] = {HD, a.kv.n_kv, int64_t(1) << a.kv.page_shift, a.kv.n_pages}, st[3] = {head, pos, page};
+      const int box[4] = {64, 1, p.box, 1};
+      if (!make_map(m, base, 4, dims, st, box)) return cudaErrorInvalidValue;
+    } else {
+      const int64_t dims[3] = {HD, a.kv.n_kv, a.b.n_tokens}, st[2] = {head, pos};
+      const int box[3] = {64, 1, kKeys};
+      if (!make_map(m, base, 3, dims, st, box)) return cudaErrorInvalidValue;
+    }
+  }
+  constexpr int smem = Shape<HD>::kSmem;
+  static_assert(smem <= 232448, "shared memory of one CTA");
+  static bool configured[64] = {false};
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<HD, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  // the lengths are on the device: at most this many units exist
+  const int64_t most = ((a.b.n_tokens + U - 1) / U + a.b.n_seqs) * a.kv.n_kv;
+  const dim3 grid((unsigned)(most < sms ? most : sms));
+  prompt_kernel<HD, BF><<<grid, kPThreads, smem, s>>>(mq, mk, mv, p);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) count_launches(1);
+  return e;
+}
+
+}  // namespace
+
+cudaError_t prompt_attn_launch(const PagedAttnArgs& a, cudaStream_t s) {
+  if (!a.b.n_tokens) return cudaSuccess;
+  if (a.kv.hd == 128) return a.kv.bf16 ? prompt_go<128, true>(a, s) : prompt_go<128, false>(a, s);
+  return a.kv.bf16 ? prompt_go<64, true>(a, s) : prompt_go<64, false>(a, s);
+}
+
+}  // namespace rpgc

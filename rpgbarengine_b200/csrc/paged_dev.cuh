@@ -68,5 +68,82 @@ RPGC_DEV int seq_of_row(const PagedSeqs& b, int64_t r, int lane) {
   return r < seq_row(b, lo + 1) ? lo : -1;
 }
 
+// Attention of packed row r (of sequence s) and query head h by one warp, from
+// the visible keys alone: 32 keys a step, lane l scoring key l, then every
+// lane adding the keys' values for its own dims; fp32 throughout.  qs: HD
+// floats of shared memory of this warp.
+template <int HD, bool BF>
+__device__ __noinline__ void attn_row(const PagedAttnArgs& a, int s, int64_t r, int h, int lane) {
+  constexpr int E = HD / 32;
+  const int kh = h / (a.n_heads / a.kv.n_kv);
+  const int64_t r0 = seq_row(a.b, s), r1 = seq_row(a.b, s + 1);
+  const int64_t len = a.b.table ? (int64_t)a.b.kv_lens[s] : r1 - r0;
+  int64_t end = len - (r1 - r0) + (r - r0) + 1;  // keys [0, end)
+  if (a.b.table) end = min(end, table_reach(a.kv, a.b));
+  const uint4* qp =
+      reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + r * a.q_tok + h * a.q_head);
+  float m = -INFINITY, l = 0.0f, o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = 0.0f;
+  const int64_t mask = (1 << a.kv.page_shift) - 1;
+  for (int64_t t0 = 0; t0 < end; t0 += 32) {
+    const int64_t t = t0 + lane;
+    bool ok = t < end;
+    int64_t ko = 0, vo = 0;
+    if (ok) {
+      if (a.b.table) {
+        const int32_t p = page_of(a.kv, a.b, s, t);
+        ok = p >= 0;
+        ko = (int64_t)p * a.kv.k_page + (t & mask) * a.kv.k_pos;
+        vo = (int64_t)p * a.kv.v_page + (t & mask) * a.kv.v_pos;
+      } else {
+        ko = (r0 + t) * a.kv.k_pos;
+        vo = (r0 + t) * a.kv.v_pos;
+      }
+    }
+    float sc = -INFINITY;
+    if (ok) {
+      const uint4* kp = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.kv.k) + ko + kh * a.kv.k_head);
+      sc = 0.0f;
+#pragma unroll 4
+      for (int i = 0; i < HD / 8; ++i) {
+        const uint4 u = kp[i], v = qp[i];
+        const uint32_t ws[4] = {u.x, u.y, u.z, u.w}, qs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack2<BF>(ws[j]), q = unpack2<BF>(qs[j]);
+          sc += q.x * f.x + q.y * f.y;
+        }
+      }
+      sc *= a.scale;
+    }
+    const uint32_t live = __ballot_sync(0xffffffffu, ok);
+    if (!live) continue;
+    const float mn = fmaxf(m, warp_max(sc));
+    const float base = mn == -INFINITY ? 0.0f : mn;
+    const float corr = expf(m - base), p = ok ? expf(sc - base) : 0.0f;
+    m = mn;
+    l = l * corr + warp_sum(p);
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] *= corr;
+    for (int j = 0; j < 32; ++j) {
+      if (!(live >> j & 1)) continue;
+      const float pj = __shfl_sync(0xffffffffu, p, j);
+      const int64_t vj = __shfl_sync(0xffffffffu, vo, j);
+      const uint16_t* vp = static_cast<const uint16_t*>(a.kv.v) + vj + kh * a.kv.v_head + E * lane;
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        const float2 f = unpack2<BF>(*reinterpret_cast<const uint32_t*>(vp + i));
+        o[i] += pj * f.x;
+        o[i + 1] += pj * f.y;
+      }
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* op = static_cast<uint16_t*>(a.out) + (r * a.n_heads + h) * HD + E * lane;
+#pragma unroll
+  for (int i = 0; i < E; i += 2) *reinterpret_cast<uint32_t*>(op + i) = pack2<BF>(o[i] * inv, o[i + 1] * inv);
+}
+
 }  // namespace paged
 }  // namespace rpgc
