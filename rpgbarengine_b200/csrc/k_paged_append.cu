@@ -1,9 +1,9 @@
-// k_paged.cu -- the paged KV cache: QK-norm + RoPE + write of new tokens into
-// pages, and attention over the pages.
+// k_paged_append.cu -- QK-norm + RoPE + write of new tokens into the pages of
+// the KV cache.
 //
 // Reference: QK-norm before RoPE (src/qwen3.cc:141-152), half-split RoPE
-// (src/kernels.h:108-120), the cache write (src/kv_cache.cc:5-33),
-// AttentionFromCache (src/qwen3.cc:79-117); the reference's cache has no pages.
+// (src/kernels.h:108-120), the cache write (src/kv_cache.cc:5-33); the
+// reference's cache has no pages.
 #include <cuda_runtime.h>
 
 #include "paged_dev.cuh"
@@ -116,33 +116,6 @@ cudaError_t append_go(const PagedAppendArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// -------------------------------------------------------------- attention
-// One warp per (row, query head).  Simple and right for every shape; bound by
-// the keys' rows, which each lane reads by itself.
-template <int HD, bool BF>
-__global__ void __launch_bounds__(128) attn_row_kernel(const PagedAttnArgs a) {
-  const int lane = threadIdx.x & 31, wi = threadIdx.x >> 5;
-  const int64_t w = (int64_t)blockIdx.x * 4 + wi;
-  if (w >= a.b.n_tokens * a.n_heads) return;
-  const int64_t r = w / a.n_heads;
-  const int s = seq_of_row(a.b, r, lane);
-  if (s >= 0) attn_row<HD, BF>(a, s, r, (int)(w % a.n_heads), lane);
-}
-
-cudaError_t attn_row_go(const PagedAttnArgs& a, cudaStream_t s) {
-  const dim3 grid((unsigned)((a.b.n_tokens * a.n_heads + 3) / 4));
-  if (a.kv.hd == 128) {
-    if (a.kv.bf16) attn_row_kernel<128, true><<<grid, 128, 0, s>>>(a);
-    else attn_row_kernel<128, false><<<grid, 128, 0, s>>>(a);
-  } else {
-    if (a.kv.bf16) attn_row_kernel<64, true><<<grid, 128, 0, s>>>(a);
-    else attn_row_kernel<64, false><<<grid, 128, 0, s>>>(a);
-  }
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) count_launches(1);
-  return e;
-}
-
 }  // namespace
 
 cudaError_t paged_append_launch(const PagedAppendArgs& a, cudaStream_t s) {
@@ -155,12 +128,6 @@ cudaError_t paged_append_launch(const PagedAppendArgs& a, cudaStream_t s) {
     e = in == kInF32 ? append_go<64, kInF32>(a, s) : in == kInF16 ? append_go<64, kInF16>(a, s) : append_go<64, kInBF16>(a, s);
   if (e == cudaSuccess) count_launches(1);
   return e;
-}
-
-int64_t paged_decode_workspace(const PagedView& kv, int32_t n_seqs, int32_t n_heads) { return 16; }
-
-cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s) {
-  return a.b.n_tokens ? attn_row_go(a, s) : cudaSuccess;
 }
 
 }  // namespace rpgc

@@ -1,0 +1,504 @@
+// k_paged_decode.cu -- attention of one new token per sequence over the pages
+// of the KV cache.
+//
+// Mathematics: out = sum_t p_t v_t / sum_t p_t with p_t = 2^(c s_t - m),
+// s_t = q . k_t, c = scale * log2(e): one pass over the keys with a reference m
+// that follows the running maximum once it has grown by kGrow, so that most
+// steps rescale nothing.  Reference: AttentionFromCache (src/qwen3.cc:79-117).
+//
+// Bound: every K and V byte is read once, so HBM is the limit.  The key tiles
+// (64 keys) of all (sequence, kv head) items form one list, cut into equal
+// ranges, one per CTA and SM: batches of any mix of lengths, and one long
+// sequence as well, give every SM the same bytes.  An item that several CTAs
+// share is joined by the last of them to finish, from partial results in the
+// workspace, in the order of the pieces (the same result whoever is last).
+//
+// A CTA: one warp walks its range and issues TMA copies of K and V tiles into
+// a ring of 6 (hd 128), so ~190 KB are in flight per SM; 4 warps take 16 keys each of
+// every tile: S^T = K Q^T (m16n8k16, the kv head's query heads are the N side),
+// P^T turned from the accumulator layout into an operand by movmatrix,
+// O^T += V^T P^T.  The warps' sums meet in shared memory at an item's end.
+#include <cuda_runtime.h>
+
+#include "paged_dev.cuh"
+#include "paged_tma.cuh"
+
+namespace rpgc {
+namespace {
+
+using namespace paged;
+
+constexpr int kTile = 64;  // keys of a tile
+constexpr int kWarps = 4;  // consumer warps, 16 keys each
+constexpr int kDThreads = (kWarps + 1) * 32;
+constexpr float kGrow = 8.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int HD, int NT>
+struct DShape {
+  static constexpr int kPanels = HD / 64;
+  static constexpr int kPanel = kTile * 128;
+  static constexpr int kHalf = kPanels * kPanel;  // K (or V) of a tile
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int kStages = HD == 128 ? 6 : 12;
+  static constexpr int kHeads = 8 * NT;           // query heads of a kv head, padded
+  static constexpr int kPad = HD + 4;             // row of the merge buffer: no bank conflicts
+  static constexpr int kMerge = kWarps * kHeads * kPad * 4;
+  static constexpr int kSmem = 1024 + kStages * kStage + kMerge + 2 * kWarps * kHeads * 4 + 512;
+};
+
+struct DecodeParams {
+  PagedAttnArgs a;
+  uint32_t* counters;  // [n_seqs * n_kv] pieces of an item that are done
+  float* part;         // [2 * CTAs][G][HD] partial sums
+  float* part_ml;      // [2 * CTAs][G][2] their reference and weight
+  int32_t G;
+  int32_t box;         // rows of one TMA copy
+};
+
+template <bool BF>
+RPGC_DEV void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+RPGC_DEV void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+RPGC_DEV void ldsm4_t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+RPGC_DEV uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// The list of key tiles: sequence by sequence, kv head by kv head.
+RPGC_DEV int32_t seen(const PagedAttnArgs& a, int s) {  // positions the token of sequence s sees
+  const int64_t n = min((int64_t)max(0, __ldg(a.b.kv_lens + s)), table_reach(a.kv, a.b));
+  return (int32_t)n;
+}
+RPGC_DEV int64_t tiles_of(int32_t n) { return (n + (int64_t)kTile - 1) / kTile; }
+
+// One CTA's range of the list, item by item; every warp walks it by itself.
+struct Walk {
+  int64_t total, lo, hi;  // all tiles; this CTA's
+  int32_t seq, kh, len;   // the item
+  int64_t i0, i1;         // its tiles in the list
+  RPGC_DEV int64_t begin(int64_t b, int64_t n) const { return b * total / n; }
+  RPGC_DEV bool start(const PagedAttnArgs& a, int lane, int ctas, int cta, int* active) {
+    const int64_t kv = a.kv.n_kv;
+    int64_t sum = 0;
+    for (int s = lane; s < a.b.n_seqs; s += 32) sum += tiles_of(seen(a, s));
+    total = warp_sum(sum) * kv;
+    const int n = (int)(total < ctas ? total : ctas);
+    *active = n;
+    if (cta >= n) return false;
+    lo = begin(cta, n);
+    hi = begin(cta + 1, n);
+    int64_t before = 0;  // tiles of the sequences before s0
+    for (int s0 = 0;; s0 += 32) {
+      const int64_t mine = s0 + lane < a.b.n_seqs ? tiles_of(seen(a, s0 + lane)) * kv : 0;
+      int64_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const uint32_t in = __ballot_sync(0xffffffffu, before + upto > lo);
+      if (in) {
+        const int src = __ffs(in) - 1;
+        const int64_t first = before + __shfl_sync(0xffffffffu, upto - mine, src);
+        seq = s0 + src;
+        len = seen(a, seq);
+        kh = (int32_t)((lo - first) / tiles_of(len));
+        i0 = first + kh * tiles_of(len);
+        i1 = i0 + tiles_of(len);
+        return true;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  RPGC_DEV bool next(const PagedAttnArgs& a) {
+    if (i1 >= hi) return false;
+    if (++kh == a.kv.n_kv) {
+      kh = 0;
+      do len = seen(a, ++seq);
+      while (!len);  // (a later item exists: i1 < hi <= total)
+    }
+    i0 = i1;
+    i1 = i0 + tiles_of(len);
+    return true;
+  }
+};
+
+RPGC_DEV void bar_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+
+template <int HD, bool BF, int NT>
+__global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_constant__ CUtensorMap tm_k,
+                                                              const __grid_constant__ CUtensorMap tm_v,
+                                                              const __grid_constant__ DecodeParams p) {
+  using S = DShape<HD, NT>;
+  constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad;
+  constexpr float kLift = BF ? 0.0f : 6.0f;  // fp16 probabilities carry 2^6: small ones keep their bits
+  extern __shared__ uint8_t dsm_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
+  float* wo = reinterpret_cast<float*>(ring + kStages * S::kStage);  // [warp][head][kPad]
+  float* wm = wo + kWarps * kHeads * kPad;                           // [warp][head]
+  float* wl = wm + kWarps * kHeads;
+  uint64_t* full = reinterpret_cast<uint64_t*>(wl + kWarps * kHeads);
+  uint64_t* empty = full + kStages;
+  uint32_t* there = reinterpret_cast<uint32_t*>(empty + kStages);  // [kStages] groups of 16 keys that are there
+  volatile int32_t* gave_up = reinterpret_cast<volatile int32_t*>(there + kStages);
+  int32_t* last = const_cast<int32_t*>(gave_up) + 1;
+  const PagedAttnArgs& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, kWarps);
+    }
+    *gave_up = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, a.b.status); };
+  int active;
+  Walk w;
+  const bool work = w.start(a, lane, gridDim.x, blockIdx.x, &active);
+
+  if (warp == kWarps) {
+    // ---------------------------------------------------------------- loads
+    if (!work) return;
+    int st = 0;
+    uint32_t ph = 0;
+    const int per = kTile / p.box;  // copies per panel
+    const int pshift = a.kv.page_shift;
+    do {
+      const int32_t* tab = a.b.table + (int64_t)w.seq * a.b.table_stride;
+      const int t0 = (int)(max(w.lo, w.i0) - w.i0), t1 = (int)(min(w.hi, w.i1) - w.i0);
+      // page ids ahead of their use: lane l holds the one of copy l of the next 32
+      const int copies = (t1 - t0) * per;
+      const int64_t base = (int64_t)t0 * kTile;
+      auto entry = [&](int c) {
+        const int64_t e = (base + (int64_t)c * p.box) >> pshift;
+        return c < copies && e < a.b.max_pages ? __ldg(tab + e) : -1;
+      };
+      int32_t ids = entry(lane), ids_next = entry(32 + lane);
+      for (int t = t0, c = 0; t < t1; ++t, c += per) {
+        if (c && !(c & 31)) {
+          ids = ids_next;
+          ids_next = entry(c + 32 + lane);
+        }
+        int32_t page = __shfl_sync(0xffffffffu, ids, (c + lane) & 31);  // (per divides 32: never past the 32)
+        const bool ok = (uint32_t)page < (uint32_t)a.kv.n_pages;
+        if (!ok) page = a.kv.n_pages;  // past the pool: TMA fills zeros
+        const uint32_t have = __ballot_sync(0xffffffffu, lane < per && ok);
+        wait(empty + st, ph ^ 1u);
+        if (*gave_up) break;
+        if (lane == 0) {
+          uint32_t groups = 0;  // a copy of 16, 32 or 64 rows covers 1, 2 or 4 groups
+          const int g = p.box >> 4;
+          for (int i = 0; i < per; ++i)
+            if (have >> i & 1u) groups |= ((1u << g) - 1u) << (i * g);
+          there[st] = groups;
+          mbar_arrive_expect_tx(full + st, S::kStage);
+        }
+        __syncwarp();
+        if (lane < per) {
+          const int at = (int)((base + (int64_t)(c + lane) * p.box) & ((1 << pshift) - 1));
+          uint8_t* dst = ring + st * S::kStage + lane * p.box * 128;
+#pragma unroll
+          for (int h = 0; h < S::kPanels; ++h) {
+            tma_4d(dst + h * S::kPanel, &tm_k, 64 * h, w.kh, at, page, full + st);
+            tma_4d(dst + S::kHalf + h * S::kPanel, &tm_v, 64 * h, w.kh, at, page, full + st);
+          }
+        }
+        if (++st == kStages) st = 0, ph ^= 1u;
+      }
+      if (*gave_up) break;
+    } while (w.next(a));
+    if (*gave_up)  // copies in flight end before the CTA does
+      for (int i = 0; i < kStages; ++i)
+        for (int k = 0; k < 1 << 12; ++k)
+          if (mbar_try_wait(full + i, ph ^ (i < st ? 0u : 1u))) break;
+    return;
+  }
+
+  // ----------------------------------------------------------- attention
+  // sequences that see nothing: zeros, their rows dealt over the CTAs
+  for (int s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x)
+    if (seen(a, s) == 0)
+      for (int i = tid; i < a.n_heads * HD / 8; i += kWarps * 32)
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)s * a.n_heads * HD)[i] = make_uint4(0, 0, 0, 0);
+  if (!work) return;
+  const int gr = lane >> 2, tq = lane & 3, G = p.G;
+  const float c = a.scale * kLog2e;
+  // ldmatrix rows of this lane in the warp's 16 keys: K as stored, V transposed
+  const int mi = lane >> 3, mr = lane & 7;
+  const int krow = 16 * warp + mr + 8 * (mi & 1), kc = mi >> 1;
+  const int vrow = 16 * warp + mr + 8 * (mi >> 1), vc = mi & 1;
+  int st = 0;
+  uint32_t ph = 0;
+  do {
+    const int t0 = (int)(max(w.lo, w.i0) - w.i0), t1 = (int)(min(w.hi, w.i1) - w.i0);
+    // Q^T as the B operand: head 8 n + gr, dims 16 k + 2 tq (+8)
+    uint32_t q[NT][HD / 16][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int h = 8 * n + gr;
+      const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)w.seq * a.q_tok + (int64_t)(w.kh * G + h) * a.q_head + 2 * tq;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        q[n][k][0] = h < G ? __ldg(reinterpret_cast<const uint32_t*>(qp + 16 * k)) : 0u;
+        q[n][k][1] = h < G ? __ldg(reinterpret_cast<const uint32_t*>(qp + 16 * k + 8)) : 0u;
+      }
+    }
+    float o[NT][HD / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.0f;
+    }
+    for (int t = t0; t < t1; ++t) {
+      wait(full + st, ph);
+      const int left = w.len - t * kTile - 16 * warp;  // keys of this warp's group
+      if (left > 0 && (there[st] >> warp & 1u)) {
+        const uint32_t kb = smem_u32(ring + st * S::kStage), vb = kb + S::kHalf;
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          uint32_t f[4];
+          ldsm4(kb + (k >> 2) * S::kPanel + krow * 128 + (((2 * (k & 3) + kc) ^ (krow & 7)) << 4), f);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma<BF>(s[n], f, q[n][k][0], q[n][k][1]);
+        }
+        // s: (key gr, head 2 tq), (gr, 2 tq + 1), (gr + 8, 2 tq), (gr + 8, 2 tq + 1)
+        const bool in0 = gr < left, in1 = gr + 8 < left;
+        bool grown = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[n][e] = (e < 2 ? in0 : in1) ? s[n][e] * c : -INFINITY;
+            grown |= s[n][e] > m[n][e & 1] + kGrow || (m[n][e & 1] == -INFINITY && s[n][e] > -INFINITY);
+          }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(s[n][e], s[n][e + 2]);
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              x = fmaxf(x, m[n][e]);
+              const float f = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - x);
+              m[n][e] = x;
+              l[n][e] *= f;
+#pragma unroll
+              for (int d = 0; d < HD / 16; ++d) {
+                o[n][d][e] *= f;
+                o[n][d][e + 2] *= f;
+              }
+            }
+        }
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[e] = exp2_fast(s[n][e] - ((m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]) - kLift));
+          l[n][0] += x[0] + x[2];
+          l[n][1] += x[1] + x[3];
+          b[n][0] = transpose8(pack2<BF>(x[0], x[1]));
+          b[n][1] = transpose8(pack2<BF>(x[2], x[3]));
+        }
+        // keys 2 tq, 2 tq + 1 (and + 8) of the V operand; what lies past the
+        // last position is cleared, for 0 * NaN is NaN
+        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+        if (left < 16) {
+          keep0 = 2 * tq + 1 < left ? 0xffffffffu : 2 * tq < left ? 0xffffu : 0u;
+          keep1 = 2 * tq + 9 < left ? 0xffffffffu : 2 * tq + 8 < left ? 0xffffu : 0u;
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+          uint32_t f[4];
+          ldsm4_t(vb + (d >> 2) * S::kPanel + vrow * 128 + (((2 * (d & 3) + vc) ^ (vrow & 7)) << 4), f);
+          f[0] &= keep0;
+          f[1] &= keep0;
+          f[2] &= keep1;
+          f[3] &= keep1;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma<BF>(o[n][d], f, b[n][0], b[n][1]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + st);
+      if (++st == kStages) st = 0, ph ^= 1u;
+    }
+    // ---- the warps' sums meet
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[n][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int h = 8 * n + 2 * tq + e;
+        if (gr == 0) {
+          wm[warp * kHeads + h] = m[n][e];
+          wl[warp * kHeads + h] = x;
+        }
+        float* row = wo + (warp * kHeads + h) * kPad + gr;
+        if (h < G)
+#pragma unroll
+          for (int d = 0; d < HD / 16; ++d) {
+            row[16 * d] = o[n][d][e];
+            row[16 * d + 8] = o[n][d][e + 2];
+          }
+      }
+    bar_consumers();
+    const bool whole = w.i0 >= w.lo && w.i1 <= w.hi;
+    const int slot = 2 * blockIdx.x + (w.lo < w.i0 ? 1 : 0);
+    for (int i = tid; i < G * HD / 4; i += kWarps * 32) {
+      const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
+      float M = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, wm[k * kHeads + h]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float mk = wm[k * kHeads + h];
+        const float f = mk == -INFINITY ? 0.0f : exp2_fast(mk - M);
+        const float4 v = *reinterpret_cast<const float4*>(wo + (k * kHeads + h) * kPad + d);
+        acc.x += f * v.x;
+        acc.y += f * v.y;
+        acc.z += f * v.z;
+        acc.w += f * v.w;
+        L += f * wl[k * kHeads + h];
+      }
+      if (whole) {
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        uint16_t* op = static_cast<uint16_t*>(a.out) + ((int64_t)w.seq * a.n_heads + w.kh * G + h) * HD + d;
+        *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv));
+      } else {
+        __stcg(reinterpret_cast<float4*>(p.part + ((int64_t)slot * G + h) * HD + d), acc);
+        if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml) + (int64_t)slot * G + h, make_float2(M, L));
+      }
+    }
+    if (!whole) {
+      // ---- the last CTA to finish a shared item joins its pieces
+      const int b0 = (int)(((w.i0 + 1) * active - 1) / w.total), b1 = (int)((w.i1 * active - 1) / w.total);
+      __threadfence();
+      bar_consumers();
+      if (tid == 0) *last = atomicInc(p.counters + (int64_t)w.seq * a.kv.n_kv + w.kh, (uint32_t)(b1 - b0)) == (uint32_t)(b1 - b0);
+      bar_consumers();
+      if (*last) {
+        __threadfence();
+        for (int i = tid; i < G * HD / 4; i += kWarps * 32) {
+          const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
+          auto at = [&](int k) { return (int64_t)(2 * k + (w.begin(k, active) < w.i0 ? 1 : 0)) * G + h; };
+          float M = -INFINITY;
+          for (int k = b0; k <= b1; ++k) M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(p.part_ml) + at(k)).x);
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float L = 0.0f;
+#pragma unroll 4
+          for (int k = b0; k <= b1; ++k) {
+            const int64_t sl = at(k);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + sl);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + sl * HD + d));
+            const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - M);
+            acc.x += f * v.x;
+            acc.y += f * v.y;
+            acc.z += f * v.z;
+            acc.w += f * v.w;
+            L += f * ml.y;
+          }
+          const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+          uint16_t* op = static_cast<uint16_t*>(a.out) + ((int64_t)w.seq * a.n_heads + w.kh * G + h) * HD + d;
+          *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv));
+        }
+      }
+    }
+    bar_consumers();  // the merge buffer is free again
+  } while (w.next(a));
+}
+
+int device_sms() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) cudaGetLastError();
+  return sm_count(dev);
+}
+
+int64_t counter_bytes(const PagedView& kv, int32_t n_seqs) { return ((int64_t)n_seqs * kv.n_kv * 4 + 255) / 256 * 256; }
+
+template <int HD, bool BF, int NT>
+cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
+  const int sms = device_sms();
+  DecodeParams p{};
+  p.a = a;
+  p.G = a.n_heads / a.kv.n_kv;
+  p.box = a.kv.page_shift < 6 ? 1 << a.kv.page_shift : kTile;
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  p.counters = reinterpret_cast<uint32_t*>(ws);
+  p.part = reinterpret_cast<float*>(ws + counter_bytes(a.kv, a.b.n_seqs));
+  p.part_ml = p.part + (int64_t)2 * sms * p.G * HD;
+  CUtensorMap mk, mv;
+  if (!make_kv_map(&mk, a, false, p.box) || !make_kv_map(&mv, a, true, p.box)) return cudaErrorInvalidValue;
+  constexpr int smem = DShape<HD, NT>::kSmem;
+  static_assert(smem <= 232448, "shared memory of one CTA");
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static bool configured[64] = {false};
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(decode_kernel<HD, BF, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  decode_kernel<HD, BF, NT><<<sms, kDThreads, smem, s>>>(mk, mv, p);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) count_launches(1);
+  return e;
+}
+
+template <int HD, bool BF>
+cudaError_t decode_heads(const PagedAttnArgs& a, cudaStream_t s) {
+  return a.n_heads / a.kv.n_kv <= 8 ? decode_go<HD, BF, 1>(a, s) : decode_go<HD, BF, 2>(a, s);
+}
+
+}  // namespace
+
+int64_t paged_decode_workspace(const PagedView& kv, int32_t n_seqs, int32_t n_heads) {
+  const int64_t rows = (int64_t)2 * device_sms() * (n_heads / kv.n_kv);
+  return counter_bytes(kv, n_seqs) + rows * (kv.hd + 2) * 4;
+}
+
+cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s) {
+  if (!a.b.n_tokens) return cudaSuccess;
+  if (a.kv.hd == 128) return a.kv.bf16 ? decode_heads<128, true>(a, s) : decode_heads<128, false>(a, s);
+  return a.kv.bf16 ? decode_heads<64, true>(a, s) : decode_heads<64, false>(a, s);
+}
+
+}  // namespace rpgc

@@ -20,13 +20,10 @@
 // While the softmax of one tile runs, the tensor core works on the other.
 //
 // TMEM columns: S/P of A 0-127, of B 128-255, O of A 256-, of B 384-.
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
-#include <mutex>
-
 #include "paged_dev.cuh"
+#include "paged_tma.cuh"
 #include "tc_dev.cuh"
 
 namespace rpgc {
@@ -72,21 +69,6 @@ struct PromptParams {
   int32_t box;     // K/V rows of one TMA copy
 };
 
-RPGC_DEV void tma_3d(void* dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
-RPGC_DEV void tma_4d(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
-
 // V as the B operand of O += P V: rows are keys (the MMA's K), the 64 values
 // of a panel row are N.  128-byte swizzle; 1024 B between groups of 8 keys,
 // one panel between 64-column blocks.
@@ -130,29 +112,6 @@ RPGC_DEV void tmem_st16_nowait(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-
-RPGC_DEV float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Bounded wait of one role (about two seconds); after the first that gives up,
-// the CTA's other waits end at once and the call's status says so.
-constexpr long long kWaitClocks = 4000000000ll;
-RPGC_DEV bool wait_for(uint64_t* bar, uint32_t parity, volatile int32_t* gave_up, int32_t* status) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  for (;;) {
-    for (int i = 0; i < 16; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
-    if (*gave_up) return false;
-    if (clock64() - t0 > kWaitClocks) break;
-  }
-  *gave_up = 1;
-  if (status) atomicOr(status, kStatusTimeout);
-  return false;
 }
 
 // ---------------------------------------------------------- the unit list
@@ -645,42 +604,6 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    cudaDriverEntryPointQueryResult q;
-    void* f = nullptr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  });
-  return fn;
-}
-
-// A map of 16-bit values: rows of hd values, `rank` - 1 strides in elements.
-bool make_map(CUtensorMap* m, const void* base, int rank, const int64_t* dims, const int64_t* strides, const int* box) {
-  auto enc = encoder();
-  if (!enc) return false;
-  cuuint64_t d[4], st[3];
-  cuuint32_t b[4], es[4] = {1, 1, 1, 1};
-  for (int i = 0; i < rank; ++i) {
-    d[i] = (cuuint64_t)dims[i];
-    b[i] = (cuuint32_t)box[i];
-    if (i) st[i - 1] = (cuuint64_t)strides[i - 1] * 2;
-  }
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, b, es,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-int sm_count(int dev) {
-  static int sms[64] = {0};
-  if (dev < 0 || dev >= 64) return 148;
-  if (!sms[dev]) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-  return sms[dev] > 0 ? sms[dev] : 148;
-}
-
 template <int HD, bool BF>
 cudaError_t prompt_go(const PagedAttnArgs& a, cudaStream_t s) {
   PromptParams p{};
@@ -700,20 +623,7 @@ cudaError_t prompt_go(const PagedAttnArgs& a, cudaStream_t s) {
     const int box[3] = {64, p.G, p.T};
     if (!make_map(&mq, a.q, 3, dims, st, box)) return cudaErrorInvalidValue;
   }
-  for (int v = 0; v < 2; ++v) {
-    const void* base = v ? a.kv.v : a.kv.k;
-    const int64_t pos = v ? a.kv.v_pos : a.kv.k_pos, head = v ? a.kv.v_head : a.kv.k_head, page = v ? a.kv.v_page : a.kv.k_page;
-    CUtensorMap* m = v ? &mv : &mk;
-    if (a.b.table) {
-      const int64_t dims[4] = {HD, a.kv.n_kv, int64_t(1) << a.kv.page_shift, a.kv.n_pages}, st[3] = {head, pos, page};
-      const int box[4] = {64, 1, p.box, 1};
-      if (!make_map(m, base, 4, dims, st, box)) return cudaErrorInvalidValue;
-    } else {
-      const int64_t dims[3] = {HD, a.kv.n_kv, a.b.n_tokens}, st[2] = {head, pos};
-      const int box[3] = {64, 1, kKeys};
-      if (!make_map(m, base, 3, dims, st, box)) return cudaErrorInvalidValue;
-    }
-  }
+  if (!make_kv_map(&mk, a, false, p.box) || !make_kv_map(&mv, a, true, p.box)) return cudaErrorInvalidValue;
   constexpr int smem = Shape<HD>::kSmem;
   static_assert(smem <= 232448, "shared memory of one CTA");
   static bool configured[64] = {false};
