@@ -43,7 +43,10 @@ struct DShape {
   static constexpr int kStages = HD == 128 ? 6 : 12;
   static constexpr int kHeads = 8 * NT;           // query heads of a kv head, padded
   static constexpr int kPad = HD + 4;             // row of the merge buffer: no bank conflicts
-  static constexpr int kMerge = kWarps * kHeads * kPad * 4;
+  static constexpr int kMaxCtas = 256;
+  // the warps' sums, later the join's table: per piece a slot and 8 bytes a head
+  static constexpr int kSums = kWarps * kHeads * kPad * 4, kTable = kMaxCtas * (2 * kHeads + 1) * 4;
+  static constexpr int kMerge = kSums > kTable ? kSums : kTable;
   static constexpr int kSmem = 1024 + kStages * kStage + kMerge + 2 * kWarps * kHeads * 4 + 512;
 };
 
@@ -417,24 +420,39 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
       bar_consumers();
       if (*last) {
         __threadfence();
+        // every piece's (reference, weight) of every head at once, one read each;
+        // then the sums, eight pieces' rows in flight
+        const int pieces = b1 - b0 + 1;
+        float2* ml = reinterpret_cast<float2*>(wo);                      // [piece][head]
+        int32_t* slots = reinterpret_cast<int32_t*>(ml + pieces * G);    // [piece]
+        for (int k = tid; k < pieces; k += kWarps * 32) slots[k] = 2 * (b0 + k) + (w.begin(b0 + k, active) < w.i0 ? 1 : 0);
+        bar_consumers();
+        for (int i = tid; i < pieces * G; i += kWarps * 32)
+          ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + (int64_t)slots[i / G] * G + i % G);
+        bar_consumers();
         for (int i = tid; i < G * HD / 4; i += kWarps * 32) {
           const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
-          auto at = [&](int k) { return (int64_t)(2 * k + (w.begin(k, active) < w.i0 ? 1 : 0)) * G + h; };
+          const float* part = p.part + h * HD + d;
           float M = -INFINITY;
-          for (int k = b0; k <= b1; ++k) M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(p.part_ml) + at(k)).x);
+          for (int k = 0; k < pieces; ++k) M = fmaxf(M, ml[k * G + h].x);
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
           float L = 0.0f;
-#pragma unroll 4
-          for (int k = b0; k <= b1; ++k) {
-            const int64_t sl = at(k);
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + sl);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + sl * HD + d));
-            const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - M);
-            acc.x += f * v.x;
-            acc.y += f * v.y;
-            acc.z += f * v.z;
-            acc.w += f * v.w;
-            L += f * ml.y;
+          for (int k0 = 0; k0 < pieces; k0 += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (k0 + k < pieces) v[k] = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)slots[k0 + k] * G * HD));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              if (k0 + k >= pieces) break;
+              const float2 x = ml[(k0 + k) * G + h];
+              const float f = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - M);
+              acc.x += f * v[k].x;
+              acc.y += f * v[k].y;
+              acc.z += f * v[k].z;
+              acc.w += f * v[k].w;
+              L += f * x.y;
+            }
           }
           const float inv = L == 0.0f ? 0.0f : 1.0f / L;
           uint16_t* op = static_cast<uint16_t*>(a.out) + ((int64_t)w.seq * a.n_heads + w.kh * G + h) * HD + d;
@@ -456,7 +474,7 @@ int64_t counter_bytes(const PagedView& kv, int32_t n_seqs) { return ((int64_t)n_
 
 template <int HD, bool BF, int NT>
 cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
-  const int sms = device_sms();
+  const int sms = min(device_sms(), DShape<HD, NT>::kMaxCtas);
   DecodeParams p{};
   p.a = a;
   p.G = a.n_heads / a.kv.n_kv;

@@ -69,6 +69,28 @@ struct PromptParams {
   int32_t box;     // K/V rows of one TMA copy
 };
 
+// Two fp32 operations at once.
+RPGC_DEV uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+RPGC_DEV float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+RPGC_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+RPGC_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // V as the B operand of O += P V: rows are keys (the MMA's K), the 64 values
 // of a panel row are N.  128-byte swizzle; 1024 B between groups of 8 keys,
 // one panel between 64-column blocks.
@@ -85,24 +107,36 @@ RPGC_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_
       "r"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 
-RPGC_DEV void tmem_ld32_nowait(uint32_t taddr, uint32_t* r) {
+// 128 consecutive columns of this warp's lanes, complete when this returns.
+RPGC_DEV void tmem_ld128(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-// The registers pass through the wait, so that nothing uses them before it.
-RPGC_DEV void tmem_wait_ld32(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
-                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31])::"memory");
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%128];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%129];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
+      "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95}, [%130];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
+      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%131];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr), "r"(taddr + 32u), "r"(taddr + 64u), "r"(taddr + 96u)
+      : "memory");
 }
 RPGC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 RPGC_DEV void tmem_st16_nowait(uint32_t taddr, const uint32_t* r) {
@@ -215,12 +249,11 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
   const uint32_t tmem = *tslot;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, status); };
 
+  // Registers move from the control warps to the softmax warps (8 x 32 x 200 +
+  // 4 x 32 x 104 = the launch's 384 x 168), each at the head of its own branch:
+  // code that both paths reached would have to fit the smaller share.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-  }
-
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 10) {
     // ---------------------------------------------------- finds the units
     const int32_t U = p.T * (p.dual ? 2 : 1);
@@ -450,7 +483,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
     if (lane == 0) mma_commit(done);
     for (int k = 0; k < 1 << 14; ++k)
       if (mbar_try_wait(done, 0)) break;
-  } else if (warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------------------------------------------------- softmax
     const int g = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -462,13 +497,17 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
     for (int it = 0;; ++it) {
       wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
       const Unit* up = units + it % kUnits;
-      const int seq = up->seq, rows = up->rows[g], tiles = up->tiles[g], first = up->pos0 + g * p.T, reach = up->reach;
-      const int h = up->kh * p.G + head;
-      const int64_t row = up->row0 + g * p.T + tok;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(u_empty + it % kUnits);
+      const int seq = up->seq, rows = up->rows[g], tiles = up->tiles[g];
       if (seq < 0 || *gave_up) break;
-      if (!rows) continue;
+      auto release = [&] {  // the unit's description is read no more
+        __syncwarp();
+        if (lane == 0) mbar_arrive(u_empty + it % kUnits);
+      };
+      if (!rows) {
+        release();
+        continue;
+      }
+      const int first = up->pos0 + g * p.T, reach = up->reach;
       const bool live = tok < rows;  // (rows past T * G have tok >= T >= rows)
       const int lim = live ? (int)max((int64_t)0, min((int64_t)first + tok + 1, (int64_t)reach)) : 0;
       const int whole = max(0, min(first + 1, reach)) / kKeys;  // key tiles that every row sees whole
@@ -488,11 +527,14 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         wait(s_full + g, sp);
         sp ^= 1u;
         tc_fence_after();
-        // the row is read twice, 32 columns at a time: for its maximum, then for
-        // the probabilities; a column that the row does not see counts as -inf
+        // the row's 128 scores stay in registers; one that the row does not see is -inf
+        uint32_t x[128];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         const bool some = j >= whole || gone;
         const int n = lim - j * kKeys;
-        auto masked = [&](uint32_t* s, int q) {
+        tmem_ld128(ts, x);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
           if (some) {
             const int k = n - 32 * q;
             uint32_t on = k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
@@ -500,19 +542,11 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
             if (gone >> ((32 * q + 16) >> shift) & 1u) on &= 0x0000ffffu;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!(on >> i & 1u)) s[i] = 0xff800000u;
+              if (!(on >> i & 1u)) x[32 * q + i] = 0xff800000u;
           }
-        };
-        uint32_t s[2][32];
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_ld32_nowait(ts, s[0]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          tmem_wait_ld32(s[q & 1]);
-          tmem_ld32_nowait(ts + 32u * ((q + 1) & 3), s[(q + 1) & 1]);
-          masked(s[q & 1], q);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[q & 1][i]));
+          for (int i = 0; i < 32; i += 2)
+            mx[(i >> 1) & 3] = fmaxf(fmaxf(mx[(i >> 1) & 3], __uint_as_float(x[32 * q + i])), __uint_as_float(x[32 * q + i + 1]));
         }
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
         // (a row that has seen nothing has m = -inf and takes the new maximum)
@@ -522,34 +556,35 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
           if (j > 0) {  // O's row: P(j-1) V(j-1) was done before S(j)
             l *= f;
 #pragma unroll 1
-            for (int q = 0; q < HD / 32; ++q) {
-              float t[32];
-              tmem_ld32(to + 32u * q, t);
+            for (int q = 0; q < HD / 16; ++q) {
+              float t[16];
+              tmem_ld16(to + 16u * q, t);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) t[i] *= f;
-              tmem_st32(to + 32u * q, t);
+              for (int i = 0; i < 16; ++i) t[i] *= f;
+              tmem_st16_nowait(to + 16u * q, reinterpret_cast<const uint32_t*>(t));
             }
           }
           m = mn;
         }
-        const float base = (m == -INFINITY ? 0.0f : m) - kLift;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float base = kLift - (m == -INFINITY ? 0.0f : m);
+        const uint64_t c2 = pair(c, c), base2 = pair(base, base);
+        uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          tmem_wait_ld32(s[q & 1]);
-          if (q < 3) tmem_ld32_nowait(ts + 32u * (q + 1), s[(q + 1) & 1]);
-          masked(s[q & 1], q);
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float x = exp2_fast(fmaf(__uint_as_float(s[q & 1][2 * i]), c, -base));
-            const float y = exp2_fast(fmaf(__uint_as_float(s[q & 1][2 * i + 1]), c, -base));
-            sum[i & 3] += x + y;
-            w[i] = pack2<BF>(x, y);
+            const float2 y = unpair(fma2(pair(__uint_as_float(x[32 * q + 2 * i]), __uint_as_float(x[32 * q + 2 * i + 1])), c2, base2));
+            const float e0 = exp2_fast(y.x), e1 = exp2_fast(y.y);
+            sum[i & 1] = add2(sum[i & 1], pair(e0, e1));
+            w[i] = pack2<BF>(e0, e1);
           }
           tmem_st16_nowait(ts + 16u * q, w);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        {
+          const float2 u = unpair(add2(sum[0], sum[1]));
+          l += u.x + u.y;
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -557,6 +592,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         if (*gave_up) break;
       }
       // ------------------------------------------------------- the rows out
+      const int64_t row = up->row0 + g * p.T + tok;
+      const int h = up->kh * p.G + head;
+      release();
       uint16_t* out = static_cast<uint16_t*>(a.out) + (row * a.n_heads + h) * HD;
       if (!tiles) {
         if (live)

@@ -34,67 +34,66 @@ class _Batch(C.Structure):
 
 
 _S2 = C.c_int64 * 2
+_mods = []
+
+
+def _torch():
+    if not _mods:
+        import torch
+        _mods.append(torch)
+    return _mods[0]
+
+
+def _refuse(msg):
+    raise RpgcError(E_ARG, msg)
 
 
 def _need(ok, msg):
     if not ok:
-        raise RpgcError(E_ARG, msg)
+        _refuse(msg)
 
 
 def _type(t):
-    import torch
-    ty = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
-    _need(ty is not None, f"{t.dtype} is not supported")
-    return ty
+    torch = _torch()
+    d = t.dtype
+    return BF16 if d is torch.bfloat16 else F16 if d is torch.float16 else F32 if d is torch.float32 else \
+        _refuse(f"{d} is not supported")
 
 
 def _ints(t, what, dims):
-    import torch
-    _need(t.is_cuda and t.dtype == torch.int32 and t.dim() == dims, f"{what} must be a {dims}-D int32 CUDA tensor")
+    _need(t.is_cuda and t.dtype is _torch().int32 and t.dim() == dims, f"{what} must be a {dims}-D int32 CUDA tensor")
 
 
-def _rows(t, what, dev, shape):
-    """Strides of a [token, head, dim] tensor with contiguous rows on `dev`."""
-    _need(t.device == dev and t.dim() == 3, f"{what} must be a 3-D tensor on {dev}")
-    _need(all(a == b for a, b in zip(t.shape, shape) if b is not None), f"{what} has shape {tuple(t.shape)}")
-    s = t.stride()
-    _need(s[2] == 1, f"{what}: rows of head_dim values must be contiguous")
-    return _S2(s[0], s[1])
+def _rows(t, what, index, n, heads, d):
+    """Strides of a [token, head, dim] tensor with contiguous rows on device `index`."""
+    shape, st = t.shape, t.stride()
+    if t.get_device() != index or len(shape) != 3 or shape[0] != n or shape[2] != d or (heads and shape[1] != heads) or st[2] != 1:
+        _refuse(f"{what} must be [{n}, {heads or 'heads'}, {d}] on CUDA device {index}, each row of {d} contiguous; "
+                f"got {tuple(shape)} with strides {tuple(st)} on {t.device}")
+    # (a dimension of one has no stride to speak of)
+    return _S2(st[0] if n > 1 else shape[1] * d, st[1] if shape[1] > 1 else d)
 
 
-def _result(out, shape, dtype, dev, what):
-    import torch
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    _need(out.device == dev and out.dtype == dtype and tuple(out.shape) == tuple(shape) and out.is_contiguous(),
-          f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
+def _result(out, like, shape, dtype):
+    if out.shape != shape or out.dtype != dtype or out.get_device() != like.get_device() or not out.is_contiguous():
+        _refuse(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device}")
     return out
 
 
-class _On:
-    """The stream a call runs on, with its device current."""
-
-    def __init__(self, dev, stream):
-        import torch
-        self.cuda = torch.cuda
-        self.guard = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else None
-        self.other = stream
-        self.ptr = int(torch.cuda.current_stream(dev).cuda_stream if stream is None else stream)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
-
-    def keep(self, t):
-        """A result made here on the current stream and used on another one
-        keeps its memory until that stream is done with it."""
-        if self.other is not None:
-            t.record_stream(self.cuda.ExternalStream(self.ptr, device=t.device))
+def _run(fn, index, stream, made, *args):
+    """fn(*args, stream) with device `index` current.  `made`: a result allocated
+    here, whose memory must outlive its use on a stream that is not the current one."""
+    cuda = _torch().cuda
+    ptr = _torch()._C._cuda_getCurrentRawStream(index) if stream is None else int(stream)
+    if index == cuda.current_device():
+        rc = fn(*args, ptr)
+    else:
+        with cuda.device(index):
+            rc = fn(*args, ptr)
+    if rc < 0:
+        _check(rc)
+    if made is not None and stream is not None:
+        made.record_stream(cuda.ExternalStream(ptr, device=made.device))
 
 
 class PagedKV:
@@ -106,20 +105,20 @@ class PagedKV:
         _need(k.is_cuda and k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device,
               "k and v must be 4-D CUDA tensors of one shape and type")
         _need(k.stride(3) == 1 and v.stride(3) == 1, "rows of head_dim values must be contiguous")
-        self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype
+        self.k, self.v, self.index, self.dtype = k, v, k.get_device(), k.dtype
         n, p, h, d = k.shape
         ty = _type(k)
         _need(ty != F32, "a paged cache holds float16 or bfloat16")
-        self.c = _KV(k.data_ptr(), v.data_ptr(), (C.c_int64 * 3)(*k.stride()[:3]), (C.c_int64 * 3)(*v.stride()[:3]),
-                     ty, n, p, h, d)
+        strides = [(C.c_int64 * 3)(*[st if size > 1 else d for st, size in zip(t.stride(), t.shape[:3])]) for t in (k, v)]
+        self.c = _KV(k.data_ptr(), v.data_ptr(), strides[0], strides[1], ty, n, p, h, d)
         self.ref = C.byref(self.c)
-        self.page_size, self.n_kv_heads, self.head_dim = p, h, d
+        self.page_size, self.n_kv_heads, self.head_dim, self.scale = p, h, d, d ** -0.5
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=None, device="cuda") -> "PagedKV":
         """New pools (bfloat16 unless said otherwise); their values are never
         read before append writes them."""
-        import torch
+        torch = _torch()
         shape, dt = (n_pages, page_size, n_kv_heads, head_dim), dtype or torch.bfloat16
         return cls(torch.empty(shape, dtype=dt, device=device), torch.empty(shape, dtype=dt, device=device))
 
@@ -147,8 +146,8 @@ class PagedBatch:
         if status is not None:
             _ints(status, "status", 1)
         self.keep = (block_table, kv_lens, cu_q, status)
-        self.device = kv_lens.device
-        _need(all(t is None or t.device == self.device for t in self.keep), "the batch's tensors must be on one device")
+        self.index = kv_lens.get_device()
+        _need(all(t is None or t.get_device() == self.index for t in self.keep), "the batch's tensors must be on one device")
         self.n_seqs, self.n_tokens = n, n if n_tokens is None else int(n_tokens)
         p = [None if t is None else t.data_ptr() for t in self.keep]
         self.c = _Batch(p[0], max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], n, p[1], p[2],
@@ -161,9 +160,12 @@ class PagedBatch:
         key = (n_heads, cache.n_kv_heads, cache.head_dim)
         ws = self._ws.get(key)
         if ws is None:
-            import torch
-            n = _check(lib().rpgc_paged_decode_workspace(cache.ref, self.n_seqs, n_heads))
-            ws = self._ws[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            torch = _torch()
+            with torch.cuda.device(self.index):
+                n = _check(lib().rpgc_paged_decode_workspace(cache.ref, self.n_seqs, n_heads))
+                buf = torch.zeros(n, dtype=torch.uint8, device="cuda")
+                torch.cuda.current_stream().synchronize()  # zeroed for every stream, once
+            ws = self._ws[key] = (buf, buf.data_ptr(), n)
         return ws
 
 
@@ -174,66 +176,63 @@ def paged_append(cache: PagedKV, batch: PagedBatch, q, k, v, q_norm=None, k_norm
     n_heads, head_dim], k and v [n_tokens, n_kv_heads, head_dim], of one type
     (float32, float16 or bfloat16); q_norm / k_norm: fp32 gains [head_dim] or
     None; rope: fp32 [positions, head_dim] (rope_table) or None."""
-    import torch
-    dev, n, d = cache.device, batch.n_tokens, cache.head_dim
-    _need(batch.device == dev, "cache and batch are on different devices")
+    torch = _torch()
+    index, n, d, kv = cache.index, batch.n_tokens, cache.head_dim, cache.n_kv_heads
+    _need(batch.index == index, "cache and batch are on different devices")
     ty = _type(k)
-    _need(v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "q, k and v must have one type")
-    ks = _rows(k, "k", dev, (n, cache.n_kv_heads, d))
-    vs = _rows(v, "v", dev, (n, cache.n_kv_heads, d))
-    qs = None if q is None else _rows(q, "q", dev, (n, None, d))
+    _need(v.dtype is k.dtype and (q is None or q.dtype is k.dtype), "q, k and v must have one type")
+    ks, vs = _rows(k, "k", index, n, kv, d), _rows(v, "v", index, n, kv, d)
     for g in (q_norm, k_norm):
-        _need(g is None or (g.device == dev and g.dtype == torch.float32 and g.shape == (d,) and (g.stride(0) == 1)),
-              "norm gains must be contiguous float32 [head_dim]")
-    _need(rope is None or (rope.device == dev and rope.dtype == torch.float32 and rope.dim() == 2 and
-                           rope.shape[1] == d and rope.is_contiguous()), "rope must be contiguous float32 [positions, head_dim]")
-    heads = 0 if q is None else q.shape[1]
-    with _On(dev, stream) as on:
-        made = q is not None and q_out is None
-        q_out = None if q is None else _result(q_out, (n, heads, d), cache.dtype, dev, "q_out")
-        _check(lib().rpgc_paged_append(
-            cache.ref, batch.ref, ty, None if q is None else q.data_ptr(), qs, heads, k.data_ptr(), ks, v.data_ptr(), vs,
-            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-            None if rope is None else rope.data_ptr(), 0 if rope is None else rope.shape[0],
-            None if q is None else q_out.data_ptr(), on.ptr))
-        if made:
-            on.keep(q_out)
+        if g is not None and not (g.get_device() == index and g.dtype is torch.float32 and g.shape == (d,) and g.is_contiguous()):
+            _refuse("norm gains must be contiguous float32 [head_dim] on the cache's device")
+    if rope is not None and not (rope.get_device() == index and rope.dtype is torch.float32 and rope.dim() == 2 and
+                                 rope.shape[1] == d and rope.is_contiguous()):
+        _refuse("rope must be contiguous float32 [positions, head_dim] on the cache's device")
+    qs, heads, qp, op, made = None, 0, None, None, None
+    if q is not None:
+        qs, heads, qp = _rows(q, "q", index, n, 0, d), q.shape[1], q.data_ptr()
+        if q_out is None:
+            q_out = made = torch.empty(q.shape, dtype=cache.dtype, device=q.device)
+        else:
+            _result(q_out, q, q.shape, cache.dtype)
+        op = q_out.data_ptr()
+    else:
+        _need(q_out is None, "q_out without q")
+    _run(lib().rpgc_paged_append, index, stream, made, cache.ref, batch.ref, ty, qp, qs, heads, k.data_ptr(), ks, v.data_ptr(), vs,
+         None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+         None if rope is None else rope.data_ptr(), 0 if rope is None else rope.shape[0], op)
     return q_out
+
+
+def _attend(cache, batch, q, out):
+    """Strides of q, the result and whether it was made here."""
+    if q.dtype is not cache.dtype or batch.index != cache.index:
+        _refuse("q, cache and batch must share their device, and q the cache's type")
+    qs = _rows(q, "q", cache.index, batch.n_tokens, 0, cache.head_dim)
+    if out is None:
+        out = q.new_empty(q.shape)
+        return qs, out, out
+    return qs, _result(out, q, q.shape, q.dtype), None
 
 
 def paged_attention_decode(cache: PagedKV, batch: PagedBatch, q, scale=None, out=None, stream=None):
     """Attention of one new token per sequence, q [n_seqs, n_heads, head_dim],
     over the sequence's positions; returns the same shape.  scale: default
     head_dim ** -0.5."""
-    dev, d = cache.device, cache.head_dim
-    _need(batch.device == dev and q.dtype == cache.dtype, "q, cache and batch must share their device, q the cache's type")
-    qs = _rows(q, "q", dev, (batch.n_tokens, None, d))
+    qs, out, made = _attend(cache, batch, q, out)
     heads = q.shape[1]
-    with _On(dev, stream) as on:
-        made = out is None
-        out = _result(out, q.shape, cache.dtype, dev, "out")
-        ws = batch.workspace(cache, heads)
-        _check(lib().rpgc_paged_attention_decode(cache.ref, batch.ref, q.data_ptr(), qs, heads,
-                                                 d ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(),
-                                                 ws.numel(), on.ptr))
-        if made:
-            on.keep(out)
+    ws = batch.workspace(cache, heads)
+    _run(lib().rpgc_paged_attention_decode, cache.index, stream, made, cache.ref, batch.ref, q.data_ptr(), qs, heads,
+         cache.scale if scale is None else scale, out.data_ptr(), ws[1], ws[2])
     return out
 
 
 def paged_attention_prompt(cache: PagedKV, batch: PagedBatch, q, scale=None, out=None, stream=None):
     """Causal attention of the batch's new tokens, q [n_tokens, n_heads,
     head_dim], over their sequences' pages (a cached prefix included)."""
-    dev, d = cache.device, cache.head_dim
-    _need(batch.device == dev and q.dtype == cache.dtype, "q, cache and batch must share their device, q the cache's type")
-    qs = _rows(q, "q", dev, (batch.n_tokens, None, d))
-    with _On(dev, stream) as on:
-        made = out is None
-        out = _result(out, q.shape, cache.dtype, dev, "out")
-        _check(lib().rpgc_paged_attention_prompt(cache.ref, batch.ref, q.data_ptr(), qs, q.shape[1],
-                                                 d ** -0.5 if scale is None else scale, out.data_ptr(), on.ptr))
-        if made:
-            on.keep(out)
+    qs, out, made = _attend(cache, batch, q, out)
+    _run(lib().rpgc_paged_attention_prompt, cache.index, stream, made, cache.ref, batch.ref, q.data_ptr(), qs, q.shape[1],
+         cache.scale if scale is None else scale, out.data_ptr())
     return out
 
 
@@ -241,26 +240,24 @@ def attention_prompt(q, k, v, cu_seqlens, scale=None, out=None, status=None, str
     """Causal attention of packed prompts: q [n_tokens, n_heads, head_dim], k
     and v [n_tokens, n_kv_heads, head_dim] in float16 or bfloat16, sequence s
     in rows [cu_seqlens[s], cu_seqlens[s+1]); returns q's shape."""
-    dev = q.device
-    _need(q.is_cuda and q.dim() == 3 and k.dim() == 3, "q, k and v must be 3-D CUDA tensors")
-    n, heads, d = q.shape
-    _need(q.dtype == k.dtype == v.dtype, "q, k and v must have one type")
-    qs, ks = _rows(q, "q", dev, (n, heads, d)), _rows(k, "k", dev, (n, None, d))
-    vs = _rows(v, "v", dev, k.shape)
+    if not q.is_cuda or q.dim() != 3 or k.dim() != 3 or q.dtype is not k.dtype or q.dtype is not v.dtype:
+        _refuse("q, k and v must be 3-D CUDA tensors of one type")
+    index, (n, heads, d), kv = q.get_device(), q.shape, k.shape[1]
+    qs, ks, vs = _rows(q, "q", index, n, heads, d), _rows(k, "k", index, n, kv, d), _rows(v, "v", index, n, kv, d)
     _ints(cu_seqlens, "cu_seqlens", 1)
-    _need(cu_seqlens.device == dev and cu_seqlens.shape[0] >= 1 and cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous, n_seqs + 1 values")
+    if cu_seqlens.get_device() != index or cu_seqlens.shape[0] < 1 or not cu_seqlens.is_contiguous():
+        _refuse("cu_seqlens must be n_seqs + 1 contiguous values on q's device")
     if status is not None:
         _ints(status, "status", 1)
-        _need(status.device == dev, f"status must be on {dev}")
-    with _On(dev, stream) as on:
-        made = out is None
-        out = _result(out, q.shape, q.dtype, dev, "out")
-        _check(lib().rpgc_attention_prompt(_type(q), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-                                           cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, n, heads, k.shape[1], d,
-                                           d ** -0.5 if scale is None else scale, out.data_ptr(),
-                                           None if status is None else status.data_ptr(), on.ptr))
-        if made:
-            on.keep(out)
+        _need(status.get_device() == index, "status must be on q's device")
+    made = None
+    if out is None:
+        out = made = q.new_empty(q.shape)
+    else:
+        _result(out, q, q.shape, q.dtype)
+    _run(lib().rpgc_attention_prompt, index, stream, made, _type(q), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+         cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, n, heads, kv, d, d ** -0.5 if scale is None else scale, out.data_ptr(),
+         None if status is None else status.data_ptr())
     return out
 
 
@@ -269,7 +266,7 @@ def rope_table(positions: int, head_dim: int, theta: float = 1e6, device="cuda")
     position * theta^(-2i/head_dim), computed in double as BuildRopeTable does
     (src/model.cc:122-145)."""
     import numpy as np
-    import torch
+    torch = _torch()
     inv = np.array([1.0 / math.pow(theta, 2.0 * i / head_dim) for i in range(head_dim // 2)])
     ang = np.arange(positions, dtype=np.float64)[:, None] * inv
     return torch.from_numpy(np.concatenate([np.cos(ang), np.sin(ang)], 1).astype(np.float32)).to(device)
