@@ -99,6 +99,13 @@ RPGC_DEV uint64_t vdesc(const void* p, uint32_t panel) {
   return ((a >> 4) & 0x3FFFull) | ((uint64_t)(panel >> 4) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// True in one lane of a converged warp; the compiler knows that only one.
+RPGC_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred P;\n elect.sync _|P, 0xffffffff;\n selp.b32 %0, 1, 0, P;\n}" : "=r"(p));
+  return p != 0;
+}
+
 // D += A B with A (16-bit) in TMEM.
 RPGC_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -389,6 +396,10 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
     int st = 0;
     uint32_t ph = 0;
     uint32_t pp[2] = {0u, 0u};  // parity of p_full
+    // One elected lane issues, from descriptors that differ by constants: with
+    // anything more to compute between two MMAs the issue, not the tensor
+    // core, sets the pace (150 clocks an MMA instead of 64).
+    const uint64_t q_desc = sdesc(Qs), k_desc = sdesc(ring), v_desc = vdesc(ring, kPanel);
     int nq = 0;
     auto next = [&] {
       if (++st == kStages) st = 0, ph ^= 1u;
@@ -403,20 +414,19 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       if (!nt) continue;
       const int end = max(un.end[0], un.end[1]);
       auto issue_s = [&](int g, int stage) {  // S of tile g over the K tile in `stage`
-        if (lane == 0) {
-          const uint8_t* q = Qs + g * kHalves * kPanel;
-          const uint8_t* k = ring + stage * S::kStage;
+        if (elect_one()) {
+          const uint64_t q = q_desc + (uint64_t)(g * kHalves * kPanel / 16), k = k_desc + (uint64_t)(stage * (S::kStage / 16));
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
-            const int o = (kk >> 2) * kPanel + (kk & 3) * 32;
-            mma_f16(tmem + 128u * g, sdesc(q + o), sdesc(k + o), kIdS, kk > 0);
+            const uint64_t o = ((kk >> 2) * kPanel + (kk & 3) * 32) / 16;
+            mma_f16(tmem + 128u * g, q + o, k + o, kIdS, kk > 0);
           }
           mma_commit(s_full + g);
         }
         __syncwarp();
       };
       auto commit = [&](uint64_t* bar) {
-        if (lane == 0) mma_commit(bar);
+        if (elect_one()) mma_commit(bar);
         __syncwarp();
       };
       wait(q_full, (uint32_t)nq & 1u);
@@ -456,9 +466,17 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
             pp[g] ^= 1u;
             tc_fence_after();
             const int steps = (min(kKeys, un.end[g] - j * kKeys) + 15) >> 4;
-            if (lane == 0)
-              for (int kk = 0; kk < steps; ++kk)
-                mma_ts(tmem + 256u + 128u * g, tmem + 128u * g + 8u * kk, vdesc(v + kk * 2048, kPanel), kIdO, j > 0 || kk > 0);
+            if (elect_one()) {
+              const uint64_t vd = v_desc + (uint64_t)(vst * (S::kStage / 16));
+              const uint32_t o = tmem + 256u + 128u * g, pt = tmem + 128u * g;
+              mma_ts(o, pt, vd, kIdO, j > 0);
+              if (steps == 8) {
+#pragma unroll
+                for (int kk = 1; kk < 8; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
+              } else {
+                for (int kk = 1; kk < steps; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
+              }
+            }
             __syncwarp();
             if (j + 1 == un.tiles[g]) commit(o_full + g);
           }
@@ -480,7 +498,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       }
       if (*gave_up) break;
     }
-    if (lane == 0) mma_commit(done);
+    if (elect_one()) mma_commit(done);
+    __syncwarp();
     for (int k = 0; k < 1 << 14; ++k)
       if (mbar_try_wait(done, 0)) break;
   }
