@@ -3,11 +3,11 @@
 //
 // Mathematics: out_i = sum_t p_t v_t / sum_t p_t with p_t = 2^(c s_t - m),
 // s_t = q_i . k_t, c = scale * log2(e), over the keys t that row i sees, one
-// pass over the keys with a running reference m.  m follows the running
-// maximum only when that has grown by more than kGrow: until then the
-// probabilities exceed 1 by at most 2^kGrow, which 16-bit floats hold, and the
-// sums need no rescaling (in fp32, so nothing is lost).  fp16 probabilities
-// carry another 2^kLift, so that small ones keep their 11 bits.
+// pass over the keys with a reference m.  m is the maximum of the first key
+// tile and stays until a later tile's sum says that its scores have outgrown
+// it: fp32 sums and bf16 probabilities have the exponents for 2^40, fp16
+// probabilities (which carry another 2^kLift, so that small ones keep their
+// 11 bits) for 2^15.  Until then no maximum is taken and nothing is rescaled.
 //
 // Layout: the G query heads of a kv head share its keys, so a tile of 128 MMA
 // rows holds T = 128 / G tokens x G heads; a work unit is two such tiles (A,
@@ -36,7 +36,7 @@ constexpr int kRows = 128;  // MMA rows of a tile
 constexpr int kKeys = 128;  // keys of a tile
 constexpr int kPThreads = 384;
 constexpr int kUnits = 2;   // units in flight between the finder and the other warps
-constexpr float kGrow = 8.0f;
+constexpr int kPoly = 1, kPolyOf = 8;  // of every 8 pairs of a row, those on the FMA pipe
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Unit {
@@ -91,6 +91,47 @@ RPGC_DEV uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// max that carries NaN
+RPGC_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+RPGC_DEV float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^y of two values on the FMA pipe, for part of a row's probabilities: the
+// special-function unit gives 16 exponentials per clock and SM, half of what the
+// MMAs of the same tile would need.  y = n + f with n the nearest integer (added
+// and taken off 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial fitted to it
+// for the smallest relative error (7.5e-5 for degree 3, 2.7e-6 for degree 4,
+// against 2^-9 and 2^-12 of the 16-bit rounding that follows), n added to the exponent.
+// Below 2^-126 the result stays there; NaN is not carried (see `m`).
+template <bool BF>
+RPGC_DEV float2 exp2_poly(uint64_t y) {
+  constexpr float kMagic = 12582912.0f;
+  const float2 v = unpair(y);
+  const uint64_t x = pair(fminf(max_nan(v.x, -126.0f), 127.0f), fminf(max_nan(v.y, -126.0f), 127.0f));
+  const uint64_t t = add2(x, pair(kMagic, kMagic));
+  const uint64_t f = fma2(add2(t, pair(-kMagic, -kMagic)), pair(-1.0f, -1.0f), x);
+  uint64_t r;
+  if (BF) {
+    r = fma2(pair(0.0551716685f, 0.0551716685f), f, pair(0.242611125f, 0.242611125f));
+    r = fma2(r, f, pair(0.693260968f, 0.693260968f));
+    r = fma2(r, f, pair(0.999928057f, 0.999928057f));
+  } else {
+    r = fma2(pair(0.00957010221f, 0.00957010221f), f, pair(0.0559178591f, 0.0559178591f));
+    r = fma2(r, f, pair(0.240247443f, 0.240247443f));
+    r = fma2(r, f, pair(0.693121791f, 0.693121791f));
+    r = fma2(r, f, pair(0.999999285f, 0.999999285f));
+  }
+  const float2 a = unpair(t), b = unpair(r);
+  return make_float2(__uint_as_float(__float_as_uint(b.x) + (__float_as_uint(a.x) << 23)),
+                     __uint_as_float(__float_as_uint(b.y) + (__float_as_uint(a.y) << 23)));
+}
 // V as the B operand of O += P V: rows are keys (the MMA's K), the 64 values
 // of a panel row are N.  128-byte swizzle; 1024 B between groups of 8 keys,
 // one panel between 64-column blocks.
@@ -114,36 +155,24 @@ RPGC_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_
       "r"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 
-// 128 consecutive columns of this warp's lanes, complete when this returns.
-RPGC_DEV void tmem_ld128(uint32_t taddr, uint32_t* r) {
+// 32 consecutive columns of this warp's lanes; `r` holds them after tmem_landed.
+RPGC_DEV void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%128];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%129];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
-      "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95}, [%130];\n"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
-      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%131];\n"
-      "tcgen05.wait::ld.sync.aligned;"
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
-      : "r"(taddr), "r"(taddr + 32u), "r"(taddr + 64u), "r"(taddr + 96u)
-      : "memory");
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// The registers pass through the wait, so that nothing uses them before it.
+RPGC_DEV void tmem_landed(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 RPGC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 RPGC_DEV void tmem_st16_nowait(uint32_t taddr, const uint32_t* r) {
@@ -201,6 +230,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
   constexpr uint32_t kIdS = kIdBase | ((uint32_t)(kKeys >> 3) << 17);
   constexpr uint32_t kIdO = kIdBase | ((uint32_t)(HD >> 3) << 17) | (1u << 16);
   constexpr float kLift = BF ? 0.0f : 6.0f;
+  constexpr float kMost = BF ? 1.0e12f : 32768.0f;  // sum of a row's 128 probabilities that needs no new reference
 
   extern __shared__ uint8_t psm_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(psm_raw) + 1023) & ~uintptr_t(1023));
@@ -530,7 +560,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       const bool live = tok < rows;  // (rows past T * G have tok >= T >= rows)
       const int lim = live ? (int)max((int64_t)0, min((int64_t)first + tok + 1, (int64_t)reach)) : 0;
       const int whole = max(0, min(first + 1, reach)) / kKeys;  // key tiles that every row sees whole
-      float m = -INFINITY, l = 0.0f;
+      // a row that sees nothing (or is none) has nothing to wait for
+      float m = lim > 0 ? -INFINITY : 0.0f, l = 0.0f;
       const int32_t* tab = paged ? a.b.table + (int64_t)seq * a.b.table_stride : nullptr;
       auto entry = [&](int j) {  // page of this lane's part of key tile j
         const int64_t e = (((int64_t)j * kKeys) >> a.kv.page_shift) + lane;
@@ -546,64 +577,96 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         wait(s_full + g, sp);
         sp ^= 1u;
         tc_fence_after();
-        // the row's 128 scores stay in registers; one that the row does not see is -inf
-        uint32_t x[128];
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const bool some = j >= whole || gone;
-        const int n = lim - j * kKeys;
-        tmem_ld128(ts, x);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (some) {
+        // One pass over the row with the reference it has: the probabilities are
+        // made, summed and kept in 16 bits while S stays where it is.  Only where a row
+        // has no reference yet, or its sum shows that the scores have outgrown it
+        // (or hold NaN: the comparison fails), the row's maximum is looked for
+        // first: m becomes it, O and l follow, and the pass is done again.
+        if (j >= whole || gone) {
+          // scores that the row does not see become -inf where they lie, so that
+          // the pass itself has no branches (they made every tile 200 clocks longer)
+          const int n = lim - j * kKeys;
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
             const int k = n - 32 * q;
             uint32_t on = k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
             if (gone >> ((32 * q) >> shift) & 1u) on &= 0xffff0000u;
             if (gone >> ((32 * q + 16) >> shift) & 1u) on &= 0x0000ffffu;
+            if (__all_sync(0xffffffffu, on == 0xffffffffu)) continue;
+            uint32_t x[32];
+            tmem_ld32_async(ts + 32u * q, x);
+            tmem_landed(x);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!(on >> i & 1u)) x[32 * q + i] = 0xff800000u;
+              if (!(on >> i & 1u)) x[i] = 0xff800000u;
+            tmem_st16_nowait(ts + 32u * q, x);
+            tmem_st16_nowait(ts + 32u * q + 16u, x + 16);
           }
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            mx[(i >> 1) & 3] = fmaxf(fmaxf(mx[(i >> 1) & 3], __uint_as_float(x[32 * q + i])), __uint_as_float(x[32 * q + i + 1]));
+          tmem_wait_st();
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-        // (a row that has seen nothing has m = -inf and takes the new maximum)
-        if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top > m))) {
-          const float mn = fmaxf(m, top);
-          const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
-          if (j > 0) {  // O's row: P(j-1) V(j-1) was done before S(j)
-            l *= f;
+        uint32_t w[64];
+        float tile_sum;
+        bool look = __any_sync(0xffffffffu, m == -INFINITY);
 #pragma unroll 1
-            for (int q = 0; q < HD / 16; ++q) {
-              float t[16];
-              tmem_ld16(to + 16u * q, t);
+        for (;;) {
+          uint32_t x[2][32];
+          if (look) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              tmem_ld32_async(ts + 32u * q, x[0]);
+              tmem_landed(x[0]);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) t[i] *= f;
-              tmem_st16_nowait(to + 16u * q, reinterpret_cast<const uint32_t*>(t));
+              for (int i = 0; i < 32; i += 2)
+                mx[(i >> 1) & 3] = max_nan(mx[(i >> 1) & 3], __uint_as_float(x[0][i]), __uint_as_float(x[0][i + 1]));
+            }
+            const float top = max_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]) * c;
+            const float mn = max_nan(m, top);
+            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+            if (j > 0) {  // O's row: P(j-1) V(j-1) was done before S(j)
+              l *= f;
+#pragma unroll 1
+              for (int q = 0; q < HD / 16; ++q) {
+                float t[16];
+                tmem_ld16(to + 16u * q, t);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) t[i] *= f;
+                tmem_st16_nowait(to + 16u * q, reinterpret_cast<const uint32_t*>(t));
+              }
+            }
+            m = mn;
+          }
+          const float base = kLift - (m == -INFINITY ? 0.0f : m);
+          const uint64_t c2 = pair(c, c), base2 = pair(base, base);
+          uint64_t sum[2] = {0ull, 0ull};
+          tmem_ld32_async(ts, x[0]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            tmem_landed(x[q & 1]);
+            if (q < 3) tmem_ld32_async(ts + 32u * (q + 1), x[(q + 1) & 1]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint64_t y =
+                  fma2(pair(__uint_as_float(x[q & 1][2 * i]), __uint_as_float(x[q & 1][2 * i + 1])), c2, base2);
+              float2 e;
+              if (i % kPolyOf < kPoly) {
+                e = exp2_poly<BF>(y);
+              } else {
+                const float2 z = unpair(y);
+                e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+              }
+              sum[i & 1] = add2(sum[i & 1], pair(e.x, e.y));
+              w[16 * q + i] = pack2<BF>(e.x, e.y);
             }
           }
-          m = mn;
-        }
-        const float base = kLift - (m == -INFINITY ? 0.0f : m);
-        const uint64_t c2 = pair(c, c), base2 = pair(base, base);
-        uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 y = unpair(fma2(pair(__uint_as_float(x[32 * q + 2 * i]), __uint_as_float(x[32 * q + 2 * i + 1])), c2, base2));
-            const float e0 = exp2_fast(y.x), e1 = exp2_fast(y.y);
-            sum[i & 1] = add2(sum[i & 1], pair(e0, e1));
-            w[i] = pack2<BF>(e0, e1);
-          }
-          tmem_st16_nowait(ts + 16u * q, w);
-        }
-        {
           const float2 u = unpair(add2(sum[0], sum[1]));
-          l += u.x + u.y;
+          tile_sum = u.x + u.y;
+          if (look || !__any_sync(0xffffffffu, !(tile_sum <= kMost))) break;
+          look = true;
         }
+        l += tile_sum;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_st16_nowait(ts + 16u * q, w + 16 * q);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -624,8 +687,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       wait(o_full + g, op);
       op ^= 1u;
       tc_fence_after();
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      float bad = 0.0f;
+      const float inv = l == 0.0f || m == -INFINITY ? 0.0f : 1.0f / l;
+      float bad = m * 0.0f;  // (m = -inf: no visible key with a score above it, the sum is zero)
+      if (m == -INFINITY) bad = 0.0f;
 #pragma unroll 1
       for (int q = 0; q < HD / 32; ++q) {
         float t[32];
@@ -643,7 +707,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       }
       // 0 * x is NaN for an infinite or NaN x in a place that a row does not
       // see: such rows are computed again from their visible keys alone
-      uint32_t again = __ballot_sync(0xffffffffu, live && bad != 0.0f);
+      uint32_t again = __ballot_sync(0xffffffffu, live && !(bad == 0.0f));
       tc_fence_before();
       while (again) {
         const int src = __ffs(again) - 1;

@@ -42,12 +42,12 @@ constexpr long long kWaitClocks = 4000000000ll;
 RPGC_DEV bool wait_for(uint64_t* bar, uint32_t parity, volatile int32_t* gave_up, int32_t* status) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
-  for (;;) {
-    for (int i = 0; i < 16; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
+  do {
+    // suspended for up to 2 us at a time: a spinning warp would take issue
+    // slots from the warps it waits for
+    if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
     if (*gave_up) return false;
-    if (clock64() - t0 > kWaitClocks) break;
-  }
+  } while (clock64() - t0 < kWaitClocks);
   *gave_up = 1;
   if (status) atomicOr(status, kStatusTimeout);
   return false;
