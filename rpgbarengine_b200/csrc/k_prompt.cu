@@ -67,7 +67,15 @@ struct PromptParams {
   int32_t G;       // heads per kv head
   int32_t dual;    // two tiles per unit
   int32_t box;     // K/V rows of one TMA copy
+  int32_t wide;    // out lies on a 32-byte boundary
 };
+
+// 32 bytes, a whole sector, at a 32-byte boundary.
+RPGC_DEV void st_32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 
 // Two fp32 operations at once.
 RPGC_DEV uint64_t pair(float a, float b) {
@@ -687,7 +695,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       wait(o_full + g, op);
       op ^= 1u;
       tc_fence_after();
-      const float inv = l == 0.0f || m == -INFINITY ? 0.0f : 1.0f / l;
+      const float inv = l == 0.0f || m == -INFINITY || lim <= 0 ? 0.0f : 1.0f / l;
       float bad = m * 0.0f;  // (m = -inf: no visible key with a score above it, the sum is zero)
       if (m == -INFINITY) bad = 0.0f;
 #pragma unroll 1
@@ -702,8 +710,15 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         }
         if (live)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            reinterpret_cast<uint4*>(out)[4 * q + i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          for (int i = 0; i < 2; ++i) {
+            if (p.wide) {
+              st_32(out + 32 * q + 16 * i, w + 8 * i);
+            } else {
+              uint4* o = reinterpret_cast<uint4*>(out + 32 * q + 16 * i);
+              o[0] = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
+              o[1] = make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
+            }
+          }
       }
       // 0 * x is NaN for an infinite or NaN x in a place that a row does not
       // see: such rows are computed again from their visible keys alone
@@ -731,6 +746,7 @@ cudaError_t prompt_go(const PagedAttnArgs& a, cudaStream_t s) {
   p.a = a;
   p.G = a.n_heads / a.kv.n_kv;
   p.T = kRows / p.G;
+  p.wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
   int dev = 0;
   cudaGetDevice(&dev);
   const int sms = sm_count(dev);
