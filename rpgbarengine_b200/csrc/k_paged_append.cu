@@ -55,6 +55,9 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Pag
   constexpr int E = HD / 32;
   const int lane = threadIdx.x & 31, kv = a.kv.n_kv, heads = a.n_heads + 2 * kv;
   const int h0 = ((int)blockIdx.y * ((int)blockDim.x >> 5) + ((int)threadIdx.x >> 5)) * kHeads;
+  // launched as a programmatic dependent: its inputs come from earlier kernels
+  grid_dep_wait();
+  grid_dep_launch();
   if (h0 >= heads) return;  // whole warps
   const int64_t r = blockIdx.x;
   float x[kHeads][E];
@@ -131,9 +134,7 @@ template <int HD, int IN>
 cudaError_t append_go(const PagedAppendArgs& a, cudaStream_t s) {
   const int groups = (a.n_heads + 2 * a.kv.n_kv + kHeads - 1) / kHeads, rows = (groups + 7) / 8;
   const dim3 grid((unsigned)a.b.n_tokens, (unsigned)rows), block(32u * (unsigned)((groups + rows - 1) / rows));
-  if (a.kv.bf16) append_kernel<HD, IN, true><<<grid, block, 0, s>>>(a);
-  else append_kernel<HD, IN, false><<<grid, block, 0, s>>>(a);
-  return cudaGetLastError();
+  return a.kv.bf16 ? launch_pdl(append_kernel<HD, IN, true>, grid, block, 0, s, a) : launch_pdl(append_kernel<HD, IN, false>, grid, block, 0, s, a);
 }
 
 }  // namespace

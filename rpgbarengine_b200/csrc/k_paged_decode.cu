@@ -178,7 +178,11 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
     *gave_up = 0;
     fence_barrier_init();
   }
+  if (warp == kWarps && lane < 2) prefetch_map(lane ? &tm_v : &tm_k);
   __syncthreads();
+  // launched as a programmatic dependent: nothing that a kernel wrote is read before this
+  grid_dep_wait();
+  grid_dep_launch();
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, a.b.status); };
   int active;
   Walk w;
@@ -495,8 +499,7 @@ cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  decode_kernel<HD, BF, NT><<<sms, kDThreads, smem, s>>>(mk, mv, p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_pdl(decode_kernel<HD, BF, NT>, dim3((unsigned)sms), dim3(kDThreads), smem, s, mk, mv, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }

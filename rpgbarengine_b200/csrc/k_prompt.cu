@@ -288,9 +288,14 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tslot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (warp == 9 && lane < 3) prefetch_map(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // launched as a programmatic dependent: all of the above runs under the
+  // previous kernel's tail, nothing that a kernel wrote is read before this
+  grid_dep_wait();
+  grid_dep_launch();
   const uint32_t tmem = *tslot;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, status); };
 
@@ -772,8 +777,7 @@ cudaError_t prompt_go(const PagedAttnArgs& a, cudaStream_t s) {
   // the lengths are on the device: at most this many units exist
   const int64_t most = ((a.b.n_tokens + U - 1) / U + a.b.n_seqs) * a.kv.n_kv;
   const dim3 grid((unsigned)(most < sms ? most : sms));
-  prompt_kernel<HD, BF><<<grid, kPThreads, smem, s>>>(mq, mk, mv, p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_pdl(prompt_kernel<HD, BF>, grid, dim3(kPThreads), smem, s, mq, mk, mv, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }

@@ -30,6 +30,10 @@ RPGC_DEV void tma_4d(void* dst, const CUtensorMap* m, int x, int y, int z, int w
       : "memory");
 }
 
+RPGC_DEV void prefetch_map(const CUtensorMap* m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
+
 RPGC_DEV float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
