@@ -13,61 +13,54 @@ namespace {
 
 using namespace paged;
 
-// One warp per token and kHeads heads (q heads first, then k, then v): lane l
-// holds dims E*l .. E*l + E - 1 (E = HD / 32), so the rotation's partner dim
-// (d +- HD/2) is in lane l ^ 16.  Bound by memory: every input row is loaded
-// before the token's position and page are looked up, so that a warp has
-// kHeads rows in flight behind one chain of dependent reads (length -> page
-// and rope row).
-constexpr int kHeads = 4;
+// A warp takes one token and kSteps x 32 / (HD / 8) of its heads (q heads first,
+// then k, then v): HD / 8 lanes hold a row, each with 4 dims of its first half and
+// the 4 dims they rotate with, so the rotation needs no exchange and a row's
+// sum of squares few.  Bound by memory as long as instructions are few: with a
+// row over the whole warp and the rotation through shuffles the kernel issued
+// twice as many and took 1.5 times as long.  Every input row is loaded before
+// the token's position and page are looked up (one chain of dependent reads).
+constexpr int kSteps = 2;
 enum { kInF32 = 0, kInF16 = 1, kInBF16 = 2 };
 
-// E values of a row, from this lane's first.
-template <int IN, int E>
-RPGC_DEV void load_row(const uint8_t* p, float* x) {
+// Four consecutive values.
+template <int IN>
+RPGC_DEV void load4(const void* base, int64_t off, float* x) {
   if (IN == kInF32) {
-    if (E == 4) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(p));
-      x[0] = f.x, x[1] = f.y, x[E - 2] = f.z, x[E - 1] = f.w;
-    } else {
-      const float2 f = __ldg(reinterpret_cast<const float2*>(p));
-      x[0] = f.x, x[1] = f.y;
-    }
+    const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + off));
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
   } else {
-    uint32_t w[2];
-    if (E == 4) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-      w[0] = u.x, w[1] = u.y;
-    } else {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-    }
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const float2 f = unpack2<IN == kInBF16>(w[i]);
-      x[2 * i] = f.x, x[2 * i + 1] = f.y;
-    }
+    const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + off));
+    const float2 f = unpack2<IN == kInBF16>(u.x), g = unpack2<IN == kInBF16>(u.y);
+    x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
   }
 }
 
 template <int HD, int IN, bool BF>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ PagedAppendArgs a) {
-  constexpr int E = HD / 32, kIn = IN == kInF32 ? 4 : 2;
+  constexpr int kLanes = HD / 8, kRows = 32 / kLanes, kHalf = HD / 2;
   const int lane = threadIdx.x & 31, kv = a.kv.n_kv, nk = a.n_heads + kv, heads = nk + kv;
-  const int h0 = ((int)blockIdx.y * ((int)blockDim.x >> 5) + ((int)threadIdx.x >> 5)) * kHeads;
+  const int w = (int)blockIdx.y * ((int)blockDim.x >> 5) + ((int)threadIdx.x >> 5);
+  const int h0 = w * kSteps * kRows, hl = h0 + lane / kLanes, d = 4 * (lane % kLanes);
   // launched as a programmatic dependent: its inputs come from earlier kernels
   grid_dep_wait();
   grid_dep_launch();
   if (h0 >= heads) return;  // whole warps
   const int64_t r = blockIdx.x;
-  const int nh = min(kHeads, heads - h0);
-  float x[kHeads][E];
+  float x[kSteps][8];  // dims d .. d + 3, then kHalf + d ..
 #pragma unroll
-  for (int j = 0; j < kHeads; ++j) {
-    const int h = h0 + j;
+  for (int j = 0; j < kSteps; ++j) {
+    const int h = hl + j * kRows;
     const bool isq = h < a.n_heads, isk = h < nk;
     const void* base = isq ? a.q : isk ? a.k : a.v;
-    const int64_t off = isq ? r * a.q_tok + h * a.q_head : isk ? r * a.k_tok + (h - a.n_heads) * a.k_head : r * a.v_tok + (h - nk) * a.v_head;
-    if (j < nh) load_row<IN, E>(static_cast<const uint8_t*>(base) + (off + E * lane) * kIn, x[j]);
+    const int64_t off = (isq ? r * a.q_tok + h * a.q_head : isk ? r * a.k_tok + (h - a.n_heads) * a.k_head : r * a.v_tok + (h - nk) * a.v_head) + d;
+    if (h < heads) {
+      load4<IN>(base, off, x[j]);
+      load4<IN>(base, off + kHalf, x[j] + 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
+    }
   }
   const int s = seq_of_row(a.b, r, lane);
   if (s < 0) return;
@@ -76,55 +69,63 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Pag
   const int32_t page = pos >= 0 ? page_of(a.kv, a.b, s, pos) : -1;
   const bool drop = page < 0 || (a.rope && pos >= a.rope_rows);
   if (drop && h0 == 0 && lane == 0 && a.b.status) atomicOr(a.b.status, kStatusDropped);
-  const bool turn = a.rope && !drop;
-  float c[E], sn[E], g[2][E];  // gains of q and of k
-#pragma unroll
-  for (int i = 0; i < E; ++i) c[i] = 1.0f, sn[i] = 0.0f, g[0][i] = g[1][i] = 1.0f;
+  const bool turn = a.rope && !drop, norm = a.k_norm != nullptr;
+  float c[4], sn[4];
   if (turn) {
-    const uint8_t* cs = reinterpret_cast<const uint8_t*>(a.rope + pos * HD + ((E * lane) & (HD / 2 - 1)));
-    load_row<kInF32, E>(cs, c);
-    load_row<kInF32, E>(cs + HD * 2, sn);
-#pragma unroll
-    for (int i = 0; i < E; ++i) sn[i] = lane < 16 ? -sn[i] : sn[i];
+    load4<kInF32>(a.rope, pos * HD + d, c);
+    load4<kInF32>(a.rope, pos * HD + kHalf + d, sn);
   }
-  if (a.q_norm && h0 < a.n_heads) load_row<kInF32, E>(reinterpret_cast<const uint8_t*>(a.q_norm + E * lane), g[0]);
-  if (a.k_norm && h0 + nh > a.n_heads) load_row<kInF32, E>(reinterpret_cast<const uint8_t*>(a.k_norm + E * lane), g[1]);
   const int64_t slot = pos & ((1 << a.kv.page_shift) - 1);
-  uint16_t* qd = static_cast<uint16_t*>(a.q_out) + r * a.n_heads * HD + E * lane;
-  uint16_t* kd = static_cast<uint16_t*>(const_cast<void*>(a.kv.k)) + page * a.kv.k_page + slot * a.kv.k_pos + E * lane;
-  uint16_t* vd = static_cast<uint16_t*>(const_cast<void*>(a.kv.v)) + page * a.kv.v_page + slot * a.kv.v_pos + E * lane;
+  uint16_t* qd = static_cast<uint16_t*>(a.q_out) + r * a.n_heads * HD + d;
+  uint16_t* kd = static_cast<uint16_t*>(const_cast<void*>(a.kv.k)) + page * a.kv.k_page + slot * a.kv.k_pos + d;
+  uint16_t* vd = static_cast<uint16_t*>(const_cast<void*>(a.kv.v)) + page * a.kv.v_page + slot * a.kv.v_pos + d;
 #pragma unroll
-  for (int j = 0; j < kHeads; ++j) {
-    if (j >= nh) break;  // whole warps
-    const int h = h0 + j;
+  for (int j = 0; j < kSteps; ++j) {
+    const int hs = h0 + j * kRows, h = hl + j * kRows;  // the step's first head; this lane's
+    if (hs >= heads) break;                             // whole warps
     const bool isq = h < a.n_heads, isk = h < nk;
-    if (isk && (isq ? a.q_norm : a.k_norm)) {
-      float ss = 0.0f;
+    if (hs < nk) {  // (a step's rows may be of two kinds: v's keep their values)
+      float y[8];
 #pragma unroll
-      for (int i = 0; i < E; ++i) ss += x[j][i] * x[j][i];
-      const float f = rsqrtf(warp_sum(ss) * (1.0f / HD) + a.eps);  // (2 ulp: far below the 16-bit rounding)
+      for (int i = 0; i < 8; ++i) y[i] = x[j][i];
+      if (norm) {
+        float ss = 0.0f, g[8];
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[j][i] = x[j][i] * f * (isq ? g[0][i] : g[1][i]);
+        for (int i = 0; i < 8; ++i) ss += y[i] * y[i];
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float f = rsqrtf(ss * (1.0f / HD) + a.eps);  // (2 ulp: far below the 16-bit rounding)
+        const float* gain = isq ? a.q_norm : a.k_norm;
+        load4<kInF32>(gain, d, g);
+        load4<kInF32>(gain, kHalf + d, g + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * f * g[i];
+      }
+      if (turn)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u = y[i], v = y[i + 4];
+          y[i] = u * c[i] - v * sn[i];
+          y[i + 4] = v * c[i] + u * sn[i];
+        }
+      if (isk)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[j][i] = y[i];
     }
-    if (isk && turn)
+    if (h >= heads || (drop && !isq)) continue;
+    if (drop)  // no place in the cache: q's row is zeros
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[j][i] = x[j][i] * c[i] + __shfl_xor_sync(0xffffffffu, x[j][i], 16) * sn[i];
-    if (drop) {  // no place in the cache; q's row is zeros
-      if (!isq) break;
-#pragma unroll
-      for (int i = 0; i < E; ++i) x[j][i] = 0.0f;
-    }
+      for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
     uint16_t* dst = isq ? qd + h * HD : isk ? kd + (h - a.n_heads) * a.kv.k_head : vd + (h - nk) * a.kv.v_head;
-    if (E == 4)
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF>(x[j][0], x[j][1]), pack2<BF>(x[j][E - 2], x[j][E - 1]));
-    else
-      *reinterpret_cast<uint32_t*>(dst) = pack2<BF>(x[j][0], x[j][1]);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF>(x[j][0], x[j][1]), pack2<BF>(x[j][2], x[j][3]));
+    *reinterpret_cast<uint2*>(dst + kHalf) = make_uint2(pack2<BF>(x[j][4], x[j][5]), pack2<BF>(x[j][6], x[j][7]));
   }
 }
 
 template <int HD, int IN>
 cudaError_t append_go(const PagedAppendArgs& a, cudaStream_t s) {
-  const int groups = (a.n_heads + 2 * a.kv.n_kv + kHeads - 1) / kHeads, rows = (groups + 7) / 8;
+  const int per = kSteps * 256 / HD;  // heads of a warp
+  const int groups = (a.n_heads + 2 * a.kv.n_kv + per - 1) / per, rows = (groups + 7) / 8;
   const dim3 grid((unsigned)a.b.n_tokens, (unsigned)rows), block(32u * (unsigned)((groups + rows - 1) / rows));
   return a.kv.bf16 ? launch_pdl(append_kernel<HD, IN, true>, grid, block, 0, s, a) : launch_pdl(append_kernel<HD, IN, false>, grid, block, 0, s, a);
 }
