@@ -14,8 +14,8 @@
 // workspace, in the order of the pieces (the same result whoever is last).
 //
 // A CTA: one warp walks its range and issues TMA copies of K and V tiles into
-// a ring of 6 (hd 128), so ~190 KB are in flight per SM; 4 warps take 16 keys each of
-// every tile: S^T = K Q^T (m16n8k16, the kv head's query heads are the N side),
+// a ring of 6 (hd 128), so ~190 KB are in flight per SM; two groups of 4 warps
+// take the tiles in turn, 16 keys a warp: S^T = K Q^T (m16n8k16, the kv head's query heads are the N side),
 // P^T turned from the accumulator layout into an operand by movmatrix,
 // O^T += V^T P^T.  The warps' sums meet in shared memory at an item's end.
 #include <cuda_runtime.h>
@@ -29,8 +29,7 @@ namespace {
 using namespace paged;
 
 constexpr int kTile = 64;  // keys of a tile
-constexpr int kWarps = 4;  // consumer warps, 16 keys each
-constexpr int kDThreads = (kWarps + 1) * 32;
+constexpr int kGroup = 4;  // consumer warps on a tile, 16 keys each
 constexpr float kGrow = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -40,7 +39,8 @@ struct DShape {
   static constexpr int kPanel = kTile * 128;
   static constexpr int kHalf = kPanels * kPanel;  // K (or V) of a tile
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kStages = HD == 128 ? 6 : 12;
+  static constexpr int kStages = HD == 128 ? 6 : 12;  // (even: the groups take them in turn)
+  static constexpr int kGroups = NT == 1 ? 2 : 1, kWarps = kGroups * kGroup, kThreads = (kWarps + 1) * 32;
   static constexpr int kHeads = 8 * NT;           // query heads of a kv head, padded
   static constexpr int kPad = HD + 4;             // row of the merge buffer: no bank conflicts
   static constexpr int kMaxCtas = 256;
@@ -149,14 +149,17 @@ struct Walk {
   }
 };
 
-RPGC_DEV void bar_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+template <int N>
+RPGC_DEV void bar_consumers() {
+  asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
+}
 
 template <int HD, bool BF, int NT>
-__global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_constant__ CUtensorMap tm_k,
+__global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(const __grid_constant__ CUtensorMap tm_k,
                                                               const __grid_constant__ CUtensorMap tm_v,
                                                               const __grid_constant__ DecodeParams p) {
   using S = DShape<HD, NT>;
-  constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad;
+  constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps;
   constexpr float kLift = BF ? 0.0f : 6.0f;  // fp16 probabilities carry 2^6: small ones keep their bits
   extern __shared__ uint8_t dsm_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, kWarps);
+      mbar_init(empty + i, kGroup);
     }
     *gave_up = 0;
     fence_barrier_init();
@@ -254,11 +257,12 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
         reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)s * a.n_heads * HD)[i] = make_uint4(0, 0, 0, 0);
   if (!work) return;
   const int gr = lane >> 2, tq = lane & 3, G = p.G;
+  const int part = warp % kGroup, group = warp / kGroup;  // 16 keys of a tile; every second tile
   const float c = a.scale * kLog2e;
   // ldmatrix rows of this lane in the warp's 16 keys: K as stored, V transposed
   const int mi = lane >> 3, mr = lane & 7;
-  const int krow = 16 * warp + mr + 8 * (mi & 1), kc = mi >> 1;
-  const int vrow = 16 * warp + mr + 8 * (mi >> 1), vc = mi & 1;
+  const int krow = 16 * part + mr + 8 * (mi & 1), kc = mi >> 1;
+  const int vrow = 16 * part + mr + 8 * (mi >> 1), vc = mi & 1;
   int st = 0;
   uint32_t ph = 0;
   do {
@@ -284,9 +288,13 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
       for (int d = 0; d < HD / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.0f;
     }
     for (int t = t0; t < t1; ++t) {
+      if (S::kGroups > 1 && (st & 1) != group) {
+        if (++st == kStages) st = 0, ph ^= 1u;
+        continue;
+      }
       wait(full + st, ph);
-      const int left = w.len - t * kTile - 16 * warp;  // keys of this warp's group
-      if (left > 0 && (there[st] >> warp & 1u)) {
+      const int left = w.len - t * kTile - 16 * part;  // keys of this warp's part
+      if (left > 0 && (there[st] >> part & 1u)) {
         const uint32_t kb = smem_u32(ring + st * S::kStage), vb = kb + S::kHalf;
         float s[NT][4];
 #pragma unroll
@@ -385,7 +393,7 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
             row[16 * d + 8] = o[n][d][e + 2];
           }
       }
-    bar_consumers();
+    bar_consumers<kWarps * 32>();
     const bool whole = w.i0 >= w.lo && w.i1 <= w.hi;
     const int slot = 2 * blockIdx.x + (w.lo < w.i0 ? 1 : 0);
     for (int i = tid; i < G * HD / 4; i += kWarps * 32) {
@@ -419,9 +427,9 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
       // ---- the last CTA to finish a shared item joins its pieces
       const int b0 = (int)(((w.i0 + 1) * active - 1) / w.total), b1 = (int)((w.i1 * active - 1) / w.total);
       __threadfence();
-      bar_consumers();
+      bar_consumers<kWarps * 32>();
       if (tid == 0) *last = atomicInc(p.counters + (int64_t)w.seq * a.kv.n_kv + w.kh, (uint32_t)(b1 - b0)) == (uint32_t)(b1 - b0);
-      bar_consumers();
+      bar_consumers<kWarps * 32>();
       if (*last) {
         __threadfence();
         // every piece's (reference, weight) of every head at once, one read each;
@@ -430,10 +438,10 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
         float2* ml = reinterpret_cast<float2*>(wo);                      // [piece][head]
         int32_t* slots = reinterpret_cast<int32_t*>(ml + pieces * G);    // [piece]
         for (int k = tid; k < pieces; k += kWarps * 32) slots[k] = 2 * (b0 + k) + (w.begin(b0 + k, active) < w.i0 ? 1 : 0);
-        bar_consumers();
+        bar_consumers<kWarps * 32>();
         for (int i = tid; i < pieces * G; i += kWarps * 32)
           ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + (int64_t)slots[i / G] * G + i % G);
-        bar_consumers();
+        bar_consumers<kWarps * 32>();
         for (int i = tid; i < G * HD / 4; i += kWarps * 32) {
           const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
           const float* part = p.part + h * HD + d;
@@ -464,7 +472,7 @@ __global__ void __launch_bounds__(kDThreads, 1) decode_kernel(const __grid_const
         }
       }
     }
-    bar_consumers();  // the merge buffer is free again
+    bar_consumers<kWarps * 32>();  // the merge buffer is free again
   } while (w.next(a));
 }
 
@@ -499,7 +507,7 @@ cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const cudaError_t e = launch_pdl(decode_kernel<HD, BF, NT>, dim3((unsigned)sms), dim3(kDThreads), smem, s, mk, mv, p);
+  const cudaError_t e = launch_pdl(decode_kernel<HD, BF, NT>, dim3((unsigned)sms), dim3(DShape<HD, NT>::kThreads), smem, s, mk, mv, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
