@@ -7,15 +7,16 @@
 // steps rescale nothing.  Reference: AttentionFromCache (src/qwen3.cc:79-117).
 //
 // Bound: every K and V byte is read once, so HBM is the limit.  The key tiles
-// (64 keys) of all (sequence, kv head) items form one list, cut into equal
+// of all (sequence, kv head) items form one list, cut into equal
 // ranges, one per CTA and SM: batches of any mix of lengths, and one long
 // sequence as well, give every SM the same bytes.  An item that several CTAs
 // share is joined by the last of them to finish, from partial results in the
 // workspace, in the order of the pieces (the same result whoever is last).
 //
-// A CTA: one warp walks its range and issues TMA copies of K and V tiles into
-// a ring of 6 (hd 128), so ~190 KB are in flight per SM; two groups of 4 warps
-// take the tiles in turn, 16 keys a warp: S^T = K Q^T (m16n8k16, the kv head's query heads are the N side),
+// A CTA: two warps walk its range and issue the TMA copies of K and of V into a
+// ring of 6 tiles, so 192 KB are in flight per SM (with one warp for both, pages of
+// 16 positions of 64 dims were issued at 2.8 TB/s).  Two groups of 4 warps (hd 128)
+// or one of 8 take the tiles, 16 keys a warp: S^T = K Q^T (m16n8k16, the kv head's query heads are the N side),
 // P^T turned from the accumulator layout into an operand by movmatrix,
 // O^T += V^T P^T.  The warps' sums meet in shared memory at an item's end.
 #include <cuda_runtime.h>
@@ -28,19 +29,19 @@ namespace {
 
 using namespace paged;
 
-constexpr int kTile = 64;  // keys of a tile
-constexpr int kGroup = 4;  // consumer warps on a tile, 16 keys each
 constexpr float kGrow = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD, int NT>
 struct DShape {
+  static constexpr int kTile = HD == 128 ? 64 : 128;  // keys: 32 KB of K and V either way
+  static constexpr int kGroup = kTile / 16;           // consumer warps on a tile, 16 keys each
   static constexpr int kPanels = HD / 64;
   static constexpr int kPanel = kTile * 128;
   static constexpr int kHalf = kPanels * kPanel;  // K (or V) of a tile
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kStages = HD == 128 ? 6 : 12;  // (even: the groups take them in turn)
-  static constexpr int kGroups = NT == 1 ? 2 : 1, kWarps = kGroups * kGroup, kThreads = (kWarps + 1) * 32;
+  static constexpr int kGroups = HD == 128 && NT == 1 ? 2 : 1, kWarps = kGroups * kGroup, kThreads = (kWarps + 2) * 32;
+  static constexpr int kStages = HD == 64 && NT == 2 ? 5 : 6;  // (even where two groups take them in turn)
   static constexpr int kHeads = 8 * NT;           // query heads of a kv head, padded
   static constexpr int kPad = HD + 4;             // row of the merge buffer: no bank conflicts
   static constexpr int kMaxCtas = 256;
@@ -95,9 +96,13 @@ RPGC_DEV int32_t seen(const PagedAttnArgs& a, int s) {  // positions the token o
   const int64_t n = min((int64_t)max(0, __ldg(a.b.kv_lens + s)), table_reach(a.kv, a.b));
   return (int32_t)n;
 }
-RPGC_DEV int64_t tiles_of(int32_t n) { return (n + (int64_t)kTile - 1) / kTile; }
+template <int T>
+RPGC_DEV int64_t tiles_of(int32_t n) {
+  return (n + (int64_t)T - 1) / T;
+}
 
 // One CTA's range of the list, item by item; every warp walks it by itself.
+template <int T>
 struct Walk {
   int64_t total, lo, hi;  // all tiles; this CTA's
   int32_t seq, kh, len;   // the item
@@ -106,7 +111,7 @@ struct Walk {
   RPGC_DEV bool start(const PagedAttnArgs& a, int lane, int ctas, int cta, int* active) {
     const int64_t kv = a.kv.n_kv;
     int64_t sum = 0;
-    for (int s = lane; s < a.b.n_seqs; s += 32) sum += tiles_of(seen(a, s));
+    for (int s = lane; s < a.b.n_seqs; s += 32) sum += tiles_of<T>(seen(a, s));
     total = warp_sum(sum) * kv;
     const int n = (int)(total < ctas ? total : ctas);
     *active = n;
@@ -115,7 +120,7 @@ struct Walk {
     hi = begin(cta + 1, n);
     int64_t before = 0;  // tiles of the sequences before s0
     for (int s0 = 0;; s0 += 32) {
-      const int64_t mine = s0 + lane < a.b.n_seqs ? tiles_of(seen(a, s0 + lane)) * kv : 0;
+      const int64_t mine = s0 + lane < a.b.n_seqs ? tiles_of<T>(seen(a, s0 + lane)) * kv : 0;
       int64_t upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -128,9 +133,9 @@ struct Walk {
         const int64_t first = before + __shfl_sync(0xffffffffu, upto - mine, src);
         seq = s0 + src;
         len = seen(a, seq);
-        kh = (int32_t)((lo - first) / tiles_of(len));
-        i0 = first + kh * tiles_of(len);
-        i1 = i0 + tiles_of(len);
+        kh = (int32_t)((lo - first) / tiles_of<T>(len));
+        i0 = first + kh * tiles_of<T>(len);
+        i1 = i0 + tiles_of<T>(len);
         return true;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
@@ -144,7 +149,7 @@ struct Walk {
       while (!len);  // (a later item exists: i1 < hi <= total)
     }
     i0 = i1;
-    i1 = i0 + tiles_of(len);
+    i1 = i0 + tiles_of<T>(len);
     return true;
   }
 };
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
                                                               const __grid_constant__ CUtensorMap tm_v,
                                                               const __grid_constant__ DecodeParams p) {
   using S = DShape<HD, NT>;
-  constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps;
+  constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps, kTile = S::kTile, kGroup = S::kGroup;
   constexpr float kLift = BF ? 0.0f : 6.0f;  // fp16 probabilities carry 2^6: small ones keep their bits
   extern __shared__ uint8_t dsm_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
@@ -175,7 +180,7 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full + i, 2);
       mbar_init(empty + i, kGroup);
     }
     *gave_up = 0;
@@ -188,10 +193,10 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
   grid_dep_launch();
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, a.b.status); };
   int active;
-  Walk w;
+  Walk<kTile> w;
   const bool work = w.start(a, lane, gridDim.x, blockIdx.x, &active);
 
-  if (warp == kWarps) {
+  if (warp >= kWarps) {  // one warp copies K, the other V
     // ---------------------------------------------------------------- loads
     if (!work) return;
     int st = 0;
@@ -221,22 +226,20 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
         wait(empty + st, ph ^ 1u);
         if (*gave_up) break;
         if (lane == 0) {
-          uint32_t groups = 0;  // a copy of 16, 32 or 64 rows covers 1, 2 or 4 groups
+          uint32_t groups = 0;  // a copy of 16, 32, .. rows covers 1, 2, .. groups of 16
           const int g = p.box >> 4;
           for (int i = 0; i < per; ++i)
             if (have >> i & 1u) groups |= ((1u << g) - 1u) << (i * g);
-          there[st] = groups;
-          mbar_arrive_expect_tx(full + st, S::kStage);
+          if (warp == kWarps) there[st] = groups;
+          mbar_arrive_expect_tx(full + st, S::kHalf);
         }
         __syncwarp();
         if (lane < per) {
           const int at = (int)((base + (int64_t)(c + lane) * p.box) & ((1 << pshift) - 1));
-          uint8_t* dst = ring + st * S::kStage + lane * p.box * 128;
+          const bool v = warp > kWarps;
+          uint8_t* dst = ring + st * S::kStage + (v ? S::kHalf : 0) + lane * p.box * 128;
 #pragma unroll
-          for (int h = 0; h < S::kPanels; ++h) {
-            tma_4d(dst + h * S::kPanel, &tm_k, 64 * h, w.kh, at, page, full + st);
-            tma_4d(dst + S::kHalf + h * S::kPanel, &tm_v, 64 * h, w.kh, at, page, full + st);
-          }
+          for (int h = 0; h < S::kPanels; ++h) tma_4d(dst + h * S::kPanel, v ? &tm_v : &tm_k, 64 * h, w.kh, at, page, full + st);
         }
         if (++st == kStages) st = 0, ph ^= 1u;
       }
@@ -490,13 +493,14 @@ cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
   DecodeParams p{};
   p.a = a;
   p.G = a.n_heads / a.kv.n_kv;
-  p.box = a.kv.page_shift < 6 ? 1 << a.kv.page_shift : kTile;
+  p.box = (1 << a.kv.page_shift) < DShape<HD, NT>::kTile ? 1 << a.kv.page_shift : DShape<HD, NT>::kTile;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.counters = reinterpret_cast<uint32_t*>(ws);
   p.part = reinterpret_cast<float*>(ws + counter_bytes(a.kv, a.b.n_seqs));
   p.part_ml = p.part + (int64_t)2 * sms * p.G * HD;
   CUtensorMap mk, mv;
-  if (!make_kv_map(&mk, a, false, p.box) || !make_kv_map(&mv, a, true, p.box)) return cudaErrorInvalidValue;
+  const CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
+  if (!make_kv_map(&mk, a, false, p.box, promo) || !make_kv_map(&mv, a, true, p.box, promo)) return cudaErrorInvalidValue;
   constexpr int smem = DShape<HD, NT>::kSmem;
   static_assert(smem <= 232448, "shared memory of one CTA");
   int dev = 0;

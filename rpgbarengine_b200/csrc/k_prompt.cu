@@ -763,7 +763,7 @@ cudaError_t prompt_go(const PagedAttnArgs& a, cudaStream_t s) {
   {
     const int64_t dims[3] = {HD, a.n_heads, a.b.n_tokens}, st[2] = {a.q_head, a.q_tok};
     const int box[3] = {64, p.G, p.T};
-    if (!make_map(&mq, a.q, 3, dims, st, box)) return cudaErrorInvalidValue;
+    if (!make_map(&mq, a.q, 3, dims, st, box, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return cudaErrorInvalidValue;
   }
   if (!make_kv_map(&mk, a, false, p.box) || !make_kv_map(&mv, a, true, p.box)) return cudaErrorInvalidValue;
   constexpr int smem = Shape<HD>::kSmem;

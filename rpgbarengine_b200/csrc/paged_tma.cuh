@@ -71,7 +71,8 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 }
 
 // A map of 16-bit values: rows of hd values, `rank` - 1 strides in elements.
-inline bool make_map(CUtensorMap* m, const void* base, int rank, const int64_t* dims, const int64_t* strides, const int* box) {
+inline bool make_map(CUtensorMap* m, const void* base, int rank, const int64_t* dims, const int64_t* strides, const int* box,
+                     CUtensorMapL2promotion promo) {
   auto enc = encoder();
   if (!enc) return false;
   cuuint64_t d[4], st[3];
@@ -82,7 +83,7 @@ inline bool make_map(CUtensorMap* m, const void* base, int rank, const int64_t* 
     if (i) st[i - 1] = (cuuint64_t)strides[i - 1] * 2;
   }
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, b, es,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promo,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -95,17 +96,18 @@ inline int sm_count(int dev) {
 
 // K or V as TMA sees it, copies of `box` rows: {dim, kv head, position, page},
 // or {dim, kv head, row} where K and V are packed.
-inline bool make_kv_map(CUtensorMap* m, const PagedAttnArgs& a, bool v, int box) {
+inline bool make_kv_map(CUtensorMap* m, const PagedAttnArgs& a, bool v, int box,
+                        CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
   const void* base = v ? a.kv.v : a.kv.k;
   const int64_t pos = v ? a.kv.v_pos : a.kv.k_pos, head = v ? a.kv.v_head : a.kv.k_head, page = v ? a.kv.v_page : a.kv.k_page;
   if (!a.b.table) {
     const int64_t dims[3] = {a.kv.hd, a.kv.n_kv, a.b.n_tokens}, st[2] = {head, pos};
     const int b[3] = {64, 1, box};
-    return make_map(m, base, 3, dims, st, b);
+    return make_map(m, base, 3, dims, st, b, promo);
   }
   const int64_t dims[4] = {a.kv.hd, a.kv.n_kv, int64_t(1) << a.kv.page_shift, a.kv.n_pages}, st[3] = {head, pos, page};
   const int b[4] = {64, 1, box, 1};
-  return make_map(m, base, 4, dims, st, b);
+  return make_map(m, base, 4, dims, st, b, promo);
 }
 
 }  // namespace paged
