@@ -96,31 +96,56 @@ RPGC_DEV int32_t seen(const PagedAttnArgs& a, int s) {  // positions the token o
   const int64_t n = min((int64_t)max(0, __ldg(a.b.kv_lens + s)), table_reach(a.kv, a.b));
   return (int32_t)n;
 }
+// What an item weighs in the list: its key tiles, and the end of an item (the
+// warps' sums, a share's join) as kEnd tiles more, at its front.  An item that sees
+// nothing weighs nothing.
+constexpr int kEnd = 2;
 template <int T>
-RPGC_DEV int64_t tiles_of(int32_t n) {
-  return (n + (int64_t)T - 1) / T;
+RPGC_DEV int64_t weight_of(int32_t n) {
+  return n ? (n + (int64_t)T - 1) / T + kEnd : 0;
 }
 
 // One CTA's range of the list, item by item; every warp walks it by itself.
 template <int T>
 struct Walk {
-  int64_t total, lo, hi;  // all tiles; this CTA's
+  int64_t total, lo, hi;  // weight of the list; this CTA's range
   int32_t seq, kh, len;   // the item
-  int64_t i0, i1;         // its tiles in the list
-  RPGC_DEV int64_t begin(int64_t b, int64_t n) const { return b * total / n; }
+  int64_t i0, i1;         // its key tiles in the list
+  int32_t t0, t1;         // those that are this CTA's
+  // where range b of n begins, and the range that holds place t
+  RPGC_DEV int64_t begin(int b, int n) const {
+    return total < (1 << 23) ? (int64_t)((uint32_t)b * (uint32_t)total / (uint32_t)n) : b * total / n;  // (n <= 256)
+  }
+  RPGC_DEV int holder(int64_t t, int n) const {
+    return total < (1 << 23) ? (int)((((uint32_t)t + 1) * (uint32_t)n - 1) / (uint32_t)total) : (int)(((t + 1) * n - 1) / total);
+  }
+  RPGC_DEV void item(int64_t first) {
+    i0 = first + kEnd;
+    i1 = first + weight_of<T>(len);
+    t0 = (int32_t)(lo > i0 ? lo - i0 : 0);
+    t1 = (int32_t)((hi < i1 ? hi : i1) - i0);
+  }
   RPGC_DEV bool start(const PagedAttnArgs& a, int lane, int ctas, int cta, int* active) {
     const int64_t kv = a.kv.n_kv;
+    // the first 128 lengths stay in registers for the second look
+    int32_t n[4];
     int64_t sum = 0;
-    for (int s = lane; s < a.b.n_seqs; s += 32) sum += tiles_of<T>(seen(a, s));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = 32 * i + lane < a.b.n_seqs ? seen(a, 32 * i + lane) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += weight_of<T>(n[i]);
+    for (int s = 128 + lane; s < a.b.n_seqs; s += 32) sum += weight_of<T>(seen(a, s));
     total = warp_sum(sum) * kv;
-    const int n = (int)(total < ctas ? total : ctas);
-    *active = n;
-    if (cta >= n) return false;
-    lo = begin(cta, n);
-    hi = begin(cta + 1, n);
-    int64_t before = 0;  // tiles of the sequences before s0
+    const int parts = (int)(total < ctas ? total : ctas);
+    *active = parts;
+    if (cta >= parts) return false;
+    lo = begin(cta, parts);
+    hi = begin(cta + 1, parts);
+    int64_t before = 0;  // weight of the sequences before s0
+#pragma unroll 1
     for (int s0 = 0;; s0 += 32) {
-      const int64_t mine = s0 + lane < a.b.n_seqs ? tiles_of<T>(seen(a, s0 + lane)) * kv : 0;
+      const int32_t ln = s0 >= 128 ? (s0 + lane < a.b.n_seqs ? seen(a, s0 + lane) : 0) : s0 == 0 ? n[0] : s0 == 32 ? n[1] : s0 == 64 ? n[2] : n[3];
+      const int64_t mine = weight_of<T>(ln) * kv;
       int64_t upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -132,10 +157,10 @@ struct Walk {
         const int src = __ffs(in) - 1;
         const int64_t first = before + __shfl_sync(0xffffffffu, upto - mine, src);
         seq = s0 + src;
-        len = seen(a, seq);
-        kh = (int32_t)((lo - first) / tiles_of<T>(len));
-        i0 = first + kh * tiles_of<T>(len);
-        i1 = i0 + tiles_of<T>(len);
+        len = __shfl_sync(0xffffffffu, ln, src);
+        const int64_t w = weight_of<T>(len), at = lo - first;
+        kh = at < (int64_t)0x7fffffff ? (int32_t)((uint32_t)at / (uint32_t)w) : (int32_t)(at / w);
+        item(first + kh * w);
         return true;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
@@ -148,8 +173,7 @@ struct Walk {
       do len = seen(a, ++seq);
       while (!len);  // (a later item exists: i1 < hi <= total)
     }
-    i0 = i1;
-    i1 = i0 + tiles_of<T>(len);
+    item(i1);
     return true;
   }
 };
@@ -205,7 +229,8 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
     const int pshift = a.kv.page_shift;
     do {
       const int32_t* tab = a.b.table + (int64_t)w.seq * a.b.table_stride;
-      const int t0 = (int)(max(w.lo, w.i0) - w.i0), t1 = (int)(min(w.hi, w.i1) - w.i0);
+      const int t0 = w.t0, t1 = w.t1;
+      if (t1 <= t0) continue;  // (the range ends in the item's front)
       // page ids ahead of their use: lane l holds the one of copy l of the next 32
       const int copies = (t1 - t0) * per;
       const int64_t base = (int64_t)t0 * kTile;
@@ -269,7 +294,8 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
   int st = 0;
   uint32_t ph = 0;
   do {
-    const int t0 = (int)(max(w.lo, w.i0) - w.i0), t1 = (int)(min(w.hi, w.i1) - w.i0);
+    const int t0 = w.t0, t1 = w.t1;
+    if (t1 <= t0) continue;
     // Q^T as the B operand: head 8 n + gr, dims 16 k + 2 tq (+8)
     uint32_t q[NT][HD / 16][2];
 #pragma unroll
@@ -428,13 +454,15 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
     }
     if (!whole) {
       // ---- the last CTA to finish a shared item joins its pieces
-      const int b0 = (int)(((w.i0 + 1) * active - 1) / w.total), b1 = (int)((w.i1 * active - 1) / w.total);
-      __threadfence();
+      const int b0 = w.holder(w.i0, active), b1 = w.holder(w.i1 - 1, active);
       bar_consumers<kWarps * 32>();
-      if (tid == 0) *last = atomicInc(p.counters + (int64_t)w.seq * a.kv.n_kv + w.kh, (uint32_t)(b1 - b0)) == (uint32_t)(b1 - b0);
+      if (tid == 0) {
+        __threadfence();  // (of all the warps' partial results: they are before this by the barrier)
+        *last = atomicInc(p.counters + (int64_t)w.seq * a.kv.n_kv + w.kh, (uint32_t)(b1 - b0)) == (uint32_t)(b1 - b0);
+        __threadfence();
+      }
       bar_consumers<kWarps * 32>();
       if (*last) {
-        __threadfence();
         // every piece's (reference, weight) of every head at once, one read each;
         // then the sums, eight pieces' rows in flight
         const int pieces = b1 - b0 + 1;
