@@ -12,7 +12,9 @@
 // Layout: the G query heads of a kv head share its keys, so a tile of 128 MMA
 // rows holds T = 128 / G tokens x G heads; a work unit is two such tiles (A,
 // B) of one sequence and kv head, one CTA per SM taking units from a list
-// sorted by cost, longest first.  Warps 0-3 / 4-7: softmax of tile A / B, one
+// sorted by cost, longest first.  Where that would leave SMs without a unit, a
+// unit is one tile of rows, A takes its even key tiles and B the odd ones, and
+// their sums meet at the end.  Warps 0-3 / 4-7: softmax of tile A / B, one
 // row per thread; warp 8: issues the MMAs; warp 9: TMA; warp 10: finds the
 // next unit.  S = Q K^T goes to TMEM (128 fp32 columns per tile); the softmax
 // warps read their row, write P over it in 16 bits, and O += P V takes P from
@@ -65,7 +67,7 @@ struct PromptParams {
   PagedAttnArgs a;
   int32_t T;       // tokens of a tile
   int32_t G;       // heads per kv head
-  int32_t dual;    // two tiles per unit
+  int32_t dual;    // two tiles of rows per unit; else one, its key tiles in turn on A and B
   int32_t box;     // K/V rows of one TMA copy
   int32_t wide;    // out lies on a 32-byte boundary
 };
@@ -207,21 +209,19 @@ RPGC_DEV SeqLens seq_lens(const PagedSeqs& b, int s) {
   }
   return q;
 }
-// First tile of the sequence whose cost is at least c (all later ones cost more).
+// First tile of the sequence whose cost is at least c (all later ones cost
+// more).  c is at most 2^23 + 2^17: positions past 2^30 count as 2^30 here.
 RPGC_DEV int32_t first_tile(SeqLens q, int32_t U, int32_t c) {
-  const int32_t tiles = (q.n + U - 1) / U;
+  const int32_t pre = min(q.pre, 1 << 30), x = kKeys * (c - 1) + 1;
   if (c <= 0) return 0;
-  const int32_t pre = min(q.pre, 1 << 30);
-  const int64_t x = (int64_t)kKeys * (c - 1) + 1;
-  if (pre + q.n < x) return tiles;
-  const int64_t d = x - pre;
-  return d <= 0 ? 0 : (int32_t)((d - 1) / U);
+  if (pre + q.n < x) return (int32_t)((uint32_t)(q.n + U - 1) / (uint32_t)U);
+  return x <= pre ? 0 : (int32_t)((uint32_t)(x - pre - 1) / (uint32_t)U);
 }
 RPGC_DEV int32_t tiles_at_least(const PagedSeqs& b, SeqLens mine, int32_t U, int32_t c, int lane) {
-  int32_t n = (mine.n + U - 1) / U - first_tile(mine, U, c);
+  int32_t n = (int32_t)((uint32_t)(mine.n + U - 1) / (uint32_t)U) - first_tile(mine, U, c);
   for (int s = lane + 32; s < b.n_seqs; s += 32) {
     const SeqLens q = seq_lens(b, s);
-    n += (q.n + U - 1) / U - first_tile(q, U, c);
+    n += (int32_t)((uint32_t)(q.n + U - 1) / (uint32_t)U) - first_tile(q, U, c);
   }
   return __reduce_add_sync(0xffffffffu, n);
 }
@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
   uint64_t* o_full = p_full + 2;           // [2] last P V of the unit done
   uint64_t* u_full = o_full + 2;           // [kUnits] unit described
   uint64_t* u_empty = u_full + kUnits;     // [kUnits] read by every role
-  uint64_t* done = u_empty + kUnits;
+  uint64_t* x_bar = u_empty + kUnits;      // the softmax groups, at the end of a unit of one tile
+  uint64_t* done = x_bar + 1;
   Unit* units = reinterpret_cast<Unit*>(done + 1);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(units + kUnits);
   volatile int32_t* gave_up = reinterpret_cast<volatile int32_t*>(tslot + 1);
@@ -280,6 +281,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       mbar_init(u_full + i, 1);
       mbar_init(u_empty + i, 10);
     }
+    mbar_init(x_bar, 8);
     mbar_init(done, 1);
     *gave_up = 0;
     fence_barrier_init();
@@ -356,8 +358,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
             un.reach = (int32_t)min(reach, (int64_t)0x7fffffff);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-              const int32_t first = g * p.T;
-              un.rows[g] = (g == 0 || p.dual) ? max(0, min(p.T, n_new - t0 - first)) : 0;
+              const int32_t first = p.dual ? g * p.T : 0;
+              un.rows[g] = max(0, min(p.T, n_new - t0 - first));
               un.end[g] = un.rows[g] ? (int32_t)max((int64_t)0, min((int64_t)un.pos0 + first + un.rows[g], reach)) : 0;
               un.tiles[g] = (un.end[g] + kKeys - 1) / kKeys;
             }
@@ -392,10 +394,11 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       ++nq;
       if (lane == 0) {
         const uint32_t bytes = (uint32_t)(p.T * p.G * 128 * kHalves);
-        mbar_arrive_expect_tx(q_full, bytes * (un.rows[1] ? 2 : 1));
+        const bool two = p.dual && un.rows[1];
+        mbar_arrive_expect_tx(q_full, bytes * (two ? 2 : 1));
 #pragma unroll
         for (int g = 0; g < 2; ++g)
-          if (g == 0 || un.rows[1])
+          if (g == 0 || two)
 #pragma unroll
           for (int h = 0; h < kHalves; ++h)
             tma_3d(Qs + (g * kHalves + h) * kPanel, &tm_q, 64 * h, un.kh * p.G, (int)(un.row0 + g * p.T), q_full);
@@ -436,16 +439,64 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------- MMAs
-    int st = 0;
-    uint32_t ph = 0;
+    uint32_t at = 0;            // the unit's first place in the ring: K tile j at + 2 j, V tile j after it
     uint32_t pp[2] = {0u, 0u};  // parity of p_full
     // One elected lane issues, from descriptors that differ by constants: with
     // anything more to compute between two MMAs the issue, not the tensor
     // core, sets the pace (150 clocks an MMA instead of 64).
     const uint64_t q_desc = sdesc(Qs), k_desc = sdesc(ring), v_desc = vdesc(ring, kPanel);
     int nq = 0;
-    auto next = [&] {
-      if (++st == kStages) st = 0, ph ^= 1u;
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) mma_commit(bar);
+      __syncwarp();
+    };
+    auto landed = [&](uint32_t c) {
+      wait(full + c % kStages, (c / kStages) & 1u);
+      tc_fence_after();
+    };
+    // S of accumulator g = Q (tile qt) K^T, K at ring place c
+    auto issue_s = [&](int g, int qt, uint32_t c) {
+      if (elect_one()) {
+        const uint64_t q = q_desc + (uint64_t)(qt * kHalves * kPanel / 16), k = k_desc + (uint64_t)(c % kStages * (S::kStage / 16));
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint64_t o = ((kk >> 2) * kPanel + (kk & 3) * 32) / 16;
+          mma_f16(tmem + 128u * g, q + o, k + o, kIdS, kk > 0);
+        }
+        mma_commit(s_full + g);
+      }
+      __syncwarp();
+    };
+    // O of accumulator g += P V, V at ring place c, once P is there
+    auto issue_pv = [&](int g, uint32_t c, int keys, bool first) {
+      wait(p_full + g, pp[g]);
+      pp[g] ^= 1u;
+      tc_fence_after();
+      const int steps = (keys + 15) >> 4;
+      if (elect_one()) {
+        const uint64_t vd = v_desc + (uint64_t)(c % kStages * (S::kStage / 16));
+        const uint32_t o = tmem + 256u + 128u * g, pt = tmem + 128u * g;
+        mma_ts(o, pt, vd, kIdO, !first);
+        if (steps == 8) {
+#pragma unroll
+          for (int kk = 1; kk < 8; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
+        } else {
+          for (int kk = 1; kk < steps; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
+        }
+      }
+      __syncwarp();
+    };
+    // the values past the last position of the last step of 16 keys become zeros
+    auto clear_tail = [&](uint32_t c, int keys) {
+      if (!(keys & 15)) return;
+      uint8_t* v = ring + c % kStages * S::kStage;
+      const int stop = (keys + 15) & ~15;
+      for (int i = lane; i < (stop - keys) * 8 * kHalves; i += 32) {
+        const int h = i / ((stop - keys) * 8), k = i % ((stop - keys) * 8);
+        *reinterpret_cast<uint4*>(v + h * kPanel + (keys + (k >> 3)) * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
     };
     for (int it = 0;; ++it) {
       wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
@@ -453,92 +504,66 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(u_empty + it % kUnits);
       if (un.seq < 0 || *gave_up) break;
-      const int nt = max(un.tiles[0], un.tiles[1]);
+      const int nt = max(un.tiles[0], un.tiles[1]), end = max(un.end[0], un.end[1]);
       if (!nt) continue;
-      const int end = max(un.end[0], un.end[1]);
-      auto issue_s = [&](int g, int stage) {  // S of tile g over the K tile in `stage`
-        if (elect_one()) {
-          const uint64_t q = q_desc + (uint64_t)(g * kHalves * kPanel / 16), k = k_desc + (uint64_t)(stage * (S::kStage / 16));
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint64_t o = ((kk >> 2) * kPanel + (kk & 3) * 32) / 16;
-            mma_f16(tmem + 128u * g, q + o, k + o, kIdS, kk > 0);
-          }
-          mma_commit(s_full + g);
-        }
-        __syncwarp();
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) mma_commit(bar);
-        __syncwarp();
-      };
       wait(q_full, (uint32_t)nq & 1u);
       ++nq;
-      wait(full + st, ph);
-      tc_fence_after();
+      if (p.dual) {
+        landed(at);
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (un.tiles[g] > 0) issue_s(g, st);
-      commit(empty + st);
-      if (nt == 1) commit(q_empty);
-      next();
-      for (int j = 0; j < nt; ++j) {
-        const int vst = st;
-        wait(full + st, ph);
-        next();
-        const int kst = st;
-        const uint32_t kph = ph;
-        const bool more = j + 1 < nt;
-        if (more) next();
-        uint8_t* v = ring + vst * S::kStage;
-        const int keys = min(kKeys, end - j * kKeys);
-        if (keys & 15) {  // the values past the last position of the last step of 16 become zeros
-          const int stop = (keys + 15) & ~15;
-          for (int i = lane; i < (stop - keys) * 8 * kHalves; i += 32) {
-            const int h = i / ((stop - keys) * 8), c = i % ((stop - keys) * 8);
-            *reinterpret_cast<uint4*>(v + h * kPanel + (keys + (c >> 3)) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-        bool waited = false;
+        for (int g = 0; g < 2; ++g)
+          if (un.tiles[g] > 0) issue_s(g, g, at);
+        commit(empty + at % kStages);
+        if (nt == 1) commit(q_empty);
+        for (int j = 0; j < nt && !*gave_up; ++j) {
+          const uint32_t vc = at + 2 * j + 1, kc = vc + 1;
+          const bool more = j + 1 < nt;
+          landed(vc);
+          clear_tail(vc, min(kKeys, end - j * kKeys));
+          bool waited = false;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (j < un.tiles[g]) {
-            wait(p_full + g, pp[g]);
-            pp[g] ^= 1u;
-            tc_fence_after();
-            const int steps = (min(kKeys, un.end[g] - j * kKeys) + 15) >> 4;
-            if (elect_one()) {
-              const uint64_t vd = v_desc + (uint64_t)(vst * (S::kStage / 16));
-              const uint32_t o = tmem + 256u + 128u * g, pt = tmem + 128u * g;
-              mma_ts(o, pt, vd, kIdO, j > 0);
-              if (steps == 8) {
-#pragma unroll
-                for (int kk = 1; kk < 8; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
-              } else {
-                for (int kk = 1; kk < steps; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
-              }
+          for (int g = 0; g < 2; ++g) {
+            if (j < un.tiles[g]) {
+              issue_pv(g, vc, min(kKeys, un.end[g] - j * kKeys), j == 0);
+              if (j + 1 == un.tiles[g]) commit(o_full + g);
             }
-            __syncwarp();
-            if (j + 1 == un.tiles[g]) commit(o_full + g);
-          }
-          if (j + 1 < un.tiles[g]) {
-            if (!waited) {
-              wait(full + kst, kph);
-              tc_fence_after();
+            if (j + 1 < un.tiles[g]) {
+              if (!waited) landed(kc);
               waited = true;
+              issue_s(g, g, kc);
             }
-            issue_s(g, kst);
           }
-        }
-        commit(empty + vst);
-        if (more) {
-          commit(empty + kst);
+          commit(empty + vc % kStages);
+          if (more) commit(empty + kc % kStages);
           if (j + 2 == nt) commit(q_empty);
         }
-        if (*gave_up) break;
+      } else {
+        // one tile of rows: accumulator A takes its even key tiles, B the odd ones
+        for (int j = 0; j < 2 && j < nt; ++j) {
+          const uint32_t kc = at + 2 * j;
+          landed(kc);
+          issue_s(j, 0, kc);
+          commit(empty + kc % kStages);
+        }
+        if (nt <= 2) commit(q_empty);
+        for (int j = 0; j < nt && !*gave_up; ++j) {
+          const uint32_t vc = at + 2 * j + 1, kc = vc + 3;
+          const int keys = min(kKeys, end - j * kKeys);
+          landed(vc);
+          clear_tail(vc, keys);
+          if (j & 1) issue_pv(1, vc, keys, j < 2);
+          else issue_pv(0, vc, keys, j < 2);
+          if (j + 2 >= nt) commit(o_full + (j & 1));
+          commit(empty + vc % kStages);
+          if (j + 2 < nt) {
+            landed(kc);
+            issue_s(j & 1, 0, kc);
+            commit(empty + kc % kStages);
+            if (j + 3 == nt) commit(q_empty);
+          }
+        }
       }
+      at += 2 * nt;
       if (*gave_up) break;
     }
     if (elect_one()) mma_commit(done);
@@ -555,7 +580,14 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
     const int tok = r / p.G, head = r - tok * p.G;
     const float c = a.scale * kLog2e;
     const int shift = paged ? min(a.kv.page_shift, 7) : 7, npg = paged ? (shift < 7 ? kKeys >> shift : 1) : 0;
-    uint32_t sp = 0, op = 0;
+    uint32_t sp = 0, op = 0, op_b = 0, xp = 0;
+    const int step = p.dual ? 1 : 2, j0 = p.dual ? 0 : g;  // this group's key tiles
+    auto both = [&] {  // the two groups meet
+      __syncwarp();
+      if (lane == 0) mbar_arrive(x_bar);
+      wait(x_bar, xp);
+      xp ^= 1u;
+    };
     for (int it = 0;; ++it) {
       wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
       const Unit* up = units + it % kUnits;
@@ -569,7 +601,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         release();
         continue;
       }
-      const int first = up->pos0 + g * p.T, reach = up->reach;
+      const int off = p.dual ? g * p.T : 0, first = up->pos0 + off, reach = up->reach;
       const bool live = tok < rows;  // (rows past T * G have tok >= T >= rows)
       const int lim = live ? (int)max((int64_t)0, min((int64_t)first + tok + 1, (int64_t)reach)) : 0;
       const int whole = max(0, min(first + 1, reach)) / kKeys;  // key tiles that every row sees whole
@@ -580,12 +612,12 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         const int64_t e = (((int64_t)j * kKeys) >> a.kv.page_shift) + lane;
         return lane < npg && e < a.b.max_pages ? __ldg(tab + e) : 0;
       };
-      int32_t pg = paged && tiles ? entry(0) : 0;
-      for (int j = 0; j < tiles; ++j) {
+      int32_t pg = paged && j0 < tiles ? entry(j0) : 0;
+      for (int j = j0; j < tiles; j += step) {
         uint32_t gone = 0;  // this tile's pages that are not there
         if (paged) {
           gone = __ballot_sync(0xffffffffu, lane < npg && (uint32_t)pg >= (uint32_t)a.kv.n_pages);
-          if (j + 1 < tiles) pg = entry(j + 1);
+          if (j + step < tiles) pg = entry(j + step);
         }
         wait(s_full + g, sp);
         sp ^= 1u;
@@ -636,7 +668,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
             const float top = max_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]) * c;
             const float mn = max_nan(m, top);
             const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
-            if (j > 0) {  // O's row: P(j-1) V(j-1) was done before S(j)
+            if (j > j0) {  // O's row: the last P V was done before this S
               l *= f;
 #pragma unroll 1
               for (int q = 0; q < HD / 16; ++q) {
@@ -687,32 +719,67 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         if (*gave_up) break;
       }
       // ------------------------------------------------------- the rows out
-      const int64_t row = up->row0 + g * p.T + tok;
+      const int64_t row = up->row0 + off + tok;
       const int h = up->kh * p.G + head;
       release();
-      uint16_t* out = static_cast<uint16_t*>(a.out) + (row * a.n_heads + h) * HD;
+      // with one tile of rows, each group has half the columns to write
+      const int col0 = p.dual ? 0 : HD / 2 * g, cols = p.dual ? HD : HD / 2;
+      uint16_t* out = static_cast<uint16_t*>(a.out) + (row * a.n_heads + h) * HD + col0;
       if (!tiles) {
         if (live)
-#pragma unroll
-          for (int i = 0; i < HD / 8; ++i) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < cols / 8; ++i) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
         continue;
       }
-      wait(o_full + g, op);
-      op ^= 1u;
+      float mine = 1.0f, other = 0.0f;  // weights of this group's sums and of the other's
+      if (p.dual) {
+        wait(o_full + g, op);
+        op ^= 1u;
+      } else {
+        volatile float2* ml = reinterpret_cast<volatile float2*>(Qs + kHalves * kPanel);  // (tile B's place: there is none)
+        ml[g * kRows + r].x = m;
+        ml[g * kRows + r].y = l;
+        both();
+        const float mo = ml[(g ^ 1) * kRows + r].x, lo = ml[(g ^ 1) * kRows + r].y;
+        const float top = max_nan(m, mo);
+        mine = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+        other = mo == -INFINITY ? 0.0f : exp2_fast(mo - top);
+        l = l * mine + lo * other;
+        m = top;
+        wait(o_full, op);
+        op ^= 1u;
+        if (tiles > 1) {
+          wait(o_full + 1, op_b);
+          op_b ^= 1u;
+        }
+      }
       tc_fence_after();
       const float inv = l == 0.0f || m == -INFINITY || lim <= 0 ? 0.0f : 1.0f / l;
+      mine *= inv;
+      other *= inv;
       float bad = m * 0.0f;  // (m = -inf: no visible key with a score above it, the sum is zero)
       if (m == -INFINITY) bad = 0.0f;
+      const bool have = p.dual || g < tiles, two = !p.dual && (g ^ 1) < tiles;
+      const uint32_t to2 = tmem + lanes + 256u + 128u * (g ^ 1);
 #pragma unroll 1
-      for (int q = 0; q < HD / 32; ++q) {
+      for (int q = 0; q < cols / 32; ++q) {
         float t[32];
-        tmem_ld32(to + 32u * q, t);
+        if (have) {
+          tmem_ld32(to + col0 + 32u * q, t);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) bad = fmaf(t[i], 0.0f, bad), t[i] *= mine;  // NaN where one is not finite
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) t[i] = 0.0f;
+        }
+        if (two) {
+          float v[32];
+          tmem_ld32(to2 + col0 + 32u * q, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) bad = fmaf(v[i], 0.0f, bad), t[i] = fmaf(v[i], other, t[i]);
+        }
         uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          bad = fmaf(t[2 * i], 0.0f, fmaf(t[2 * i + 1], 0.0f, bad));  // NaN where one is not finite
-          w[i] = pack2<BF>(t[2 * i] * inv, t[2 * i + 1] * inv);
-        }
+        for (int i = 0; i < 16; ++i) w[i] = pack2<BF>(t[2 * i], t[2 * i + 1]);
         if (live)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -725,16 +792,17 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
             }
           }
       }
+      tc_fence_before();
+      if (!p.dual) both();  // both have read O: the next unit's may go over it
       // 0 * x is NaN for an infinite or NaN x in a place that a row does not
       // see: such rows are computed again from their visible keys alone
       uint32_t again = __ballot_sync(0xffffffffu, live && !(bad == 0.0f));
-      tc_fence_before();
       while (again) {
         const int src = __ffs(again) - 1;
         again &= again - 1;
         const int64_t rr = __shfl_sync(0xffffffffu, row, src);
         const int hh = __shfl_sync(0xffffffffu, h, src);
-        attn_row<HD, BF>(a, seq, rr, hh, lane);
+        attn_row<HD, BF>(a, seq, rr, hh, p.dual ? -1 : g, lane);
       }
     }
   }

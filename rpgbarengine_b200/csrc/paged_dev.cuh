@@ -70,10 +70,10 @@ RPGC_DEV int seq_of_row(const PagedSeqs& b, int64_t r, int lane) {
 
 // Attention of packed row r (of sequence s) and query head h by one warp, from
 // the visible keys alone: 32 keys a step, lane l scoring key l, then every
-// lane adding the keys' values for its own dims; fp32 throughout.  qs: HD
-// floats of shared memory of this warp.
+// lane adding the keys' values for its own dims; fp32 throughout.  Half hf of
+// the row is written (-1: all of it).
 template <int HD, bool BF>
-__device__ __noinline__ void attn_row(const PagedAttnArgs& a, int s, int64_t r, int h, int lane) {
+__device__ __noinline__ void attn_row(const PagedAttnArgs& a, int s, int64_t r, int h, int hf, int lane) {
   constexpr int E = HD / 32;
   const int kh = h / (a.n_heads / a.kv.n_kv);
   const int64_t r0 = seq_row(a.b, s), r1 = seq_row(a.b, s + 1);
@@ -140,6 +140,7 @@ __device__ __noinline__ void attn_row(const PagedAttnArgs& a, int s, int64_t r, 
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (hf >= 0 && lane >> 4 != hf) return;
   uint16_t* op = static_cast<uint16_t*>(a.out) + (r * a.n_heads + h) * HD + E * lane;
 #pragma unroll
   for (int i = 0; i < E; i += 2) *reinterpret_cast<uint32_t*>(op + i) = pack2<BF>(o[i] * inv, o[i + 1] * inv);

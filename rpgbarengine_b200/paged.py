@@ -74,6 +74,12 @@ def _rows(t, what, index, n, heads, d):
     return _S2(st[0] if n > 1 else shape[1] * d, st[1] if shape[1] > 1 else d)
 
 
+def _new(like, dtype=None):
+    """A contiguous tensor of `like`'s shape (the cheapest call that makes one)."""
+    torch = _torch()
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _result(out, like, shape, dtype):
     if out.shape != shape or out.dtype != dtype or out.get_device() != like.get_device() or not out.is_contiguous():
         _refuse(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device}")
@@ -192,7 +198,7 @@ def paged_append(cache: PagedKV, batch: PagedBatch, q, k, v, q_norm=None, k_norm
     if q is not None:
         qs, heads, qp = _rows(q, "q", index, n, 0, d), q.shape[1], q.data_ptr()
         if q_out is None:
-            q_out = made = torch.empty(q.shape, dtype=cache.dtype, device=q.device)
+            q_out = made = _new(q, cache.dtype)
         else:
             _result(q_out, q, q.shape, cache.dtype)
         op = q_out.data_ptr()
@@ -210,7 +216,7 @@ def _attend(cache, batch, q, out):
         _refuse("q, cache and batch must share their device, and q the cache's type")
     qs = _rows(q, "q", cache.index, batch.n_tokens, 0, cache.head_dim)
     if out is None:
-        out = q.new_empty(q.shape)
+        out = _new(q)
         return qs, out, out
     return qs, _result(out, q, q.shape, q.dtype), None
 
@@ -252,7 +258,7 @@ def attention_prompt(q, k, v, cu_seqlens, scale=None, out=None, status=None, str
         _need(status.get_device() == index, "status must be on q's device")
     made = None
     if out is None:
-        out = made = q.new_empty(q.shape)
+        out = made = _new(q)
     else:
         _result(out, q, q.shape, q.dtype)
     _run(lib().rpgc_attention_prompt, index, stream, made, _type(q), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
