@@ -2,9 +2,10 @@
 // of the KV cache.
 //
 // Mathematics: out = sum_t p_t v_t / sum_t p_t with p_t = 2^(c s_t - m),
-// s_t = q . k_t, c = scale * log2(e): one pass over the keys with a reference m
-// that follows the running maximum once it has grown by kGrow, so that most
-// steps rescale nothing.  Reference: AttentionFromCache (src/qwen3.cc:79-117).
+// s_t = q . k_t, c = scale * log2(e): one pass over the keys with a reference m,
+// the maximum of a warp's first keys until a later probability outgrows what 16
+// bits hold (2^40 in bf16, 2^15 in fp16), so that most steps look for no
+// maximum and rescale nothing.  Reference: AttentionFromCache (src/qwen3.cc:79-117).
 //
 // Bound: every K and V byte is read once, so HBM is the limit.  The key tiles
 // of all (sequence, kv head) items form one list, cut into equal
@@ -29,7 +30,8 @@ namespace {
 
 using namespace paged;
 
-constexpr float kGrow = 8.0f;
+constexpr int kJoin = 8;   // pieces of a share whose sums are in flight at once
+constexpr int kAhead = 4;  // V operands loaded ahead of the probabilities
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD, int NT>
@@ -45,8 +47,8 @@ struct DShape {
   static constexpr int kHeads = 8 * NT;           // query heads of a kv head, padded
   static constexpr int kPad = HD + 4;             // row of the merge buffer: no bank conflicts
   static constexpr int kMaxCtas = 256;
-  // the warps' sums, later the join's table: per piece a slot and 8 bytes a head
-  static constexpr int kSums = kWarps * kHeads * kPad * 4, kTable = kMaxCtas * (2 * kHeads + 1) * 4;
+  // the warps' sums, later the join's table: 8 bytes per piece and head
+  static constexpr int kSums = kWarps * kHeads * kPad * 4, kTable = kMaxCtas * kHeads * 8;
   static constexpr int kMerge = kSums > kTable ? kSums : kTable;
   static constexpr int kSmem = 1024 + kStages * kStage + kMerge + 2 * kWarps * kHeads * 4 + 512;
 };
@@ -190,6 +192,7 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
   using S = DShape<HD, NT>;
   constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps, kTile = S::kTile, kGroup = S::kGroup;
   constexpr float kLift = BF ? 0.0f : 6.0f;  // fp16 probabilities carry 2^6: small ones keep their bits
+  constexpr float kMost = BF ? 1.0e12f : 32768.0f;  // a probability that needs no new reference
   extern __shared__ uint8_t dsm_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
   float* wo = reinterpret_cast<float*>(ring + kStages * S::kStage);  // [warp][head][kPad]
@@ -325,57 +328,79 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
       const int left = w.len - t * kTile - 16 * part;  // keys of this warp's part
       if (left > 0 && (there[st] >> part & 1u)) {
         const uint32_t kb = smem_u32(ring + st * S::kStage), vb = kb + S::kHalf;
-        float s[NT][4];
+        // two chains of MMAs, so that one's latency hides the other's
+        float s[NT][4], s2[NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.0f;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           uint32_t f[4];
           ldsm4(kb + (k >> 2) * S::kPanel + krow * 128 + (((2 * (k & 3) + kc) ^ (krow & 7)) << 4), f);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma<BF>(s[n], f, q[n][k][0], q[n][k][1]);
+          for (int n = 0; n < NT; ++n) mma<BF>(k & 1 ? s2[n] : s[n], f, q[n][k][0], q[n][k][1]);
         }
+        // the first values are on their way while the probabilities are made
+        uint32_t v[kAhead][4];
+        auto load_v = [&](int d, uint32_t* f) {
+          ldsm4_t(vb + (d >> 2) * S::kPanel + vrow * 128 + (((2 * (d & 3) + vc) ^ (vrow & 7)) << 4), f);
+        };
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) load_v(d, v[d]);
         // s: (key gr, head 2 tq), (gr, 2 tq + 1), (gr + 8, 2 tq), (gr + 8, 2 tq + 1)
         const bool in0 = gr < left, in1 = gr + 8 < left;
-        bool grown = false;
+        bool fresh = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[n][e] = (e < 2 ? in0 : in1) ? s[n][e] * c : -INFINITY;
-            grown |= s[n][e] > m[n][e & 1] + kGrow || (m[n][e & 1] == -INFINITY && s[n][e] > -INFINITY);
+          for (int e = 0; e < 4; ++e) s[n][e] = (e < 2 ? in0 : in1) ? (s[n][e] + s2[n][e]) * c : -INFINITY;
+          fresh |= m[n][0] == -INFINITY || m[n][1] == -INFINITY;
+        }
+        // probabilities by the reference there is; where there is none yet, or one
+        // has outgrown it (or is NaN), the maximum becomes it and they are made again
+        float x[NT][4];
+        bool look = __any_sync(0xffffffffu, fresh);
+#pragma unroll 1
+        for (;;) {
+          if (look) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float t = fmaxf(s[n][e], s[n][e + 2]);
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                t = fmaxf(t, m[n][e]);
+                const float f = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - t);
+                m[n][e] = t;
+                l[n][e] *= f;
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) {
+                  o[n][d][e] *= f;
+                  o[n][d][e + 2] *= f;
+                }
+              }
           }
-        if (__any_sync(0xffffffffu, grown)) {
+          bool grown = false;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = fmaxf(s[n][e], s[n][e + 2]);
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-              x = fmaxf(x, m[n][e]);
-              const float f = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - x);
-              m[n][e] = x;
-              l[n][e] *= f;
-#pragma unroll
-              for (int d = 0; d < HD / 16; ++d) {
-                o[n][d][e] *= f;
-                o[n][d][e + 2] *= f;
-              }
+            for (int e = 0; e < 4; ++e) {
+              x[n][e] = exp2_fast(s[n][e] - ((m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]) - kLift));
+              grown |= !(x[n][e] <= kMost);
             }
+          if (look || !__any_sync(0xffffffffu, grown)) break;
+          look = true;
         }
         uint32_t b[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[e] = exp2_fast(s[n][e] - ((m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]) - kLift));
-          l[n][0] += x[0] + x[2];
-          l[n][1] += x[1] + x[3];
-          b[n][0] = transpose8(pack2<BF>(x[0], x[1]));
-          b[n][1] = transpose8(pack2<BF>(x[2], x[3]));
+          l[n][0] += x[n][0] + x[n][2];
+          l[n][1] += x[n][1] + x[n][3];
+          b[n][0] = transpose8(pack2<BF>(x[n][0], x[n][1]));
+          b[n][1] = transpose8(pack2<BF>(x[n][2], x[n][3]));
         }
         // keys 2 tq, 2 tq + 1 (and + 8) of the V operand; what lies past the
         // last position is cleared, for 0 * NaN is NaN
@@ -386,8 +411,8 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
         }
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) {
-          uint32_t f[4];
-          ldsm4_t(vb + (d >> 2) * S::kPanel + vrow * 128 + (((2 * (d & 3) + vc) ^ (vrow & 7)) << 4), f);
+          uint32_t f[4] = {v[d % kAhead][0], v[d % kAhead][1], v[d % kAhead][2], v[d % kAhead][3]};
+          if (d + kAhead < HD / 16) load_v(d + kAhead, v[d % kAhead]);
           f[0] &= keep0;
           f[1] &= keep0;
           f[2] &= keep1;
@@ -463,30 +488,34 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
       }
       bar_consumers<kWarps * 32>();
       if (*last) {
-        // every piece's (reference, weight) of every head at once, one read each;
-        // then the sums, eight pieces' rows in flight
+        // every piece's (reference, weight) of every head at once, the first rows of
+        // partial sums in flight beside them.  Piece k is in its CTA's first slot,
+        // but the first piece's CTA may have had an item before.
         const int pieces = b1 - b0 + 1;
-        float2* ml = reinterpret_cast<float2*>(wo);                      // [piece][head]
-        int32_t* slots = reinterpret_cast<int32_t*>(ml + pieces * G);    // [piece]
-        for (int k = tid; k < pieces; k += kWarps * 32) slots[k] = 2 * (b0 + k) + (w.begin(b0 + k, active) < w.i0 ? 1 : 0);
-        bar_consumers<kWarps * 32>();
+        const int front = w.begin(b0, active) < w.i0 ? 1 : 0;
+        auto slot_of = [&](int k) { return (int64_t)(2 * (b0 + k) + (k ? 0 : front)); };
+        float2* ml = reinterpret_cast<float2*>(wo);  // [piece][head]
+        float4 v[kJoin];
+        auto fetch = [&](int i, int k0) {
+          const float* part = p.part + (i / (HD / 4)) * HD + 4 * (i % (HD / 4));
+#pragma unroll
+          for (int k = 0; k < kJoin; ++k)
+            if (k0 + k < pieces) v[k] = __ldcg(reinterpret_cast<const float4*>(part + slot_of(k0 + k) * G * HD));
+        };
+        if (tid < G * HD / 4) fetch(tid, 0);
         for (int i = tid; i < pieces * G; i += kWarps * 32)
-          ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + (int64_t)slots[i / G] * G + i % G);
+          ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot_of(i / G) * G + i % G);
         bar_consumers<kWarps * 32>();
         for (int i = tid; i < G * HD / 4; i += kWarps * 32) {
           const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
-          const float* part = p.part + h * HD + d;
           float M = -INFINITY;
           for (int k = 0; k < pieces; ++k) M = fmaxf(M, ml[k * G + h].x);
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
           float L = 0.0f;
-          for (int k0 = 0; k0 < pieces; k0 += 8) {
-            float4 v[8];
+          for (int k0 = 0; k0 < pieces; k0 += kJoin) {
+            if (k0 || i != tid) fetch(i, k0);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (k0 + k < pieces) v[k] = __ldcg(reinterpret_cast<const float4*>(part + (int64_t)slots[k0 + k] * G * HD));
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < kJoin; ++k) {
               if (k0 + k >= pieces) break;
               const float2 x = ml[(k0 + k) * G + h];
               const float f = x.x == -INFINITY ? 0.0f : exp2_fast(x.x - M);
