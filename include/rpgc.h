@@ -374,7 +374,7 @@ RPGC_API int rpgc_sample(const float* logits, int64_t n, float temperature, int3
  * name them -1) and not written by append.
  *
  * The values of a sequence's slots past its length, and of pages no sequence
- * names, are never used, whatever they are. */
+ * names, are never used, whatever they are.  Outputs do not overlap inputs. */
 typedef struct rpgc_paged_kv {
   void* k; /* slot (page, position, head) at page*stride[0] + position*stride[1] + head*stride[2] */
   void* v;

@@ -129,44 +129,51 @@ struct Walk {
   }
   RPGC_DEV bool start(const PagedAttnArgs& a, int lane, int ctas, int cta, int* active) {
     const int64_t kv = a.kv.n_kv;
-    // the first 128 lengths stay in registers for the second look
-    int32_t n[4];
+    // each lane adds up a run of sequences; then the run that holds this CTA's
+    // first place is looked through 32 sequences at a time
+    const int run = (a.b.n_seqs + 31) / 32;
     int64_t sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) n[i] = 32 * i + lane < a.b.n_seqs ? seen(a, 32 * i + lane) : 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum += weight_of<T>(n[i]);
-    for (int s = 128 + lane; s < a.b.n_seqs; s += 32) sum += weight_of<T>(seen(a, s));
-    total = warp_sum(sum) * kv;
+#pragma unroll 4
+    for (int i = 0; i < run; ++i) {
+      const int s = lane * run + i;
+      if (s < a.b.n_seqs) sum += weight_of<T>(seen(a, s));
+    }
+    sum *= kv;
+    int64_t upto = scan(sum, lane);
+    total = __shfl_sync(0xffffffffu, upto, 31);
     const int parts = (int)(total < ctas ? total : ctas);
     *active = parts;
     if (cta >= parts) return false;
     lo = begin(cta, parts);
     hi = begin(cta + 1, parts);
-    int64_t before = 0;  // weight of the sequences before s0
+    const int src = __ffs(__ballot_sync(0xffffffffu, upto > lo)) - 1;
+    int64_t before = __shfl_sync(0xffffffffu, upto - sum, src);  // weight of the sequences before s0
 #pragma unroll 1
-    for (int s0 = 0;; s0 += 32) {
-      const int32_t ln = s0 >= 128 ? (s0 + lane < a.b.n_seqs ? seen(a, s0 + lane) : 0) : s0 == 0 ? n[0] : s0 == 32 ? n[1] : s0 == 64 ? n[2] : n[3];
+    for (int s0 = src * run;; s0 += 32) {
+      const int32_t ln = s0 + lane < a.b.n_seqs ? seen(a, s0 + lane) : 0;
       const int64_t mine = weight_of<T>(ln) * kv;
-      int64_t upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
+      upto = scan(mine, lane);
       const uint32_t in = __ballot_sync(0xffffffffu, before + upto > lo);
       if (in) {
-        const int src = __ffs(in) - 1;
-        const int64_t first = before + __shfl_sync(0xffffffffu, upto - mine, src);
-        seq = s0 + src;
-        len = __shfl_sync(0xffffffffu, ln, src);
-        const int64_t w = weight_of<T>(len), at = lo - first;
-        kh = at < (int64_t)0x7fffffff ? (int32_t)((uint32_t)at / (uint32_t)w) : (int32_t)(at / w);
+        const int at = __ffs(in) - 1;
+        const int64_t first = before + __shfl_sync(0xffffffffu, upto - mine, at);
+        seq = s0 + at;
+        len = __shfl_sync(0xffffffffu, ln, at);
+        const int64_t w = weight_of<T>(len), in_seq = lo - first;
+        kh = in_seq < (int64_t)0x7fffffff ? (int32_t)((uint32_t)in_seq / (uint32_t)w) : (int32_t)(in_seq / w);
         item(first + kh * w);
         return true;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
+  }
+  RPGC_DEV int64_t scan(int64_t v, int lane) const {  // inclusive sums over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += x;
+    }
+    return v;
   }
   RPGC_DEV bool next(const PagedAttnArgs& a) {
     if (i1 >= hi) return false;

@@ -318,7 +318,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
     cmax = __reduce_max_sync(0xffffffffu, cmax);
     const int32_t total = tiles_at_least(a.b, mine, U, 0, lane);
     const int64_t units_n = (int64_t)total * a.kv.n_kv;
-    int32_t hi = cmax;
+    // the current cost c: tiles that cost at least c, and more; the sequences from
+    // s0 on are still to be looked through, `before` tiles of cost c lie before them
+    int32_t c = cmax + 1, at_least = 0, more = 0, s0 = 0, before = 0;
     for (int it = 0;; ++it) {
       // there and back over the CTAs, so that nobody gets the longest of every round
       const int64_t u = (int64_t)it * gridDim.x + ((it & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
@@ -326,27 +328,33 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       Unit un;
       un.seq = -1;
       if (u < units_n) {
-        const int32_t k = (int32_t)(u / a.kv.n_kv);
-        int32_t lo = 0;  // largest c with more than k tiles of at least that cost
-        while (lo < hi) {
-          const int32_t mid = (lo + hi + 1) >> 1;
-          if (tiles_at_least(a.b, mine, U, mid, lane) > k) lo = mid;
-          else hi = mid - 1;
+        const int32_t k = (int32_t)(u / a.kv.n_kv);  // (never less than the last)
+        if (k >= at_least) {  // the largest lower cost that more than k tiles reach
+          int32_t lo = 0, hi = c - 1;
+          while (lo < hi) {
+            const int32_t mid = (lo + hi + 1) >> 1;
+            if (tiles_at_least(a.b, mine, U, mid, lane) > k) lo = mid;
+            else hi = mid - 1;
+          }
+          c = lo;
+          more = tiles_at_least(a.b, mine, U, c + 1, lane);
+          at_least = tiles_at_least(a.b, mine, U, c, lane);
+          s0 = before = 0;
         }
-        int32_t r = k - tiles_at_least(a.b, mine, U, lo + 1, lane);
-        for (int s0 = 0; s0 < a.b.n_seqs; s0 += 32) {
+        const int32_t r = k - more;  // among the tiles of cost c
+        for (; s0 < a.b.n_seqs; s0 += 32) {
           const SeqLens q = s0 ? seq_lens(a.b, s0 + lane) : mine;
-          const int32_t f = first_tile(q, U, lo), n = first_tile(q, U, lo + 1) - f;
+          const int32_t f = first_tile(q, U, c), n = first_tile(q, U, c + 1) - f;
           int32_t sum = n;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += x;
           }
-          const uint32_t in = __ballot_sync(0xffffffffu, r < sum);
+          const uint32_t in = __ballot_sync(0xffffffffu, r - before < sum);
           if (in) {
             const int src = __ffs(in) - 1;
-            const int32_t i = __shfl_sync(0xffffffffu, f + r - (sum - n), src);
+            const int32_t i = __shfl_sync(0xffffffffu, f + r - before - (sum - n), src);
             const int32_t n_new = __shfl_sync(0xffffffffu, q.n, src), pre = __shfl_sync(0xffffffffu, q.pre, src);
             const int32_t t0 = i * U;
             un.seq = s0 + src;
@@ -355,19 +363,18 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
             un.row0 = un.key0 + t0;
             un.pos0 = pre + t0;
             const int64_t reach = paged ? table_reach(a.kv, a.b) : (int64_t)n_new;
-            un.reach = (int32_t)min(reach, (int64_t)0x7fffffff);
+            un.reach = (int32_t)min(reach, (int64_t)0x7fffff00);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const int32_t first = p.dual ? g * p.T : 0;
               un.rows[g] = max(0, min(p.T, n_new - t0 - first));
-              un.end[g] = un.rows[g] ? (int32_t)max((int64_t)0, min((int64_t)un.pos0 + first + un.rows[g], reach)) : 0;
+              un.end[g] = un.rows[g] ? (int32_t)max((int64_t)0, min((int64_t)un.pos0 + first + un.rows[g], (int64_t)un.reach)) : 0;
               un.tiles[g] = (un.end[g] + kKeys - 1) / kKeys;
             }
             break;
           }
-          r -= __shfl_sync(0xffffffffu, sum, 31);
+          before += __shfl_sync(0xffffffffu, sum, 31);
         }
-        hi = lo;
       }
       if (lane == 0) {
         units[it % kUnits] = un;

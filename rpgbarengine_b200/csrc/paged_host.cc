@@ -64,6 +64,10 @@ void need_ptr(const void* p, const char* what) {
   if (reinterpret_cast<uintptr_t>(p) & 15) fail(RPGC_E_ARG, "%s must be 16-byte aligned", what);
 }
 
+void need_words(const void* p, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) & 3) fail(RPGC_E_ARG, "%s must be 4-byte aligned", what);
+}
+
 // A stride in elements of `size` bytes: not negative, a multiple of 16
 // bytes, and small enough that no product with a count overflows.
 void need_stride(int64_t st, int size, const char* what) {
@@ -123,6 +127,10 @@ PagedSeqs seqs_of(const rpgc_paged_batch* b) {
   if (b->n_seqs > 0 && (!b->block_table || !b->kv_lens)) fail(RPGC_E_ARG, "block_table or kv_lens is NULL");
   if (!b->cu_q && b->n_tokens != b->n_seqs)
     fail(RPGC_E_ARG, "without cu_q there is one token per sequence: n_tokens %lld, n_seqs %d", (long long)b->n_tokens, b->n_seqs);
+  need_words(b->block_table, "block_table");
+  need_words(b->kv_lens, "kv_lens");
+  need_words(b->cu_q, "cu_q");
+  need_words(b->status, "status");
   PagedSeqs s{};
   s.table = b->block_table;
   s.table_stride = b->table_stride;
@@ -259,6 +267,8 @@ int rpgc_attention_prompt(uint32_t type, const void* q, const int64_t* q_stride,
     need_counts(n_seqs, n_tokens);
     if (n_seqs == 0 || n_tokens == 0) return RPGC_OK;
     if (!cu) fail(RPGC_E_ARG, "cu is NULL");
+    need_words(cu, "cu");
+    need_words(status, "status");
     need_attn(q, q_stride, scale, out);
     need_ptr(k, "k");
     need_ptr(v, "v");

@@ -136,7 +136,8 @@ class PagedBatch:
     [cu_q[s], cu_q[s+1]) of n_tokens (None: one new token per sequence).  All on
     the device, and read there at each call, so a decode loop updates them in
     place and keeps the batch.  status: optional int32 tensor of one word that
-    receives DROPPED / TIMEOUT bits.  The batch also holds decode's workspace:
+    receives DROPPED / TIMEOUT bits.  The batch also holds decode's workspace
+    (made at its first decode call, which is therefore not a captured one):
     calls on one batch are made in stream order."""
 
     def __init__(self, block_table, kv_lens, cu_q=None, n_tokens=None, status=None):

@@ -298,6 +298,36 @@ def test_decode_lengths_change_between_calls_and_in_a_graph():
         assert torch.equal(a, out)
 
 
+def test_many_sequences():
+    # more sequences than a warp's lanes many times over, most of them empty or
+    # of one position, in decode and as prompts of one and of a few tokens
+    page, kv, H, hd = 16, 2, 4, 64
+    lens = [0 if i % 3 == 0 else 1 if i % 7 else (i * 37) % 90 for i in range(3001)]
+    k, v, table, q = decode_case(lens, H, kv, hd, page, "f16", False, 4)
+    cache = rb.PagedKV(k, v)
+    tab, ln = i32(table), i32(lens)
+    kk, vv = (x.double()[tab.clamp(min=0).long()].flatten(1, 2) for x in (k, v))  # [sequence, place, head, dim]
+
+    def want(qs, seq, last):
+        s = torch.einsum("nhgd,nthd->nhgt", qs.double().view(len(seq), kv, H // kv, hd), kk[seq]) * hd ** -0.5
+        far = torch.arange(kk.shape[1], device="cuda") > last[:, None]
+        p = torch.where(far[:, None, None], 0.0, torch.exp(s))
+        p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+        f = lambda x: torch.einsum("nhgt,nthd->nhgd", p, x[seq]).reshape(len(seq), H, hd)  # noqa: E731
+        return f(vv), f(vv.abs())
+
+    seq = torch.arange(len(lens), device="cuda")
+    close(rb.paged_attention_decode(cache, rb.PagedBatch(tab, ln), q), *want(q, seq, ln.long() - 1))
+    close(rb.paged_attention_prompt(cache, rb.PagedBatch(tab, ln), q), *want(q, seq, ln.long() - 1))
+    new = [min(n, 5) for n in lens]
+    cu = i32(np.concatenate([[0], np.cumsum(new)]).tolist())
+    n = sum(new)
+    qp = randn(gen(1), n, H, hd, dtype=torch.float16)
+    seq = torch.repeat_interleave(seq, torch.tensor(new, device="cuda"))
+    last = ln.long()[seq] - cu.long()[seq + 1] + torch.arange(n, device="cuda")
+    close(rb.paged_attention_prompt(cache, rb.PagedBatch(tab, ln, cu, n), qp), *want(qp, seq, last))
+
+
 def test_decode_offsets_past_32_bits():
     # a pool of more than 2^31 values whose last pages hold the sequence
     page, kv, H, hd = 256, 8, 16, 128

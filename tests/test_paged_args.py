@@ -53,6 +53,7 @@ def test_cache_is_checked(kw, word):
 @pytest.mark.parametrize("kw,word", [
     (dict(block_table=None), "block_table"), (dict(kv_lens=None), "kv_lens"), (dict(max_pages=0), "max_pages"),
     (dict(table_stride=3), "table_stride"), (dict(n_seqs=-1), "n_seqs"), (dict(n_tokens=3), "one token per sequence"),
+    (dict(block_table=P + 2), "block_table"), (dict(kv_lens=P + 1), "kv_lens"), (dict(status=P + 2), "status"),
     (dict(n_tokens=-1), "n_tokens"), (dict(n_tokens=1 << 25), "n_tokens"), (dict(cu_q=P), "cu_q"),
 ])
 def test_batch_is_checked(kw, word):
