@@ -133,10 +133,12 @@ struct Walk {
     // first place is looked through 32 sequences at a time
     const int run = (a.b.n_seqs + 31) / 32;
     int64_t sum = 0;
+    int32_t ln = 0;
 #pragma unroll 4
     for (int i = 0; i < run; ++i) {
       const int s = lane * run + i;
-      if (s < a.b.n_seqs) sum += weight_of<T>(seen(a, s));
+      ln = s < a.b.n_seqs ? seen(a, s) : 0;
+      sum += weight_of<T>(ln);
     }
     sum *= kv;
     int64_t upto = scan(sum, lane);
@@ -150,7 +152,8 @@ struct Walk {
     int64_t before = __shfl_sync(0xffffffffu, upto - sum, src);  // weight of the sequences before s0
 #pragma unroll 1
     for (int s0 = src * run;; s0 += 32) {
-      const int32_t ln = s0 + lane < a.b.n_seqs ? seen(a, s0 + lane) : 0;
+      if (run > 1) ln = s0 + lane < a.b.n_seqs ? seen(a, s0 + lane) : 0;
+      else ln = __shfl_sync(0xffffffffu, ln, (src + lane) & 31);  // (only lane 0's counts: the run is one sequence)
       const int64_t mine = weight_of<T>(ln) * kv;
       upto = scan(mine, lane);
       const uint32_t in = __ballot_sync(0xffffffffu, before + upto > lo);
@@ -401,13 +404,22 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
           if (look || !__any_sync(0xffffffffu, grown)) break;
           look = true;
         }
-        uint32_t b[NT][2];
+        // each probability as two 16-bit values, itself rounded and what that left:
+        // the products with V keep 16 bits of it or more.  The memory sets the
+        // pace here, so the second product costs nothing; rounded to one value
+        // it would be as large an error as the output's own rounding.
+        uint32_t b[NT][2], b_lo[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           l[n][0] += x[n][0] + x[n][2];
           l[n][1] += x[n][1] + x[n][3];
-          b[n][0] = transpose8(pack2<BF>(x[n][0], x[n][1]));
-          b[n][1] = transpose8(pack2<BF>(x[n][2], x[n][3]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t hi = pack2<BF>(x[n][2 * e], x[n][2 * e + 1]);
+            const float2 h = unpack2<BF>(hi);
+            b[n][e] = transpose8(hi);
+            b_lo[n][e] = transpose8(pack2<BF>(x[n][2 * e] - h.x, x[n][2 * e + 1] - h.y));
+          }
         }
         // keys 2 tq, 2 tq + 1 (and + 8) of the V operand; what lies past the
         // last position is cleared, for 0 * NaN is NaN
@@ -425,7 +437,10 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
           f[2] &= keep1;
           f[3] &= keep1;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma<BF>(o[n][d], f, b[n][0], b[n][1]);
+          for (int n = 0; n < NT; ++n) {
+            mma<BF>(o[n][d], f, b[n][0], b[n][1]);
+            mma<BF>(o[n][d], f, b_lo[n][0], b_lo[n][1]);
+          }
         }
       }
       __syncwarp();
