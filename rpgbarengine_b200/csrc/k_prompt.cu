@@ -713,7 +713,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
           }
           const float2 u = unpair(add2(sum[0], sum[1]));
           tile_sum = u.x + u.y;
-          if (look || !__any_sync(0xffffffffu, !(tile_sum <= kMost))) break;
+          // (rows that see nothing have no say: their queries may be anything)
+          if (look || !__any_sync(0xffffffffu, lim > 0 && !(tile_sum <= kMost))) break;
           look = true;
         }
         l += tile_sum;

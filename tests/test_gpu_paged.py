@@ -417,6 +417,22 @@ def test_packed_prompt_growing_scores():
         check_packed(got, q, k, v, [n], float(np.float32(0.02)))
 
 
+@pytest.mark.parametrize("H,kv", [(6, 2), (5, 1), (12, 12), (14, 2), (16, 2)])
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+def test_packed_prompt_repeats_bit_for_bit(H, kv, ty):
+    # rows of a tile that belong to no token hold what an earlier call left
+    # there: whatever that was, the tokens' rows come out the same
+    g = gen(H)
+    lens = [900, 77, 300]
+    q, k, v = packed_inputs(g, sum(lens), H, kv, 128, DT[ty], False)
+    cu = i32([0, 900, 977, 1277])
+    want = rb.attention_prompt(q, k, v, cu)
+    for scale in (1e3, 1e-3, float("inf")):
+        junk = (randn(g, 2000, 8, 128) * scale).to(DT[ty])
+        rb.attention_prompt(junk, junk, junk, i32([0, 2000]))
+        assert torch.equal(rb.attention_prompt(q, k, v, cu), want)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_packed_prompt_later_positions_do_not_leak(bad):
     # what a row may not see cannot change it, whatever it holds: the key and
