@@ -761,11 +761,11 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         }
       }
       tc_fence_after();
-      const float inv = l == 0.0f || m == -INFINITY || lim <= 0 ? 0.0f : 1.0f / l;
+      // a visible score that is NaN or +inf (then m is too) makes the row NaN
+      const float inv = l == 0.0f || m == -INFINITY || lim <= 0 ? 0.0f : m < INFINITY ? 1.0f / l : __int_as_float(0x7fffffff);
       mine *= inv;
       other *= inv;
-      float bad = m * 0.0f;  // (m = -inf: no visible key with a score above it, the sum is zero)
-      if (m == -INFINITY) bad = 0.0f;
+      float bad = 0.0f;
       const bool have = p.dual || g < tiles, two = !p.dual && (g ^ 1) < tiles;
       const uint32_t to2 = tmem + lanes + 256u + 128u * (g ^ 1);
 #pragma unroll 1
@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       if (!p.dual) both();  // both have read O: the next unit's may go over it
       // 0 * x is NaN for an infinite or NaN x in a place that a row does not
       // see: such rows are computed again from their visible keys alone
-      uint32_t again = __ballot_sync(0xffffffffu, live && !(bad == 0.0f));
+      uint32_t again = __ballot_sync(0xffffffffu, live && m < INFINITY && !(bad == 0.0f));
       while (again) {
         const int src = __ffs(again) - 1;
         again &= again - 1;

@@ -40,9 +40,9 @@ RPGC_DEV float exp2_fast(float x) {
   return y;
 }
 
-// Bounded wait of one role (about two seconds); after the first that gives up,
+// Bounded wait of one role (about ten seconds); after the first that gives up,
 // the CTA's other waits end at once and the call's status says so.
-constexpr long long kWaitClocks = 4000000000ll;
+constexpr long long kWaitClocks = 20000000000ll;
 RPGC_DEV bool wait_for(uint64_t* bar, uint32_t parity, volatile int32_t* gave_up, int32_t* status) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();

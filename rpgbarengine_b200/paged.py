@@ -34,6 +34,7 @@ class _Batch(C.Structure):
 
 
 _S2 = C.c_int64 * 2
+_strides = {}  # (token, head) strides -> their C array
 _mods = []
 
 
@@ -71,12 +72,20 @@ def _rows(t, what, index, n, heads, d):
         _refuse(f"{what} must be [{n}, {heads or 'heads'}, {d}] on CUDA device {index}, each row of {d} contiguous; "
                 f"got {tuple(shape)} with strides {tuple(st)} on {t.device}")
     # (a dimension of one has no stride to speak of)
-    return _S2(st[0] if n > 1 else shape[1] * d, st[1] if shape[1] > 1 else d)
+    key = st[0] if n > 1 else shape[1] * d, st[1] if shape[1] > 1 else d
+    c = _strides.get(key)
+    if c is None:
+        if len(_strides) > 1000:
+            _strides.clear()
+        c = _strides[key] = _S2(*key)
+    return c
 
 
 def _new(like, dtype=None):
     """A contiguous tensor of `like`'s shape (the cheapest call that makes one)."""
     torch = _torch()
+    if dtype is None and like.is_contiguous():
+        return torch.empty_like(like)
     return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
 
 
@@ -86,20 +95,26 @@ def _result(out, like, shape, dtype):
     return out
 
 
+def _on(index, stream):
+    """The stream of a call on device `index`, or None where another device is current."""
+    c = _torch()._C
+    if c._cuda_getDevice() != index:
+        return None
+    return c._cuda_getCurrentRawStream(index) if stream is None else int(stream)
+
+
 def _run(fn, index, stream, made, *args):
     """fn(*args, stream) with device `index` current.  `made`: a result allocated
     here, whose memory must outlive its use on a stream that is not the current one."""
-    cuda = _torch().cuda
-    ptr = _torch()._C._cuda_getCurrentRawStream(index) if stream is None else int(stream)
-    if index == cuda.current_device():
-        rc = fn(*args, ptr)
-    else:
-        with cuda.device(index):
-            rc = fn(*args, ptr)
+    ptr = _on(index, stream)
+    if ptr is None:
+        with _torch().cuda.device(index):
+            return _run(fn, index, stream, made, *args)
+    rc = fn(*args, ptr)
     if rc < 0:
         _check(rc)
     if made is not None and stream is not None:
-        made.record_stream(cuda.ExternalStream(ptr, device=made.device))
+        made.record_stream(_torch().cuda.ExternalStream(ptr, device=made.device))
 
 
 class PagedKV:

@@ -448,6 +448,13 @@ def test_packed_prompt_later_positions_do_not_leak(bad):
     got = rb.attention_prompt(q, k2, v2, cu)
     check_packed(got[:300], q[:300], k[:300], v[:300], [300], hd ** -0.5)
     assert torch.isfinite(want).all()
+    assert torch.isnan(got[300:430]).all()  # these see it (infinite keys give scores of both signs at once)
+    q2 = q.clone()
+    q2[77], q2[78, 3] = bad, bad
+    got = rb.attention_prompt(q2, k, v, cu)
+    ok = torch.ones(500, H, dtype=torch.bool, device="cuda")
+    ok[77], ok[78, 3] = False, False
+    assert torch.isnan(got[~ok]).all() and torch.equal(got[ok], want[ok])
 
 
 def test_prompt_rows_outside_every_sequence_are_left_alone():
