@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       const float inv = l == 0.0f || m == -INFINITY || lim <= 0 ? 0.0f : m < INFINITY ? 1.0f / l : __int_as_float(0x7fffffff);
       mine *= inv;
       other *= inv;
-      float bad = 0.0f;
+      float bad[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN where a value is not finite
       const bool have = p.dual || g < tiles, two = !p.dual && (g ^ 1) < tiles;
       const uint32_t to2 = tmem + lanes + 256u + 128u * (g ^ 1);
 #pragma unroll 1
@@ -774,7 +774,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         if (have) {
           tmem_ld32(to + col0 + 32u * q, t);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) bad = fmaf(t[i], 0.0f, bad), t[i] *= mine;  // NaN where one is not finite
+          for (int i = 0; i < 32; ++i) bad[i & 3] = fmaf(t[i], 0.0f, bad[i & 3]), t[i] *= mine;
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) t[i] = 0.0f;
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
           float v[32];
           tmem_ld32(to2 + col0 + 32u * q, v);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) bad = fmaf(v[i], 0.0f, bad), t[i] = fmaf(v[i], other, t[i]);
+          for (int i = 0; i < 32; ++i) bad[i & 3] = fmaf(v[i], 0.0f, bad[i & 3]), t[i] = fmaf(v[i], other, t[i]);
         }
         uint32_t w[16];
 #pragma unroll
@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       if (!p.dual) both();  // both have read O: the next unit's may go over it
       // 0 * x is NaN for an infinite or NaN x in a place that a row does not
       // see: such rows are computed again from their visible keys alone
-      uint32_t again = __ballot_sync(0xffffffffu, live && m < INFINITY && !(bad == 0.0f));
+      uint32_t again = __ballot_sync(0xffffffffu, live && m < INFINITY && !(bad[0] + bad[1] + bad[2] + bad[3] == 0.0f));
       while (again) {
         const int src = __ffs(again) - 1;
         again &= again - 1;
