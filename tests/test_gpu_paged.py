@@ -537,6 +537,63 @@ def test_one_token_each_through_the_prompt_call_agrees_with_decode():
     check_decode(rb.paged_attention_prompt(cache, batch, q), q, k, v, table, lens, 128 ** -0.5)
 
 
+# ---------------------------------------------------------- other layouts
+@pytest.mark.parametrize("hd", [64, 128])
+def test_pools_in_one_tensor_strided_rows_and_outputs_off_a_sector(hd):
+    # K and V interleaved in one pool with room between heads, every second head
+    # of a wider q, results on a 16-byte boundary that is no 32-byte one
+    g = gen(hd)
+    page, kv, H, pages = 32, 3, 6, 40
+    pool = randn(g, pages, page, 2, kv + 1, 2 * hd, dtype=torch.bfloat16)
+    before = pool.clone()
+    k, v = pool[:, :, 0, :kv, :hd], pool[:, :, 1, 1:, hd:]
+    lens, new = [300, 33, 130], [130, 1, 64]
+    perm = torch.randperm(pages, generator=g, device="cuda").tolist()
+    table = [perm[:10], perm[10:12] + [-1] * 8, perm[12:17] + [-1] * 5]
+    n = sum(new)
+    cu = i32(np.concatenate([[0], np.cumsum(new)]).tolist())
+    wide = randn(g, n, 2 * H + 1, hd, dtype=torch.bfloat16)
+    q = wide[:, 1::2]
+    cache, batch = rb.PagedKV(k, v), rb.PagedBatch(i32(table), i32(lens), cu, n)
+
+    def odd(shape):
+        size = int(np.prod(shape))
+        buf = torch.full((size + 16,), 5.0, dtype=torch.bfloat16, device="cuda")
+        assert buf.data_ptr() % 32 == 0
+        return buf, buf[8:8 + size].view(shape)
+
+    buf, out = odd(q.shape)
+    got = rb.paged_attention_prompt(cache, batch, q, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    check_paged(out, q, k, v, table, new, lens, hd ** -0.5)
+    assert bool((buf[:8] == 5).all()) and bool((buf[-8:] == 5).all())
+    qd = q[:3]
+    buf, out = odd(qd.shape)
+    rb.paged_attention_decode(cache, rb.PagedBatch(i32(table), i32(lens)), qd, out=out)
+    check_decode(out, qd, k, v, table, lens, hd ** -0.5)
+    assert bool((buf[:8] == 5).all()) and bool((buf[-8:] == 5).all())
+    buf, out = odd(q.shape)
+    kk, vv = randn(g, n, 2 * kv, hd, dtype=torch.bfloat16)[:, ::2], randn(g, n, kv, 2 * hd, dtype=torch.bfloat16)[..., hd:]
+    rb.attention_prompt(q, kk, vv, cu, out=out)
+    check_packed(out, q, kk, vv, new, hd ** -0.5)
+    assert bool((buf[:8] == 5).all()) and bool((buf[-8:] == 5).all())
+    assert torch.equal(pool, before)
+    # append into the same pool touches the new tokens' slots alone
+    q_out = rb.paged_append(cache, batch, q, kk, vv)
+    assert torch.equal(q_out, q)
+    touched = torch.zeros_like(pool, dtype=torch.bool)
+    at = 0
+    for s, m in enumerate(new):
+        for i in range(m):
+            p = lens[s] - m + i
+            pg, sl = table[s][p // page], p % page
+            assert torch.equal(k[pg, sl], kk[at]) and torch.equal(v[pg, sl], vv[at])
+            touched[pg, sl, 0, :kv, :hd] = True
+            touched[pg, sl, 1, 1:, hd:] = True
+            at += 1
+    assert torch.equal(pool[~touched], before[~touched])
+
+
 # ------------------------------------------------------ streams, refusals
 def test_calls_on_another_stream():
     g = gen(6)
