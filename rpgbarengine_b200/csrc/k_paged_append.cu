@@ -26,17 +26,24 @@ using namespace paged;
 constexpr int kSteps = 2;
 enum { kInF32 = 0, kInF16 = 1, kInBF16 = 2 };
 
-// Four consecutive values.
+// Four consecutive values.  (__ldcg, not __ldg: the kernel before may still be
+// writing the inputs when this one is launched.)
 template <int IN>
 RPGC_DEV void load4(const void* base, int64_t off, float* x) {
   if (IN == kInF32) {
-    const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + off));
+    const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + off));
     x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
   } else {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + off));
+    const uint2 u = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + off));
     const float2 f = unpack2<IN == kInBF16>(u.x), g = unpack2<IN == kInBF16>(u.y);
     x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
   }
+}
+
+// The same of tables that stay as they are: gains and rope rows.
+RPGC_DEV void table4(const float* p, float* x) {
+  const float4 f = __ldg(reinterpret_cast<const float4*>(p));
+  x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
 }
 
 template <int HD, int IN, bool BF>
@@ -68,15 +75,15 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
   const int s = seq_of_row(a.b, r, lane);
   if (s < 0) return;
   const int64_t r0 = seq_row(a.b, s), r1 = seq_row(a.b, s + 1);
-  const int64_t pos = (int64_t)__ldg(a.b.kv_lens + s) - (r1 - r0) + (r - r0);
+  const int64_t pos = (int64_t)a.b.kv_lens[s] - (r1 - r0) + (r - r0);
   const int32_t page = pos >= 0 ? page_of(a.kv, a.b, s, pos) : -1;
   const bool drop = page < 0 || (a.rope && pos >= a.rope_rows);
   if (drop && h0 == 0 && lane == 0 && a.b.status) atomicOr(a.b.status, kStatusDropped);
   const bool turn = a.rope && !drop, norm = a.k_norm != nullptr;
   float c[4], sn[4];
   if (turn) {
-    load4<kInF32>(a.rope, pos * HD + d, c);
-    load4<kInF32>(a.rope, pos * HD + kHalf + d, sn);
+    table4(a.rope + pos * HD + d, c);
+    table4(a.rope + pos * HD + kHalf + d, sn);
   }
   const int64_t slot = pos & ((1 << a.kv.page_shift) - 1);
   uint16_t* qd = static_cast<uint16_t*>(a.q_out) + r * a.n_heads * HD + d;
@@ -99,8 +106,8 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
         for (int o = 1; o < kLanes; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float f = rsqrtf(ss * (1.0f / HD) + a.eps);  // (2 ulp: far below the 16-bit rounding)
         const float* gain = isq ? a.q_norm : a.k_norm;
-        load4<kInF32>(gain, d, g);
-        load4<kInF32>(gain, kHalf + d, g + 4);
+        table4(gain + d, g);
+        table4(gain + kHalf + d, g + 4);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = y[i] * f * g[i];
       }

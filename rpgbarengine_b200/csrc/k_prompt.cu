@@ -22,6 +22,14 @@
 // While the softmax of one tile runs, the tensor core works on the other.
 //
 // TMEM columns: S/P of A 0-127, of B 128-255, O of A 256-, of B 384-.
+//
+// Bound: per pair of tiles and 128 keys the tensor core needs 2048 clocks and the
+// special-function unit as many for the exponentials (an eighth of them go to
+// the FMA pipe); a pair takes ~2600, and long prompts run at the board's power
+// limit.  Measured with 32 query and 8 kv heads of 128, bf16: 8192 tokens 465-500
+// us (1.1-1.18 PFLOP/s), 512 tokens 12.1 us, 16 sequences of ~734 tokens after 256
+// cached ones 147-170 us; the end of a unit costs 3 k clocks (O is read, scaled
+// and stored), a first or a masked key tile 1 k more than another.
 #include <cuda_runtime.h>
 
 #include "paged_dev.cuh"
@@ -205,7 +213,7 @@ RPGC_DEV SeqLens seq_lens(const PagedSeqs& b, int s) {
   SeqLens q{0, 0};
   if (s < b.n_seqs) {
     q.n = max(0, (int32_t)(seq_row(b, s + 1) - seq_row(b, s)));
-    if (b.table) q.pre = max(0, __ldg(b.kv_lens + s)) - q.n;
+    if (b.table) q.pre = max(0, b.kv_lens[s]) - q.n;
   }
   return q;
 }
@@ -306,278 +314,278 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
   // code that both paths reached would have to fit the smaller share.
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  if (warp == 10) {
-    // ---------------------------------------------------- finds the units
-    const int32_t U = p.T * (p.dual ? 2 : 1);
-    const SeqLens mine = seq_lens(a.b, lane);
-    int32_t cmax = (max(0, min(mine.pre, 1 << 30) + mine.n) + kKeys - 1) / kKeys;
-    for (int s = lane + 32; s < a.b.n_seqs; s += 32) {
-      const SeqLens q = seq_lens(a.b, s);
-      cmax = max(cmax, (max(0, min(q.pre, 1 << 30) + q.n) + kKeys - 1) / kKeys);
-    }
-    cmax = __reduce_max_sync(0xffffffffu, cmax);
-    const int32_t total = tiles_at_least(a.b, mine, U, 0, lane);
-    const int64_t units_n = (int64_t)total * a.kv.n_kv;
-    // the current cost c: tiles that cost at least c, and more; the sequences from
-    // s0 on are still to be looked through, `before` tiles of cost c lie before them
-    int32_t c = cmax + 1, at_least = 0, more = 0, s0 = 0, before = 0;
-    for (int it = 0;; ++it) {
-      // there and back over the CTAs, so that nobody gets the longest of every round
-      const int64_t u = (int64_t)it * gridDim.x + ((it & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-      if (it >= kUnits) wait(u_empty + it % kUnits, (uint32_t)((it / kUnits) - 1) & 1u);
-      Unit un;
-      un.seq = -1;
-      if (u < units_n) {
-        const int32_t k = (int32_t)(u / a.kv.n_kv);  // (never less than the last)
-        if (k >= at_least) {  // the largest lower cost that more than k tiles reach
-          int32_t lo = 0, hi = c - 1;
-          while (lo < hi) {
-            const int32_t mid = (lo + hi + 1) >> 1;
-            if (tiles_at_least(a.b, mine, U, mid, lane) > k) lo = mid;
-            else hi = mid - 1;
+    if (warp == 10) {
+      // ---------------------------------------------------- finds the units
+      const int32_t U = p.T * (p.dual ? 2 : 1);
+      const SeqLens mine = seq_lens(a.b, lane);
+      int32_t cmax = (max(0, min(mine.pre, 1 << 30) + mine.n) + kKeys - 1) / kKeys;
+      for (int s = lane + 32; s < a.b.n_seqs; s += 32) {
+        const SeqLens q = seq_lens(a.b, s);
+        cmax = max(cmax, (max(0, min(q.pre, 1 << 30) + q.n) + kKeys - 1) / kKeys);
+      }
+      cmax = __reduce_max_sync(0xffffffffu, cmax);
+      const int32_t total = tiles_at_least(a.b, mine, U, 0, lane);
+      const int64_t units_n = (int64_t)total * a.kv.n_kv;
+      // the current cost c: tiles that cost at least c, and more; the sequences from
+      // s0 on are still to be looked through, `before` tiles of cost c lie before them
+      int32_t c = cmax + 1, at_least = 0, more = 0, s0 = 0, before = 0;
+      for (int it = 0;; ++it) {
+        // there and back over the CTAs, so that nobody gets the longest of every round
+        const int64_t u = (int64_t)it * gridDim.x + ((it & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (it >= kUnits) wait(u_empty + it % kUnits, (uint32_t)((it / kUnits) - 1) & 1u);
+        Unit un;
+        un.seq = -1;
+        if (u < units_n) {
+          const int32_t k = (int32_t)(u / a.kv.n_kv);  // (never less than the last)
+          if (k >= at_least) {  // the largest lower cost that more than k tiles reach
+            int32_t lo = 0, hi = c - 1;
+            while (lo < hi) {
+              const int32_t mid = (lo + hi + 1) >> 1;
+              if (tiles_at_least(a.b, mine, U, mid, lane) > k) lo = mid;
+              else hi = mid - 1;
+            }
+            c = lo;
+            more = tiles_at_least(a.b, mine, U, c + 1, lane);
+            at_least = tiles_at_least(a.b, mine, U, c, lane);
+            s0 = before = 0;
           }
-          c = lo;
-          more = tiles_at_least(a.b, mine, U, c + 1, lane);
-          at_least = tiles_at_least(a.b, mine, U, c, lane);
-          s0 = before = 0;
-        }
-        const int32_t r = k - more;  // among the tiles of cost c
-        for (; s0 < a.b.n_seqs; s0 += 32) {
-          const SeqLens q = s0 ? seq_lens(a.b, s0 + lane) : mine;
-          const int32_t f = first_tile(q, U, c), n = first_tile(q, U, c + 1) - f;
-          int32_t sum = n;
+          const int32_t r = k - more;  // among the tiles of cost c
+          for (; s0 < a.b.n_seqs; s0 += 32) {
+            const SeqLens q = s0 ? seq_lens(a.b, s0 + lane) : mine;
+            const int32_t f = first_tile(q, U, c), n = first_tile(q, U, c + 1) - f;
+            int32_t sum = n;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += x;
+            for (int o = 1; o < 32; o <<= 1) {
+              const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
+              if (lane >= o) sum += x;
+            }
+            const uint32_t in = __ballot_sync(0xffffffffu, r - before < sum);
+            if (in) {
+              const int src = __ffs(in) - 1;
+              const int32_t i = __shfl_sync(0xffffffffu, f + r - before - (sum - n), src);
+              const int32_t n_new = __shfl_sync(0xffffffffu, q.n, src), pre = __shfl_sync(0xffffffffu, q.pre, src);
+              const int32_t t0 = i * U;
+              un.seq = s0 + src;
+              un.kh = (int32_t)(u % a.kv.n_kv);
+              un.key0 = seq_row(a.b, un.seq);
+              un.row0 = un.key0 + t0;
+              un.pos0 = pre + t0;
+              const int64_t reach = paged ? table_reach(a.kv, a.b) : (int64_t)n_new;
+              un.reach = (int32_t)min(reach, (int64_t)0x7fffff00);
+#pragma unroll
+              for (int g = 0; g < 2; ++g) {
+                const int32_t first = p.dual ? g * p.T : 0;
+                un.rows[g] = max(0, min(p.T, n_new - t0 - first));
+                un.end[g] = un.rows[g] ? (int32_t)max((int64_t)0, min((int64_t)un.pos0 + first + un.rows[g], (int64_t)un.reach)) : 0;
+                un.tiles[g] = (un.end[g] + kKeys - 1) / kKeys;
+              }
+              break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
           }
-          const uint32_t in = __ballot_sync(0xffffffffu, r - before < sum);
-          if (in) {
-            const int src = __ffs(in) - 1;
-            const int32_t i = __shfl_sync(0xffffffffu, f + r - before - (sum - n), src);
-            const int32_t n_new = __shfl_sync(0xffffffffu, q.n, src), pre = __shfl_sync(0xffffffffu, q.pre, src);
-            const int32_t t0 = i * U;
-            un.seq = s0 + src;
-            un.kh = (int32_t)(u % a.kv.n_kv);
-            un.key0 = seq_row(a.b, un.seq);
-            un.row0 = un.key0 + t0;
-            un.pos0 = pre + t0;
-            const int64_t reach = paged ? table_reach(a.kv, a.b) : (int64_t)n_new;
-            un.reach = (int32_t)min(reach, (int64_t)0x7fffff00);
+        }
+        if (lane == 0) {
+          units[it % kUnits] = un;
+          mbar_arrive(u_full + it % kUnits);
+        }
+        __syncwarp();
+        if (un.seq < 0 || *gave_up) break;
+      }
+    } else if (warp == 9) {
+      // ------------------------------------------------------------ loads
+      int st = 0;
+      uint32_t ph = 0;
+      int nq = 0;
+      const int per = kKeys / p.box;  // copies of a tile and panel
+      for (int it = 0;; ++it) {
+        wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
+        const Unit un = units[it % kUnits];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(u_empty + it % kUnits);
+        if (un.seq < 0 || *gave_up) break;
+        const int nt = max(un.tiles[0], un.tiles[1]);
+        if (!nt) continue;
+        if (nq) wait(q_empty, (uint32_t)(nq - 1) & 1u);
+        ++nq;
+        if (lane == 0) {
+          const uint32_t bytes = (uint32_t)(p.T * p.G * 128 * kHalves);
+          const bool two = p.dual && un.rows[1];
+          mbar_arrive_expect_tx(q_full, bytes * (two ? 2 : 1));
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+            if (g == 0 || two)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+              tma_3d(Qs + (g * kHalves + h) * kPanel, &tm_q, 64 * h, un.kh * p.G, (int)(un.row0 + g * p.T), q_full);
+        }
+        for (int j = 0; j < nt; ++j) {
+          // lane l: the page of copy l; a page that is not there becomes the one
+          // past the last, which TMA fills with zeros
+          int page = 0, at = 0;
+          if (paged) {
+            const int64_t t = (int64_t)j * kKeys + (int64_t)lane * p.box;
+            if (lane < per) page = page_of(a.kv, a.b, un.seq, t);
+            if (page < 0) page = a.kv.n_pages;
+            at = (int)(t & ((1 << a.kv.page_shift) - 1));
+          }
+          for (int v = 0; v < 2; ++v) {
+            wait(empty + st, ph ^ 1u);
+            uint8_t* dst = ring + st * S::kStage;
+            const CUtensorMap* m = v ? &tm_v : &tm_k;
+            if (lane == 0) mbar_arrive_expect_tx(full + st, S::kStage);
+            __syncwarp();
+            if (lane < per) {
+#pragma unroll
+              for (int h = 0; h < kHalves; ++h) {
+                uint8_t* d = dst + h * kPanel + lane * p.box * 128;
+                if (paged) tma_4d(d, m, 64 * h, un.kh, at, page, full + st);
+                else tma_3d(d, m, 64 * h, un.kh, (int)un.key0 + j * kKeys, full + st);
+              }
+            }
+            if (++st == kStages) st = 0, ph ^= 1u;
+          }
+          if (*gave_up) break;
+        }
+      }
+      if (*gave_up) {  // copies in flight end before the CTA does
+        for (int i = 0; i < kStages; ++i)
+          for (int k = 0; k < 1 << 12; ++k)
+            if (mbar_try_wait(full + i, ph ^ (i < st ? 0u : 1u))) break;
+      }
+    } else if (warp == 8) {
+      // ------------------------------------------------------------- MMAs
+      uint32_t at = 0;            // the unit's first place in the ring: K tile j at + 2 j, V tile j after it
+      uint32_t pp[2] = {0u, 0u};  // parity of p_full
+      // One elected lane issues, from descriptors that differ by constants: with
+      // anything more to compute between two MMAs the issue, not the tensor
+      // core, sets the pace (150 clocks an MMA instead of 64).
+      const uint64_t q_desc = sdesc(Qs), k_desc = sdesc(ring), v_desc = vdesc(ring, kPanel);
+      int nq = 0;
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) mma_commit(bar);
+        __syncwarp();
+      };
+      auto landed = [&](uint32_t c) {
+        wait(full + c % kStages, (c / kStages) & 1u);
+        tc_fence_after();
+      };
+      // S of accumulator g = Q (tile qt) K^T, K at ring place c
+      auto issue_s = [&](int g, int qt, uint32_t c) {
+        if (elect_one()) {
+          const uint64_t q = q_desc + (uint64_t)(qt * kHalves * kPanel / 16), k = k_desc + (uint64_t)(c % kStages * (S::kStage / 16));
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint64_t o = ((kk >> 2) * kPanel + (kk & 3) * 32) / 16;
+            mma_f16(tmem + 128u * g, q + o, k + o, kIdS, kk > 0);
+          }
+          mma_commit(s_full + g);
+        }
+        __syncwarp();
+      };
+      // O of accumulator g += P V, V at ring place c, once P is there
+      auto issue_pv = [&](int g, uint32_t c, int keys, bool first) {
+        wait(p_full + g, pp[g]);
+        pp[g] ^= 1u;
+        tc_fence_after();
+        const int steps = (keys + 15) >> 4;
+        if (elect_one()) {
+          const uint64_t vd = v_desc + (uint64_t)(c % kStages * (S::kStage / 16));
+          const uint32_t o = tmem + 256u + 128u * g, pt = tmem + 128u * g;
+          mma_ts(o, pt, vd, kIdO, !first);
+          if (steps == 8) {
+#pragma unroll
+            for (int kk = 1; kk < 8; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
+          } else {
+            for (int kk = 1; kk < steps; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
+          }
+        }
+        __syncwarp();
+      };
+      // the values past the last position of the last step of 16 keys become zeros
+      auto clear_tail = [&](uint32_t c, int keys) {
+        if (!(keys & 15)) return;
+        uint8_t* v = ring + c % kStages * S::kStage;
+        const int stop = (keys + 15) & ~15;
+        for (int i = lane; i < (stop - keys) * 8 * kHalves; i += 32) {
+          const int h = i / ((stop - keys) * 8), k = i % ((stop - keys) * 8);
+          *reinterpret_cast<uint4*>(v + h * kPanel + (keys + (k >> 3)) * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      };
+      for (int it = 0;; ++it) {
+        wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
+        const Unit un = units[it % kUnits];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(u_empty + it % kUnits);
+        if (un.seq < 0 || *gave_up) break;
+        const int nt = max(un.tiles[0], un.tiles[1]), end = max(un.end[0], un.end[1]);
+        if (!nt) continue;
+        wait(q_full, (uint32_t)nq & 1u);
+        ++nq;
+        if (p.dual) {
+          landed(at);
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+            if (un.tiles[g] > 0) issue_s(g, g, at);
+          commit(empty + at % kStages);
+          if (nt == 1) commit(q_empty);
+          for (int j = 0; j < nt && !*gave_up; ++j) {
+            const uint32_t vc = at + 2 * j + 1, kc = vc + 1;
+            const bool more = j + 1 < nt;
+            landed(vc);
+            clear_tail(vc, min(kKeys, end - j * kKeys));
+            bool waited = false;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-              const int32_t first = p.dual ? g * p.T : 0;
-              un.rows[g] = max(0, min(p.T, n_new - t0 - first));
-              un.end[g] = un.rows[g] ? (int32_t)max((int64_t)0, min((int64_t)un.pos0 + first + un.rows[g], (int64_t)un.reach)) : 0;
-              un.tiles[g] = (un.end[g] + kKeys - 1) / kKeys;
+              if (j < un.tiles[g]) {
+                issue_pv(g, vc, min(kKeys, un.end[g] - j * kKeys), j == 0);
+                if (j + 1 == un.tiles[g]) commit(o_full + g);
+              }
+              if (j + 1 < un.tiles[g]) {
+                if (!waited) landed(kc);
+                waited = true;
+                issue_s(g, g, kc);
+              }
             }
-            break;
+            commit(empty + vc % kStages);
+            if (more) commit(empty + kc % kStages);
+            if (j + 2 == nt) commit(q_empty);
           }
-          before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-      }
-      if (lane == 0) {
-        units[it % kUnits] = un;
-        mbar_arrive(u_full + it % kUnits);
-      }
-      __syncwarp();
-      if (un.seq < 0 || *gave_up) break;
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ loads
-    int st = 0;
-    uint32_t ph = 0;
-    int nq = 0;
-    const int per = kKeys / p.box;  // copies of a tile and panel
-    for (int it = 0;; ++it) {
-      wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
-      const Unit un = units[it % kUnits];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(u_empty + it % kUnits);
-      if (un.seq < 0 || *gave_up) break;
-      const int nt = max(un.tiles[0], un.tiles[1]);
-      if (!nt) continue;
-      if (nq) wait(q_empty, (uint32_t)(nq - 1) & 1u);
-      ++nq;
-      if (lane == 0) {
-        const uint32_t bytes = (uint32_t)(p.T * p.G * 128 * kHalves);
-        const bool two = p.dual && un.rows[1];
-        mbar_arrive_expect_tx(q_full, bytes * (two ? 2 : 1));
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          if (g == 0 || two)
-#pragma unroll
-          for (int h = 0; h < kHalves; ++h)
-            tma_3d(Qs + (g * kHalves + h) * kPanel, &tm_q, 64 * h, un.kh * p.G, (int)(un.row0 + g * p.T), q_full);
-      }
-      for (int j = 0; j < nt; ++j) {
-        // lane l: the page of copy l; a page that is not there becomes the one
-        // past the last, which TMA fills with zeros
-        int page = 0, at = 0;
-        if (paged) {
-          const int64_t t = (int64_t)j * kKeys + (int64_t)lane * p.box;
-          if (lane < per) page = page_of(a.kv, a.b, un.seq, t);
-          if (page < 0) page = a.kv.n_pages;
-          at = (int)(t & ((1 << a.kv.page_shift) - 1));
-        }
-        for (int v = 0; v < 2; ++v) {
-          wait(empty + st, ph ^ 1u);
-          uint8_t* dst = ring + st * S::kStage;
-          const CUtensorMap* m = v ? &tm_v : &tm_k;
-          if (lane == 0) mbar_arrive_expect_tx(full + st, S::kStage);
-          __syncwarp();
-          if (lane < per) {
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-              uint8_t* d = dst + h * kPanel + lane * p.box * 128;
-              if (paged) tma_4d(d, m, 64 * h, un.kh, at, page, full + st);
-              else tma_3d(d, m, 64 * h, un.kh, (int)un.key0 + j * kKeys, full + st);
+        } else {
+          // one tile of rows: accumulator A takes its even key tiles, B the odd ones
+          for (int j = 0; j < 2 && j < nt; ++j) {
+            const uint32_t kc = at + 2 * j;
+            landed(kc);
+            issue_s(j, 0, kc);
+            commit(empty + kc % kStages);
+          }
+          if (nt <= 2) commit(q_empty);
+          for (int j = 0; j < nt && !*gave_up; ++j) {
+            const uint32_t vc = at + 2 * j + 1, kc = vc + 3;
+            const int keys = min(kKeys, end - j * kKeys);
+            landed(vc);
+            clear_tail(vc, keys);
+            if (j & 1) issue_pv(1, vc, keys, j < 2);
+            else issue_pv(0, vc, keys, j < 2);
+            if (j + 2 >= nt) commit(o_full + (j & 1));
+            commit(empty + vc % kStages);
+            if (j + 2 < nt) {
+              landed(kc);
+              issue_s(j & 1, 0, kc);
+              commit(empty + kc % kStages);
+              if (j + 3 == nt) commit(q_empty);
             }
           }
-          if (++st == kStages) st = 0, ph ^= 1u;
         }
+        at += 2 * nt;
         if (*gave_up) break;
       }
+      if (elect_one()) mma_commit(done);
+      __syncwarp();
+      for (int k = 0; k < 1 << 14; ++k)
+        if (mbar_try_wait(done, 0)) break;
     }
-    if (*gave_up) {  // copies in flight end before the CTA does
-      for (int i = 0; i < kStages; ++i)
-        for (int k = 0; k < 1 << 12; ++k)
-          if (mbar_try_wait(full + i, ph ^ (i < st ? 0u : 1u))) break;
-    }
-  } else if (warp == 8) {
-    // ------------------------------------------------------------- MMAs
-    uint32_t at = 0;            // the unit's first place in the ring: K tile j at + 2 j, V tile j after it
-    uint32_t pp[2] = {0u, 0u};  // parity of p_full
-    // One elected lane issues, from descriptors that differ by constants: with
-    // anything more to compute between two MMAs the issue, not the tensor
-    // core, sets the pace (150 clocks an MMA instead of 64).
-    const uint64_t q_desc = sdesc(Qs), k_desc = sdesc(ring), v_desc = vdesc(ring, kPanel);
-    int nq = 0;
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) mma_commit(bar);
-      __syncwarp();
-    };
-    auto landed = [&](uint32_t c) {
-      wait(full + c % kStages, (c / kStages) & 1u);
-      tc_fence_after();
-    };
-    // S of accumulator g = Q (tile qt) K^T, K at ring place c
-    auto issue_s = [&](int g, int qt, uint32_t c) {
-      if (elect_one()) {
-        const uint64_t q = q_desc + (uint64_t)(qt * kHalves * kPanel / 16), k = k_desc + (uint64_t)(c % kStages * (S::kStage / 16));
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint64_t o = ((kk >> 2) * kPanel + (kk & 3) * 32) / 16;
-          mma_f16(tmem + 128u * g, q + o, k + o, kIdS, kk > 0);
-        }
-        mma_commit(s_full + g);
-      }
-      __syncwarp();
-    };
-    // O of accumulator g += P V, V at ring place c, once P is there
-    auto issue_pv = [&](int g, uint32_t c, int keys, bool first) {
-      wait(p_full + g, pp[g]);
-      pp[g] ^= 1u;
-      tc_fence_after();
-      const int steps = (keys + 15) >> 4;
-      if (elect_one()) {
-        const uint64_t vd = v_desc + (uint64_t)(c % kStages * (S::kStage / 16));
-        const uint32_t o = tmem + 256u + 128u * g, pt = tmem + 128u * g;
-        mma_ts(o, pt, vd, kIdO, !first);
-        if (steps == 8) {
-#pragma unroll
-          for (int kk = 1; kk < 8; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
-        } else {
-          for (int kk = 1; kk < steps; ++kk) mma_ts(o, pt + 8u * kk, vd + kk * 128, kIdO, 1u);
-        }
-      }
-      __syncwarp();
-    };
-    // the values past the last position of the last step of 16 keys become zeros
-    auto clear_tail = [&](uint32_t c, int keys) {
-      if (!(keys & 15)) return;
-      uint8_t* v = ring + c % kStages * S::kStage;
-      const int stop = (keys + 15) & ~15;
-      for (int i = lane; i < (stop - keys) * 8 * kHalves; i += 32) {
-        const int h = i / ((stop - keys) * 8), k = i % ((stop - keys) * 8);
-        *reinterpret_cast<uint4*>(v + h * kPanel + (keys + (k >> 3)) * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-    };
-    for (int it = 0;; ++it) {
-      wait(u_full + it % kUnits, (uint32_t)(it / kUnits) & 1u);
-      const Unit un = units[it % kUnits];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(u_empty + it % kUnits);
-      if (un.seq < 0 || *gave_up) break;
-      const int nt = max(un.tiles[0], un.tiles[1]), end = max(un.end[0], un.end[1]);
-      if (!nt) continue;
-      wait(q_full, (uint32_t)nq & 1u);
-      ++nq;
-      if (p.dual) {
-        landed(at);
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          if (un.tiles[g] > 0) issue_s(g, g, at);
-        commit(empty + at % kStages);
-        if (nt == 1) commit(q_empty);
-        for (int j = 0; j < nt && !*gave_up; ++j) {
-          const uint32_t vc = at + 2 * j + 1, kc = vc + 1;
-          const bool more = j + 1 < nt;
-          landed(vc);
-          clear_tail(vc, min(kKeys, end - j * kKeys));
-          bool waited = false;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            if (j < un.tiles[g]) {
-              issue_pv(g, vc, min(kKeys, un.end[g] - j * kKeys), j == 0);
-              if (j + 1 == un.tiles[g]) commit(o_full + g);
-            }
-            if (j + 1 < un.tiles[g]) {
-              if (!waited) landed(kc);
-              waited = true;
-              issue_s(g, g, kc);
-            }
-          }
-          commit(empty + vc % kStages);
-          if (more) commit(empty + kc % kStages);
-          if (j + 2 == nt) commit(q_empty);
-        }
-      } else {
-        // one tile of rows: accumulator A takes its even key tiles, B the odd ones
-        for (int j = 0; j < 2 && j < nt; ++j) {
-          const uint32_t kc = at + 2 * j;
-          landed(kc);
-          issue_s(j, 0, kc);
-          commit(empty + kc % kStages);
-        }
-        if (nt <= 2) commit(q_empty);
-        for (int j = 0; j < nt && !*gave_up; ++j) {
-          const uint32_t vc = at + 2 * j + 1, kc = vc + 3;
-          const int keys = min(kKeys, end - j * kKeys);
-          landed(vc);
-          clear_tail(vc, keys);
-          if (j & 1) issue_pv(1, vc, keys, j < 2);
-          else issue_pv(0, vc, keys, j < 2);
-          if (j + 2 >= nt) commit(o_full + (j & 1));
-          commit(empty + vc % kStages);
-          if (j + 2 < nt) {
-            landed(kc);
-            issue_s(j & 1, 0, kc);
-            commit(empty + kc % kStages);
-            if (j + 3 == nt) commit(q_empty);
-          }
-        }
-      }
-      at += 2 * nt;
-      if (*gave_up) break;
-    }
-    if (elect_one()) mma_commit(done);
-    __syncwarp();
-    for (int k = 0; k < 1 << 14; ++k)
-      if (mbar_try_wait(done, 0)) break;
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------------------------------------------------- softmax
@@ -617,7 +625,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       const int32_t* tab = paged ? a.b.table + (int64_t)seq * a.b.table_stride : nullptr;
       auto entry = [&](int j) {  // page of this lane's part of key tile j
         const int64_t e = (((int64_t)j * kKeys) >> a.kv.page_shift) + lane;
-        return lane < npg && e < a.b.max_pages ? __ldg(tab + e) : 0;
+        return lane < npg && e < a.b.max_pages ? tab[e] : 0;
       };
       int32_t pg = paged && j0 < tiles ? entry(j0) : 0;
       for (int j = j0; j < tiles; j += step) {
