@@ -9,25 +9,27 @@
 //
 // Bound: every K and V byte is read once, so HBM is the limit.  The key tiles of
 // all (sequence, kv head) items form one list, cut into equal ranges, one per
-// CTA and SM: batches of any mix of lengths, and one long sequence as well, give
-// every SM the same bytes.  An item that several CTAs share is joined by the last
-// of them to finish, from partial results in the workspace, in the order of the
+// CTA: batches of any mix of lengths, and one long sequence as well, give every
+// SM the same bytes.  An item that several CTAs share is joined by the last of
+// them to finish, from partial results in the workspace, in the order of the
 // pieces (the same result whoever is last).
 //
 // A CTA: two warps walk its range and issue the TMA copies of K and of V into a
-// ring of 6 tiles, so 192 KB are in flight per SM (with one warp for both, pages of
-// 16 positions of 64 dims were issued at 2.8 TB/s).  Two groups of 4 warps (hd
-// 128) or one of 8 take the tiles, 16 keys a warp: S^T = K Q^T (m16n8k16, the kv
-// head's query heads are the N side), P^T turned from the accumulator layout
+// ring (with one warp for both, pages of 16 positions of 64 dims were issued at
+// 2.8 TB/s); 4 warps take 16 keys each of every tile: S^T = K Q^T (m16n8k16, the
+// kv head's query heads are the N side), P^T turned from the accumulator layout
 // into an operand by movmatrix, O^T += V^T P^T.  (mma.sync: at 4 to 16 rows a
 // head group has nothing for wider MMAs.)  The warps' sums meet in shared memory
-// at an item's end.
+// at an item's end.  Two such CTAs on an SM, 192 KB in flight between them: while
+// one ends an item or looks for the next, the other's tiles go on (one CTA of 8
+// warps took 1.5 times as long on 128 sequences of 20 positions, 1.08 times on
+// 128 of 500).
 //
 // Measured with 32 query and 8 kv heads of 128, bf16: 128 sequences of 1-8192
-// positions 325 us (2.17 GB, 6.67 TB/s), 64 of ~1100 53.5 us (5.4 TB/s; 8 us of
-// it are the look-ups before the first tile and the last joins), one of 4200
-// 9.7 us, one of 33 (16 heads) 4.1 us; 48 sequences with 12 heads of 64 in
-// pages of 16, 167 MB, 42 us.
+// positions 318 us (2.17 GB, 6.8 TB/s), 64 of ~1100 52 us (5.5 TB/s; 8 us of it
+// are the look-ups before the first tile and the last joins), 128 of 200 28 us
+// (3.7 TB/s), one of 4200 10.0 us, one of 33 (16 heads) 4.0 us; 48 sequences with
+// 12 heads of 64 in pages of 16, 167 MB, 39 us.
 #include <cuda_runtime.h>
 
 #include "paged_dev.cuh"
@@ -44,21 +46,21 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD, int NT>
 struct DShape {
-  static constexpr int kTile = HD == 128 ? 64 : 128;  // keys: 32 KB of K and V either way
-  static constexpr int kGroup = kTile / 16;           // consumer warps on a tile, 16 keys each
+  static constexpr int kCtas = NT == 1 ? 2 : 1;       // CTAs on an SM
+  static constexpr int kTile = HD == 128 || NT == 1 ? 64 : 128;  // keys
+  static constexpr int kWarps = kTile / 16;           // consumer warps, 16 keys of a tile each
+  static constexpr int kThreads = (kWarps + 2) * 32;
   static constexpr int kPanels = HD / 64;
   static constexpr int kPanel = kTile * 128;
   static constexpr int kHalf = kPanels * kPanel;  // K (or V) of a tile
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kGroups = HD == 128 && NT == 1 ? 2 : 1, kWarps = kGroups * kGroup, kThreads = (kWarps + 2) * 32;
-  static constexpr int kStages = HD == 64 && NT == 2 ? 5 : 6;  // (even where two groups take them in turn)
   static constexpr int kHeads = 8 * NT;           // query heads of a kv head, padded
   static constexpr int kPad = HD + 4;             // row of the merge buffer: no bank conflicts
-  static constexpr int kMaxCtas = 256;
-  // the warps' sums, later the join's table: 8 bytes per piece and head
-  static constexpr int kSums = kWarps * kHeads * kPad * 4, kTable = kMaxCtas * kHeads * 8;
-  static constexpr int kMerge = kSums > kTable ? kSums : kTable;
-  static constexpr int kSmem = 1024 + kStages * kStage + kMerge + 2 * kWarps * kHeads * 4 + 512;
+  static constexpr int kMerge = kWarps * kHeads * kPad * 4;  // the warps' sums; later the join's table, 8 bytes per piece and head
+  static constexpr int kRest = kMerge + 2 * kWarps * kHeads * 4 + 256;
+  // what an SM has, less a kilobyte for each CTA, goes to the ring
+  static constexpr int kStages = ((233472 / kCtas - 1024) - kRest) / kStage;
+  static constexpr int kSmem = kStages * kStage + kRest;
 };
 
 struct DecodeParams {
@@ -109,7 +111,8 @@ RPGC_DEV int32_t seen(const PagedAttnArgs& a, int s) {  // positions the token o
 // What an item weighs in the list: its key tiles, and the end of an item (the
 // warps' sums, a share's join) as kEnd tiles more, at its front.  An item that sees
 // nothing weighs nothing.
-constexpr int kEnd = 2;
+constexpr int kEnd = 3;
+constexpr int kPieces = 18;  // of an item, at most on average: one of 4200 positions takes 11.6 us in 37 pieces, 10.0 in 18
 template <int T>
 RPGC_DEV int64_t weight_of(int32_t n) {
   return n ? (n + (int64_t)T - 1) / T + kEnd : 0;
@@ -124,7 +127,7 @@ struct Walk {
   int32_t t0, t1;         // those that are this CTA's
   // where range b of n begins, and the range that holds place t
   RPGC_DEV int64_t begin(int b, int n) const {
-    return total < (1 << 23) ? (int64_t)((uint32_t)b * (uint32_t)total / (uint32_t)n) : b * total / n;  // (n <= 256)
+    return total < (1 << 23) ? (int64_t)((uint32_t)b * (uint32_t)total / (uint32_t)n) : b * total / n;  // (n < 512)
   }
   RPGC_DEV int holder(int64_t t, int n) const {
     return total < (1 << 23) ? (int)((((uint32_t)t + 1) * (uint32_t)n - 1) / (uint32_t)total) : (int)(((t + 1) * n - 1) / total);
@@ -141,17 +144,20 @@ struct Walk {
     // first place is looked through 32 sequences at a time
     const int run = (a.b.n_seqs + 31) / 32;
     int64_t sum = 0;
-    int32_t ln = 0;
+    int32_t ln = 0, some = 0;
 #pragma unroll 4
     for (int i = 0; i < run; ++i) {
       const int s = lane * run + i;
       ln = s < a.b.n_seqs ? seen(a, s) : 0;
       sum += weight_of<T>(ln);
+      some += ln > 0;
     }
     sum *= kv;
     int64_t upto = scan(sum, lane);
     total = __shfl_sync(0xffffffffu, upto, 31);
-    const int parts = (int)(total < ctas ? total : ctas);
+    // no more CTAs than there is weight, nor so many that a join is long
+    const int64_t items = (int64_t)__reduce_add_sync(0xffffffffu, some) * kv;
+    const int parts = (int)min(min(total, (int64_t)ctas), items * kPieces);
     *active = parts;
     if (cta >= parts) return false;
     lo = begin(cta, parts);
@@ -204,15 +210,14 @@ RPGC_DEV void bar_consumers() {
 }
 
 template <int HD, bool BF, int NT>
-__global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(const __grid_constant__ CUtensorMap tm_k,
+__global__ void __launch_bounds__(DShape<HD, NT>::kThreads, DShape<HD, NT>::kCtas) decode_kernel(const __grid_constant__ CUtensorMap tm_k,
                                                               const __grid_constant__ CUtensorMap tm_v,
                                                               const __grid_constant__ DecodeParams p) {
   using S = DShape<HD, NT>;
-  constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps, kTile = S::kTile, kGroup = S::kGroup;
+  constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps, kTile = S::kTile;
   constexpr float kLift = BF ? 0.0f : 6.0f;  // fp16 probabilities carry 2^6: small ones keep their bits
   constexpr float kMost = BF ? 1.0e12f : 32768.0f;  // a probability that needs no new reference
-  extern __shared__ uint8_t dsm_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t ring[];  // (swizzled tiles start on 1024 bytes; the kernel has no other shared memory)
   float* wo = reinterpret_cast<float*>(ring + kStages * S::kStage);  // [warp][head][kPad]
   float* wm = wo + kWarps * kHeads * kPad;                           // [warp][head]
   float* wl = wm + kWarps * kHeads;
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(full + i, 2);
-      mbar_init(empty + i, kGroup);
+      mbar_init(empty + i, kWarps);
     }
     *gave_up = 0;
     fence_barrier_init();
@@ -306,12 +311,11 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
         reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)s * a.n_heads * HD)[i] = make_uint4(0, 0, 0, 0);
   if (!work) return;
   const int gr = lane >> 2, tq = lane & 3, G = p.G;
-  const int part = warp % kGroup, group = warp / kGroup;  // 16 keys of a tile; every second tile
   const float c = a.scale * kLog2e;
   // ldmatrix rows of this lane in the warp's 16 keys: K as stored, V transposed
   const int mi = lane >> 3, mr = lane & 7;
-  const int krow = 16 * part + mr + 8 * (mi & 1), kc = mi >> 1;
-  const int vrow = 16 * part + mr + 8 * (mi >> 1), vc = mi & 1;
+  const int krow = 16 * warp + mr + 8 * (mi & 1), kc = mi >> 1;
+  const int vrow = 16 * warp + mr + 8 * (mi >> 1), vc = mi & 1;
   int st = 0;
   uint32_t ph = 0;
   do {
@@ -338,13 +342,9 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, 1) decode_kernel(con
       for (int d = 0; d < HD / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.0f;
     }
     for (int t = t0; t < t1; ++t) {
-      if (S::kGroups > 1 && (st & 1) != group) {
-        if (++st == kStages) st = 0, ph ^= 1u;
-        continue;
-      }
       wait(full + st, ph);
-      const int left = w.len - t * kTile - 16 * part;  // keys of this warp's part
-      if (left > 0 && (there[st] >> part & 1u)) {
+      const int left = w.len - t * kTile - 16 * warp;  // keys of this warp's part
+      if (left > 0 && (there[st] >> warp & 1u)) {
         const uint32_t kb = smem_u32(ring + st * S::kStage), vb = kb + S::kHalf;
         // two chains of MMAs, so that one's latency hides the other's
         float s[NT][4], s2[NT][4];
@@ -574,9 +574,17 @@ int device_sms() {
 
 int64_t counter_bytes(const PagedView& kv, int32_t n_seqs) { return ((int64_t)n_seqs * kv.n_kv * 4 + 255) / 256 * 256; }
 
+// As many CTAs as run at once, and no more than the join's table has room for.
+template <int HD, int NT>
+int decode_ctas(int G) {
+  using S = DShape<HD, NT>;
+  const int n = device_sms() * S::kCtas, most = S::kMerge / (8 * G);
+  return n < most ? n : most;
+}
+
 template <int HD, bool BF, int NT>
 cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
-  const int sms = min(device_sms(), DShape<HD, NT>::kMaxCtas);
+  const int ctas = decode_ctas<HD, NT>(a.n_heads / a.kv.n_kv);
   DecodeParams p{};
   p.a = a;
   p.G = a.n_heads / a.kv.n_kv;
@@ -584,12 +592,12 @@ cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.counters = reinterpret_cast<uint32_t*>(ws);
   p.part = reinterpret_cast<float*>(ws + counter_bytes(a.kv, a.b.n_seqs));
-  p.part_ml = p.part + (int64_t)2 * sms * p.G * HD;
+  p.part_ml = p.part + (int64_t)2 * ctas * p.G * HD;
   CUtensorMap mk, mv;
   const CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
   if (!make_kv_map(&mk, a, false, p.box, promo) || !make_kv_map(&mv, a, true, p.box, promo)) return cudaErrorInvalidValue;
   constexpr int smem = DShape<HD, NT>::kSmem;
-  static_assert(smem <= 232448, "shared memory of one CTA");
+  static_assert(smem <= 233472 / DShape<HD, NT>::kCtas - 1024, "shared memory of one CTA");
   int dev = 0;
   cudaGetDevice(&dev);
   static bool configured[64] = {false};
@@ -598,7 +606,7 @@ cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const cudaError_t e = launch_pdl(decode_kernel<HD, BF, NT>, dim3((unsigned)sms), dim3(DShape<HD, NT>::kThreads), smem, s, mk, mv, p);
+  const cudaError_t e = launch_pdl(decode_kernel<HD, BF, NT>, dim3((unsigned)ctas), dim3(DShape<HD, NT>::kThreads), smem, s, mk, mv, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
@@ -611,7 +619,7 @@ cudaError_t decode_heads(const PagedAttnArgs& a, cudaStream_t s) {
 }  // namespace
 
 int64_t paged_decode_workspace(const PagedView& kv, int32_t n_seqs, int32_t n_heads) {
-  const int64_t rows = (int64_t)2 * device_sms() * (n_heads / kv.n_kv);
+  const int64_t rows = (int64_t)2 * 2 * device_sms() * (n_heads / kv.n_kv);  // (two CTAs an SM at most, two items each)
   return counter_bytes(kv, n_seqs) + rows * (kv.hd + 2) * 4;
 }
 
