@@ -773,29 +773,44 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       const float inv = l == 0.0f || m == -INFINITY || lim <= 0 ? 0.0f : m < INFINITY ? 1.0f / l : __int_as_float(0x7fffffff);
       mine *= inv;
       other *= inv;
-      float bad[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN where a value is not finite
+      uint64_t bad[2] = {0ull, 0ull};  // NaN where a value is not finite
+      const uint64_t mine2 = pair(mine, mine), other2 = pair(other, other);
       const bool have = p.dual || g < tiles, two = !p.dual && (g ^ 1) < tiles;
       const uint32_t to2 = tmem + lanes + 256u + 128u * (g ^ 1);
 #pragma unroll 1
       for (int q = 0; q < cols / 32; ++q) {
-        float t[32];
+        uint64_t t[16];
         if (have) {
-          tmem_ld32(to + col0 + 32u * q, t);
+          uint32_t x[32];
+          tmem_ld32_async(to + col0 + 32u * q, x);
+          tmem_landed(x);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) bad[i & 3] = fmaf(t[i], 0.0f, bad[i & 3]), t[i] *= mine;
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t y = pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+            bad[i & 1] = fma2(y, 0ull, bad[i & 1]);
+            t[i] = fma2(y, mine2, 0ull);
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) t[i] = 0.0f;
+          for (int i = 0; i < 16; ++i) t[i] = 0ull;
         }
         if (two) {
-          float v[32];
-          tmem_ld32(to2 + col0 + 32u * q, v);
+          uint32_t x[32];
+          tmem_ld32_async(to2 + col0 + 32u * q, x);
+          tmem_landed(x);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) bad[i & 3] = fmaf(v[i], 0.0f, bad[i & 3]), t[i] = fmaf(v[i], other, t[i]);
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t y = pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+            bad[i & 1] = fma2(y, 0ull, bad[i & 1]);
+            t[i] = fma2(y, other2, t[i]);
+          }
         }
         uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = pack2<BF>(t[2 * i], t[2 * i + 1]);
+        for (int i = 0; i < 16; ++i) {
+          const float2 z = unpair(t[i]);
+          w[i] = pack2<BF>(z.x, z.y);
+        }
         if (live)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -812,7 +827,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
       if (!p.dual) both();  // both have read O: the next unit's may go over it
       // 0 * x is NaN for an infinite or NaN x in a place that a row does not
       // see: such rows are computed again from their visible keys alone
-      uint32_t again = __ballot_sync(0xffffffffu, live && m < INFINITY && !(bad[0] + bad[1] + bad[2] + bad[3] == 0.0f));
+      const float2 bad2 = unpair(add2(bad[0], bad[1]));
+      uint32_t again = __ballot_sync(0xffffffffu, live && m < INFINITY && !(bad2.x + bad2.y == 0.0f));
       while (again) {
         const int src = __ffs(again) - 1;
         again &= again - 1;
