@@ -22,23 +22,35 @@ using namespace paged;
 // the token's position and page are looked up (one chain of dependent reads).
 // Two steps a warp: one has too little in flight (33.0 us), three and more cost
 // registers and with them warps (32.3, 34.7 us).  4096 tokens of 32 + 2 x 8 heads
-// of 128, fp32 in, bf16 out: 29.3 us, 153 MB, 5.2 TB/s; 64 tokens: 3.2 us.
+// of 128, fp32 in, bf16 out: 29.3 us, 153 MB, 5.2 TB/s; 64 tokens: 3.1 us.  12114
+// ragged tokens of 12 + 2 x 4 heads of 64, fp16: 18.3 us, 65 MB, 3.6 TB/s (what
+// bounds it is the latency of 40 warps an SM with 1 KB of input each).
 constexpr int kSteps = 2;
 enum { kInF32 = 0, kInF16 = 1, kInBF16 = 2 };
 
-// Four consecutive values.  (__ldcg, not __ldg: the kernel before may still be
-// writing the inputs when this one is launched.)
+// Four consecutive values as they are read, and as floats.  16-bit ones stay as
+// they are until they are used: half the registers and with that more warps (13
+// to 18 % faster).  (__ldcg, not __ldg: the kernel before may still be writing
+// the inputs when this one is launched.)
 template <int IN>
-RPGC_DEV void load4(const void* base, int64_t off, float* x) {
-  if (IN == kInF32) {
-    const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + off));
-    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-  } else {
-    const uint2 u = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + off));
+struct Four {
+  uint2 u;
+  RPGC_DEV void load(const void* base, int64_t off) {
+    u = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + off));
+  }
+  RPGC_DEV void get(float* x) const {
     const float2 f = unpack2<IN == kInBF16>(u.x), g = unpack2<IN == kInBF16>(u.y);
     x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
   }
-}
+};
+template <>
+struct Four<kInF32> {
+  float4 f;
+  RPGC_DEV void load(const void* base, int64_t off) {
+    f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + off));
+  }
+  RPGC_DEV void get(float* x) const { x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w; }
+};
 
 // The same of tables that stay as they are: gains and rope rows.
 RPGC_DEV void table4(const float* p, float* x) {
@@ -57,7 +69,7 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
   grid_dep_launch();
   if (h0 >= heads) return;  // whole warps
   const int64_t r = blockIdx.x;
-  float x[kSteps][8];  // dims d .. d + 3, then kHalf + d ..
+  Four<IN> in[kSteps][2] = {};  // dims d .. d + 3, then kHalf + d ..
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) {
     const int h = hl + j * kRows;
@@ -65,11 +77,8 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
     const void* base = isq ? a.q : isk ? a.k : a.v;
     const int64_t off = (isq ? r * a.q_tok + h * a.q_head : isk ? r * a.k_tok + (h - a.n_heads) * a.k_head : r * a.v_tok + (h - nk) * a.v_head) + d;
     if (h < heads) {
-      load4<IN>(base, off, x[j]);
-      load4<IN>(base, off + kHalf, x[j] + 4);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
+      in[j][0].load(base, off);
+      in[j][1].load(base, off + kHalf);
     }
   }
   const int s = seq_of_row(a.b, r, lane);
@@ -94,10 +103,13 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
     const int hs = h0 + j * kRows, h = hl + j * kRows;  // the step's first head; this lane's
     if (hs >= heads) break;                             // whole warps
     const bool isq = h < a.n_heads, isk = h < nk;
+    float x[8];
+    in[j][0].get(x);
+    in[j][1].get(x + 4);
     if (hs < nk) {  // (a step's rows may be of two kinds: v's keep their values)
       float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[j][i];
+      for (int i = 0; i < 8; ++i) y[i] = x[i];
       if (norm) {
         float ss = 0.0f, g[8];
 #pragma unroll
@@ -120,15 +132,15 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
         }
       if (isk)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][i] = y[i];
+        for (int i = 0; i < 8; ++i) x[i] = y[i];
     }
     if (h >= heads || (drop && !isq)) continue;
     if (drop)  // no place in the cache: q's row is zeros
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
+      for (int i = 0; i < 8; ++i) x[i] = 0.0f;
     uint16_t* dst = isq ? qd + h * HD : isk ? kd + (h - a.n_heads) * a.kv.k_head : vd + (h - nk) * a.kv.v_head;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF>(x[j][0], x[j][1]), pack2<BF>(x[j][2], x[j][3]));
-    *reinterpret_cast<uint2*>(dst + kHalf) = make_uint2(pack2<BF>(x[j][4], x[j][5]), pack2<BF>(x[j][6], x[j][7]));
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]));
+    *reinterpret_cast<uint2*>(dst + kHalf) = make_uint2(pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7]));
   }
 }
 
