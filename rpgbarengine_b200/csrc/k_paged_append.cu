@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include "paged_dev.cuh"
+#include "paged_tma.cuh"
 
 namespace rpgc {
 namespace {
@@ -20,12 +21,15 @@ using namespace paged;
 // row over the whole warp and the rotation through shuffles the kernel issued
 // twice as many and took 1.5 times as long.  Every input row is loaded before
 // the token's position and page are looked up (one chain of dependent reads).
-// Two steps a warp: one has too little in flight (33.0 us), three and more cost
-// registers and with them warps (32.3, 34.7 us).  4096 tokens of 32 + 2 x 8 heads
-// of 128, fp32 in, bf16 out: 29.3 us, 153 MB, 5.2 TB/s; 64 tokens: 3.1 us.  12114
-// ragged tokens of 12 + 2 x 4 heads of 64, fp16: 18.3 us, 65 MB, 3.6 TB/s (what
-// bounds it is the latency of 40 warps an SM with 1 KB of input each).
-constexpr int kSteps = 2;
+// Steps a warp: one where all warps run at once all the same, kAtOnce of them an
+// SM, so that only the latency counts (64 tokens of 32 + 2 x 8 heads of 128, fp32:
+// 2.8 us, 3.1 with two; 128 tokens fp16 3.0 and 3.4 with three; 192 tokens, 31 warps
+// an SM, 4.1 and 3.6); else two of fp32 (4096 tokens: one 33.0 us, two 28.9, three
+// 32.3 for the registers they take) and three of 16-bit rows (two 26.4, three 24.6,
+// four 25.4).  So 4096 fp32 tokens take 28.9 us, 153 MB, 5.3 TB/s, and 12114 ragged
+// tokens of 12 + 2 x 4 heads of 64, fp16, 16.9 us, 65 MB, 3.9 TB/s (bound by the
+// latency of its warps).
+constexpr int kAtOnce = 24;
 enum { kInF32 = 0, kInF16 = 1, kInBF16 = 2 };
 
 // Four consecutive values as they are read, and as floats.  16-bit ones stay as
@@ -58,7 +62,7 @@ RPGC_DEV void table4(const float* p, float* x) {
   x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
 }
 
-template <int HD, int IN, bool BF>
+template <int HD, int IN, bool BF, int kSteps>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ PagedAppendArgs a) {
   constexpr int kLanes = HD / 8, kRows = 32 / kLanes, kHalf = HD / 2;
   const int lane = threadIdx.x & 31, kv = a.kv.n_kv, nk = a.n_heads + kv, heads = nk + kv;
@@ -85,15 +89,16 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
   if (s < 0) return;
   const int64_t r0 = seq_row(a.b, s), r1 = seq_row(a.b, s + 1);
   const int64_t pos = (int64_t)a.b.kv_lens[s] - (r1 - r0) + (r - r0);
+  // (the two look-ups that pos leads to run beside each other)
+  float c[4] = {}, sn[4] = {};
+  if (a.rope && pos >= 0 && pos < a.rope_rows) {
+    table4(a.rope + pos * HD + d, c);
+    table4(a.rope + pos * HD + kHalf + d, sn);
+  }
   const int32_t page = pos >= 0 ? page_of(a.kv, a.b, s, pos) : -1;
   const bool drop = page < 0 || (a.rope && pos >= a.rope_rows);
   if (drop && h0 == 0 && lane == 0 && a.b.status) atomicOr(a.b.status, kStatusDropped);
   const bool turn = a.rope && !drop, norm = a.k_norm != nullptr;
-  float c[4], sn[4];
-  if (turn) {
-    table4(a.rope + pos * HD + d, c);
-    table4(a.rope + pos * HD + kHalf + d, sn);
-  }
   const int64_t slot = pos & ((1 << a.kv.page_shift) - 1);
   uint16_t* qd = static_cast<uint16_t*>(a.q_out) + r * a.n_heads * HD + d;
   uint16_t* kd = static_cast<uint16_t*>(const_cast<void*>(a.kv.k)) + page * a.kv.k_page + slot * a.kv.k_pos + d;
@@ -144,12 +149,22 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
   }
 }
 
-template <int HD, int IN>
-cudaError_t append_go(const PagedAppendArgs& a, cudaStream_t s) {
+template <int HD, int IN, int kSteps>
+cudaError_t append_steps(const PagedAppendArgs& a, cudaStream_t s) {
   const int per = kSteps * 256 / HD;  // heads of a warp
   const int groups = (a.n_heads + 2 * a.kv.n_kv + per - 1) / per, rows = (groups + 3) / 4;  // blocks of at most 4 warps: 5 % faster than of 8
   const dim3 grid((unsigned)a.b.n_tokens, (unsigned)rows), block(32u * (unsigned)((groups + rows - 1) / rows));
-  return a.kv.bf16 ? launch_pdl(append_kernel<HD, IN, true>, grid, block, 0, s, a) : launch_pdl(append_kernel<HD, IN, false>, grid, block, 0, s, a);
+  return a.kv.bf16 ? launch_pdl(append_kernel<HD, IN, true, kSteps>, grid, block, 0, s, a)
+                   : launch_pdl(append_kernel<HD, IN, false, kSteps>, grid, block, 0, s, a);
+}
+
+template <int HD, int IN>
+cudaError_t append_go(const PagedAppendArgs& a, cudaStream_t s) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int64_t warps = (a.n_heads + 2 * a.kv.n_kv + 256 / HD - 1) / (256 / HD) * a.b.n_tokens;
+  if (warps <= (int64_t)kAtOnce * sm_count(dev)) return append_steps<HD, IN, 1>(a, s);
+  return append_steps<HD, IN, IN == kInF32 ? 2 : 3>(a, s);
 }
 
 }  // namespace

@@ -188,6 +188,50 @@ def test_append_drops_tokens_without_a_place():
         assert changed == [[2, 0], [4, 1]], changed
 
 
+# Enough tokens that a warp takes several heads: counts that leave the last warp
+# and its last step part full, q, k and v rows in one step, pages that are not there.
+MANY = [  # heads, kv, hd, in, fused
+    (5, 1, 64, "f16", True),
+    (5, 1, 128, "f32", False),
+    (7, 7, 128, "bf16", False),
+    (12, 4, 64, "f32", True),
+    (32, 8, 128, "f16", True),
+    (9, 3, 64, "bf16", True),
+    (1, 1, 128, "f16", False),
+]
+
+
+@pytest.mark.parametrize("H,kv,hd,ty,fused", MANY)
+def test_append_of_many_tokens(H, kv, hd, ty, fused):
+    g = gen(H + hd)
+    new, pre, page, dt = [2500, 0, 1, 3100, 777], [17, 5, 0, 300, 64], 32, torch.bfloat16 if ty == "bf16" else torch.float16
+    lens, n = [a + b for a, b in zip(new, pre)], sum(new)
+    k, v, table = make_pool(g, lens, page, kv, hd, dt)
+    table[0][3], table[3][100] = -1, k.shape[0]  # the pages of 64 new tokens
+    k0, v0 = k.clone(), v.clone()
+    q, kn, vn = append_inputs(g, n, H, kv, hd, ty, fused)
+    qg, kg, tab = 1 + 0.1 * randn(g, hd), 1 + 0.1 * randn(g, hd), rb.rope_table(max(lens), hd)
+    cu, status = i32(np.concatenate([[0], np.cumsum(new)]).tolist()), i32([0])
+    got = rb.paged_append(rb.PagedKV(k, v), rb.PagedBatch(i32(table), i32(lens), cu, n, status), q, kn, vn, qg, kg, 1e-6, tab)
+    pos = torch.tensor([b + i for a, b in zip(new, pre) for i in range(a)], device="cuda")
+    seq = torch.tensor([s for s, a in enumerate(new) for _ in range(a)], device="cuda")
+    pages = i32(table)[seq, pos // page].long()
+    there = (pages >= 0) & (pages < k.shape[0])
+    assert int((~there).sum()) == 64 and int(status) == paged.DROPPED
+    assert bool((got[~there] == 0).all())
+    u, pg, sl = U[dt], pages[there], pos[there] % page
+
+    def near(a, want):
+        assert bool(((a.double() - want).abs() <= u * want.abs() + 2.0 ** -20 * want.abs().amax(-1, keepdim=True) + 2.0 ** -25).all())
+
+    near(got[there], turned(q, qg, tab, pos, 1e-6)[there])
+    near(k[pg, sl], turned(kn, kg, tab, pos, 1e-6)[there])
+    near(v[pg, sl], vn.double()[there])
+    touched = torch.zeros(k.shape[:2], dtype=torch.bool, device="cuda")
+    touched[pg, sl] = True
+    assert torch.equal(k[~touched], k0[~touched]) and torch.equal(v[~touched], v0[~touched])
+
+
 # ------------------------------------------------------------------ decode
 DECODE = [  # lens, heads, kv, hd, page, cache, hnd
     ([1], 16, 8, 128, 16, "f16", False),
