@@ -28,7 +28,7 @@
 // the FMA pipe); a pair takes ~2600, and long prompts run at the board's power
 // limit.  Measured with 32 query and 8 kv heads of 128, bf16: 8192 tokens 465-500
 // us (1.1-1.18 PFLOP/s), 512 tokens 12.1 us, 16 sequences of ~734 tokens after 256
-// cached ones 147-170 us; the end of a unit costs 3 k clocks (O is read, scaled
+// cached ones 147-177 us; the end of a unit costs 3 k clocks (O is read, scaled
 // and stored), a first or a masked key tile 1 k more than another.
 #include <cuda_runtime.h>
 
