@@ -421,8 +421,9 @@ RPGC_API int rpgc_paged_append(const rpgc_paged_kv* kv, const rpgc_paged_batch* 
  * scale finite and > 0.  A sequence with no position to see gets zeros.
  * Sequences are split over their length as far as the GPU has room: workspace holds
  * the partial results (rpgc_paged_decode_workspace bytes, 16-byte aligned, filled
- * with zeros before its first use; every call leaves it ready for the next).
- * Calls that share a workspace must be ordered. */
+ * with zeros before its first use; every call leaves it ready for the next, of any
+ * batch, head count, head size or type that it is large enough for).  Calls that
+ * share a workspace must be ordered. */
 RPGC_API int64_t rpgc_paged_decode_workspace(const rpgc_paged_kv* kv, int32_t n_seqs, int32_t n_heads);
 RPGC_API int rpgc_paged_attention_decode(const rpgc_paged_kv* kv, const rpgc_paged_batch* b, const void* q,
                                          const int64_t* q_stride, int32_t n_heads, float scale, void* out,

@@ -65,7 +65,7 @@ struct DShape {
 
 struct DecodeParams {
   PagedAttnArgs a;
-  uint32_t* counters;  // [n_seqs * n_kv] pieces of an item that are done
+  uint32_t* counters;  // [CTAs] pieces that are done of the shared item that begins in a CTA's range
   float* part;         // [2 * CTAs][G][HD] partial sums
   float* part_ml;      // [2 * CTAs][G][2] their reference and weight
   int32_t G;
@@ -513,7 +513,8 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, DShape<HD, NT>::kCta
       bar_consumers<kWarps * 32>();
       if (tid == 0) {
         __threadfence();  // (of all the warps' partial results: they are before this by the barrier)
-        *last = atomicInc(p.counters + (int64_t)w.seq * a.kv.n_kv + w.kh, (uint32_t)(b1 - b0)) == (uint32_t)(b1 - b0);
+        // (only the last item of a range goes on past it: one counter per CTA, back at 0 after the join)
+        *last = atomicInc(p.counters + b0, (uint32_t)(b1 - b0)) == (uint32_t)(b1 - b0);
         __threadfence();
       }
       bar_consumers<kWarps * 32>();
@@ -572,7 +573,10 @@ int device_sms() {
   return sm_count(dev);
 }
 
-int64_t counter_bytes(const PagedView& kv, int32_t n_seqs) { return ((int64_t)n_seqs * kv.n_kv * 4 + 255) / 256 * 256; }
+// The workspace: counters, one per CTA (two CTAs an SM at most), then the partial
+// results.  The counters alone have to be zero when a call begins, so they lie
+// where no call of any shape puts anything else.
+int64_t counter_bytes() { return ((int64_t)2 * device_sms() * 4 + 255) / 256 * 256; }
 
 // As many CTAs as run at once, and no more than the join's table has room for.
 template <int HD, int NT>
@@ -591,7 +595,7 @@ cudaError_t decode_go(const PagedAttnArgs& a, cudaStream_t s) {
   p.box = (1 << a.kv.page_shift) < DShape<HD, NT>::kTile ? 1 << a.kv.page_shift : DShape<HD, NT>::kTile;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.counters = reinterpret_cast<uint32_t*>(ws);
-  p.part = reinterpret_cast<float*>(ws + counter_bytes(a.kv, a.b.n_seqs));
+  p.part = reinterpret_cast<float*>(ws + counter_bytes());
   p.part_ml = p.part + (int64_t)2 * ctas * p.G * HD;
   CUtensorMap mk, mv;
   const CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
@@ -618,9 +622,9 @@ cudaError_t decode_heads(const PagedAttnArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-int64_t paged_decode_workspace(const PagedView& kv, int32_t n_seqs, int32_t n_heads) {
-  const int64_t rows = (int64_t)2 * 2 * device_sms() * (n_heads / kv.n_kv);  // (two CTAs an SM at most, two items each)
-  return counter_bytes(kv, n_seqs) + rows * (kv.hd + 2) * 4;
+int64_t paged_decode_workspace(const PagedView& kv, int32_t n_heads) {
+  const int64_t rows = (int64_t)2 * 2 * device_sms() * (n_heads / kv.n_kv);  // (two items of each CTA)
+  return counter_bytes() + rows * (kv.hd + 2) * 4;
 }
 
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s) {

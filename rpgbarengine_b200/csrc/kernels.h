@@ -377,7 +377,7 @@ struct PagedAttnArgs {
   void* workspace;
 };
 cudaError_t paged_append_launch(const PagedAppendArgs& a, cudaStream_t s);
-int64_t paged_decode_workspace(const PagedView& kv, int32_t n_seqs, int32_t n_heads);
+int64_t paged_decode_workspace(const PagedView& kv, int32_t n_heads);
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s);
 cudaError_t prompt_attn_launch(const PagedAttnArgs& a, cudaStream_t s);
 

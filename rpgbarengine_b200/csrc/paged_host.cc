@@ -226,7 +226,7 @@ int64_t rpgc_paged_decode_workspace(const rpgc_paged_kv* kv, int32_t n_seqs, int
     const PagedView v = view_of(kv);
     need_counts(n_seqs, 0);
     need_heads(n_heads, v.n_kv, v.hd);
-    return rpgc::paged_decode_workspace(v, n_seqs, n_heads);
+    return rpgc::paged_decode_workspace(v, n_heads);
   });
 }
 
@@ -238,7 +238,7 @@ int rpgc_paged_attention_decode(const rpgc_paged_kv* kv, const rpgc_paged_batch*
     if (a.b.cu) fail(RPGC_E_ARG, "decode takes one new token per sequence: cu_q must be NULL");
     if (!a.b.n_seqs) return RPGC_OK;
     need_ptr(workspace, "workspace");
-    const int64_t need = rpgc::paged_decode_workspace(a.kv, a.b.n_seqs, n_heads);
+    const int64_t need = rpgc::paged_decode_workspace(a.kv, n_heads);
     if (workspace_bytes < need)
       fail(RPGC_E_ARG, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes, (long long)need);
     a.workspace = workspace;
