@@ -384,7 +384,7 @@ typedef struct rpgc_paged_kv {
 } rpgc_paged_kv;
 
 typedef struct rpgc_paged_batch {
-  const int32_t* block_table; /* [n_seqs] rows of max_pages ids, table_stride apart */
+  const int32_t* block_table; /* [n_seqs] rows of max_pages ids, table_stride apart (0: one row for all) */
   int64_t table_stride;
   int32_t max_pages;
   int32_t n_seqs;

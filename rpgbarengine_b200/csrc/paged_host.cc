@@ -122,8 +122,9 @@ PagedSeqs seqs_of(const rpgc_paged_batch* b) {
   if (!b) fail(RPGC_E_ARG, "batch is NULL");
   need_counts(b->n_seqs, b->n_tokens);
   if (b->max_pages <= 0 || b->max_pages > (1 << 26)) fail(RPGC_E_ARG, "max_pages %d out of range", b->max_pages);
-  if (b->table_stride < b->max_pages || b->table_stride > (int64_t(1) << 40))
-    fail(RPGC_E_ARG, "table_stride %lld must be at least max_pages %d", (long long)b->table_stride, b->max_pages);
+  // (0: one row that all sequences share; the kernels only read the table)
+  if ((b->table_stride && b->table_stride < b->max_pages) || b->table_stride > (int64_t(1) << 40))
+    fail(RPGC_E_ARG, "table_stride %lld must be 0 or at least max_pages %d", (long long)b->table_stride, b->max_pages);
   if (b->n_seqs > 0 && (!b->block_table || !b->kv_lens)) fail(RPGC_E_ARG, "block_table or kv_lens is NULL");
   if (!b->cu_q && b->n_tokens != b->n_seqs)
     fail(RPGC_E_ARG, "without cu_q there is one token per sequence: n_tokens %lld, n_seqs %d", (long long)b->n_tokens, b->n_seqs);

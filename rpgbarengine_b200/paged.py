@@ -146,7 +146,7 @@ class PagedKV:
 
 class PagedBatch:
     """The sequences of a call.  block_table: int32 [n_seqs, max_pages] page
-    ids; kv_lens: int32 [n_seqs] cache lengths, the call's new tokens included;
+    ids (one row expanded to n_seqs: all sequences over the same pages); kv_lens: int32 [n_seqs] cache lengths, the call's new tokens included;
     cu_q: int32 [n_seqs + 1], sequence s's new tokens are rows
     [cu_q[s], cu_q[s+1]) of n_tokens (None: one new token per sequence).  All on
     the device, and read there at each call, so a decode loop updates them in
@@ -159,7 +159,10 @@ class PagedBatch:
         _ints(block_table, "block_table", 2)
         _ints(kv_lens, "kv_lens", 1)
         n = kv_lens.shape[0]
-        _need(block_table.shape[0] == n and block_table.stride(1) == 1, "block_table needs one contiguous row per sequence")
+        width = block_table.shape[1]
+        stride = block_table.stride(0) if n > 1 else width  # (one row has no stride to speak of)
+        _need(block_table.shape[0] == n and (block_table.stride(1) == 1 or width < 2), "block_table needs one contiguous row per sequence")
+        _need(stride == 0 or stride >= width, "block_table's rows overlap: they must be apart, or one row expanded to all sequences")
         _need(kv_lens.stride(0) == 1 or n < 2, "kv_lens must be contiguous")
         if cu_q is not None:
             _ints(cu_q, "cu_q", 1)
@@ -172,8 +175,7 @@ class PagedBatch:
         _need(all(t is None or t.get_device() == self.index for t in self.keep), "the batch's tensors must be on one device")
         self.n_seqs, self.n_tokens = n, n if n_tokens is None else int(n_tokens)
         p = [None if t is None else t.data_ptr() for t in self.keep]
-        self.c = _Batch(p[0], max(block_table.stride(0), block_table.shape[1]), block_table.shape[1], n, p[1], p[2],
-                        self.n_tokens, p[3])
+        self.c = _Batch(p[0], stride, width, n, p[1], p[2], self.n_tokens, p[3])
         self.ref = C.byref(self.c)
         self._ws = {}
 

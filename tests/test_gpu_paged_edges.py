@@ -9,7 +9,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import rpgbarengine_b200 as rb  # noqa: E402
-from test_gpu_paged import check_decode, decode_case, i32  # noqa: E402
+from test_gpu_paged import append_inputs, check_decode, check_paged, decode_case, gen, i32, make_pool, randn  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -53,3 +53,26 @@ def test_one_workspace_serves_calls_of_every_shape():
                                                ws.data_ptr(), size, stream)
             assert rc == rb.OK
             assert torch.equal(out, want), i
+
+
+# ------------------------------------------------------------ block tables
+def test_one_row_of_pages_expanded_to_all_sequences():
+    # sequences of different lengths over the same pages, named once
+    page, H, kv, hd = 32, 8, 2, 128
+    lens, new = [300, 17, 299, 64], [40, 17, 1, 30]
+    g = gen(23)
+    k, v, table = make_pool(g, [300], page, kv, hd, torch.bfloat16)
+    shared, n = i32(table).expand(4, -1), sum(new)
+    q = randn(g, n, H, hd, dtype=torch.bfloat16)
+    cache, cu = rb.PagedKV(k, v), i32([0, 40, 57, 58, 88])
+    check_paged(rb.paged_attention_prompt(cache, rb.PagedBatch(shared, i32(lens), cu, n), q), q, k, v, table * 4, new, lens, hd ** -0.5)
+    check_decode(rb.paged_attention_decode(cache, rb.PagedBatch(shared, i32(lens)), q[:4]), q[:4], k, v, table * 4, lens, hd ** -0.5)
+    # append: sequences that end at different positions of the pages
+    qn, kn, vn = append_inputs(g, 4, H, kv, hd, "bf16", False)
+    k0, v0 = k.clone(), v.clone()
+    assert torch.equal(rb.paged_append(cache, rb.PagedBatch(shared, i32(lens)), qn, kn, vn), qn)
+    for i, m in enumerate(lens):
+        at = table[0][(m - 1) // page], (m - 1) % page
+        assert torch.equal(k[at], kn[i]) and torch.equal(v[at], vn[i])
+        k0[at], v0[at] = kn[i], vn[i]
+    assert torch.equal(k, k0) and torch.equal(v, v0)
