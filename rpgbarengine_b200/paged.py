@@ -9,14 +9,15 @@
   rope_table               the cosine and sine rows paged_append reads
 
 Lengths, tables and page ids live on the device and are read there when the
-call runs: nothing here waits for the GPU, and all calls can be captured.
+call runs: nothing here waits for the GPU, and all calls can be captured
+(decode's once its batch has a workspace, which an earlier call makes).
 """
 from __future__ import annotations
 
 import ctypes as C
 import math
 
-from . import BF16, E_ARG, F16, F32, RpgcError, _check, lib
+from . import BF16, E_ARG, E_STATE, F16, F32, RpgcError, _check, lib
 
 DROPPED, TIMEOUT = 1, 2  # PagedBatch.status bits
 
@@ -151,9 +152,13 @@ class PagedBatch:
     [cu_q[s], cu_q[s+1]) of n_tokens (None: one new token per sequence).  All on
     the device, and read there at each call, so a decode loop updates them in
     place and keeps the batch.  status: optional int32 tensor of one word that
-    receives DROPPED / TIMEOUT bits.  The batch also holds decode's workspace
-    (made at its first decode call, which is therefore not a captured one):
-    calls on one batch are made in stream order."""
+    receives DROPPED / TIMEOUT bits.
+
+    The batch also holds decode's workspaces, one for each stream that it is
+    used on, made by the first call there.  A captured call uses one that is
+    there already (of a call outside the graph), so the batch is kept until the
+    graph's last replay has ended, and replays are ordered with each other and with
+    other calls on that stream."""
 
     def __init__(self, block_table, kv_lens, cu_q=None, n_tokens=None, status=None):
         _ints(block_table, "block_table", 2)
@@ -179,17 +184,25 @@ class PagedBatch:
         self.ref = C.byref(self.c)
         self._ws = {}
 
-    def workspace(self, cache: PagedKV, n_heads: int):
-        """Decode's workspace for this batch and head count (made once)."""
-        key = (n_heads, cache.n_kv_heads, cache.head_dim)
-        ws = self._ws.get(key)
+    def workspace(self, cache: PagedKV, n_heads: int, stream: int):
+        """Decode's workspace for this batch, head count and stream (made
+        once).  It is zeroed and used on that stream, and its memory is the
+        stream's: when the batch is dropped, what gets it next runs after the
+        calls that are still using it."""
+        shape = n_heads, cache.n_kv_heads, cache.head_dim
+        ws = self._ws.get((shape, stream))
         if ws is None:
             torch = _torch()
-            with torch.cuda.device(self.index):
+            on = torch.cuda.ExternalStream(stream, device=self.index) if stream else torch.cuda.default_stream(self.index)
+            with torch.cuda.device(self.index), torch.cuda.stream(on):
+                if torch.cuda.is_current_stream_capturing():
+                    for key, ws in self._ws.items():
+                        if key[0] == shape:
+                            return ws
+                    raise RpgcError(E_STATE, "a captured decode call needs the workspace of an earlier one on its batch: make a call outside the graph first")
                 n = _check(lib().rpgc_paged_decode_workspace(cache.ref, self.n_seqs, n_heads))
                 buf = torch.zeros(n, dtype=torch.uint8, device="cuda")
-                torch.cuda.current_stream().synchronize()  # zeroed for every stream, once
-            ws = self._ws[key] = (buf, buf.data_ptr(), n)
+            ws = self._ws[shape, stream] = (buf, buf.data_ptr(), n)
         return ws
 
 
@@ -245,7 +258,7 @@ def paged_attention_decode(cache: PagedKV, batch: PagedBatch, q, scale=None, out
     head_dim ** -0.5."""
     qs, out, made = _attend(cache, batch, q, out)
     heads = q.shape[1]
-    ws = batch.workspace(cache, heads)
+    ws = batch.workspace(cache, heads, _torch()._C._cuda_getCurrentRawStream(cache.index) if stream is None else int(stream))
     _run(lib().rpgc_paged_attention_decode, cache.index, stream, made, cache.ref, batch.ref, q.data_ptr(), qs, heads,
          cache.scale if scale is None else scale, out.data_ptr(), ws[1], ws[2])
     return out

@@ -76,3 +76,48 @@ def test_one_row_of_pages_expanded_to_all_sequences():
         assert torch.equal(k[at], kn[i]) and torch.equal(v[at], vn[i])
         k0[at], v0[at] = kn[i], vn[i]
     assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+# ---------------------------------------------------------------- streams
+def test_a_batch_dropped_while_its_call_runs():
+    # the calls run on a stream that is not current, late; their batch is gone at once and
+    # its memory asked for again: the results are right and nobody's memory is written
+    lens, H, kv, hd = [4000, 1, 700], 32, 8, 128
+    k, v, table, q = decode_case(lens, H, kv, hd, 64, "bf16", False, 6)
+    tab, ln, cache = i32(table), i32(lens), rb.PagedKV(k, v)
+    want = rb.paged_attention_decode(cache, rb.PagedBatch(tab, ln), q)
+    size = rb.lib().rpgc_paged_decode_workspace(cache.ref, len(lens), H)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for how in ("argument", "current", "second stream"):
+        batch = rb.PagedBatch(tab, ln)
+        if how == "second stream":
+            rb.paged_attention_decode(cache, batch, q)
+            torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(50_000_000)
+            if how == "current":
+                got = rb.paged_attention_decode(cache, batch, q)
+        if how != "current":
+            got = rb.paged_attention_decode(cache, batch, q, stream=side.cuda_stream)
+        del batch
+        mine = [torch.full((size,), 0xA5, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), how
+        assert all(bool((m == 0xA5).all()) for m in mine), how
+
+
+def test_one_batch_on_two_streams_at_once():
+    lens, H, kv, hd = [3000 + i for i in range(6)], 32, 8, 128
+    k, v, table, q = decode_case(lens, H, kv, hd, 64, "bf16", False, 7)
+    cache, batch = rb.PagedKV(k, v), rb.PagedBatch(i32(table), i32(lens))
+    want = rb.paged_attention_decode(cache, batch, q)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got += [rb.paged_attention_decode(cache, batch, q) for _ in range(5)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x in got)

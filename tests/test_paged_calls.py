@@ -71,3 +71,109 @@ def test_the_entry_point_takes_a_row_that_all_sequences_share():
         b = paged._Batch(p, stride, 4, 2, p, None, 2, None)
         rc = rb.lib().rpgc_paged_attention_decode(C.byref(kv), C.byref(b), p, paged._S2(1024, 128), 16, 0.0, p, p, 1 << 40, None)
         assert rc == rb.E_ARG and word in rb.lib().rpgc_last_error().decode()
+
+
+# ------------------------------------------------------------ streams
+class Recorder:
+    """torch and the library as paged.py uses them around a decode call: which stream is
+    current when memory is made, which memory and stream each launch gets."""
+    uint8, int32 = torch.uint8, torch.int32
+
+    def __init__(self):
+        self.current, self.capturing, self.made, self.launches, outer = 0, set(), {}, [], self
+
+        class Stream:
+            def __init__(self, handle):
+                self.cuda_stream = handle
+
+        class On:
+            def __init__(self, stream):
+                self.new = stream.cuda_stream
+
+            def __enter__(self):
+                self.old, outer.current = outer.current, self.new
+
+            def __exit__(self, *_):
+                outer.current = self.old
+
+        class Nothing:
+            def __init__(self, *_):
+                pass
+
+            __enter__ = __exit__ = lambda *_: None
+
+        class Cuda:
+            device, stream = Nothing, On
+            ExternalStream = staticmethod(lambda handle, device=None: Stream(handle))
+            default_stream = staticmethod(lambda device=None: Stream(0))
+            current_stream = staticmethod(lambda device=None: Waits(outer.current))
+            is_current_stream_capturing = staticmethod(lambda: outer.current in outer.capturing)
+
+        class Waits(Stream):
+            def synchronize(self):
+                assert self.cuda_stream not in outer.capturing, "waits inside a capture"
+
+        class Raw:
+            _cuda_getDevice = staticmethod(lambda: 0)
+            _cuda_getCurrentRawStream = staticmethod(lambda index: outer.current)
+
+        self.cuda, self._C, self.On, self.Stream = Cuda, Raw, On, Stream
+
+    def zeros(self, n, **_):
+        t = torch.zeros(n, dtype=torch.uint8)
+        self.made[t.data_ptr()] = (self.current, t)
+        return t
+
+    def rpgc_paged_decode_workspace(self, kv, n_seqs, n_heads):
+        return 64 * n_heads
+
+    def rpgc_paged_attention_decode(self, kv, b, q, st, heads, scale, out, ws, ws_bytes, stream):
+        assert ws_bytes == 64 * heads
+        self.launches.append((ws, stream))
+        return 0
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    r = Recorder()
+    monkeypatch.setattr(paged, "_torch", lambda: r)
+    monkeypatch.setattr(paged, "lib", lambda: r)
+    return r
+
+
+def decode_inputs():
+    class Cache:
+        dtype, index, n_kv_heads, head_dim, scale, ref = torch.bfloat16, 0, 2, 64, 0.125, None
+
+    q = Dev(torch.zeros(3, 4, 64, dtype=torch.bfloat16))
+    out = Dev(torch.zeros(3, 4, 64, dtype=torch.bfloat16))
+    return Cache, rb.PagedBatch(ints([[0, 1]] * 3), ints([5] * 3)), q, out
+
+
+def test_a_workspace_is_used_on_the_stream_that_owns_its_memory_alone(recorder):
+    # memory goes back to the stream that it was made on when the batch is dropped: a call
+    # still running on another would share it with whatever the allocator puts there
+    cache, batch, q, out = decode_inputs()
+    rb.paged_attention_decode(cache, batch, q, out=out)
+    rb.paged_attention_decode(cache, batch, q, out=out, stream=0x50)
+    with recorder.On(recorder.Stream(0x70)):
+        rb.paged_attention_decode(cache, batch, q, out=out)
+        rb.paged_attention_decode(cache, batch, q, out=out, stream=0)
+    rb.paged_attention_decode(cache, batch, q, out=out)
+    assert [s for _, s in recorder.launches] == [0, 0x50, 0x70, 0, 0]
+    for ws, stream in recorder.launches:
+        assert recorder.made[ws][0] == stream
+    assert len(recorder.made) == 3  # (made once per stream)
+
+
+def test_a_captured_call_uses_a_workspace_that_is_there(recorder):
+    cache, batch, q, out = decode_inputs()
+    recorder.capturing.add(0x90)
+    with recorder.On(recorder.Stream(0x90)):
+        with pytest.raises(rb.RpgcError) as e:  # nothing is made or waited for inside a capture
+            rb.paged_attention_decode(cache, batch, q, out=out)
+    assert e.value.code == rb.E_STATE and not recorder.made and not recorder.launches
+    rb.paged_attention_decode(cache, batch, q, out=out)
+    with recorder.On(recorder.Stream(0x90)):
+        rb.paged_attention_decode(cache, batch, q, out=out)
+    assert recorder.launches[1] == (recorder.launches[0][0], 0x90) and len(recorder.made) == 1
