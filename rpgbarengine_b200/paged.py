@@ -104,6 +104,12 @@ def _on(index, stream):
     return c._cuda_getCurrentRawStream(index) if stream is None else int(stream)
 
 
+def _stream_at(index, handle):
+    """The stream of a handle (torch makes a new one of handle 0, which is the default stream)."""
+    cuda = _torch().cuda
+    return cuda.ExternalStream(handle, device=index) if handle else cuda.default_stream(index)
+
+
 def _run(fn, index, stream, made, *args):
     """fn(*args, stream) with device `index` current.  `made`: a result allocated
     here, whose memory must outlive its use on a stream that is not the current one."""
@@ -115,7 +121,7 @@ def _run(fn, index, stream, made, *args):
     if rc < 0:
         _check(rc)
     if made is not None and stream is not None:
-        made.record_stream(_torch().cuda.ExternalStream(ptr, device=made.device))
+        made.record_stream(_stream_at(index, ptr))
 
 
 class PagedKV:
@@ -193,8 +199,7 @@ class PagedBatch:
         ws = self._ws.get((shape, stream))
         if ws is None:
             torch = _torch()
-            on = torch.cuda.ExternalStream(stream, device=self.index) if stream else torch.cuda.default_stream(self.index)
-            with torch.cuda.device(self.index), torch.cuda.stream(on):
+            with torch.cuda.device(self.index), torch.cuda.stream(_stream_at(self.index, stream)):
                 if torch.cuda.is_current_stream_capturing():
                     for key, ws in self._ws.items():
                         if key[0] == shape:

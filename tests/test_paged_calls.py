@@ -177,3 +177,18 @@ def test_a_captured_call_uses_a_workspace_that_is_there(recorder):
     with recorder.On(recorder.Stream(0x90)):
         rb.paged_attention_decode(cache, batch, q, out=out)
     assert recorder.launches[1] == (recorder.launches[0][0], 0x90) and len(recorder.made) == 1
+
+
+@pytest.mark.parametrize("handle", [0, 0x50])
+def test_a_result_outlives_its_use_on_the_stream_that_was_asked_for(recorder, monkeypatch, handle):
+    # made on the current stream, written on another, the default one (handle 0) among them
+    cache, batch, q, out = decode_inputs()
+    recorded = []
+    out.record_stream, out.device = lambda s: recorded.append(s.cuda_stream), "cuda:0"
+    pool = iter(range(0x1000, 0x2000))
+    monkeypatch.setattr(recorder.cuda, "ExternalStream",  # (as torch has it: no handle, a stream of the pool)
+                        staticmethod(lambda handle, device=None: recorder.Stream(handle or next(pool))))
+    monkeypatch.setattr(paged, "_new", lambda like, dtype=None: out)
+    with recorder.On(recorder.Stream(0x70)):
+        rb.paged_attention_decode(cache, batch, q, stream=handle)
+    assert recorder.launches[-1][1] == handle and recorded == [handle]
