@@ -103,6 +103,11 @@ RPGC_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+RPGC_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 RPGC_DEV uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -124,15 +129,18 @@ RPGC_DEV float max_nan(float a, float b, float c) {
 // 2^y of two values on the FMA pipe, for part of a row's probabilities: the
 // special-function unit gives 16 exponentials per clock and SM, half of what the
 // MMAs of the same tile would need.  y = n + f with n the nearest integer (added
-// and taken off 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial fitted to it
+// to and taken off 1.5 * 2^23 + 127), 2^f on [-1/2, 1/2] by a polynomial fitted to it
 // for the smallest relative error (7.5e-5 for degree 3, 2.7e-6 for degree 4,
-// against 2^-9 and 2^-12 of the 16-bit rounding that follows), n added to the exponent.
-// Below 2^-126 the result stays there; NaN is not carried (see `m`).
+// against 2^-9 and 2^-12 of the 16-bit rounding that follows), times 2^n: the sum's
+// last bits are n + 127, moved up they are the bits of 2^n.  For n = -127, where y
+// stops, those of 0: -inf, the score of a key that the row does not see, has to give
+// a weight of 0 (2^-126, which bf16 holds, times a value near its largest is 4).
+// NaN is not carried (see `m`).
 template <bool BF>
 RPGC_DEV float2 exp2_poly(uint64_t y) {
-  constexpr float kMagic = 12582912.0f;
+  constexpr float kMagic = 12582912.0f + 127.0f;
   const float2 v = unpair(y);
-  const uint64_t x = pair(fminf(max_nan(v.x, -126.0f), 127.0f), fminf(max_nan(v.y, -126.0f), 127.0f));
+  const uint64_t x = pair(fminf(max_nan(v.x, -127.0f), 127.0f), fminf(max_nan(v.y, -127.0f), 127.0f));
   const uint64_t t = add2(x, pair(kMagic, kMagic));
   const uint64_t f = fma2(add2(t, pair(-kMagic, -kMagic)), pair(-1.0f, -1.0f), x);
   uint64_t r;
@@ -146,9 +154,8 @@ RPGC_DEV float2 exp2_poly(uint64_t y) {
     r = fma2(r, f, pair(0.693121791f, 0.693121791f));
     r = fma2(r, f, pair(0.999999285f, 0.999999285f));
   }
-  const float2 a = unpair(t), b = unpair(r);
-  return make_float2(__uint_as_float(__float_as_uint(b.x) + (__float_as_uint(a.x) << 23)),
-                     __uint_as_float(__float_as_uint(b.y) + (__float_as_uint(a.y) << 23)));
+  const float2 a = unpair(t);
+  return unpair(mul2(r, pair(__uint_as_float(__float_as_uint(a.x) << 23), __uint_as_float(__float_as_uint(a.y) << 23))));
 }
 // V as the B operand of O += P V: rows are keys (the MMA's K), the 64 values
 // of a panel row are N.  128-byte swizzle; 1024 B between groups of 8 keys,

@@ -9,7 +9,8 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import rpgbarengine_b200 as rb  # noqa: E402
-from test_gpu_paged import append_inputs, check_decode, check_paged, decode_case, gen, i32, make_pool, randn  # noqa: E402
+from test_gpu_paged import (DT, append_inputs, check_decode, check_packed, check_paged, decode_case, gen, i32, make_pool,  # noqa: E402
+                            packed_inputs, randn)
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -121,3 +122,48 @@ def test_one_batch_on_two_streams_at_once():
                 got += [rb.paged_attention_decode(cache, batch, q) for _ in range(5)]
         torch.cuda.synchronize()
         assert all(torch.equal(x, want) for x in got)
+
+
+# ------------------------------------- values that a row does not see
+HUGE = {"bf16": 3.0e38, "f16": 65504.0}  # finite, so that only a weight of zero keeps them out
+
+
+@pytest.mark.parametrize("lens,H,kv,hd", [([430, 70], 8, 2, 128), ([1500, 300], 32, 8, 128), ([430, 70], 12, 4, 64)])
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+def test_large_values_of_later_positions_do_not_leak_into_prompts(lens, H, kv, hd, ty):
+    g = gen(sum(lens))
+    n, at = sum(lens), 300
+    q, k, v = packed_inputs(g, n, H, kv, hd, DT[ty], False)
+    cu = i32([0, lens[0], n])
+    want = rb.attention_prompt(q, k, v, cu)
+    check_packed(want, q, k, v, lens, hd ** -0.5)
+    for sign in (1, -1):
+        v2 = v.clone()
+        v2[at:] = sign * HUGE[ty]
+        assert torch.equal(rb.attention_prompt(q, k, v2, cu)[:at], want[:at])
+
+
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+def test_large_values_past_the_end_do_not_leak_over_pages(ty):
+    # later tokens of the prompt, and slots that no sequence holds
+    page, H, kv, hd = 32, 8, 2, 128
+    g = gen(17)
+    lens, new, at = [500, 77], [200, 77], 120  # rows [0, at) see positions below 420
+    k, v, table = make_pool(g, lens, page, kv, hd, DT[ty])
+    q = randn(g, sum(new), H, hd, dtype=DT[ty])
+    cache = rb.PagedKV(k, v)
+    batch = rb.PagedBatch(i32(table), i32(lens), i32([0, 200, 277]), 277)
+    one = rb.PagedBatch(i32(table), i32(lens))
+    want, want1 = rb.paged_attention_prompt(cache, batch, q), rb.paged_attention_decode(cache, one, q[:2])
+    used = torch.zeros(k.shape[:2], dtype=torch.bool, device="cuda")
+    for s, n in enumerate(lens):
+        for j, p in enumerate(table[s]):
+            if p >= 0:
+                used[p, : max(0, min(page, n - j * page))] = True
+    for sign in (1, -1):
+        k[~used], v[~used] = sign * HUGE[ty], sign * HUGE[ty]
+        assert torch.equal(rb.paged_attention_prompt(cache, batch, q), want)
+        assert torch.equal(rb.paged_attention_decode(cache, one, q[:2]), want1)
+    for p in range(420, 500):
+        v[table[0][p // page], p % page] = HUGE[ty]
+    assert torch.equal(rb.paged_attention_prompt(cache, batch, q)[:at], want[:at])
