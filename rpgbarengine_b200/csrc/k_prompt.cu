@@ -648,7 +648,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         // made, summed and kept in 16 bits while S stays where it is.  Only where a row
         // has no reference yet, or its sum shows that the scores have outgrown it
         // (or hold NaN: the comparison fails), the row's maximum is looked for
-        // first: m becomes it, O and l follow, and the pass is done again.
+        // first: m becomes it, O and l follow, and the pass is done again.  The other
+        // rows of the warp keep theirs, so that what they give does not
+        // depend on scores that they do not see.
         if (j >= whole || gone) {
           // scores that the row does not see become -inf where they lie, so that
           // the pass itself has no branches (they made every tile 200 clocks longer)
@@ -673,11 +675,11 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         }
         uint32_t w[64];
         float tile_sum;
-        bool look = __any_sync(0xffffffffu, m == -INFINITY);
+        bool due = m == -INFINITY;  // this row's maximum has to be looked for
 #pragma unroll 1
-        for (;;) {
+        for (int pass = 0;; ++pass) {
           uint32_t x[2][32];
-          if (look) {
+          if (__any_sync(0xffffffffu, due)) {
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
@@ -688,8 +690,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
                 mx[(i >> 1) & 3] = max_nan(mx[(i >> 1) & 3], __uint_as_float(x[0][i]), __uint_as_float(x[0][i + 1]));
             }
             const float top = max_nan(max_nan(mx[0], mx[1]), mx[2], mx[3]) * c;
-            const float mn = max_nan(m, top);
-            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - mn);
+            const float mn = due ? max_nan(m, top) : m;
+            const float f = !due ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - mn);
             if (j > j0) {  // O's row: the last P V was done before this S
               l *= f;
 #pragma unroll 1
@@ -729,8 +731,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
           const float2 u = unpair(add2(sum[0], sum[1]));
           tile_sum = u.x + u.y;
           // (rows that see nothing have no say: their queries may be anything)
-          if (look || !__any_sync(0xffffffffu, lim > 0 && !(tile_sum <= kMost))) break;
-          look = true;
+          // (the second pass settles every row: those without a reference had theirs in the first)
+          due = lim > 0 && !(tile_sum <= kMost);
+          if (pass || !__any_sync(0xffffffffu, due)) break;
         }
         l += tile_sum;
 #pragma unroll

@@ -167,3 +167,23 @@ def test_large_values_past_the_end_do_not_leak_over_pages(ty):
     for p in range(420, 500):
         v[table[0][p // page], p % page] = HUGE[ty]
     assert torch.equal(rb.paged_attention_prompt(cache, batch, q)[:at], want[:at])
+
+
+@pytest.mark.parametrize("lens,H,kv,hd", [([430, 70], 8, 2, 128), ([1500, 300], 32, 8, 128), ([430, 70], 12, 4, 64)])
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+def test_large_keys_of_later_positions_change_nothing_before_them(lens, H, kv, hd, ty):
+    # rows that see them outgrow their references by far; the rows beside them keep
+    # theirs, and with them every bit
+    g = gen(sum(lens))
+    n, at = sum(lens), 300
+    q, k, v = packed_inputs(g, n, H, kv, hd, DT[ty], False)
+    cu = i32([0, lens[0], n])
+    want = rb.attention_prompt(q, k, v, cu)
+    for big in (HUGE[ty], -HUGE[ty], 300.0):
+        k2 = k.clone()
+        k2[at:] = big
+        assert torch.equal(rb.attention_prompt(q, k2, v, cu)[:at], want[:at])
+    # queries of other rows: each row's result is its own
+    q2 = q.clone()
+    q2[1::2] *= 64
+    assert torch.equal(rb.attention_prompt(q2, k, v, cu)[::2], want[::2])
