@@ -19,7 +19,11 @@
 // 2.8 TB/s); 4 warps take 16 keys each of every tile: S^T = K Q^T (m16n8k16, the
 // kv head's query heads are the N side), P^T turned from the accumulator layout
 // into an operand by movmatrix, O^T += V^T P^T.  (mma.sync: at 4 to 16 rows a
-// head group has nothing for wider MMAs.)  The warps' sums meet in shared memory
+// head group has nothing for wider MMAs.)  A row that comes out infinite or NaN
+// though its weights are finite is computed again by one warp in fp32 (attn_row):
+// a weight's second 16-bit value may be 0 or negative, and that times a visible
+// infinity is not the infinity that the row should have; and weights of up to
+// 2^40 may overflow with values that the true weights, at most 1, do not.  The warps' sums meet in shared memory
 // at an item's end.  Two such CTAs on an SM, 192 KB in flight between them: while
 // one ends an item or looks for the next, the other's tiles go on (one CTA of 8
 // warps took 1.5 times as long on 128 sequences of 20 positions, 1.08 times on
@@ -61,6 +65,7 @@ struct DShape {
   // what an SM has, less a kilobyte for each CTA, goes to the ring
   static constexpr int kStages = ((233472 / kCtas - 1024) - kRest) / kStage;
   static constexpr int kSmem = kStages * kStage + kRest;
+  static_assert(kStages * 20 + 12 <= 256, "barriers and flags");
 };
 
 struct DecodeParams {
@@ -226,6 +231,7 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, DShape<HD, NT>::kCta
   uint32_t* there = reinterpret_cast<uint32_t*>(empty + kStages);  // [kStages] groups of 16 keys that are there
   volatile int32_t* gave_up = reinterpret_cast<volatile int32_t*>(there + kStages);
   int32_t* last = const_cast<int32_t*>(gave_up) + 1;
+  uint32_t* again = reinterpret_cast<uint32_t*>(last + 1);  // heads of the item to be computed again
   const PagedAttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -234,6 +240,7 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, DShape<HD, NT>::kCta
       mbar_init(empty + i, kWarps);
     }
     *gave_up = 0;
+    *again = 0;
     fence_barrier_init();
   }
   if (warp == kWarps && lane < 2) prefetch_map(lane ? &tm_v : &tm_k);
@@ -318,6 +325,13 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, DShape<HD, NT>::kCta
   const int vrow = 16 * warp + mr + 8 * (mi >> 1), vc = mi & 1;
   int st = 0;
   uint32_t ph = 0;
+  auto put = [&](int h, int d, const float4& acc, float L) {  // four values of the item's row of head h
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    uint16_t* op = static_cast<uint16_t*>(a.out) + ((int64_t)w.seq * a.n_heads + w.kh * G + h) * HD + d;
+    *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv));
+    const float z = fmaf(acc.x, 0.0f, fmaf(acc.y, 0.0f, fmaf(acc.z, 0.0f, acc.w * 0.0f)));  // NaN: not all finite
+    if (__builtin_expect(z != 0.0f && L < INFINITY, 0)) atomicOr(again, 1u << h);
+  };
   do {
     const int t0 = w.t0, t1 = w.t1;
     if (t1 <= t0) continue;
@@ -499,9 +513,7 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, DShape<HD, NT>::kCta
         L += f * wl[k * kHeads + h];
       }
       if (whole) {
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        uint16_t* op = static_cast<uint16_t*>(a.out) + ((int64_t)w.seq * a.n_heads + w.kh * G + h) * HD + d;
-        *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv));
+        put(h, d, acc, L);
       } else {
         __stcg(reinterpret_cast<float4*>(p.part + ((int64_t)slot * G + h) * HD + d), acc);
         if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml) + (int64_t)slot * G + h, make_float2(M, L));
@@ -557,13 +569,19 @@ __global__ void __launch_bounds__(DShape<HD, NT>::kThreads, DShape<HD, NT>::kCta
               L += f * x.y;
             }
           }
-          const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-          uint16_t* op = static_cast<uint16_t*>(a.out) + ((int64_t)w.seq * a.n_heads + w.kh * G + h) * HD + d;
-          *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv));
+          put(h, d, acc, L);
         }
       }
     }
     bar_consumers<kWarps * 32>();  // the merge buffer is free again
+    // (attn_row inlined: a kernel that calls takes 0.2 us longer to begin)
+    const uint32_t todo = *again;
+    if (__builtin_expect(todo != 0, 0)) {
+      for (int h = warp; h < G; h += kWarps)
+        if (todo >> h & 1u) attn_row<HD, BF>(a, w.seq, w.seq, w.kh * G + h, -1, lane);
+      bar_consumers<kWarps * 32>();
+      if (tid == 0) *again = 0;
+    }
   } while (w.next(a));
 }
 

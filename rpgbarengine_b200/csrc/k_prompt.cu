@@ -241,6 +241,12 @@ RPGC_DEV int32_t tiles_at_least(const PagedSeqs& b, SeqLens mine, int32_t U, int
   return __reduce_add_sync(0xffffffffu, n);
 }
 
+// (a call of its own, so that its registers are not the pass's)
+template <int HD, bool BF>
+__device__ __noinline__ void row_again(const PagedAttnArgs& a, int s, int64_t r, int h, int hf, int lane) {
+  attn_row<HD, BF>(a, s, r, h, hf, lane);
+}
+
 template <int HD, bool BF>
 __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_constant__ CUtensorMap tm_q,
                                                               const __grid_constant__ CUtensorMap tm_k,
@@ -844,7 +850,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const __grid_const
         again &= again - 1;
         const int64_t rr = __shfl_sync(0xffffffffu, row, src);
         const int hh = __shfl_sync(0xffffffffu, h, src);
-        attn_row<HD, BF>(a, seq, rr, hh, p.dual ? -1 : g, lane);
+        row_again<HD, BF>(a, seq, rr, hh, p.dual ? -1 : g, lane);
       }
     }
   }

@@ -187,3 +187,67 @@ def test_large_keys_of_later_positions_change_nothing_before_them(lens, H, kv, h
     q2 = q.clone()
     q2[1::2] *= 64
     assert torch.equal(rb.attention_prompt(q2, k, v, cu)[::2], want[::2])
+
+
+# -------------------------------------------- infinities that a row sees
+def slot(pool, table, s, p):
+    return pool[table[s][p // pool.shape[1]], p % pool.shape[1]]
+
+
+@pytest.mark.parametrize("call", ["paged_attention_decode", "paged_attention_prompt"])
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+def test_visible_infinite_values_give_infinities(ty, call):
+    # a positive weight times an infinity is that infinity, both signs make NaN;
+    # the other dims and the other kv head's rows keep their values
+    lens, H, kv, hd = [40, 3000, 5, 700], 8, 2, 128
+    k, v, table, q = decode_case(lens, H, kv, hd, 32, ty, False, 3)
+    cache, batch = rb.PagedKV(k, v), rb.PagedBatch(i32(table), i32(lens))
+    run = getattr(rb, call)
+    base, clean = run(cache, batch, q), v.clone()
+    for s, n in enumerate(lens):
+        a, b = slot(v, table, s, n // 2)[1], slot(v, table, s, n - 1)[1]
+        a[3], a[5], a[7], b[7], b[9] = float("inf"), float("-inf"), float("inf"), float("-inf"), float("nan")
+    got = run(cache, batch, q)
+    assert torch.equal(got[:, :4], base[:, :4])
+    assert bool((got[:, 4:, 3] == float("inf")).all()) and bool((got[:, 4:, 5] == float("-inf")).all())
+    assert bool(got[:, 4:, [7, 9]].isnan().all())
+    got[:, 4:, [3, 5, 7, 9]] = base[:, 4:, [3, 5, 7, 9]]
+    check_decode(got, q, k, clean, table, lens, hd ** -0.5)
+
+
+def ramp_case(scores, ty, hd=128):
+    """One sequence whose position t scores scores[t] (scale 1) for the one query head, values of one."""
+    n, page = len(scores), 64
+    pages = -(-n // page)
+    k = torch.zeros(pages, page, 1, hd, dtype=DT[ty], device="cuda")
+    k.view(-1, hd)[:n, 0] = torch.tensor(scores, device="cuda").to(DT[ty])
+    q = torch.zeros(1, 1, hd, dtype=DT[ty], device="cuda")
+    q[0, 0, 0] = 1
+    table = [list(range(pages))]
+    return k, torch.ones_like(k), table, q
+
+
+@pytest.mark.parametrize("call", ["paged_attention_decode", "paged_attention_prompt"])
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+def test_an_infinite_value_of_little_weight_still_counts(ty, call):
+    # e^-40 of the largest weight: nothing in 16 bits, but not zero
+    scores = [0.0] * 200
+    scores[150] = -40.0
+    k, v, table, q = ramp_case(scores, ty)
+    v[2, 150 - 128, 0, 6] = float("inf")
+    got = getattr(rb, call)(rb.PagedKV(k, v), rb.PagedBatch(i32(table), i32([200])), q, scale=1.0)
+    assert float(got[0, 0, 6]) == float("inf")
+    got[0, 0, 6] = 1
+    assert bool((got == 1).all())
+
+
+@pytest.mark.parametrize("call", ["paged_attention_decode", "paged_attention_prompt"])
+def test_large_values_do_not_overflow_on_the_way(call):
+    # the weights outgrow the first keys' by e^22, and the values are 1e30: their
+    # products are past fp32's range, the result is not
+    scores = ([0.0] * 128 + [22.0] * 128) * 16
+    k, v, table, q = ramp_case(scores, "bf16")
+    v *= 1e30
+    got = getattr(rb, call)(rb.PagedKV(k, v), rb.PagedBatch(i32(table), i32([4096])), q, scale=1.0)
+    want = float(v[0, 0, 0, 0])
+    assert float((got.double() - want).abs().max()) <= 2.0 ** -8 * want
