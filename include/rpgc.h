@@ -407,7 +407,9 @@ typedef struct rpgc_paged_batch {
  * n_heads * head_dim values in the cache's type; q and q_out may both be NULL.
  * Arithmetic is fp32; each output is rounded once.  Tokens whose position has
  * no page or no rope row are dropped: nothing is written to the cache, their
- * q_out rows are zeros, and RPGC_PAGED_DROPPED is set. */
+ * q_out rows are zeros, and RPGC_PAGED_DROPPED is set.  Rows that no sequence
+ * holds (cu_q may leave some out, where a captured call has a fixed n_tokens)
+ * write nothing to the cache either, and their q_out rows are zeros. */
 RPGC_API int rpgc_paged_append(const rpgc_paged_kv* kv, const rpgc_paged_batch* b, uint32_t in_type,
                                const void* q, const int64_t* q_stride, int32_t n_heads, const void* k,
                                const int64_t* k_stride, const void* v, const int64_t* v_stride,

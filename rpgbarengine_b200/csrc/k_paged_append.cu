@@ -86,7 +86,16 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
     }
   }
   const int s = seq_of_row(a.b, r, lane);
-  if (s < 0) return;
+  if (s < 0) {  // no sequence's row: zeros for q, nothing for the cache
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const int h = hl + j * kRows;
+      if (h >= a.n_heads) break;
+      uint16_t* dst = static_cast<uint16_t*>(a.q_out) + (r * a.n_heads + h) * HD + d;
+      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(dst + kHalf) = make_uint2(0u, 0u);
+    }
+    return;
+  }
   const int64_t r0 = seq_row(a.b, s), r1 = seq_row(a.b, s + 1);
   const int64_t pos = (int64_t)a.b.kv_lens[s] - (r1 - r0) + (r - r0);
   // (the two look-ups that pos leads to run beside each other)

@@ -217,7 +217,8 @@ def paged_append(cache: PagedKV, batch: PagedBatch, q, k, v, q_norm=None, k_norm
     and rotated in the cache's type (None when q is None).  q [n_tokens,
     n_heads, head_dim], k and v [n_tokens, n_kv_heads, head_dim], of one type
     (float32, float16 or bfloat16); q_norm / k_norm: fp32 gains [head_dim] or
-    None; rope: fp32 [positions, head_dim] (rope_table) or None."""
+    None; rope: fp32 [positions, head_dim] (rope_table) or None.  Rows that no
+    sequence holds are zeros in the result and write nothing to the cache."""
     torch = _torch()
     index, n, d, kv = cache.index, batch.n_tokens, cache.head_dim, cache.n_kv_heads
     _need(batch.index == index, "cache and batch are on different devices")
@@ -271,7 +272,9 @@ def paged_attention_decode(cache: PagedKV, batch: PagedBatch, q, scale=None, out
 
 def paged_attention_prompt(cache: PagedKV, batch: PagedBatch, q, scale=None, out=None, stream=None):
     """Causal attention of the batch's new tokens, q [n_tokens, n_heads,
-    head_dim], over their sequences' pages (a cached prefix included)."""
+    head_dim], over their sequences' pages (a cached prefix included).  Rows
+    that no sequence holds are not written: in a result made here they hold
+    anything."""
     qs, out, made = _attend(cache, batch, q, out)
     _run(lib().rpgc_paged_attention_prompt, cache.index, stream, made, cache.ref, batch.ref, q.data_ptr(), qs, q.shape[1],
          cache.scale if scale is None else scale, out.data_ptr())
@@ -281,7 +284,8 @@ def paged_attention_prompt(cache: PagedKV, batch: PagedBatch, q, scale=None, out
 def attention_prompt(q, k, v, cu_seqlens, scale=None, out=None, status=None, stream=None):
     """Causal attention of packed prompts: q [n_tokens, n_heads, head_dim], k
     and v [n_tokens, n_kv_heads, head_dim] in float16 or bfloat16, sequence s
-    in rows [cu_seqlens[s], cu_seqlens[s+1]); returns q's shape."""
+    in rows [cu_seqlens[s], cu_seqlens[s+1]); returns q's shape.  Rows of no
+    sequence as in paged_attention_prompt."""
     if not q.is_cuda or q.dim() != 3 or k.dim() != 3 or q.dtype is not k.dtype or q.dtype is not v.dtype:
         _refuse("q, k and v must be 3-D CUDA tensors of one type")
     index, (n, heads, d), kv = q.get_device(), q.shape, k.shape[1]

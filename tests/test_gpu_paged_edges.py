@@ -251,3 +251,33 @@ def test_large_values_do_not_overflow_on_the_way(call):
     got = getattr(rb, call)(rb.PagedKV(k, v), rb.PagedBatch(i32(table), i32([4096])), q, scale=1.0)
     want = float(v[0, 0, 0, 0])
     assert float((got.double() - want).abs().max()) <= 2.0 ** -8 * want
+
+
+# ------------------------------------------------- rows of no sequence
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_rows_that_no_sequence_holds_are_zeros(ty, norm):
+    # a call of a fixed number of rows, as a captured one is, fewer of them in use:
+    # rows before the first sequence, between the bounds' ends and past the last
+    page, H, kv, hd, n = 16, 6, 2, 128, 40
+    g = gen(11)
+    lens, cu = [20, 9, 30], [3, 8, 8, 25]
+    k, v, table = make_pool(g, lens, page, kv, hd, torch.bfloat16)
+    q, kn, vn = append_inputs(g, n, H, kv, hd, ty, False)
+    gain = 1 + 0.1 * randn(g, hd) if norm else None
+    tab, status = rb.rope_table(64, hd), i32([0])
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    k0, v0 = k.clone(), v.clone()
+    rb.paged_append(rb.PagedKV(k, v), rb.PagedBatch(i32(table), i32(lens), i32(cu), n, status), q, kn, vn, gain, gain, 1e-6, tab,
+                    q_out=out)
+    assert bool((out[:3] == 0).all()) and bool((out[25:] == 0).all())
+    assert bool((out[3:25] != 0).any(-1).all()) and bool((out[3:25] != 7).any(-1).all())
+    assert int(status) == 0
+    changed = (k != k0).any(-1).any(-1) | (v != v0).any(-1).any(-1)
+    assert int(changed.sum()) == 22
+    # no sequence at all
+    out.fill_(7)
+    empty = rb.PagedBatch(i32(table), i32(lens), i32([0, 0, 0, 0]), n, status)
+    k0, v0 = k.clone(), v.clone()
+    rb.paged_append(rb.PagedKV(k, v), empty, q, kn, vn, gain, gain, 1e-6, tab, q_out=out)
+    assert bool((out == 0).all()) and torch.equal(k, k0) and torch.equal(v, v0) and int(status) == 0
