@@ -392,10 +392,16 @@ typedef struct rpgc_paged_batch {
   const int32_t* cu_q;    /* [n_seqs + 1] sequence s's new tokens are rows [cu_q[s], cu_q[s+1]);
                              NULL: one new token per sequence, row s */
   int64_t n_tokens;       /* rows of q (and of k and v in append) */
-  int32_t* status;        /* optional: RPGC_PAGED_* bits are OR-ed into it on the device */
+  int32_t* status;        /* RPGC_PAGED_* bits are OR-ed into it on the device; NULL: into a word
+                             of the library, see rpgc_paged_status */
 } rpgc_paged_batch;
 #define RPGC_PAGED_DROPPED 1 /* append: a new token's position has no page or no rope row */
 #define RPGC_PAGED_TIMEOUT 2 /* a bounded wait inside a kernel gave up; the output is not valid */
+
+/* *bits: what the calls that had no status word of their own have reported on the
+ * current device since the last time this was asked.  The caller has waited for
+ * those calls; what one that is still running reports may be lost. */
+RPGC_API int rpgc_paged_status(int32_t* bits);
 
 /* QK-norm, rotary positions and the cache write of new tokens
  * (src/qwen3.cc:141-163, src/kv_cache.cc:5-33), from the rows the matmuls

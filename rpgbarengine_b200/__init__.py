@@ -143,6 +143,7 @@ def lib() -> C.CDLL:
         "rpgc_sample": ([vp, i64, f32, i32, f32, f32, vp, vp], C.c_int),
         "rpgc_attention_decode": ([vp, vp, vp, i64, i32, i32, i32, i64, vp, vp], C.c_int),
         "rpgc_paged_append": ([vp, vp, u32, vp, vp, i32, vp, vp, vp, vp, vp, vp, f32, vp, i64, vp, vp], C.c_int),
+        "rpgc_paged_status": ([vp], C.c_int),
         "rpgc_paged_decode_workspace": ([vp, i32, i32], i64),
         "rpgc_paged_attention_decode": ([vp, vp, vp, vp, i32, f32, vp, vp, i64, vp], C.c_int),
         "rpgc_paged_attention_prompt": ([vp, vp, vp, vp, i32, f32, vp, vp], C.c_int),
@@ -510,4 +511,4 @@ class EngineSession:
 
 
 from .paged import (PagedBatch, PagedKV, attention_prompt, paged_append, paged_attention_decode,  # noqa: E402
-                    paged_attention_prompt, rope_table)
+                    paged_attention_prompt, paged_status, rope_table)

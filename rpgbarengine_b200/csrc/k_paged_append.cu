@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
   }
   const int32_t page = pos >= 0 ? page_of(a.kv, a.b, s, pos) : -1;
   const bool drop = page < 0 || (a.rope && pos >= a.rope_rows);
-  if (drop && h0 == 0 && lane == 0 && a.b.status) atomicOr(a.b.status, kStatusDropped);
+  if (drop && h0 == 0 && lane == 0) report(a.b.status, kStatusDropped);
   const bool turn = a.rope && !drop, norm = a.k_norm != nullptr;
   const int64_t slot = pos & ((1 << a.kv.page_shift) - 1);
   uint16_t* qd = static_cast<uint16_t*>(a.q_out) + r * a.n_heads * HD + d;
@@ -177,6 +177,8 @@ cudaError_t append_go(const PagedAppendArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+cudaError_t paged_append_status(int32_t* bits) { return take_bits(bits); }
 
 cudaError_t paged_append_launch(const PagedAppendArgs& a, cudaStream_t s) {
   if (!a.b.n_tokens) return cudaSuccess;

@@ -645,6 +645,8 @@ int64_t paged_decode_workspace(const PagedView& kv, int32_t n_heads) {
   return counter_bytes() + rows * (kv.hd + 2) * 4;
 }
 
+cudaError_t paged_decode_status(int32_t* bits) { return take_bits(bits); }
+
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s) {
   if (!a.b.n_tokens) return cudaSuccess;
   if (a.kv.hd == 128) return a.kv.bf16 ? decode_heads<128, true>(a, s) : decode_heads<128, false>(a, s);

@@ -900,6 +900,8 @@ cudaError_t prompt_go(const PagedAttnArgs& a, cudaStream_t s) {
 
 }  // namespace
 
+cudaError_t prompt_attn_status(int32_t* bits) { return take_bits(bits); }
+
 cudaError_t prompt_attn_launch(const PagedAttnArgs& a, cudaStream_t s) {
   if (!a.b.n_tokens) return cudaSuccess;
   if (a.kv.hd == 128) return a.kv.bf16 ? prompt_go<128, true>(a, s) : prompt_go<128, false>(a, s);

@@ -380,5 +380,10 @@ cudaError_t paged_append_launch(const PagedAppendArgs& a, cudaStream_t s);
 int64_t paged_decode_workspace(const PagedView& kv, int32_t n_heads);
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s);
 cudaError_t prompt_attn_launch(const PagedAttnArgs& a, cudaStream_t s);
+// Adds to *bits what calls without a status word reported on the current device since
+// the last time.
+cudaError_t paged_append_status(int32_t* bits);
+cudaError_t paged_decode_status(int32_t* bits);
+cudaError_t prompt_attn_status(int32_t* bits);
 
 }  // namespace rpgc

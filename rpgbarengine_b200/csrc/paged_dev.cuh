@@ -14,6 +14,20 @@ namespace paged {
 
 constexpr int kStatusDropped = 1, kStatusTimeout = 2;  // RPGC_PAGED_*
 
+// What a call has to say goes to its status word or, where it has none, to this
+// one (each kernel's file has its own), which rpgc_paged_status reads.
+static __device__ int32_t g_status;
+RPGC_DEV void report(int32_t* status, int32_t bit) { atomicOr(status ? status : &g_status, bit); }
+
+// Host: the bits of this file's word on the current device, which starts again at 0.
+static inline cudaError_t take_bits(int32_t* bits) {
+  int32_t b = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&b, g_status, sizeof b);
+  if (e == cudaSuccess && b) e = cudaMemcpyToSymbol(g_status, &zero, sizeof zero);
+  *bits |= b;
+  return e;
+}
+
 // First packed row of sequence s (s == n_seqs: past the last), kept inside
 // [0, n_tokens] whatever cu holds.
 RPGC_DEV int64_t seq_row(const PagedSeqs& b, int s) {

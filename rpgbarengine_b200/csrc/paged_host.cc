@@ -222,6 +222,17 @@ int rpgc_paged_append(const rpgc_paged_kv* kv, const rpgc_paged_batch* b, uint32
   });
 }
 
+int rpgc_paged_status(int32_t* bits) {
+  return guard<int>([&] {
+    if (!bits) fail(RPGC_E_ARG, "bits is NULL");
+    *bits = 0;
+    check(rpgc::paged_append_status(bits), "append's status");
+    check(rpgc::paged_decode_status(bits), "single-token attention's status");
+    check(rpgc::prompt_attn_status(bits), "prompt attention's status");
+    return RPGC_OK;
+  });
+}
+
 int64_t rpgc_paged_decode_workspace(const rpgc_paged_kv* kv, int32_t n_seqs, int32_t n_heads) {
   return guard<int64_t>([&]() -> int64_t {
     const PagedView v = view_of(kv);

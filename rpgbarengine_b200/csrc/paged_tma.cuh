@@ -53,7 +53,7 @@ RPGC_DEV bool wait_for(uint64_t* bar, uint32_t parity, volatile int32_t* gave_up
     if (*gave_up) return false;
   } while (clock64() - t0 < kWaitClocks);
   *gave_up = 1;
-  if (status) atomicOr(status, kStatusTimeout);
+  report(status, kStatusTimeout);
   return false;
 }
 

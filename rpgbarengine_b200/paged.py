@@ -7,6 +7,7 @@
   paged_attention_prompt   causal attention of packed prompts over their pages
   attention_prompt         the same with K and V packed beside q
   rope_table               the cosine and sine rows paged_append reads
+  paged_status             what calls without a status word have reported
 
 Lengths, tables and page ids live on the device and are read there when the
 call runs: nothing here waits for the GPU, and all calls can be captured
@@ -157,8 +158,8 @@ class PagedBatch:
     cu_q: int32 [n_seqs + 1], sequence s's new tokens are rows
     [cu_q[s], cu_q[s+1]) of n_tokens (None: one new token per sequence).  All on
     the device, and read there at each call, so a decode loop updates them in
-    place and keeps the batch.  status: optional int32 tensor of one word that
-    receives DROPPED / TIMEOUT bits.
+    place and keeps the batch.  status: int32 tensor of one word that
+    receives DROPPED / TIMEOUT bits (None: see paged_status).
 
     The batch also holds decode's workspaces, one for each stream that it is
     used on, made by the first call there.  A captured call uses one that is
@@ -305,6 +306,18 @@ def attention_prompt(q, k, v, cu_seqlens, scale=None, out=None, status=None, str
          cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, n, heads, kv, d, d ** -0.5 if scale is None else scale, out.data_ptr(),
          None if status is None else status.data_ptr())
     return out
+
+
+def paged_status(device=None) -> int:
+    """Waits for the device and returns the DROPPED / TIMEOUT bits that calls
+    without a status tensor have reported on it since the last time: after
+    TIMEOUT the output of one of them is not valid."""
+    torch = _torch()
+    bits = C.c_int32()
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        _check(lib().rpgc_paged_status(C.byref(bits)))
+    return bits.value
 
 
 def rope_table(positions: int, head_dim: int, theta: float = 1e6, device="cuda"):

@@ -281,3 +281,20 @@ def test_append_rows_that_no_sequence_holds_are_zeros(ty, norm):
     k0, v0 = k.clone(), v.clone()
     rb.paged_append(rb.PagedKV(k, v), empty, q, kn, vn, gain, gain, 1e-6, tab, q_out=out)
     assert bool((out == 0).all()) and torch.equal(k, k0) and torch.equal(v, v0) and int(status) == 0
+
+
+# --------------------------------------------------------------- status
+def test_calls_without_a_status_word_report_to_the_library():
+    g = gen(5)
+    k, v, _ = make_pool(g, [64], 16, 2, 64, torch.float16)
+    cache, kn = rb.PagedKV(k, v), randn(g, 1, 2, 64)
+    rb.paged_status()  # whatever earlier calls left
+    rb.paged_append(cache, rb.PagedBatch(i32([[0]]), i32([5])), None, kn, kn)
+    rb.paged_attention_decode(cache, rb.PagedBatch(i32([[0]]), i32([5])), kn.half())
+    assert rb.paged_status() == 0
+    own = i32([0])
+    rb.paged_append(cache, rb.PagedBatch(i32([[-1]]), i32([5]), status=own), None, kn, kn)
+    assert rb.paged_status() == 0 and int(own) == rb.paged.DROPPED
+    rb.paged_append(cache, rb.PagedBatch(i32([[-1]]), i32([5])), None, kn, kn)
+    assert rb.paged_status() == rb.paged.DROPPED
+    assert rb.paged_status() == 0  # told once

@@ -192,3 +192,9 @@ def test_a_result_outlives_its_use_on_the_stream_that_was_asked_for(recorder, mo
     with recorder.On(recorder.Stream(0x70)):
         rb.paged_attention_decode(cache, batch, q, stream=handle)
     assert recorder.launches[-1][1] == handle and recorded == [handle]
+
+
+def test_the_status_of_calls_without_a_word_of_their_own_can_be_asked_for():
+    assert rb.lib().rpgc_paged_status(None) == rb.E_ARG
+    assert "bits is NULL" in rb.lib().rpgc_last_error().decode()
+    assert callable(rb.paged_status)
