@@ -3,13 +3,14 @@
 Where two calls do the same arithmetic on the same visible values their results
 are compared bit for bit; else against 64 bits with the bounds of
 test_gpu_paged.py."""
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import rpgbarengine_b200 as rb  # noqa: E402
-from test_gpu_paged import (DT, append_inputs, check_decode, check_packed, check_paged, decode_case, gen, i32, make_pool,  # noqa: E402
+from test_gpu_paged import (DT, U, append_inputs, check_decode, check_packed, check_paged, decode_case, gen, i32, make_pool,  # noqa: E402
                             packed_inputs, randn)
 
 
@@ -298,3 +299,75 @@ def test_calls_without_a_status_word_report_to_the_library():
     rb.paged_append(cache, rb.PagedBatch(i32([[-1]]), i32([5])), None, kn, kn)
     assert rb.paged_status() == rb.paged.DROPPED
     assert rb.paged_status() == 0  # told once
+
+
+# ------------------------------------------------------------- precision
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [96, 4000])
+def test_decode_weights_keep_more_than_16_bits(ty, n):
+    # Weights that round to 16 bits as badly as they can, values that cancel.  Every 16
+    # positions have two of score 0 and value 0, the reference of whoever takes those 16; of
+    # the others, one half weigh a little less than halfway above a 16-bit number in [1/2, 1)
+    # and hold 1, the other half a little more than halfway above another and hold -1.
+    # Bound: the output's rounding, u / 2 of the value, and 2^-13 of sum p |v| for
+    # everything before it (weights in two 16-bit parts are within 2^-17; ex2 and its
+    # fp32 argument, at most 1 here, 2^-22; fp32 sums of up to 4000 / 16 steps 2^-15).
+    # Weights of one 16-bit part err by 0.48 steps of 2^-8 (bf16) or 2^-11 (fp16) of
+    # 1/2, with the values all in one direction: 2^-8 or 2^-11 of sum p |v|, which is above
+    # the bound.
+    dt, hd, page, step = DT[ty], 64, 32, 2.0 ** (-8 if ty == "bf16" else -11)
+    kind = torch.tensor([0 if i % 16 in (0, 15) else 1 + i % 2 for i in range(n)], device="cuda")
+    s = torch.tensor([0.0, np.log(0.5 + 0.48 * step), np.log(0.5 + 7.52 * step)], dtype=torch.float64, device="cuda")
+    parts, rest = [], s.clone()
+    for _ in range(4):  # exact in a few 16-bit parts, each times 1 of q
+        parts.append(rest.to(dt))
+        rest = rest - parts[-1].double()
+    s = sum(p.double() for p in parts)  # what the scores are
+    pages = -(-n // page)
+    k = torch.zeros(pages, page, 1, hd, dtype=dt, device="cuda")
+    v = torch.zeros_like(k)
+    for i, p in enumerate(parts):
+        k.view(-1, hd)[:n, i] = p[kind]
+    w = torch.exp(s)[kind]
+    vals = torch.tensor([0.0, 1.0, -1.0], dtype=torch.float64, device="cuda")[kind].to(dt)
+    v.view(-1, hd)[:n] = vals[:, None]
+    q = torch.zeros(1, 1, hd, dtype=dt, device="cuda")
+    q[..., :4] = 1
+    got = rb.paged_attention_decode(rb.PagedKV(k, v), rb.PagedBatch(i32([list(range(pages))]), i32([n])), q, scale=1.0)
+    e, mag = (w * vals.double()).sum() / w.sum(), (w * vals.double().abs()).sum() / w.sum()
+    bound = float(U[dt] / 2 * e.abs() + 2.0 ** -13 * mag)
+    assert float((got.double() - e).abs().max()) <= bound
+    once = ((w.to(dt).double() * vals.double()).sum() / w.sum() - e).abs()
+    assert float(once) > (3 if ty == "f16" else 15) * bound  # weights rounded to 16 bits would be seen
+
+
+# ------------------------------------------------- bounds that make no sense
+@pytest.mark.parametrize("cu", [[-5, 100, 40, 9999], [300, 200, 100, 0], [0, 2 ** 31 - 1, -2 ** 31, 300], [299, 299, 300, 300]])
+def test_prompt_bounds_out_of_range_write_inside_the_result(cu):
+    # bounds that leave [0, n_tokens] or fall are kept inside it; nothing beside `out` is
+    # written, no wait gives up, rows of sequences whose bounds are in order are right
+    g = gen(31)
+    n, H, kv, hd, page = 300, 4, 2, 64, 32
+    q, k, v = packed_inputs(g, n, H, kv, hd, torch.float16, False)
+    guard = 64 * H * hd
+    buf = torch.full((n * H * hd + 2 * guard,), 3.0, dtype=torch.float16, device="cuda")
+    out, status = buf[guard:-guard].view(n, H, hd), i32([0])
+    rb.attention_prompt(q, k, v, i32(cu), out=out, status=status)
+    assert int(status) == 0
+    assert bool((buf[:guard] == 3).all()) and bool((buf[-guard:] == 3).all())
+    assert torch.isfinite(out).all()
+    bounds = [min(max(c, 0), n) for c in cu]
+    held = torch.zeros(n, dtype=torch.int32)
+    for a, b in zip(bounds, bounds[1:]):
+        held[a:b] += 1
+    assert bool((out[(held == 0).cuda()] == 3).all())
+    for a, b in zip(bounds, bounds[1:]):
+        if b > a and int(held[a:b].max()) == 1:
+            check_packed(out[a:b], q[a:b], k[a:b], v[a:b], [b - a], hd ** -0.5)
+    # over pages: the same bounds, more new rows than positions among them
+    kp, vp, table = make_pool(g, [n, n, n], page, kv, hd, torch.float16)
+    buf.fill_(3)
+    rb.paged_attention_prompt(rb.PagedKV(kp, vp), rb.PagedBatch(i32(table), i32([n, 5, n]), i32(cu), n, status), q, out=out)
+    assert int(status) == 0
+    assert bool((buf[:guard] == 3).all()) and bool((buf[-guard:] == 3).all())
+    assert torch.isfinite(out).all() and bool((out[(held == 0).cuda()] == 3).all())
