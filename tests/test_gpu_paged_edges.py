@@ -371,3 +371,26 @@ def test_prompt_bounds_out_of_range_write_inside_the_result(cu):
     assert int(status) == 0
     assert bool((buf[:guard] == 3).all()) and bool((buf[-guard:] == 3).all())
     assert torch.isfinite(out).all() and bool((out[(held == 0).cuda()] == 3).all())
+
+
+# ---------------------------------------------------------- broadcast inputs
+def test_heads_and_rows_expanded_from_one():
+    # strides of zero: one K and V head read as four, one query row as all
+    g = gen(41)
+    n, H, hd, page = 150, 8, 128, 16
+    q, k1, v1 = randn(g, 1, H, hd, dtype=torch.bfloat16), randn(g, n, 1, hd, dtype=torch.bfloat16), randn(g, n, 1, hd, dtype=torch.bfloat16)
+    q, k, v = q.expand(n, -1, -1), k1.expand(-1, 4, -1), v1.expand(-1, 4, -1)
+    cu = i32([0, 100, n])
+    assert torch.equal(rb.attention_prompt(q, k, v, cu), rb.attention_prompt(*(x.contiguous() for x in (q, k, v)), cu))
+    kp, vp, table = make_pool(g, [90, 150], page, 1, hd, torch.bfloat16)
+    wide, full = rb.PagedKV(kp.expand(-1, -1, 4, -1), vp.expand(-1, -1, 4, -1)), rb.PagedKV(kp.repeat(1, 1, 4, 1), vp.repeat(1, 1, 4, 1))
+    batch = rb.PagedBatch(i32(table), i32([90, 150]))
+    assert torch.equal(rb.paged_attention_decode(wide, batch, q[:2]), rb.paged_attention_decode(full, batch, q[:2].contiguous()))
+    batch = rb.PagedBatch(i32(table), i32([90, 150]), i32([0, 30, 100]), 100)
+    assert torch.equal(rb.paged_attention_prompt(wide, batch, q[:100]), rb.paged_attention_prompt(full, batch, q[:100].contiguous()))
+    # append of one row to every sequence
+    qa, ka = randn(g, 1, H, hd).expand(2, -1, -1), randn(g, 1, 1, hd).expand(2, 1, -1)
+    one, both = rb.PagedKV(kp.clone(), vp.clone()), rb.PagedKV(kp.clone(), vp.clone())
+    batch = rb.PagedBatch(i32(table), i32([90, 150]))
+    assert torch.equal(rb.paged_append(one, batch, qa, ka, ka), rb.paged_append(both, batch, qa.contiguous(), ka.contiguous(), ka.contiguous()))
+    assert torch.equal(one.k, both.k) and torch.equal(one.v, both.v)
