@@ -374,7 +374,11 @@ RPGC_API int rpgc_sample(const float* logits, int64_t n, float temperature, int3
  * name them -1) and not written by append.
  *
  * The values of a sequence's slots past its length, and of pages no sequence
- * names, are never used, whatever they are.  Outputs do not overlap inputs. */
+ * names, are never used, whatever they are; nor is what a token does not see.  A
+ * value that a token does see and that is infinite or NaN makes its result so, as
+ * the formula has it, but slowly: such rows are computed again one by one (a
+ * prompt takes some hundred times as long, a decode step 0.12 ms per 1000
+ * positions of that sequence).  Outputs do not overlap inputs. */
 typedef struct rpgc_paged_kv {
   void* k; /* slot (page, position, head) at page*stride[0] + position*stride[1] + head*stride[2] */
   void* v;

@@ -32,8 +32,9 @@
 // Measured with 32 query and 8 kv heads of 128, bf16: 128 sequences of 1-8192
 // positions 318 us (2.17 GB, 6.8 TB/s), 64 of ~1100 52 us (5.5 TB/s; 8 us of it
 // are the look-ups before the first tile and the last joins), 128 of 200 28 us
-// (3.7 TB/s), one of 4200 10.0 us, one of 33 (16 heads) 4.0 us; 48 sequences with
-// 12 heads of 64 in pages of 16, 167 MB, 39 us.
+// (3.7 TB/s), one of 4200 10.4 us, one of 33 (16 heads) 4.2 us; 48 sequences with
+// 12 heads of 64 in pages of 16, 167 MB, 39-41 us.  Groups of 16 (NT 2, one CTA per SM),
+// 64 of ~1090: 32 / 2 heads of 128 28 us (2.5 TB/s), 16 / 1 20.6 us (1.7 TB/s).
 #include <cuda_runtime.h>
 
 #include "paged_dev.cuh"
@@ -50,7 +51,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD, int NT>
 struct DShape {
-  static constexpr int kCtas = NT == 1 ? 2 : 1;       // CTAs on an SM
+  static constexpr int kCtas = NT == 1 ? 2 : 1;       // CTAs on an SM (NT 2: 240 registers a thread leave room for one)
   static constexpr int kTile = HD == 128 || NT == 1 ? 64 : 128;  // keys
   static constexpr int kWarps = kTile / 16;           // consumer warps, 16 keys of a tile each
   static constexpr int kThreads = (kWarps + 2) * 32;
@@ -117,7 +118,12 @@ RPGC_DEV int32_t seen(const PagedAttnArgs& a, int s) {  // positions the token o
 // warps' sums, a share's join) as kEnd tiles more, at its front.  An item that sees
 // nothing weighs nothing.
 constexpr int kEnd = 3;
-constexpr int kPieces = 18;  // of an item, at most on average: one of 4200 positions takes 11.6 us in 37 pieces, 10.0 in 18
+// Pieces of an item, at most on average: with 8 kv heads of 128, one sequence of 4200
+// positions takes 11.6 us in 37 pieces and 10.0 in 18.  Only few long items meet the
+// bound, and those of fewer kv heads than 8 lose by it: one sequence of 131072
+// positions takes 90 us with 8 kv heads (6.0 TB/s), 81 with 4 (3.3 TB/s) and 89 with one
+// (0.76 TB/s, 18 CTAs at work).
+constexpr int kPieces = 18;
 template <int T>
 RPGC_DEV int64_t weight_of(int32_t n) {
   return n ? (n + (int64_t)T - 1) / T + kEnd : 0;

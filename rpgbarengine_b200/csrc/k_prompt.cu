@@ -9,6 +9,21 @@
 // probabilities (which carry another 2^kLift, so that small ones keep their
 // 11 bits) for 2^15.  Until then no maximum is taken and nothing is rescaled.
 //
+// Precision: scores, exponentials, sums and joins in fp32.  P is rounded once to the
+// type of V, the only operand that the 16-bit MMA takes: two 16-bit parts, as the
+// single-token kernel has them, would be half as many MMAs again on the unit that sets
+// the pace.  Each result is within u / 2 (sum p |v| + its own size) for it, u = 2^-8 or
+// 2^-11 (relative L2 on normal values: 2.0e-3 to 2.3e-3 in bf16, where the result's
+// rounding alone is 1.6e-3; 2.5e-4 and 2.0e-4 in fp16).  l adds the unrounded
+// probabilities: their roundings fall both ways and are not correlated with V.
+//
+// What a row does not see: its score becomes -inf, its weight 0, and it counts for
+// nothing whatever it holds, except that 0 times an infinite or NaN V is NaN in an
+// MMA.  Rows that come out infinite or NaN though their scores are finite are computed
+// again from their visible keys (attn_row), which also settles rows that do see such
+// a V.  That is a warp per row and takes 200 to 400 times as long (512 tokens
+// 2.4 ms, 2048 tokens 11 ms).
+//
 // Layout: the G query heads of a kv head share its keys, so a tile of 128 MMA
 // rows holds T = 128 / G tokens x G heads; a work unit is two such tiles (A,
 // B) of one sequence and kv head, one CTA per SM taking units from a list
@@ -27,9 +42,11 @@
 // special-function unit as many for the exponentials (an eighth of them go to
 // the FMA pipe); a pair takes ~2600, and long prompts run at the board's power
 // limit.  Measured with 32 query and 8 kv heads of 128, bf16: 8192 tokens 465-500
-// us (1.1-1.18 PFLOP/s), 512 tokens 12.1 us, 16 sequences of ~734 tokens after 256
-// cached ones 147-177 us; the end of a unit costs 3 k clocks (O is read, scaled
-// and stored), a first or a masked key tile 1 k more than another.
+// us (1.1-1.18 PFLOP/s), 512 tokens 12.4 us, 16 sequences of ~734 tokens after 256
+// cached ones 147-178 us; a key tile's softmax pass takes 1.57 k clocks, a first or a
+// masked one 1.05 k more; the end of a unit 0.7 k for its last product and 3.2 k to read,
+// scale and store O.  Heads of 64 (the MMAs need half the clocks, the exponentials as
+// many): 8192 tokens of 32 and 8 heads 407 us, 676 TFLOP/s.
 #include <cuda_runtime.h>
 
 #include "paged_dev.cuh"
@@ -127,8 +144,10 @@ RPGC_DEV float max_nan(float a, float b, float c) {
 }
 
 // 2^y of two values on the FMA pipe, for part of a row's probabilities: the
-// special-function unit gives 16 exponentials per clock and SM, half of what the
-// MMAs of the same tile would need.  y = n + f with n the nearest integer (added
+// special-function unit gives 16 exponentials per clock and SM, which takes as many clocks
+// as the MMAs of the same tile with heads of 128 and twice as many with heads of 64.
+// (One in eight: a quarter made 8192 tokens of heads of 128 slower; at 64 other shares
+// have not been measured.)  y = n + f with n the nearest integer (added
 // to and taken off 1.5 * 2^23 + 127), 2^f on [-1/2, 1/2] by a polynomial fitted to it
 // for the smallest relative error (7.5e-5 for degree 3, 2.7e-6 for degree 4,
 // against 2^-9 and 2^-12 of the 16-bit rounding that follows), times 2^n: the sum's
