@@ -19,18 +19,18 @@
 // 2.8 TB/s); 4 warps take 16 keys each of every tile: S^T = K Q^T (m16n8k16, the
 // kv head's query heads are the N side), P^T turned from the accumulator layout
 // into an operand by movmatrix, O^T += V^T P^T.  (mma.sync: at 4 to 16 rows a
-// head group has nothing for wider MMAs.)  A row that comes out infinite or NaN
-// though its weights are finite is computed again by one warp in fp32 (attn_row):
-// a weight's second 16-bit value may be 0 or negative, and that times a visible
-// infinity is not the infinity that the row should have; and weights of up to
-// 2^40 may overflow with values that the true weights, at most 1, do not.  The warps' sums meet in shared memory
-// at an item's end.  Two such CTAs on an SM, 192 KB in flight between them: while
+// head group has nothing for wider MMAs.)  The warps' sums meet in shared memory
+// at an item's end.  A row that comes out infinite or NaN though its weights are
+// finite is computed again by one warp in fp32 (attn_row): a weight's second
+// 16-bit value may be 0 or negative, and that times a visible infinity is not the
+// infinity that the row should have; and weights of up to 2^40 may overflow with
+// values that the true weights, at most 1, do not.  Two such CTAs on an SM, 192 KB in flight between them: while
 // one ends an item or looks for the next, the other's tiles go on (one CTA of 8
 // warps took 1.5 times as long on 128 sequences of 20 positions, 1.08 times on
 // 128 of 500).
 //
 // Measured with 32 query and 8 kv heads of 128, bf16: 128 sequences of 1-8192
-// positions 318 us (2.17 GB, 6.8 TB/s), 64 of ~1100 52 us (5.5 TB/s; 8 us of it
+// positions 318-327 us (2.17 GB, 6.6-6.8 TB/s), 64 of ~1100 52.6 us (5.5 TB/s; 8 us of it
 // are the look-ups before the first tile and the last joins), 128 of 200 28 us
 // (3.7 TB/s), one of 4200 10.4 us, one of 33 (16 heads) 4.2 us; 48 sequences with
 // 12 heads of 64 in pages of 16, 167 MB, 39-41 us.  Groups of 16 (NT 2, one CTA per SM),
@@ -51,7 +51,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD, int NT>
 struct DShape {
-  static constexpr int kCtas = NT == 1 ? 2 : 1;       // CTAs on an SM (NT 2: 240 registers a thread leave room for one)
+  static constexpr int kCtas = NT == 1 ? 2 : 1;       // CTAs on an SM (NT 2: over 240 registers a thread leave room for one)
   static constexpr int kTile = HD == 128 || NT == 1 ? 64 : 128;  // keys
   static constexpr int kWarps = kTile / 16;           // consumer warps, 16 keys of a tile each
   static constexpr int kThreads = (kWarps + 2) * 32;

@@ -10,8 +10,8 @@
   paged_status             what calls without a status word have reported
 
 Lengths, tables and page ids live on the device and are read there when the
-call runs: nothing here waits for the GPU, and all calls can be captured
-(decode's once its batch has a workspace, which an earlier call makes).
+call runs: nothing here but paged_status waits for the GPU, and all calls can
+be captured (decode's once its batch has a workspace, which an earlier call makes).
 """
 from __future__ import annotations
 
@@ -154,7 +154,8 @@ class PagedKV:
 
 class PagedBatch:
     """The sequences of a call.  block_table: int32 [n_seqs, max_pages] page
-    ids (one row expanded to n_seqs: all sequences over the same pages); kv_lens: int32 [n_seqs] cache lengths, the call's new tokens included;
+    ids (one row expanded to n_seqs: all sequences over the same pages);
+    kv_lens: int32 [n_seqs] cache lengths, the call's new tokens included;
     cu_q: int32 [n_seqs + 1], sequence s's new tokens are rows
     [cu_q[s], cu_q[s+1]) of n_tokens (None: one new token per sequence).  All on
     the device, and read there at each call, so a decode loop updates them in
