@@ -458,6 +458,75 @@ RPGC_API int rpgc_attention_prompt(uint32_t type, const void* q, const int64_t* 
                                    int32_t n_kv_heads, int32_t head_dim, float scale, void* out,
                                    int32_t* status, void* stream);
 
+/* ------------------------------------------- paged KV cache in 8 bits */
+/* A layer's cache with half the bytes: a row of head_dim values (a position's K
+ * or V of one kv head) is head_dim e4m3 codes and one fp32 scale, value = scale *
+ * code.  Pages, tables, lengths and batches are those of the 16-bit cache, and so
+ * is what is said there of positions that are not there and of values that are
+ * not finite; a row written with a value that is not finite reads as NaN.
+ *
+ * Code strides count bytes and are multiples of 16, scale strides count floats
+ * and are multiples of 4: K's scale of slot (page, position, head) is at
+ * page*scale_stride[0] + head*scale_stride[1] + position, V's page_size floats
+ * after it. */
+typedef struct rpgc_paged_kv8 {
+  void* k; /* codes of slot (page, position, head) at page*stride[0] + position*stride[1] + head*stride[2] */
+  void* v;
+  int64_t k_stride[3], v_stride[3];
+  float* scales;
+  int64_t scale_stride[2];
+  uint32_t type; /* of q and of attention's results: RPGC_F16 or RPGC_BF16 */
+  int32_t n_pages, page_size, n_kv_heads, head_dim;
+} rpgc_paged_kv8;
+
+/* First positions that groups of a batch's sequences share, for single-token
+ * attention: group g is sequences [cu_seqs[g], cu_seqs[g+1]) (cu_seqs does not
+ * decrease; sequences outside all groups share nothing), and its sequences'
+ * positions [0, lens[g]) are read through row g of this table from this cache,
+ * once for the whole group.  Their own tables' entries for those positions are not
+ * looked at.  A sequence shorter than lens[g] sees as much of the prefix as it
+ * has positions.  Lengths, table and cu_seqs are device data, as in a batch. */
+typedef struct rpgc_paged_prefix {
+  const rpgc_paged_kv* kv; /* 16 bits, of the call's type, kv heads and head_dim; its pool may be the call's own */
+  const int32_t* block_table; /* [n_groups] rows of max_pages ids, table_stride apart (0: one row for all) */
+  int64_t table_stride;
+  int32_t max_pages;
+  int32_t n_groups;
+  const int32_t* lens;    /* [n_groups] */
+  const int32_t* cu_seqs; /* [n_groups + 1] */
+} rpgc_paged_prefix;
+
+/* rpgc_paged_append into 8-bit pages: a row's scale is max|x| / 448 (2^-126 at
+ * least), its codes x / scale rounded to the nearest even; NaN where a value of the
+ * row is not finite.  q_out has the cache's type.  All else as there. */
+RPGC_API int rpgc_paged8_append(const rpgc_paged_kv8* kv, const rpgc_paged_batch* b, uint32_t in_type,
+                                const void* q, const int64_t* q_stride, int32_t n_heads, const void* k,
+                                const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                                const float* q_norm, const float* k_norm, float eps, const float* rope,
+                                int64_t rope_rows, void* q_out, void* stream);
+
+/* The values of positions [0, kv_lens[s]) of every sequence, rounded once to `to`'s
+ * type, into the slots that row s of to_table names in `to` (kv heads and head_dim
+ * alike; page sizes may differ).  A position whose page is not in b's table is left
+ * out: its slot keeps what it holds.  A position without a page in to_table is
+ * dropped and RPGC_PAGED_DROPPED set.  b->cu_q is not looked at. */
+RPGC_API int rpgc_paged8_read(const rpgc_paged_kv8* kv, const rpgc_paged_batch* b, const rpgc_paged_kv* to,
+                              const int32_t* to_table, int64_t to_table_stride, int32_t to_max_pages, void* stream);
+
+/* rpgc_paged_attention_decode with a shared prefix, over 16-bit pages or (paged8)
+ * over 8-bit ones, there with a prefix or without (NULL).  The same arguments and
+ * results; the workspace, used as there, is one of its own size. */
+RPGC_API int64_t rpgc_paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
+RPGC_API int rpgc_paged_attention_decode_prefix(const rpgc_paged_kv* kv, const rpgc_paged_batch* b,
+                                                const rpgc_paged_prefix* prefix, const void* q,
+                                                const int64_t* q_stride, int32_t n_heads, float scale, void* out,
+                                                void* workspace, int64_t workspace_bytes, void* stream);
+RPGC_API int64_t rpgc_paged8_decode_workspace(const rpgc_paged_kv8* kv, int32_t n_seqs, int32_t n_heads);
+RPGC_API int rpgc_paged8_attention_decode(const rpgc_paged_kv8* kv, const rpgc_paged_batch* b,
+                                          const rpgc_paged_prefix* prefix, const void* q, const int64_t* q_stride,
+                                          int32_t n_heads, float scale, void* out, void* workspace,
+                                          int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -9,8 +9,9 @@ Python host mirror of the reference's token-level interface:
   dequantize_rows              DequantizeRow             (src/quant.h:65)
   matvec / matmul_batch        MatVec / MatMulBatch      (src/model.cc:23-69)
   sample_token                 SampleToken / ArgMax      (src/sampler.cc:96-112)
-  PagedKV, paged_* ,           a 16-bit KV cache in pages, its writer and its
-  attention_prompt             attention (paged.py; no counterpart)
+  PagedKV, PagedKV8, paged_* , a KV cache in pages of 16 or 8 bits, its writer and
+  PagedPrefix,                 its attention, with openings that sequences share
+  attention_prompt             (paged.py; no counterpart)
 
 Every call goes through librpgc.so (include/rpgc.h).  There is no CPU
 fallback: without the built library, or without a CUDA device, calls fail.
@@ -147,6 +148,12 @@ def lib() -> C.CDLL:
         "rpgc_paged_decode_workspace": ([vp, i32, i32], i64),
         "rpgc_paged_attention_decode": ([vp, vp, vp, vp, i32, f32, vp, vp, i64, vp], C.c_int),
         "rpgc_paged_attention_prompt": ([vp, vp, vp, vp, i32, f32, vp, vp], C.c_int),
+        "rpgc_paged8_append": ([vp, vp, u32, vp, vp, i32, vp, vp, vp, vp, vp, vp, f32, vp, i64, vp, vp], C.c_int),
+        "rpgc_paged8_read": ([vp, vp, vp, vp, i64, i32, vp], C.c_int),
+        "rpgc_paged_prefix_workspace": ([i32, i32, i32, i32], i64),
+        "rpgc_paged_attention_decode_prefix": ([vp, vp, vp, vp, vp, i32, f32, vp, vp, i64, vp], C.c_int),
+        "rpgc_paged8_decode_workspace": ([vp, i32, i32], i64),
+        "rpgc_paged8_attention_decode": ([vp, vp, vp, vp, vp, i32, f32, vp, vp, i64, vp], C.c_int),
         "rpgc_attention_prompt": ([u32, vp, vp, vp, vp, vp, vp, vp, i32, i64, i32, i32, i32, f32, vp, vp, vp], C.c_int),
     }
     for name, (args, res) in sig.items():
@@ -510,5 +517,5 @@ class EngineSession:
             pass
 
 
-from .paged import (PagedBatch, PagedKV, attention_prompt, paged_append, paged_attention_decode,  # noqa: E402
-                    paged_attention_prompt, paged_status, rope_table)
+from .paged import (PagedBatch, PagedKV, PagedKV8, PagedPrefix, attention_prompt, paged_append,  # noqa: E402
+                    paged_attention_decode, paged_attention_prompt, paged_read, paged_status, rope_table)

@@ -6,6 +6,9 @@
 // reference's cache has no pages.
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
+#include "paged8_dev.cuh"
 #include "paged_dev.cuh"
 #include "paged_tma.cuh"
 
@@ -62,7 +65,9 @@ RPGC_DEV void table4(const float* p, float* x) {
   x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
 }
 
-template <int HD, int IN, bool BF, int kSteps>
+// F8: k and v leave as e4m3 codes, each row with a scale that puts its largest
+// value at 448, the largest code.
+template <int HD, int IN, bool BF, int kSteps, bool F8>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ PagedAppendArgs a) {
   constexpr int kLanes = HD / 8, kRows = 32 / kLanes, kHalf = HD / 2;
   const int lane = threadIdx.x & 31, kv = a.kv.n_kv, nk = a.n_heads + kv, heads = nk + kv;
@@ -110,8 +115,9 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
   const bool turn = a.rope && !drop, norm = a.k_norm != nullptr;
   const int64_t slot = pos & ((1 << a.kv.page_shift) - 1);
   uint16_t* qd = static_cast<uint16_t*>(a.q_out) + r * a.n_heads * HD + d;
-  uint16_t* kd = static_cast<uint16_t*>(const_cast<void*>(a.kv.k)) + page * a.kv.k_page + slot * a.kv.k_pos + d;
-  uint16_t* vd = static_cast<uint16_t*>(const_cast<void*>(a.kv.v)) + page * a.kv.v_page + slot * a.kv.v_pos + d;
+  using Cell = std::conditional_t<F8, uint8_t, uint16_t>;
+  Cell* kd = static_cast<Cell*>(const_cast<void*>(a.kv.k)) + page * a.kv.k_page + slot * a.kv.k_pos + d;
+  Cell* vd = static_cast<Cell*>(const_cast<void*>(a.kv.v)) + page * a.kv.v_page + slot * a.kv.v_pos + d;
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) {
     const int hs = h0 + j * kRows, h = hl + j * kRows;  // the step's first head; this lane's
@@ -148,11 +154,32 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = y[i];
     }
+    if constexpr (F8) {
+      if (hs + kRows > a.n_heads) {  // (a step with rows of k or v; whole warps)
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (h < heads && !isq && !drop) {
+          const float sc = scale_of(top), inv = 1.0f / sc;
+          const int kh = isk ? h - a.n_heads : h - nk;
+          uint8_t* dst = isk ? kd + kh * a.kv.k_head : vd + kh * a.kv.v_head;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= inv;  // (within 1.5 ulp of the quotient)
+          *reinterpret_cast<uint32_t*>(dst) = pack_e4m3(x);
+          *reinterpret_cast<uint32_t*>(dst + kHalf) = pack_e4m3(x + 4);
+          if (d == 0) a.scales[page * a.sc_page + kh * a.sc_head + slot + (isk ? 0 : 1 << a.kv.page_shift)] = sc;
+        }
+      }
+      if (!isq) continue;
+    }
     if (h >= heads || (drop && !isq)) continue;
     if (drop)  // no place in the cache: q's row is zeros
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    uint16_t* dst = isq ? qd + h * HD : isk ? kd + (h - a.n_heads) * a.kv.k_head : vd + (h - nk) * a.kv.v_head;
+    uint16_t* dst = qd + h * HD;
+    if constexpr (!F8) dst = isq ? dst : isk ? kd + (h - a.n_heads) * a.kv.k_head : vd + (h - nk) * a.kv.v_head;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]));
     *reinterpret_cast<uint2*>(dst + kHalf) = make_uint2(pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7]));
   }
@@ -163,8 +190,11 @@ cudaError_t append_steps(const PagedAppendArgs& a, cudaStream_t s) {
   const int per = kSteps * 256 / HD;  // heads of a warp
   const int groups = (a.n_heads + 2 * a.kv.n_kv + per - 1) / per, rows = (groups + 3) / 4;  // blocks of at most 4 warps: 5 % faster than of 8
   const dim3 grid((unsigned)a.b.n_tokens, (unsigned)rows), block(32u * (unsigned)((groups + rows - 1) / rows));
-  return a.kv.bf16 ? launch_pdl(append_kernel<HD, IN, true, kSteps>, grid, block, 0, s, a)
-                   : launch_pdl(append_kernel<HD, IN, false, kSteps>, grid, block, 0, s, a);
+  if (a.scales)
+    return a.kv.bf16 ? launch_pdl(append_kernel<HD, IN, true, kSteps, true>, grid, block, 0, s, a)
+                     : launch_pdl(append_kernel<HD, IN, false, kSteps, true>, grid, block, 0, s, a);
+  return a.kv.bf16 ? launch_pdl(append_kernel<HD, IN, true, kSteps, false>, grid, block, 0, s, a)
+                   : launch_pdl(append_kernel<HD, IN, false, kSteps, false>, grid, block, 0, s, a);
 }
 
 template <int HD, int IN>

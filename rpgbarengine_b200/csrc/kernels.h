@@ -365,6 +365,9 @@ struct PagedAppendArgs {
   const float* rope;
   int64_t rope_rows;
   void* q_out;
+  // 8-bit pages: kv.k and kv.v hold e4m3 codes, scales their rows' (nullptr: 16 bits)
+  float* scales;
+  int64_t sc_page, sc_head;
 };
 struct PagedAttnArgs {
   PagedView kv;
@@ -376,7 +379,40 @@ struct PagedAttnArgs {
   void* out;
   void* workspace;
 };
+// Positions that groups of sequences share; n_groups == 0: none.
+struct PagedPrefix {
+  PagedView kv;
+  const int32_t* table;  // [n_groups] rows
+  int64_t table_stride;
+  int32_t max_pages;
+  int32_t n_groups;
+  const int32_t* lens;
+  const int32_t* cu;  // [n_groups + 1]
+};
+// Single-token attention over 8-bit pages (scales != nullptr; kv.bf16 is q's and
+// out's type then), with a shared prefix, or both.
+struct PagedOwnArgs : PagedAttnArgs {
+  const float* scales;
+  int64_t sc_page, sc_head;
+  PagedPrefix pre;
+};
+struct PagedReadArgs {
+  PagedView kv;  // codes
+  const float* scales;
+  int64_t sc_page, sc_head;
+  PagedSeqs b;
+  PagedView to;  // its k and v are written
+  const int32_t* to_table;
+  int64_t to_stride;
+  int32_t to_max;
+};
 cudaError_t paged_append_launch(const PagedAppendArgs& a, cudaStream_t s);
+cudaError_t paged_read_launch(const PagedReadArgs& a, cudaStream_t s);
+cudaError_t paged_read_status(int32_t* bits);
+// Workspaces of calls without and with a prefix.
+int64_t paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd);
+cudaError_t paged_own_decode_launch(const PagedOwnArgs& a, cudaStream_t s);
+cudaError_t paged_own_decode_status(int32_t* bits);
 int64_t paged_decode_workspace(const PagedView& kv, int32_t n_heads);
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s);
 cudaError_t prompt_attn_launch(const PagedAttnArgs& a, cudaStream_t s);

@@ -1,9 +1,12 @@
-"""Paged KV cache on the device (rpgc_paged_*, rpgc_attention_prompt).
+"""Paged KV cache on the device (rpgc_paged_*, rpgc_paged8_*, rpgc_attention_prompt).
 
   PagedKV                  one layer's K and V pools: [page, position, kv head, head_dim]
+  PagedKV8                 the same in 8 bits: e4m3 codes and a scale for each row
   PagedBatch               the sequences of a call: block table, lengths, packed rows
+  PagedPrefix              first positions that groups of sequences share
   paged_append             QK-norm + RoPE + write of new tokens into their pages
   paged_attention_decode   one new token per sequence over its pages
+  paged_read               positions of 8-bit pages back into 16-bit pages
   paged_attention_prompt   causal attention of packed prompts over their pages
   attention_prompt         the same with K and V packed beside q
   rope_table               the cosine and sine rows paged_append reads
@@ -33,6 +36,17 @@ class _Batch(C.Structure):
     _fields_ = [("block_table", C.c_void_p), ("table_stride", C.c_int64), ("max_pages", C.c_int32),
                 ("n_seqs", C.c_int32), ("kv_lens", C.c_void_p), ("cu_q", C.c_void_p),
                 ("n_tokens", C.c_int64), ("status", C.c_void_p)]
+
+
+class _KV8(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+                ("scales", C.c_void_p), ("scale_stride", C.c_int64 * 2), ("type", C.c_uint32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class _Prefix(C.Structure):
+    _fields_ = [("kv", C.POINTER(_KV)), ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("max_pages", C.c_int32),
+                ("n_groups", C.c_int32), ("lens", C.c_void_p), ("cu_seqs", C.c_void_p)]
 
 
 _S2 = C.c_int64 * 2
@@ -81,6 +95,16 @@ def _rows(t, what, index, n, heads, d):
             _strides.clear()
         c = _strides[key] = _S2(*key)
     return c
+
+
+def _table(t, what, n):
+    """Row stride and width of a block table of n rows."""
+    _ints(t, what, 2)
+    width = t.shape[1]
+    stride = t.stride(0) if n > 1 else width  # (one row has no stride to speak of)
+    _need(t.shape[0] == n and (t.stride(1) == 1 or width < 2), f"{what} needs one contiguous row per sequence")
+    _need(stride == 0 or stride >= width, f"{what}'s rows overlap: they must be apart, or one row expanded to all sequences")
+    return stride, width
 
 
 def _new(like, dtype=None):
@@ -152,6 +176,68 @@ class PagedKV:
         return cls(torch.empty(shape, dtype=dt, device=device), torch.empty(shape, dtype=dt, device=device))
 
 
+class PagedKV8:
+    """One layer's K and V pools in 8 bits: k and v float8_e4m3fn [n_pages,
+    page_size, n_kv_heads, head_dim] codes, any strides that are multiples of 16,
+    and scales float32 [n_pages, n_kv_heads, 2, page_size] (K's, then V's; a
+    page and head's contiguous): a row's values are scale * code.  dtype: the
+    type of q and of attention's results (float16 or bfloat16).  Holds
+    references to all three."""
+
+    def __init__(self, k, v, scales, dtype=None):
+        torch = _torch()
+        _need(k.is_cuda and k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype == torch.float8_e4m3fn and k.device == v.device,
+              "k and v must be 4-D CUDA tensors of one shape, float8_e4m3fn")
+        _need(k.stride(3) == 1 and v.stride(3) == 1, "rows of head_dim codes must be contiguous")
+        n, p, h, d = k.shape
+        _need(scales.device == k.device and scales.dtype is torch.float32 and scales.shape == (n, h, 2, p) and
+              scales.stride(3) == 1 and scales.stride(2) == p,
+              f"scales must be float32 [{n}, {h}, 2, {p}] on the pools' device, the last two dimensions contiguous")
+        self.k, self.v, self.scales, self.index = k, v, scales, k.get_device()
+        self.dtype = dtype or torch.bfloat16
+        _need(self.dtype in (torch.float16, torch.bfloat16), "dtype must be float16 or bfloat16")
+        strides = [(C.c_int64 * 3)(*[st if size > 1 else d for st, size in zip(t.stride(), t.shape[:3])]) for t in (k, v)]
+        st = _S2(scales.stride(0) if n > 1 else 2 * h * p, scales.stride(1) if h > 1 else 2 * p)
+        self.c = _KV8(k.data_ptr(), v.data_ptr(), strides[0], strides[1], scales.data_ptr(), st,
+                      BF16 if self.dtype is torch.bfloat16 else F16, n, p, h, d)
+        self.ref = C.byref(self.c)
+        self.page_size, self.n_kv_heads, self.head_dim, self.scale = p, h, d, d ** -0.5
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype=None, device="cuda") -> "PagedKV8":
+        """New pools; their values are never read before append writes them."""
+        torch = _torch()
+        shape = (n_pages, page_size, n_kv_heads, head_dim)
+        return cls(torch.empty(shape, dtype=torch.float8_e4m3fn, device=device), torch.empty(shape, dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty((n_pages, n_kv_heads, 2, page_size), dtype=torch.float32, device=device), dtype)
+
+
+class PagedPrefix:
+    """First positions that groups of a batch's sequences share, for
+    paged_attention_decode.  Group g is sequences [cu_seqs[g], cu_seqs[g+1]) of the
+    batch (those outside all groups share nothing); its sequences' positions
+    [0, lens[g]) are read once for all of them, through row g of block_table
+    (int32 [n_groups, max_pages]) from `cache`, a PagedKV: the batch's own, where
+    the sequences name the same pages, or another (for a batch in 8 bits, one that
+    paged_read has filled).  The sequences' own tables' entries for those
+    positions are not looked at.  lens [n_groups], cu_seqs [n_groups + 1]:
+    int32, on the device like the table, and read there at each call.  Holds
+    references to all of them."""
+
+    def __init__(self, cache: PagedKV, block_table, lens, cu_seqs):
+        _need(isinstance(cache, PagedKV), "a prefix lies in a PagedKV (16 bits)")
+        _ints(lens, "lens", 1)
+        _ints(cu_seqs, "cu_seqs", 1)
+        n = lens.shape[0]
+        stride, width = _table(block_table, "block_table", n)
+        _need(lens.stride(0) == 1 or n < 2, "lens must be contiguous")
+        _need(cu_seqs.shape[0] == n + 1 and cu_seqs.is_contiguous(), "cu_seqs must hold n_groups + 1 contiguous values")
+        self.index, self.cache, self.keep = cache.index, cache, (block_table, lens, cu_seqs)
+        _need(all(t.get_device() == self.index for t in self.keep), "the prefix's tensors must be on its cache's device")
+        self.c = _Prefix(C.pointer(cache.c), block_table.data_ptr(), stride, width, n, lens.data_ptr(), cu_seqs.data_ptr())
+        self.ref = C.byref(self.c)
+
+
 class PagedBatch:
     """The sequences of a call.  block_table: int32 [n_seqs, max_pages] page
     ids (one row expanded to n_seqs: all sequences over the same pages);
@@ -169,13 +255,9 @@ class PagedBatch:
     other calls on that stream."""
 
     def __init__(self, block_table, kv_lens, cu_q=None, n_tokens=None, status=None):
-        _ints(block_table, "block_table", 2)
         _ints(kv_lens, "kv_lens", 1)
         n = kv_lens.shape[0]
-        width = block_table.shape[1]
-        stride = block_table.stride(0) if n > 1 else width  # (one row has no stride to speak of)
-        _need(block_table.shape[0] == n and (block_table.stride(1) == 1 or width < 2), "block_table needs one contiguous row per sequence")
-        _need(stride == 0 or stride >= width, "block_table's rows overlap: they must be apart, or one row expanded to all sequences")
+        stride, width = _table(block_table, "block_table", n)
         _need(kv_lens.stride(0) == 1 or n < 2, "kv_lens must be contiguous")
         if cu_q is not None:
             _ints(cu_q, "cu_q", 1)
@@ -192,12 +274,12 @@ class PagedBatch:
         self.ref = C.byref(self.c)
         self._ws = {}
 
-    def workspace(self, cache: PagedKV, n_heads: int, stream: int):
-        """Decode's workspace for this batch, head count and stream (made
-        once).  It is zeroed and used on that stream, and its memory is the
+    def workspace(self, cache, n_heads: int, stream: int, prefix: bool = False):
+        """Decode's workspace for this batch, head count and stream, with a
+        prefix or without (made once).  It is zeroed and used on that stream, and its memory is the
         stream's: when the batch is dropped, what gets it next runs after the
         calls that are still using it."""
-        shape = n_heads, cache.n_kv_heads, cache.head_dim
+        shape = (n_heads, cache.n_kv_heads, cache.head_dim) + (("prefix",) if prefix else ())
         ws = self._ws.get((shape, stream))
         if ws is None:
             torch = _torch()
@@ -207,20 +289,23 @@ class PagedBatch:
                         if key[0] == shape:
                             return ws
                     raise RpgcError(E_STATE, "a captured decode call needs the workspace of an earlier one on its batch: make a call outside the graph first")
-                n = _check(lib().rpgc_paged_decode_workspace(cache.ref, self.n_seqs, n_heads))
+                n = _check(lib().rpgc_paged_prefix_workspace(self.n_seqs, n_heads, cache.n_kv_heads, cache.head_dim) if prefix else
+                           lib().rpgc_paged8_decode_workspace(cache.ref, self.n_seqs, n_heads) if isinstance(cache, PagedKV8) else
+                           lib().rpgc_paged_decode_workspace(cache.ref, self.n_seqs, n_heads))
                 buf = torch.zeros(n, dtype=torch.uint8, device="cuda")
             ws = self._ws[shape, stream] = (buf, buf.data_ptr(), n)
         return ws
 
 
-def paged_append(cache: PagedKV, batch: PagedBatch, q, k, v, q_norm=None, k_norm=None, eps: float = 1e-6, rope=None,
+def paged_append(cache, batch: PagedBatch, q, k, v, q_norm=None, k_norm=None, eps: float = 1e-6, rope=None,
                  q_out=None, stream=None):
     """Writes the batch's new tokens into their pages and returns q normalised
     and rotated in the cache's type (None when q is None).  q [n_tokens,
     n_heads, head_dim], k and v [n_tokens, n_kv_heads, head_dim], of one type
     (float32, float16 or bfloat16); q_norm / k_norm: fp32 gains [head_dim] or
     None; rope: fp32 [positions, head_dim] (rope_table) or None.  Rows that no
-    sequence holds are zeros in the result and write nothing to the cache."""
+    sequence holds are zeros in the result and write nothing to the cache.
+    cache: a PagedKV or a PagedKV8."""
     torch = _torch()
     index, n, d, kv = cache.index, batch.n_tokens, cache.head_dim, cache.n_kv_heads
     _need(batch.index == index, "cache and batch are on different devices")
@@ -243,7 +328,7 @@ def paged_append(cache: PagedKV, batch: PagedBatch, q, k, v, q_norm=None, k_norm
         op = q_out.data_ptr()
     else:
         _need(q_out is None, "q_out without q")
-    _run(lib().rpgc_paged_append, index, stream, made, cache.ref, batch.ref, ty, qp, qs, heads, k.data_ptr(), ks, v.data_ptr(), vs,
+    _run(lib().rpgc_paged8_append if isinstance(cache, PagedKV8) else lib().rpgc_paged_append, index, stream, made, cache.ref, batch.ref, ty, qp, qs, heads, k.data_ptr(), ks, v.data_ptr(), vs,
          None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
          None if rope is None else rope.data_ptr(), 0 if rope is None else rope.shape[0], op)
     return q_out
@@ -260,23 +345,47 @@ def _attend(cache, batch, q, out):
     return qs, _result(out, q, q.shape, q.dtype), None
 
 
-def paged_attention_decode(cache: PagedKV, batch: PagedBatch, q, scale=None, out=None, stream=None):
+def paged_attention_decode(cache, batch: PagedBatch, q, scale=None, out=None, stream=None, prefix: PagedPrefix = None):
     """Attention of one new token per sequence, q [n_seqs, n_heads, head_dim],
     over the sequence's positions; returns the same shape.  scale: default
-    head_dim ** -0.5."""
+    head_dim ** -0.5.  cache: a PagedKV or a PagedKV8.  prefix: first positions that
+    groups of the sequences share, read once for each group; the results are
+    those without it, up to rounding, where the sequences name the same pages."""
     qs, out, made = _attend(cache, batch, q, out)
-    heads = q.shape[1]
-    ws = batch.workspace(cache, heads, _torch()._C._cuda_getCurrentRawStream(cache.index) if stream is None else int(stream))
-    _run(lib().rpgc_paged_attention_decode, cache.index, stream, made, cache.ref, batch.ref, q.data_ptr(), qs, heads,
-         cache.scale if scale is None else scale, out.data_ptr(), ws[1], ws[2])
+    heads, eight = q.shape[1], isinstance(cache, PagedKV8)
+    ws = batch.workspace(cache, heads, _torch()._C._cuda_getCurrentRawStream(cache.index) if stream is None else int(stream),
+                         *(() if prefix is None else (True,)))
+    scale = cache.scale if scale is None else scale
+    if prefix is None and not eight:
+        _run(lib().rpgc_paged_attention_decode, cache.index, stream, made, cache.ref, batch.ref, q.data_ptr(), qs, heads, scale,
+             out.data_ptr(), ws[1], ws[2])
+        return out
+    if prefix is not None and prefix.index != cache.index:
+        _refuse("cache and prefix are on different devices")
+    _run(lib().rpgc_paged8_attention_decode if eight else lib().rpgc_paged_attention_decode_prefix, cache.index, stream, made, cache.ref,
+         batch.ref, None if prefix is None else prefix.ref, q.data_ptr(), qs, heads, scale, out.data_ptr(), ws[1], ws[2])
     return out
+
+
+def paged_read(cache: PagedKV8, batch: PagedBatch, to: PagedKV, to_table, stream=None):
+    """Positions [0, kv_lens[s]) of every sequence of the batch, rounded once
+    to `to`'s type, into the slots that row s of to_table (int32 [n_seqs,
+    pages]) names there: what prompt attention and a PagedPrefix read.
+    Positions whose page is not in the batch's table are left out; those without one
+    in to_table are dropped (DROPPED in the batch's status)."""
+    _need(isinstance(cache, PagedKV8) and isinstance(to, PagedKV), "paged_read goes from a PagedKV8 to a PagedKV")
+    stride, width = _table(to_table, "to_table", batch.n_seqs)
+    if not cache.index == batch.index == to.index == to_table.get_device():
+        _refuse("cache, batch, to and to_table must be on one device")
+    _run(lib().rpgc_paged8_read, cache.index, stream, None, cache.ref, batch.ref, to.ref, to_table.data_ptr(), stride, width)
 
 
 def paged_attention_prompt(cache: PagedKV, batch: PagedBatch, q, scale=None, out=None, stream=None):
     """Causal attention of the batch's new tokens, q [n_tokens, n_heads,
     head_dim], over their sequences' pages (a cached prefix included).  Rows
     that no sequence holds are not written: in a result made here they hold
-    anything."""
+    anything.  (An 8-bit cache is read back first: paged_read.)"""
+    _need(isinstance(cache, PagedKV), "prompt attention reads 16-bit pages: paged_read brings an 8-bit cache's back into some")
     qs, out, made = _attend(cache, batch, q, out)
     _run(lib().rpgc_paged_attention_prompt, cache.index, stream, made, cache.ref, batch.ref, q.data_ptr(), qs, q.shape[1],
          cache.scale if scale is None else scale, out.data_ptr())
