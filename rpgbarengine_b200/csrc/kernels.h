@@ -409,10 +409,17 @@ struct PagedReadArgs {
 cudaError_t paged_append_launch(const PagedAppendArgs& a, cudaStream_t s);
 cudaError_t paged_read_launch(const PagedReadArgs& a, cudaStream_t s);
 cudaError_t paged_read_status(int32_t* bits);
-// Workspaces of calls without and with a prefix.
+cudaError_t paged8_decode_launch(const PagedOwnArgs& a, cudaStream_t s);  // no prefix
+cudaError_t paged8_decode_status(int32_t* bits);
+// With a prefix: its sums, then own positions (two kernels that belong together).
 int64_t paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd);
-cudaError_t paged_own_decode_launch(const PagedOwnArgs& a, cudaStream_t s);
-cudaError_t paged_own_decode_status(int32_t* bits);
+void paged_prefix_parts(const PagedOwnArgs& a, int32_t** chunk, float** part, float** ml);
+cudaError_t paged_prefix_launch(const PagedOwnArgs& a, cudaStream_t s);
+cudaError_t paged_prefix_status(int32_t* bits);
+cudaError_t paged_decode_prefix_launch(const PagedOwnArgs& a, cudaStream_t s);
+cudaError_t paged_decode_prefix_status(int32_t* bits);
+cudaError_t paged8_decode_prefix_launch(const PagedOwnArgs& a, cudaStream_t s);
+cudaError_t paged8_decode_prefix_status(int32_t* bits);
 int64_t paged_decode_workspace(const PagedView& kv, int32_t n_heads);
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s);
 cudaError_t prompt_attn_launch(const PagedAttnArgs& a, cudaStream_t s);

@@ -11,13 +11,6 @@
 namespace rpgc {
 namespace paged {
 
-// max that carries NaN
-RPGC_DEV float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // Scale of a row whose largest absolute value is `top` (NaN where one was NaN).
 // 2^-126 at least, so that its inverse is finite.
 RPGC_DEV float scale_of(float top) {
@@ -49,7 +42,7 @@ RPGC_DEV float2 float2_hi(uint32_t w) { return unpack2<false>(half2_hi(w)); }
 // ------------------------------------------------------- shared prefixes
 // First sequence of group g, kept inside [0, n_seqs] whatever cu holds.
 RPGC_DEV int32_t group_seq(const PagedPrefix& p, int32_t n_seqs, int g) {
-  return min(max(p.cu[g], 0), n_seqs);
+  return min(max(__ldcg(p.cu + g), 0), n_seqs);
 }
 // Group of sequence s, or -1: the last g with group_seq(g) <= s, where s is before
 // the next one's.
@@ -70,7 +63,7 @@ struct Sight {
 };
 template <bool SH>
 RPGC_DEV Sight sight_of(const PagedOwnArgs& a, int32_t s) {
-  const int32_t n = max(0, a.b.kv_lens[s]);
+  const int32_t n = max(0, SH ? __ldcg(a.b.kv_lens + s) : a.b.kv_lens[s]);
   Sight v;
   v.group = -1;
   v.pre = v.own = 0;
@@ -78,7 +71,7 @@ RPGC_DEV Sight sight_of(const PagedOwnArgs& a, int32_t s) {
   if (SH) {
     v.group = group_of(a.pre, a.b.n_seqs, s);
     if (v.group >= 0) {
-      v.own = min(n, max(0, a.pre.lens[v.group]));
+      v.own = min(n, max(0, __ldcg(a.pre.lens + v.group)));
       v.pre = (int32_t)min((int64_t)v.own, (int64_t)a.pre.max_pages << a.pre.kv.page_shift);
       v.len = max(v.len, v.own);
     }

@@ -28,6 +28,18 @@ static inline cudaError_t take_bits(int32_t* bits) {
   return e;
 }
 
+// max that carries NaN
+RPGC_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+RPGC_DEV float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // First packed row of sequence s (s == n_seqs: past the last), kept inside
 // [0, n_tokens] whatever cu holds.
 RPGC_DEV int64_t seq_row(const PagedSeqs& b, int s) {

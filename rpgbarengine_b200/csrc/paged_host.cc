@@ -268,7 +268,14 @@ int own_decode(rpgc::PagedOwnArgs a, const rpgc_paged_batch* b, const rpgc_paged
   a.scale = scale;
   a.out = out;
   a.workspace = workspace;
-  check(rpgc::paged_own_decode_launch(a, as_stream(stream)), "paged decode attention");
+  if (!a.pre.n_groups) {
+    check(a.scales ? rpgc::paged8_decode_launch(a, as_stream(stream)) : rpgc::paged_decode_launch(a, as_stream(stream)),
+          "paged decode attention");
+    return RPGC_OK;
+  }
+  check(rpgc::paged_prefix_launch(a, as_stream(stream)), "attention over the prefix");
+  check(a.scales ? rpgc::paged8_decode_prefix_launch(a, as_stream(stream)) : rpgc::paged_decode_prefix_launch(a, as_stream(stream)),
+        "paged decode attention");
   return RPGC_OK;
 }
 
@@ -295,7 +302,10 @@ int rpgc_paged_status(int32_t* bits) {
     check(rpgc::paged_append_status(bits), "append's status");
     check(rpgc::paged_decode_status(bits), "single-token attention's status");
     check(rpgc::prompt_attn_status(bits), "prompt attention's status");
-    check(rpgc::paged_own_decode_status(bits), "single-token attention's status");
+    check(rpgc::paged8_decode_status(bits), "single-token attention's status");
+    check(rpgc::paged_decode_prefix_status(bits), "single-token attention's status");
+    check(rpgc::paged8_decode_prefix_status(bits), "single-token attention's status");
+    check(rpgc::paged_prefix_status(bits), "the prefix's status");
     check(rpgc::paged_read_status(bits), "read's status");
     return RPGC_OK;
   });
