@@ -34,11 +34,10 @@ using namespace paged;
 using namespace tc;
 
 constexpr int kRows = 128;  // MMA rows of a tile
-constexpr int kKeys = 128;  // keys of a tile
+constexpr int kKeys = kPrefixKeys;  // of a tile
 constexpr int kThreads = 384;
 constexpr int kUnits = 2;  // units in flight between the finder and the other warps
 constexpr int kPoly = 1, kPolyOf = 8;  // of every 8 pairs of a row, those on the FMA pipe
-constexpr int kPieces = 32;  // of a prefix, at most
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Unit {
@@ -67,50 +66,11 @@ struct PrefixParams {
   int32_t T;       // sequences of a tile
   int32_t G;       // heads per kv head
   int32_t box;     // K/V rows of one TMA copy
-  int32_t pieces;  // at most, by the workspace's size
+  PrefixShape shape;
   int32_t* chunk;  // positions of a piece, for the kernel that joins them
   float* part;     // [piece][sequence][head][HD]
   float* ml;       // [piece][sequence][head][2]
 };
-
-// A group as the plan sees it.
-struct Share {
-  int32_t seq, n;  // its sequences
-  int32_t end;     // positions that exist
-};
-RPGC_DEV Share share_of(const PagedOwnArgs& a, int g) {
-  Share s{0, 0, 0};
-  if (g < a.pre.n_groups) {
-    s.seq = group_seq(a.pre, a.b.n_seqs, g);
-    s.n = max(0, group_seq(a.pre, a.b.n_seqs, g + 1) - s.seq);
-    s.end = (int32_t)min((int64_t)max(0, a.pre.lens[g]), (int64_t)a.pre.max_pages << a.pre.kv.page_shift);
-    if (s.n == 0) s.end = 0;
-  }
-  return s;
-}
-RPGC_DEV int32_t tiles_of(const Share& s) { return (int32_t)(((int64_t)s.end + kKeys - 1) / kKeys); }
-
-// Key tiles of a piece.  Lane k weighs the length that cuts the longest prefix into
-// k + 1 pieces: rounds of units over the CTAs, each a piece's tiles and the cost of a
-// unit besides, kUnitCost tiles of two accumulators.
-constexpr int kUnitCost = 2;
-RPGC_DEV int32_t plan(const PrefixParams& p, int ctas, int lane) {
-  const PagedOwnArgs& a = p.a;
-  int32_t most = 0;
-  for (int g = lane; g < a.pre.n_groups; g += 32) most = max(most, tiles_of(share_of(a, g)));
-  most = __reduce_max_sync(0xffffffffu, most);
-  if (most == 0) return 1;
-  const int32_t c = (most + lane) / (lane + 1);
-  int64_t units = 0;
-  for (int g = 0; g < a.pre.n_groups; ++g) {
-    const Share s = share_of(a, g);
-    units += (int64_t)((s.n + 2 * p.T - 1) / (2 * p.T)) * ((tiles_of(s) + c - 1) / c);
-  }
-  const int64_t rounds = (units * a.kv.n_kv + ctas - 1) / ctas;
-  const int64_t cost = lane < p.pieces ? min(rounds * (c + kUnitCost), (int64_t)1 << 30) : (int64_t)1 << 31;
-  const uint32_t best = __reduce_min_sync(0xffffffffu, (uint32_t)cost);
-  return __shfl_sync(0xffffffffu, c, __ffs(__ballot_sync(0xffffffffu, (uint32_t)cost == best)) - 1);
-}
 
 template <int HD, bool BF>
 __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_constant__ CUtensorMap tm_q,
@@ -191,35 +151,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 10) {
       // ---------------------------------------------------- finds the units
-      const int32_t chunk = plan(p, gridDim.x, lane), U = 2 * p.T, kv = a.kv.n_kv;
+      const PrefixPlan pl = prefix_plan(a, p.shape, lane);
+      const int32_t chunk = pl.chunk, U = 2 * p.T, kv = a.kv.n_kv;
       if (blockIdx.x == 0 && lane == 0) *p.chunk = chunk * kKeys;
       int g0 = 0;          // the groups from g0 on are still to be looked through
-      int64_t before = 0;  // units of those before them
+      int32_t before = 0;  // units of those before them
+      Share s = pl.mine;
       for (int it = 0;; ++it) {
-        const int64_t u = (int64_t)it * gridDim.x + blockIdx.x;
+        const int32_t u = it * (int32_t)gridDim.x + (int32_t)blockIdx.x;
         if (it >= kUnits) wait(u_empty + it % kUnits, (uint32_t)((it / kUnits) - 1) & 1u);
         Unit un;
         un.seq = -1;
-        for (; g0 < a.pre.n_groups; g0 += 32) {
-          const Share s = share_of(a, g0 + lane);
+        while (g0 < a.pre.n_groups) {
           const int32_t tiles = tiles_of(s);
-          const int64_t mine = (int64_t)((s.n + U - 1) / U) * ((tiles + chunk - 1) / chunk) * kv;
-          int64_t sum = mine;
+          const int32_t mine = ((s.n + U - 1) / U) * ((tiles + chunk - 1) / chunk) * kv;
+          int32_t sum = mine;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
+            const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += x;
           }
           const uint32_t in = __ballot_sync(0xffffffffu, u - before < sum);
           if (in) {
             const int src = __ffs(in) - 1;
-            int64_t w = u - before - __shfl_sync(0xffffffffu, sum - mine, src);
+            int32_t w = u - before - __shfl_sync(0xffffffffu, sum - mine, src);
             const int32_t n = __shfl_sync(0xffffffffu, s.n, src), nt = __shfl_sync(0xffffffffu, tiles, src);
             const int32_t R = (n + U - 1) / U;
-            un.kh = (int32_t)(w % kv);
+            un.kh = w % kv;
             w /= kv;
-            const int32_t r = (int32_t)(w % R);
-            un.piece = (int32_t)(w / R);
+            const int32_t r = w % R;
+            un.piece = w / R;
             un.group = g0 + src;
             un.seq = __shfl_sync(0xffffffffu, s.seq, src) + r * U;
             un.rows[0] = min(p.T, n - r * U);
@@ -230,6 +191,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
             break;
           }
           before += __shfl_sync(0xffffffffu, sum, 31);
+          g0 += 32;
+          s = share_of(a, g0 + lane);
         }
         if (lane == 0) {
           units[it % kUnits] = un;
@@ -426,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     const int tok = r / p.G, head = r - tok * p.G;
     const float c = a.scale * kLog2e;
     const int pshift = a.pre.kv.page_shift, shift = min(pshift, 7), npg = shift < 7 ? kKeys >> shift : 1;
-    uint32_t sp = 0, op[2] = {0u, 0u}, xp = 0;
+    uint32_t sp = 0, op[2] = {0u, 0u}, xp = 0;  // parities of s_full, o_full, x_bar
     auto both = [&] {  // the two groups meet
       __syncwarp();
       if (lane == 0) mbar_arrive(x_bar);
@@ -625,13 +588,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   }
 }
 
-// Pieces that the workspace has room for: fewer for more rows, whose units fill the
-// SMs with longer ones.
-int pieces_of(int32_t n_seqs, int32_t n_heads) {
-  const int64_t rows = (int64_t)(n_seqs > 0 ? n_seqs : 1) * n_heads, n = 75776 / rows;  // (148 SMs, two tiles each, twice over)
-  return n < 1 ? 1 : n > kPieces ? kPieces : (int)n;
-}
-
 template <int HD, bool BF>
 cudaError_t prefix_go(const PagedOwnArgs& a, const PrefixParams& given, cudaStream_t s) {
   PrefixParams p = given;
@@ -659,42 +615,24 @@ cudaError_t prefix_go(const PagedOwnArgs& a, const PrefixParams& given, cudaStre
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const cudaError_t e = launch_pdl(prefix_kernel<HD, BF>, dim3((unsigned)sm_count(dev)), dim3(kThreads), smem, s, mq, mk, mv, p);
+  const cudaError_t e = launch_pdl(prefix_kernel<HD, BF>, dim3((unsigned)p.shape.ctas), dim3(kThreads), smem, s, mq, mk, mv, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
 
-// The workspace of a call with a prefix: single-token attention's, then the length of
-// a piece, the pieces' sums, their references and weights.
-int64_t front_bytes(int32_t n_heads, int32_t n_kv, int32_t hd) {
-  PagedView v{};
-  v.n_kv = n_kv;
-  v.hd = hd;
-  return (paged_decode_workspace(v, n_heads) + 255) / 256 * 256 + 256;
-}
-
 }  // namespace
-
-int64_t paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd) {
-  return front_bytes(n_heads, n_kv, hd) + (int64_t)pieces_of(n_seqs, n_heads) * n_seqs * n_heads * (hd + 2) * 4;
-}
-
-void paged_prefix_parts(const PagedOwnArgs& a, int32_t** chunk, float** part, float** ml) {
-  uint8_t* w = static_cast<uint8_t*>(a.workspace) + front_bytes(a.n_heads, a.kv.n_kv, a.kv.hd);
-  *chunk = reinterpret_cast<int32_t*>(w - 256);
-  *part = reinterpret_cast<float*>(w);
-  *ml = *part + (int64_t)pieces_of(a.b.n_seqs, a.n_heads) * a.b.n_seqs * a.n_heads * a.kv.hd;
-}
 
 cudaError_t paged_prefix_status(int32_t* bits) { return take_bits(bits); }
 
-cudaError_t paged_prefix_launch(const PagedOwnArgs& a, cudaStream_t s) {
+cudaError_t paged_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s) {
   PrefixParams p{};
   p.a = a;
   p.G = a.n_heads / a.kv.n_kv;
-  p.T = kRows / p.G;
-  p.pieces = pieces_of(a.b.n_seqs, a.n_heads);
-  paged_prefix_parts(a, &p.chunk, &p.part, &p.ml);
+  p.T = shape.T;
+  p.shape = shape;
+  p.chunk = parts.chunk;
+  p.part = parts.part;
+  p.ml = parts.ml;
   if (a.kv.hd == 128) return a.kv.bf16 ? prefix_go<128, true>(a, p, s) : prefix_go<128, false>(a, p, s);
   return a.kv.bf16 ? prefix_go<64, true>(a, p, s) : prefix_go<64, false>(a, p, s);
 }

@@ -411,14 +411,27 @@ cudaError_t paged_read_launch(const PagedReadArgs& a, cudaStream_t s);
 cudaError_t paged_read_status(int32_t* bits);
 cudaError_t paged8_decode_launch(const PagedOwnArgs& a, cudaStream_t s);  // no prefix
 cudaError_t paged8_decode_status(int32_t* bits);
-// With a prefix: its sums, then own positions (two kernels that belong together).
+// With a prefix, three kernels: sums over the prefixes, sums over the sequences' own
+// positions, and the two joined.
+struct PrefixParts {
+  int32_t* chunk;  // positions of a piece of a prefix
+  float* part;     // [piece][sequence][head][hd] sums of weights times values
+  float* ml;       // [piece][sequence][head][2] their reference and weight
+  float* own;      // [sequence][head][hd] the same over own positions
+  float* own_ml;
+};
+struct PrefixShape {
+  int32_t T;       // sequences of a tile of rows
+  int32_t ctas;    // of the prefix kernel
+  int32_t pieces;  // of a prefix, at most
+};
 int64_t paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd);
-void paged_prefix_parts(const PagedOwnArgs& a, int32_t** chunk, float** part, float** ml);
-cudaError_t paged_prefix_launch(const PagedOwnArgs& a, cudaStream_t s);
+cudaError_t paged_prefix_decode_launch(const PagedOwnArgs& a, cudaStream_t s);  // all three
+cudaError_t paged_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged_prefix_status(int32_t* bits);
-cudaError_t paged_decode_prefix_launch(const PagedOwnArgs& a, cudaStream_t s);
+cudaError_t paged_decode_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged_decode_prefix_status(int32_t* bits);
-cudaError_t paged8_decode_prefix_launch(const PagedOwnArgs& a, cudaStream_t s);
+cudaError_t paged8_decode_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged8_decode_prefix_status(int32_t* bits);
 int64_t paged_decode_workspace(const PagedView& kv, int32_t n_heads);
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s);

@@ -60,8 +60,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 template <int HD, int NT, bool F8 = false>
 struct DShape {
   static constexpr int kCtas = NT == 1 ? 2 : 1;       // CTAs on an SM (NT 2: over 240 registers a thread leave room for one)
-  static constexpr int kTile = HD == 128 || NT == 1 ? 64 : 128;  // keys
-  static constexpr int kWarps = kTile / 16;           // consumer warps, 16 keys of a tile each
+  static constexpr int kWarps = HD == 128 || NT == 1 ? 4 : 8;  // consumer warps
+  static constexpr int kSub = F8 && NT == 1 ? 2 : 1;  // 16 keys of a tile each, or two times 16
+  static constexpr int kTile = 16 * kSub * kWarps;    // keys
   static constexpr int kThreads = (kWarps + 2) * 32;
   static constexpr int kPanels = F8 ? 1 : HD / 64;
   static constexpr int kPanel = F8 ? kTile * HD : kTile * 128;
@@ -79,19 +80,17 @@ struct DShape {
   static_assert(kStages * 20 + 12 <= 256, "barriers and flags");
 };
 
-// The prefix kernel's results: positions of a piece; sums [piece][sequence][head][HD];
-// their reference and weight [piece][sequence][head][2].
-struct PrefixParts {
-  const int32_t* chunk;
-  const float* part;
-  const float* ml;
-};
+// Maps that 16-bit pages alone do without: the scales' (8-bit pages), K and V in copies
+// of 16 rows for tiles that are not whole.
 template <bool F8>
-struct ScaleMap {};
-template <>
-struct ScaleMap<true> {
-  CUtensorMap map;
+struct MoreMaps {
+  CUtensorMap k, v;
 };
+template <>
+struct MoreMaps<true> {
+  CUtensorMap k, v, s;
+};
+struct NoMaps {};
 template <bool F8, bool SH>
 struct DecodeParams {
   std::conditional_t<F8 || SH, PagedOwnArgs, PagedAttnArgs> a;
@@ -100,7 +99,8 @@ struct DecodeParams {
   float* part_ml;      // [2 * CTAs][G][2] their reference and weight
   int32_t G;
   int32_t box;         // rows of one TMA copy
-  PrefixParts pre;     // SH
+  PrefixParts pre;     // SH: own and own_ml are written
+  PrefixShape shape;
 };
 
 template <bool BF>
@@ -135,23 +135,23 @@ RPGC_DEV uint32_t transpose8(uint32_t x) {
 }
 
 // The list of key tiles: sequence by sequence, kv head by kv head.
-// What the token of sequence s sees (sight_of, without its group).
+// Positions [own, len) are what the token of sequence s sees of its pages.
 struct Seen {
-  int32_t len, own, pre;
+  int32_t len, own;
 };
 template <bool SH, typename Args>
-RPGC_DEV Seen seen(const Args& a, int s) {
+RPGC_DEV Seen seen(const Args& a, int s, int32_t kv_len, GroupAt& at) {
   if constexpr (SH) {
-    const Sight v = sight_of<true>(a, s);
-    return {v.len, v.own, v.pre};
+    const Sight v = sight_of<true>(a, s, kv_len, at);
+    return {v.len, v.own};
   } else {
-    const int64_t n = min((int64_t)max(0, a.b.kv_lens[s]), table_reach(a.kv, a.b));
-    return {(int32_t)n, 0, 0};
+    const int64_t n = min((int64_t)max(0, kv_len), table_reach(a.kv, a.b));
+    return {(int32_t)n, 0};
   }
 }
 // What an item weighs in the list: its key tiles, and the end of an item (the
 // warps' sums, a share's join) as kEnd tiles more, at its front.  An item that sees
-// nothing weighs nothing; one that sees a prefix alone has a front without tiles.
+// nothing weighs nothing.
 constexpr int kEnd = 3;
 // Pieces of an item, at most on average: with 8 kv heads of 128, one sequence of 4200
 // positions takes 11.6 us in 37 pieces and 10.0 in 18.  Only few long items meet the
@@ -165,7 +165,7 @@ RPGC_DEV int64_t tiles_of(const Seen& v) {  // from the tile on that holds its f
 }
 template <int T>
 RPGC_DEV int64_t weight_of(const Seen& v) {
-  return v.len > v.own || v.pre > 0 ? tiles_of<T>(v) + kEnd : 0;
+  return v.len > v.own ? tiles_of<T>(v) + kEnd : 0;
 }
 
 // One CTA's range of the list, item by item; every warp walks it by itself.
@@ -174,6 +174,7 @@ struct Walk {
   int64_t total, lo, hi;  // weight of the list; this CTA's range
   int32_t seq, kh;        // the item
   Seen at;                // what it sees
+  GroupAt group;          // SH: of the sequence looked up last
   int64_t i0, i1;         // its key tiles in the list
   int32_t t0, t1;         // those that are this CTA's, counted from at.own / T
   // where range b of n begins, and the range that holds place t
@@ -189,8 +190,10 @@ struct Walk {
     t0 = (int32_t)(lo > i0 ? lo - i0 : 0);
     t1 = (int32_t)((hi < i1 ? hi : i1) - i0);
   }
-  // whether this CTA has tiles of the item, or the end of one that has no tiles
-  RPGC_DEV bool mine() const { return t1 > t0 || (SH && i1 == i0 && hi >= i0); }
+  template <typename Args>
+  RPGC_DEV static int32_t length(const Args& a, int s) {
+    return s >= a.b.n_seqs ? 0 : SH ? __ldcg(a.b.kv_lens + s) : a.b.kv_lens[s];
+  }
   template <typename Args>
   RPGC_DEV bool start(const Args& a, int lane, int ctas, int cta, int* active) {
     const int64_t kv = a.kv.n_kv;
@@ -199,13 +202,19 @@ struct Walk {
     const int run = (a.b.n_seqs + 31) / 32;
     int64_t sum = 0;
     int32_t some = 0;
-    Seen ln = {0, 0, 0};
-#pragma unroll 4
-    for (int i = 0; i < run; ++i) {
-      const int s = lane * run + i;
-      ln = s < a.b.n_seqs ? seen<SH>(a, s) : Seen{0, 0, 0};
-      sum += weight_of<T>(ln);
-      some += ln.len > ln.own || ln.pre > 0;
+    Seen ln = {0, 0};
+    for (int i0 = 0; i0 < run; i0 += 4) {
+      int32_t n[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n[i] = length(a, i0 + i < run ? lane * run + i0 + i : a.b.n_seqs);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = lane * run + i0 + i;
+        if (i0 + i >= run) break;
+        ln = s < a.b.n_seqs ? seen<SH>(a, s, n[i], group) : Seen{0, 0};
+        sum += weight_of<T>(ln);
+        some += ln.len > ln.own;
+      }
     }
     sum *= kv;
     int64_t upto = scan(sum, lane);
@@ -221,7 +230,7 @@ struct Walk {
     int64_t before = __shfl_sync(0xffffffffu, upto - sum, src);  // weight of the sequences before s0
 #pragma unroll 1
     for (int s0 = src * run;; s0 += 32) {
-      if (run > 1) ln = s0 + lane < a.b.n_seqs ? seen<SH>(a, s0 + lane) : Seen{0, 0, 0};
+      if (run > 1) ln = s0 + lane < a.b.n_seqs ? seen<SH>(a, s0 + lane, length(a, s0 + lane), group) : Seen{0, 0};
       else ln = from(ln, (src + lane) & 31);  // (only lane 0's counts: the run is one sequence)
       const int64_t mine = weight_of<T>(ln) * kv;
       upto = scan(mine, lane);
@@ -240,8 +249,8 @@ struct Walk {
     }
   }
   RPGC_DEV static Seen from(const Seen& v, int lane) {
-    Seen r = {__shfl_sync(0xffffffffu, v.len, lane), 0, 0};
-    if (SH) r.own = __shfl_sync(0xffffffffu, v.own, lane), r.pre = __shfl_sync(0xffffffffu, v.pre, lane);
+    Seen r = {__shfl_sync(0xffffffffu, v.len, lane), 0};
+    if (SH) r.own = __shfl_sync(0xffffffffu, v.own, lane);
     return r;
   }
   RPGC_DEV int64_t scan(int64_t v, int lane) const {  // inclusive sums over the lanes
@@ -257,7 +266,7 @@ struct Walk {
     if (i1 >= hi) return false;
     if (++kh == a.kv.n_kv) {
       kh = 0;
-      do at = seen<SH>(a, ++seq);
+      do ++seq, at = seen<SH>(a, seq, length(a, seq), group);
       while (!weight_of<T>(at));  // (a later item exists: i1 < hi <= total)
     }
     item(i1);
@@ -270,11 +279,10 @@ RPGC_DEV void bar_consumers() {
   asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
 }
 
-// tm_s: the scales' map (F8).
 template <int HD, bool BF, int NT, bool F8, bool SH>
 __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F8>::kCtas)
     decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const __grid_constant__ ScaleMap<F8> tm_s, const __grid_constant__ DecodeParams<F8, SH> p) {
+                  const __grid_constant__ std::conditional_t<F8 || SH, MoreMaps<F8>, NoMaps> tm, const __grid_constant__ DecodeParams<F8, SH> p) {
   using S = DShape<HD, NT, F8>;
   constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps, kTile = S::kTile;
   constexpr bool MB = BF && !F8;             // the MMAs' type: bf16, else fp16
@@ -304,11 +312,12 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
   }
   if (warp == kWarps && lane < 2) prefetch_map(lane ? &tm_v : &tm_k);
   if constexpr (F8)
-    if (warp == kWarps && lane == 2) prefetch_map(&tm_s.map);
+    if (warp == kWarps && lane == 2) prefetch_map(&tm.s);
   __syncthreads();
   // launched as a programmatic dependent: nothing that a kernel wrote is read before
-  // this.  With a prefix the kernel before is the prefix's, which began its work after
-  // all that came earlier had ended: its results alone are waited for, at an item's end.
+  // this.  With a prefix the kernel before is the prefix's, whose results the next one
+  // reads, not this, and which let this one begin when all that came earlier had ended: it
+  // is waited for at the end, so that this kernel does not end before it.
   if (!SH) grid_dep_wait();
   grid_dep_launch();
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, a.b.status); };
@@ -347,6 +356,38 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
         const bool ok = (uint32_t)page < (uint32_t)a.kv.n_pages;
         if (!ok) page = a.kv.n_pages;  // past the pool: TMA fills zeros
         const uint32_t have = __ballot_sync(0xffffffffu, lane < per && ok);
+        const int at = (int)((base + (int64_t)(c + lane) * p.box) & ((1 << pshift) - 1));
+        const bool v = warp > kWarps;
+        uint8_t* dst = ring + st * S::kStage + (v ? S::kHalf : 0);
+        if constexpr (F8 || SH) {
+          // groups of 16 keys that the token sees; a tile that it does not see whole comes
+          // in copies of 16 rows, those alone
+          const int64_t tb = base + (int64_t)(t - t0) * kTile;
+          const int g0 = SH ? (int)max((int64_t)0, w.at.own - tb) >> 4 : 0, g1 = (int)min((int64_t)kTile, w.at.len - tb + 15) >> 4;
+          if (g0 > 0 || g1 < kTile / 16) {
+            int32_t fine = __shfl_sync(0xffffffffu, ids, (c + lane * 16 / p.box) & 31);
+            const bool in = lane >= g0 && lane < g1, there_is = (uint32_t)fine < (uint32_t)a.kv.n_pages;
+            if (!there_is) fine = a.kv.n_pages;
+            const uint32_t groups = __ballot_sync(0xffffffffu, in && there_is);
+            wait(empty + st, ph ^ 1u);
+            if (*gave_up) break;
+            if (lane == 0) {
+              if (warp == kWarps) there[st] = groups;
+              mbar_arrive_expect_tx(full + st, (g1 - g0) * (S::kHalf * 16 / kTile) + S::kScales);
+            }
+            __syncwarp();
+            if (in) {
+              const int at16 = (int)((tb + 16 * lane) & ((1 << pshift) - 1));
+#pragma unroll
+              for (int h = 0; h < S::kPanels; ++h)
+                tma_4d(dst + h * S::kPanel + lane * 16 * (F8 ? HD : 128), v ? &tm.v : &tm.k, 64 * h, w.kh, at16, fine, full + st);
+            }
+            if constexpr (F8)
+              if (lane < per) tma_4d(scales + (2 * st + v) * (S::kScaleRoom / 4) + lane * max(p.box, 32), &tm.s, at, v, w.kh, page, full + st);
+            if (++st == kStages) st = 0, ph ^= 1u;
+            continue;
+          }
+        }
         wait(empty + st, ph ^ 1u);
         if (*gave_up) break;
         if (lane == 0) {
@@ -359,12 +400,10 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
         }
         __syncwarp();
         if (lane < per) {
-          const int at = (int)((base + (int64_t)(c + lane) * p.box) & ((1 << pshift) - 1));
-          const bool v = warp > kWarps;
-          uint8_t* dst = ring + st * S::kStage + (v ? S::kHalf : 0) + lane * p.box * (F8 ? HD : 128);
 #pragma unroll
-          for (int h = 0; h < S::kPanels; ++h) tma_4d(dst + h * S::kPanel, v ? &tm_v : &tm_k, 64 * h, w.kh, at, page, full + st);
-          if constexpr (F8) tma_4d(scales + (2 * st + v) * (S::kScaleRoom / 4) + lane * max(p.box, 32), &tm_s.map, at, v, w.kh, page, full + st);
+          for (int h = 0; h < S::kPanels; ++h)
+            tma_4d(dst + h * S::kPanel + lane * p.box * (F8 ? HD : 128), v ? &tm_v : &tm_k, 64 * h, w.kh, at, page, full + st);
+          if constexpr (F8) tma_4d(scales + (2 * st + v) * (S::kScaleRoom / 4) + lane * max(p.box, 32), &tm.s, at, v, w.kh, page, full + st);
         }
         if (++st == kStages) st = 0, ph ^= 1u;
       }
@@ -380,8 +419,8 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
 
   // ----------------------------------------------------------- attention
   // sequences that see nothing: zeros, their rows dealt over the CTAs
-  for (int s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x)
-    if (weight_of<kTile>(seen<SH>(a, s)) == 0)
+  for (int s = blockIdx.x; !SH && s < a.b.n_seqs; s += gridDim.x)
+    if (min((int64_t)a.b.kv_lens[s], table_reach(a.kv, a.b)) <= 0)
       for (int i = tid; i < a.n_heads * HD / 8; i += kWarps * 32)
         reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)s * a.n_heads * HD)[i] = make_uint4(0, 0, 0, 0);
   if (!work) {
@@ -394,60 +433,29 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
   const int mi = lane >> 3, mr = lane & 7;
   const int krow = 16 * warp + mr + 8 * (mi & 1), kc = mi >> 1;
   const int vrow = 16 * warp + mr + 8 * (mi >> 1), vc = mi & 1;
-  // F8: 16-byte chunk c of row krow, in tiles of 128- or 64-byte rows
-  auto chunk8 = [&](uint32_t base, int c) {
-    return base + krow * HD + ((c ^ (HD == 128 ? krow & 7 : krow >> 1 & 3)) << 4);
+  // F8: 16-byte chunk c of this lane's row in group u of the warp's 16 keys, in tiles of 128- or 64-byte rows
+  auto chunk8 = [&](uint32_t base, int u, int c) {
+    const int row = 16 * ((S::kSub - 1) * warp + u) + krow;
+    return base + row * HD + ((c ^ (HD == 128 ? row & 7 : row >> 1 & 3)) << 4);
   };
   int st = 0;
   uint32_t ph = 0;
-  auto put = [&](int h, int d, const float4& acc, float L) {  // four values of the item's row of head h
+  auto put = [&](int h, int d, float M, const float4& acc, float L) {  // four values of the item's row of head h
+    if constexpr (SH) {  // its sums, for the kernel that joins them with the prefix's (weights are 2^(score - reference))
+      const int64_t row = (int64_t)w.seq * a.n_heads + w.kh * G + h;
+      __stcg(reinterpret_cast<float4*>(p.pre.own + row * HD + d), acc);
+      if (d == 0) __stcg(reinterpret_cast<float2*>(p.pre.own_ml) + row, make_float2(L == L ? M - kLift : 0.0f, L));  // (NaN stays: a score was)
+      return;
+    }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     uint16_t* op = static_cast<uint16_t*>(a.out) + ((int64_t)w.seq * a.n_heads + w.kh * G + h) * HD + d;
     *reinterpret_cast<uint2*>(op) = make_uint2(pack2<BF>(acc.x * inv, acc.y * inv), pack2<BF>(acc.z * inv, acc.w * inv));
     const float z = fmaf(acc.x, 0.0f, fmaf(acc.y, 0.0f, fmaf(acc.z, 0.0f, acc.w * 0.0f)));  // NaN: not all finite
     if (__builtin_expect(z != 0.0f && L < INFINITY, 0)) atomicOr(again, 1u << h);
   };
-  // SH: the sums over the item's prefix, piece by piece, join those over its own positions
-  auto join_prefix = [&](int h, int d, float M, float4& acc, float& L) {
-    if constexpr (SH) {
-      const int pieces = w.at.pre > 0 ? (w.at.pre - 1) / __ldcg(p.pre.chunk) + 1 : 0;
-      const int64_t row = (int64_t)w.seq * a.n_heads + w.kh * G + h, rows = (int64_t)a.b.n_seqs * a.n_heads;
-      float top = M - kLift;  // (weights are 2^(score - top))
-      for (int k0 = 0; k0 < pieces; k0 += kJoin) {
-        float2 ml[kJoin];
-        float4 v[kJoin];
-        float t = top;
-#pragma unroll
-        for (int k = 0; k < kJoin; ++k) {
-          const int64_t i = row + min(k0 + k, pieces - 1) * rows;
-          ml[k] = __ldcg(reinterpret_cast<const float2*>(p.pre.ml) + i);
-          v[k] = __ldcg(reinterpret_cast<const float4*>(p.pre.part + i * HD + d));
-        }
-#pragma unroll
-        for (int k = 0; k < kJoin; ++k) {
-          if (k0 + k >= pieces) ml[k].x = -INFINITY;
-          t = fmaxf(t, ml[k].x);
-        }
-        const float f = top == -INFINITY ? 0.0f : exp2_fast(top - t);
-        top = t;
-        acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-        L *= f;
-#pragma unroll
-        for (int k = 0; k < kJoin; ++k) {
-          if (ml[k].x == -INFINITY) continue;  // (saw nothing: what its sums hold counts for nothing)
-          const float f = exp2_fast(ml[k].x - top);
-          acc.x += f * v[k].x;
-          acc.y += f * v[k].y;
-          acc.z += f * v[k].z;
-          acc.w += f * v[k].w;
-          L += f * ml[k].y;
-        }
-      }
-    }
-  };
   do {
     const int t0 = w.t0, t1 = w.t1;
-    if (!w.mine()) continue;
+    if (t1 <= t0) continue;
     // Q^T as the B operand: head 8 n + gr, dims 16 k + 2 tq (+8)
     uint32_t q[NT][HD / 16][2];
     float cs[NT][2];  // F8: factors from scores to exponents, of heads 8 n + 2 tq (+1)
@@ -500,59 +508,69 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
     }
     for (int t = t0; t < t1; ++t) {
       wait(full + st, ph);
-      const int first = (t + (SH ? w.at.own / kTile : 0)) * kTile + 16 * warp;
+      const int first = (t + (SH ? w.at.own / kTile : 0)) * kTile + 16 * S::kSub * warp;
       const int left = w.at.len - first;          // keys of this warp's part
       const int skip = SH ? w.at.own - first : 0;  // those before that the prefix has
-      if (left > 0 && skip < 16 && (there[st] >> warp & 1u)) {
-        const uint32_t kb = smem_u32(ring + st * S::kStage), vb = kb + S::kHalf;
-        // two chains of MMAs, so that one's latency hides the other's
-        float s[NT][4], s2[NT][4];
+      if constexpr (F8) {
+        if (left > 0 && skip < 16 * S::kSub) {
+          constexpr int kSub = S::kSub, kChains = 2 / kSub;  // two chains of MMAs, so that one's latency hides the other's
+          const uint32_t kb = smem_u32(ring + st * S::kStage), vb = kb + S::kHalf, is = there[st] >> kSub * warp;
+          float s[kSub][kChains][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int u = 0; u < kSub; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.0f;
-        if constexpr (F8) {
+            for (int n = 0; n < NT * kChains * 4; ++n) (&s[u][0][0][0])[n] = 0.0f;
 #pragma unroll
-          for (int k = 0; k < HD / 16; k += 2) {
-            uint32_t f[4];
-            ldsm4(chunk8(kb, k + kc), f);
-            const uint32_t x[4] = {half2_lo(f[0]), half2_lo(f[1]), half2_hi(f[0]), half2_hi(f[1])};
-            const uint32_t y[4] = {half2_lo(f[2]), half2_lo(f[3]), half2_hi(f[2]), half2_hi(f[3])};
+          for (int k = 0; k < HD / 16; k += 2)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma<MB>(s[n], x, q[n][k][0], q[n][k][1]);
-              mma<MB>(s2[n], y, q[n][k + 1][0], q[n][k + 1][1]);
+            for (int u = 0; u < kSub; ++u) {
+              uint32_t f[4];
+              ldsm4(chunk8(kb, u, k + kc), f);
+              const uint32_t x[4] = {half2_lo(f[0]), half2_lo(f[1]), half2_hi(f[0]), half2_hi(f[1])};
+              const uint32_t y[4] = {half2_lo(f[2]), half2_lo(f[3]), half2_hi(f[2]), half2_hi(f[3])};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma<MB>(s[u][0][n], x, q[n][k][0], q[n][k][1]);
+                mma<MB>(s[u][kChains - 1][n], y, q[n][k + 1][0], q[n][k + 1][1]);
+              }
             }
-          }
-        } else {
+          // the first values (a load brings those of 32 dims) are on their way while the
+          // probabilities are made
+          constexpr int kLoads = HD / 32, kFirst = kAhead / kSub < kLoads ? kAhead / kSub : kLoads;
+          uint32_t v[kSub][kFirst][4];
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
-            uint32_t f[4];
-            ldsm4(kb + (k >> 2) * S::kPanel + krow * 128 + (((2 * (k & 3) + kc) ^ (krow & 7)) << 4), f);
+          for (int d = 0; d < kFirst; ++d)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma<MB>(k & 1 ? s2[n] : s[n], f, q[n][k][0], q[n][k][1]);
-          }
-        }
-        // the first values are on their way while the probabilities are made (F8: a load
-        // brings those of 32 dims)
-        constexpr int kLoads = F8 ? HD / 32 : HD / 16, kFirst = kAhead < kLoads ? kAhead : kLoads;
-        uint32_t v[kFirst][4];
-        auto load_v = [&](int d, uint32_t* f) {
-          ldsm4_t(F8 ? chunk8(vb, 2 * d + kc) : vb + (d >> 2) * S::kPanel + vrow * 128 + (((2 * (d & 3) + vc) ^ (vrow & 7)) << 4), f);
-        };
+            for (int u = 0; u < kSub; ++u) ldsm4_t(chunk8(vb, u, 2 * d + kc), v[u][d]);
+          // s: (key gr, head 2 tq), (gr, 2 tq + 1), (gr + 8, 2 tq), (gr + 8, 2 tq + 1)
+          bool in[kSub][2];
+          float vs[kSub][2];  // V's scales of keys gr, gr + 8 in units of vtop
+          const float* ks = scales + 2 * st * (S::kScaleRoom / 4) + (p.box == 16 ? 32 : 16) * kSub * warp + gr;
+          bool above = false, fresh = false;
 #pragma unroll
-        for (int d = 0; d < kFirst; ++d) load_v(d, v[d]);
-        // s: (key gr, head 2 tq), (gr, 2 tq + 1), (gr + 8, 2 tq), (gr + 8, 2 tq + 1)
-        const bool in0 = gr < left && gr >= skip, in1 = gr + 8 < left && gr + 8 >= skip;
-        float vs0 = 1.0f, vs1 = 1.0f;  // F8: V's scales of keys gr, gr + 8 in units of vtop
-        bool fresh = false;
-        if constexpr (F8) {
-          const float* ks = scales + 2 * st * (S::kScaleRoom / 4) + (p.box == 16 ? 32 : 16) * warp + gr;
-          const float* sv = ks + S::kScaleRoom / 4;
-          const float k0 = ks[0], k1 = ks[8];
-          vs0 = in0 ? sv[0] : 0.0f, vs1 = in1 ? sv[8] : 0.0f;
-          if (__any_sync(0xffffffffu, vs0 > vtop || vs1 > vtop)) {
-            const float t = warp_max(fmaxf(vs0, vs1));
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int key = 16 * u + 8 * e + gr;
+              in[u][e] = key < left && (!SH || key >= skip) && (is >> u & 1u);
+              const float* at = ks + (p.box == 16 ? 32 : 16) * u + 8 * e;
+              const float k = at[0] ;
+              vs[u][e] = in[u][e] ? at[S::kScaleRoom / 4] : 0.0f;
+              above |= vs[u][e] > vtop;
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  float& y = s[u][0][n][2 * e + j];
+                  if (kChains > 1) y += s[u][kChains - 1][n][2 * e + j];
+                  y = in[u][e] ? y * k * cs[n][j] : -INFINITY;
+                }
+            }
+          if (__any_sync(0xffffffffu, above)) {
+            float t = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) t = fmaxf(t, fmaxf(vs[u][0], vs[u][1]));
+            t = warp_max(t);
             const float up = __uint_as_float((uint32_t)min(max((int)(__float_as_uint(t) >> 23) + 1, 2), 252) << 23);
             const float f = vtop / up;
             vtop = up;
@@ -563,120 +581,227 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[n][d][e] *= f;
           }
-          const float down = vtop > 0.0f ? 1.0f / vtop : 0.0f;  // (a power of two: exact)
-          vs0 *= down, vs1 *= down;
+          const float down = vtop > 0.0f ? __uint_as_float(0x7f000000u - __float_as_uint(vtop)) : 0.0f;  // 1 / vtop, a power of two
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int u = 0; u < kSub; ++u) vs[u][0] *= down, vs[u][1] *= down;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[n][e] = (e < 2 ? in0 : in1) ? (s[n][e] + s2[n][e]) * (e < 2 ? k0 : k1) * cs[n][e & 1] : -INFINITY;
-        } else {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = (e < 2 ? in0 : in1) ? (s[n][e] + s2[n][e]) * c : -INFINITY;
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) fresh |= m[n][0] == -INFINITY || m[n][1] == -INFINITY;
-        // probabilities by the reference there is; where there is none yet, or one
-        // has outgrown it (or is NaN), the maximum becomes it and they are made again
-        float x[NT][4];
-        bool look = __any_sync(0xffffffffu, fresh);
-        uint32_t due = 0;  // F8, SH: heads (columns 8 n + 2 tq + e, bit 2 n + e) that need a reference
+          for (int n = 0; n < NT; ++n) fresh |= m[n][0] == -INFINITY || m[n][1] == -INFINITY;
+          // probabilities by the reference there is; where there is none yet, or one
+          // has outgrown it (or is NaN), the maximum becomes it and they are made again;
+          // the heads that are not due keep theirs, and with them every bit
+          float x[kSub][NT][4];
+          bool look = __any_sync(0xffffffffu, fresh);
+          uint32_t due = 0;  // heads (columns 8 n + 2 tq + e, bit 2 n + e) that need a reference
 #pragma unroll 1
-        for (;;) {
-          if (look) {
-            if (F8 || SH) {  // the others keep theirs, and with them every bit
+          for (;;) {
+            if (look) {
 #pragma unroll
               for (int n = 0; n < NT; ++n) due |= (m[n][0] == -INFINITY ? 1u : 0u) << 2 * n | (m[n][1] == -INFINITY ? 2u : 0u) << 2 * n;
               due |= __shfl_xor_sync(0xffffffffu, due, 4);
               due |= __shfl_xor_sync(0xffffffffu, due, 8);
               due |= __shfl_xor_sync(0xffffffffu, due, 16);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float t = m[n][e];
+#pragma unroll
+                  for (int u = 0; u < kSub; ++u) t = fmaxf(t, fmaxf(s[u][0][n][e], s[u][0][n][e + 2]));
+                  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                  if (!(due >> (2 * n + e) & 1u)) t = m[n][e];
+                  const float f = m[n][e] == -INFINITY ? 0.0f : t == m[n][e] ? 1.0f : exp2_fast(m[n][e] - t);
+                  m[n][e] = t;
+                  l[n][e] *= f;
+#pragma unroll
+                  for (int d = 0; d < HD / 16; ++d) {
+                    o[n][d][e] *= f;
+                    o[n][d][e + 2] *= f;
+                  }
+                }
             }
+            bool grown = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float t = fmaxf(s[n][e], s[n][e + 2]);
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-                t = fmaxf(t, m[n][e]);
-                if ((F8 || SH) && !(due >> (2 * n + e) & 1u)) t = m[n][e];
-                const float f = m[n][e] == -INFINITY ? 0.0f : (F8 || SH) && t == m[n][e] ? 1.0f : exp2_fast(m[n][e] - t);
-                m[n][e] = t;
-                l[n][e] *= f;
+              for (int e = 0; e < 4; ++e) {
+                const float base = (m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]) - kLift;
 #pragma unroll
-                for (int d = 0; d < HD / 16; ++d) {
-                  o[n][d][e] *= f;
-                  o[n][d][e + 2] *= f;
+                for (int u = 0; u < kSub; ++u) {
+                  x[u][n][e] = exp2_fast(s[u][0][n][e] - base);
+                  const bool g = !(x[u][n][e] <= kMost);
+                  grown |= g;
+                  due |= g ? 1u << (2 * n + (e & 1)) : 0u;
                 }
               }
+            if (look || !__any_sync(0xffffffffu, grown)) break;
+            look = true;
           }
-          bool grown = false;
+          // each weight, V's scale in it, as two fp16 values, itself rounded and what that
+          // left: the memory sets the pace here, so the second product costs nothing
+          uint32_t b[kSub][NT][2], b_lo[kSub][NT][2], keep[kSub][2];
+#pragma unroll
+          for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              l[n][0] += x[u][n][0] + x[u][n][2];
+              l[n][1] += x[u][n][1] + x[u][n][3];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float w0 = x[u][n][2 * e] * vs[u][e], w1 = x[u][n][2 * e + 1] * vs[u][e];
+                const uint32_t hi = pack2<MB>(w0, w1);
+                const float2 h = unpack2<MB>(hi);
+                b[u][n][e] = transpose8(hi);
+                b_lo[u][n][e] = transpose8(pack2<MB>(w0 - h.x, w1 - h.y));
+              }
+            }
+            // keys 2 tq, 2 tq + 1 (and + 8) of the V operand; what the token does not see is
+            // cleared, for 0 * NaN is NaN
+            keep[u][0] = keep[u][1] = is >> u & 1u ? 0xffffffffu : 0u;
+            if (left < 16 * kSub || skip > 0 || !(is >> u & 1u))
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = 16 * u + 8 * e + 2 * tq;
+                if (!(key < left && key >= skip)) keep[u][e] &= 0xffff0000u;
+                if (!(key + 1 < left && key + 1 >= skip)) keep[u][e] &= 0xffffu;
+              }
+          }
+#pragma unroll
+          for (int d = 0; d < kLoads; ++d)
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+              uint32_t f[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f[e] = v[u][d % kFirst][e];
+              if (d + kFirst < kLoads) ldsm4_t(chunk8(vb, u, 2 * (d + kFirst) + kc), v[u][d % kFirst]);
+              // a word holds dims 2 gr, 2 gr + 1 of keys 2 tq and 2 tq + 1: with the middle bytes
+              // changed over its halves are the two keys' codes of one dim.  So row gr of the
+              // operand is dim 2 gr, row gr + 8 dim 2 gr + 1.
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f[e] = __byte_perm(f[e] & keep[u][e & 1], 0u, 0x3120);
+              const uint32_t y[4] = {half2_lo(f[0]), half2_hi(f[0]), half2_lo(f[1]), half2_hi(f[1])};
+              const uint32_t z[4] = {half2_lo(f[2]), half2_hi(f[2]), half2_lo(f[3]), half2_hi(f[3])};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma<MB>(o[n][2 * d], y, b[u][n][0], b[u][n][1]);
+                mma<MB>(o[n][2 * d + 1], z, b[u][n][0], b[u][n][1]);
+                mma<MB>(o[n][2 * d], y, b_lo[u][n][0], b_lo[u][n][1]);
+                mma<MB>(o[n][2 * d + 1], z, b_lo[u][n][0], b_lo[u][n][1]);
+              }
+            }
+        }
+      } else {
+        if (left > 0 && skip < 16 && (there[st] >> warp & 1u)) {
+          const uint32_t kb = smem_u32(ring + st * S::kStage), vb = kb + S::kHalf;
+          // two chains of MMAs, so that one's latency hides the other's
+          float s[NT][4], s2[NT][4];
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[n][e] = exp2_fast(s[n][e] - ((m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]) - kLift));
-              grown |= !(x[n][e] <= kMost);
-              if (F8 || SH) due |= !(x[n][e] <= kMost) ? 1u << (2 * n + (e & 1)) : 0u;
-            }
-          if (look || !__any_sync(0xffffffffu, grown)) break;
-          look = true;
-        }
-        // each probability as two 16-bit values, itself rounded and what that left:
-        // the products with V keep 16 bits of it or more.  The memory sets the
-        // pace here, so the second product costs nothing; rounded to one value
-        // it would be as large an error as the output's own rounding.
-        uint32_t b[NT][2], b_lo[NT][2];
+            for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          l[n][0] += x[n][0] + x[n][2];
-          l[n][1] += x[n][1] + x[n][3];
-          if constexpr (F8) {  // V's scales are the weights' from here on
-            x[n][0] *= vs0, x[n][1] *= vs0;
-            x[n][2] *= vs1, x[n][3] *= vs1;
+          for (int k = 0; k < HD / 16; ++k) {
+            uint32_t f[4];
+            ldsm4(kb + (k >> 2) * S::kPanel + krow * 128 + (((2 * (k & 3) + kc) ^ (krow & 7)) << 4), f);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma<MB>(k & 1 ? s2[n] : s[n], f, q[n][k][0], q[n][k][1]);
+          }
+          // the first values are on their way while the probabilities are made
+          uint32_t v[kAhead][4];
+          auto load_v = [&](int d, uint32_t* f) {
+            ldsm4_t(vb + (d >> 2) * S::kPanel + vrow * 128 + (((2 * (d & 3) + vc) ^ (vrow & 7)) << 4), f);
+          };
+#pragma unroll
+          for (int d = 0; d < kAhead; ++d) load_v(d, v[d]);
+          // s: (key gr, head 2 tq), (gr, 2 tq + 1), (gr + 8, 2 tq), (gr + 8, 2 tq + 1)
+          const bool in0 = gr < left && gr >= skip, in1 = gr + 8 < left && gr + 8 >= skip;
+          bool fresh = false;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = (e < 2 ? in0 : in1) ? (s[n][e] + s2[n][e]) * c : -INFINITY;
+            fresh |= m[n][0] == -INFINITY || m[n][1] == -INFINITY;
+          }
+          // probabilities by the reference there is; where there is none yet, or one
+          // has outgrown it (or is NaN), the maximum becomes it and they are made again
+          float x[NT][4];
+          bool look = __any_sync(0xffffffffu, fresh);
+          uint32_t due = 0;  // F8, SH: heads (columns 8 n + 2 tq + e, bit 2 n + e) that need a reference
+#pragma unroll 1
+          for (;;) {
+            if (look) {
+              if (SH) {  // the others keep theirs, and with them every bit
+#pragma unroll
+                for (int n = 0; n < NT; ++n) due |= (m[n][0] == -INFINITY ? 1u : 0u) << 2 * n | (m[n][1] == -INFINITY ? 2u : 0u) << 2 * n;
+                due |= __shfl_xor_sync(0xffffffffu, due, 4);
+                due |= __shfl_xor_sync(0xffffffffu, due, 8);
+                due |= __shfl_xor_sync(0xffffffffu, due, 16);
+              }
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float t = fmaxf(s[n][e], s[n][e + 2]);
+                  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                  t = fmaxf(t, m[n][e]);
+                  if ((SH) && !(due >> (2 * n + e) & 1u)) t = m[n][e];
+                  const float f = m[n][e] == -INFINITY ? 0.0f : (SH) && t == m[n][e] ? 1.0f : exp2_fast(m[n][e] - t);
+                  m[n][e] = t;
+                  l[n][e] *= f;
+#pragma unroll
+                  for (int d = 0; d < HD / 16; ++d) {
+                    o[n][d][e] *= f;
+                    o[n][d][e + 2] *= f;
+                  }
+                }
+            }
+            bool grown = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                x[n][e] = exp2_fast(s[n][e] - ((m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]) - kLift));
+                grown |= !(x[n][e] <= kMost);
+                if (SH) due |= !(x[n][e] <= kMost) ? 1u << (2 * n + (e & 1)) : 0u;
+              }
+            if (look || !__any_sync(0xffffffffu, grown)) break;
+            look = true;
+          }
+          // each probability as two 16-bit values, itself rounded and what that left:
+          // the products with V keep 16 bits of it or more.  The memory sets the
+          // pace here, so the second product costs nothing; rounded to one value
+          // it would be as large an error as the output's own rounding.
+          uint32_t b[NT][2], b_lo[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            l[n][0] += x[n][0] + x[n][2];
+            l[n][1] += x[n][1] + x[n][3];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t hi = pack2<MB>(x[n][2 * e], x[n][2 * e + 1]);
+              const float2 h = unpack2<MB>(hi);
+              b[n][e] = transpose8(hi);
+              b_lo[n][e] = transpose8(pack2<MB>(x[n][2 * e] - h.x, x[n][2 * e + 1] - h.y));
+            }
+          }
+          // keys 2 tq, 2 tq + 1 (and + 8) of the V operand; what lies past the
+          // last position is cleared, for 0 * NaN is NaN
+          uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+          if (left < 16) {
+            keep0 = 2 * tq + 1 < left ? 0xffffffffu : 2 * tq < left ? 0xffffu : 0u;
+            keep1 = 2 * tq + 9 < left ? 0xffffffffu : 2 * tq + 8 < left ? 0xffffu : 0u;
+          }
+          if (SH && skip > 0) {  // (and what the prefix has)
+            keep0 &= 2 * tq >= skip ? 0xffffffffu : 2 * tq + 1 >= skip ? 0xffff0000u : 0u;
+            keep1 &= 2 * tq + 8 >= skip ? 0xffffffffu : 2 * tq + 9 >= skip ? 0xffff0000u : 0u;
           }
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t hi = pack2<MB>(x[n][2 * e], x[n][2 * e + 1]);
-            const float2 h = unpack2<MB>(hi);
-            b[n][e] = transpose8(hi);
-            b_lo[n][e] = transpose8(pack2<MB>(x[n][2 * e] - h.x, x[n][2 * e + 1] - h.y));
-          }
-        }
-        // keys 2 tq, 2 tq + 1 (and + 8) of the V operand; what lies past the
-        // last position is cleared, for 0 * NaN is NaN
-        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-        if (left < 16) {
-          keep0 = 2 * tq + 1 < left ? 0xffffffffu : 2 * tq < left ? 0xffffu : 0u;
-          keep1 = 2 * tq + 9 < left ? 0xffffffffu : 2 * tq + 8 < left ? 0xffffu : 0u;
-        }
-        if (SH && skip > 0) {  // (and what the prefix has)
-          keep0 &= 2 * tq >= skip ? 0xffffffffu : 2 * tq + 1 >= skip ? 0xffff0000u : 0u;
-          keep1 &= 2 * tq + 8 >= skip ? 0xffffffffu : 2 * tq + 9 >= skip ? 0xffff0000u : 0u;
-        }
-#pragma unroll
-        for (int d = 0; d < kLoads; ++d) {
-          uint32_t f[4] = {v[d % kFirst][0], v[d % kFirst][1], v[d % kFirst][2], v[d % kFirst][3]};
-          if (d + kFirst < kLoads) load_v(d + kFirst, v[d % kFirst]);
-          if constexpr (F8) {
-            // a word holds dims 2 gr, 2 gr + 1 of keys 2 tq and 2 tq + 1: with the middle bytes
-            // changed over its halves are the two keys' codes of one dim.  So row gr of the
-            // operand is dim 2 gr, row gr + 8 dim 2 gr + 1.
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = __byte_perm(f[e] & (e & 1 ? keep1 : keep0), 0u, 0x3120);
-            const uint32_t x4[4] = {half2_lo(f[0]), half2_hi(f[0]), half2_lo(f[1]), half2_hi(f[1])};
-            const uint32_t y4[4] = {half2_lo(f[2]), half2_hi(f[2]), half2_lo(f[3]), half2_hi(f[3])};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma<MB>(o[n][2 * d], x4, b[n][0], b[n][1]);
-              mma<MB>(o[n][2 * d], x4, b_lo[n][0], b_lo[n][1]);
-              mma<MB>(o[n][2 * d + 1], y4, b[n][0], b[n][1]);
-              mma<MB>(o[n][2 * d + 1], y4, b_lo[n][0], b_lo[n][1]);
-            }
-          } else {
+          for (int d = 0; d < HD / 16; ++d) {
+            uint32_t f[4] = {v[d % kAhead][0], v[d % kAhead][1], v[d % kAhead][2], v[d % kAhead][3]};
+            if (d + kAhead < HD / 16) load_v(d + kAhead, v[d % kAhead]);
             f[0] &= keep0;
             f[1] &= keep0;
             f[2] &= keep1;
@@ -715,7 +840,6 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
             row[16 * d + (F8 ? 1 : 8)] = F8 ? o[n][d][e + 2] * vtop : o[n][d][e + 2];
           }
       }
-    if (SH) grid_dep_wait();  // (the prefix's sums are there)
     bar_consumers<kWarps * 32>();
     const bool whole = w.i0 >= w.lo && w.i1 <= w.hi;
     const int slot = 2 * blockIdx.x + (w.lo < w.i0 ? 1 : 0);
@@ -738,8 +862,7 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
         L += f * wl[k * kHeads + h];
       }
       if (whole) {
-        if (SH) join_prefix(h, d, M, acc, L);
-        put(h, d, acc, L);
+        put(h, d, M, acc, L);
       } else {
         __stcg(reinterpret_cast<float4*>(p.part + ((int64_t)slot * G + h) * HD + d), acc);
         if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml) + (int64_t)slot * G + h, make_float2(M, L));
@@ -795,18 +918,17 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
               L += f * x.y;
             }
           }
-          if (SH) join_prefix(h, d, M, acc, L);
-          put(h, d, acc, L);
+          put(h, d, M, acc, L);
         }
       }
     }
     bar_consumers<kWarps * 32>();  // the merge buffer is free again
     // (attn_row inlined: a kernel that calls takes 0.2 us longer to begin)
-    const uint32_t todo = *again;
+    const uint32_t todo = SH ? 0u : *again;
     if (__builtin_expect(todo != 0, 0)) {
       for (int h = warp; h < G; h += kWarps)
         if (todo >> h & 1u) {
-          if constexpr (F8 || SH) own_row<HD, BF, F8, SH>(a, w.seq, w.kh * G + h, lane);
+          if constexpr (F8) own_row<HD, BF, F8, false>(a, w.seq, w.kh * G + h, lane);
           else attn_row<HD, BF>(a, w.seq, w.seq, w.kh * G + h, -1, lane);
         }
       bar_consumers<kWarps * 32>();
@@ -859,7 +981,7 @@ inline bool make_map_scales(CUtensorMap* m, const PagedOwnArgs& a, int box) {
 }
 
 template <int HD, bool BF, int NT, bool F8, bool SH, typename Args>
-cudaError_t decode_go(const Args& a, const PrefixParts& pre, cudaStream_t s) {
+cudaError_t decode_go(const Args& a, const PrefixParts& pre, const PrefixShape& shape, cudaStream_t s) {
   using S = DShape<HD, NT, F8>;
   const int ctas = decode_ctas<HD, NT, F8>(a.n_heads / a.kv.n_kv);
   DecodeParams<F8, SH> p{};
@@ -867,18 +989,21 @@ cudaError_t decode_go(const Args& a, const PrefixParts& pre, cudaStream_t s) {
   p.G = a.n_heads / a.kv.n_kv;
   p.box = (1 << a.kv.page_shift) < S::kTile ? 1 << a.kv.page_shift : S::kTile;
   p.pre = pre;
+  p.shape = shape;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.counters = reinterpret_cast<uint32_t*>(ws);
   p.part = reinterpret_cast<float*>(ws + counter_bytes());
   p.part_ml = p.part + (int64_t)2 * ctas * p.G * HD;
   CUtensorMap mk, mv;
-  ScaleMap<F8> ms{};
-  if constexpr (F8) {
-    if (!make_map8(&mk, a, false, p.box) || !make_map8(&mv, a, true, p.box) || !make_map_scales(&ms.map, a, p.box)) return cudaErrorInvalidValue;
-  } else {
-    const CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
-    if (!make_kv_map(&mk, a, false, p.box, promo) || !make_kv_map(&mv, a, true, p.box, promo)) return cudaErrorInvalidValue;
-  }
+  std::conditional_t<F8 || SH, MoreMaps<F8>, NoMaps> more{};
+  auto map = [&](CUtensorMap* m, bool v, int box) {
+    if constexpr (F8) return make_map8(m, a, v, box);
+    else return make_kv_map(m, a, v, box);
+  };
+  bool made = map(&mk, false, p.box) && map(&mv, true, p.box);
+  if constexpr (F8) made = made && make_map_scales(&more.s, a, p.box);
+  if constexpr (F8 || SH) made = made && map(&more.k, false, 16) && map(&more.v, true, 16);
+  if (!made) return cudaErrorInvalidValue;
   constexpr int smem = S::kSmem;
   static_assert(smem <= 233472 / S::kCtas - 1024, "shared memory of one CTA");
   int dev = 0;
@@ -890,16 +1015,16 @@ cudaError_t decode_go(const Args& a, const PrefixParts& pre, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(S::kThreads), smem, s, mk, mv, ms, p);
+  const cudaError_t e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(S::kThreads), smem, s, mk, mv, more, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
 
 template <bool F8, bool SH, typename Args>
-cudaError_t decode_any(const Args& a, const PrefixParts& pre, cudaStream_t s) {
+cudaError_t decode_any(const Args& a, const PrefixParts& pre, const PrefixShape& shape, cudaStream_t s) {
   auto heads = [&](auto hd, auto bf) {
-    return a.n_heads / a.kv.n_kv <= 8 ? decode_go<decltype(hd)::value, decltype(bf)::value, 1, F8, SH>(a, pre, s)
-                                      : decode_go<decltype(hd)::value, decltype(bf)::value, 2, F8, SH>(a, pre, s);
+    return a.n_heads / a.kv.n_kv <= 8 ? decode_go<decltype(hd)::value, decltype(bf)::value, 1, F8, SH>(a, pre, shape, s)
+                                      : decode_go<decltype(hd)::value, decltype(bf)::value, 2, F8, SH>(a, pre, shape, s);
   };
   using H64 = std::integral_constant<int, 64>;
   using H128 = std::integral_constant<int, 128>;

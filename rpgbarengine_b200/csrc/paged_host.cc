@@ -273,9 +273,7 @@ int own_decode(rpgc::PagedOwnArgs a, const rpgc_paged_batch* b, const rpgc_paged
           "paged decode attention");
     return RPGC_OK;
   }
-  check(rpgc::paged_prefix_launch(a, as_stream(stream)), "attention over the prefix");
-  check(a.scales ? rpgc::paged8_decode_prefix_launch(a, as_stream(stream)) : rpgc::paged_decode_prefix_launch(a, as_stream(stream)),
-        "paged decode attention");
+  check(rpgc::paged_prefix_decode_launch(a, as_stream(stream)), "paged decode attention");
   return RPGC_OK;
 }
 
