@@ -1,5 +1,5 @@
 // k_paged_join.cu -- single-token attention with a shared prefix: the workspace, the
-// launches of its three kernels, and the last of them, which joins the sums over the
+// launches of its four kernels, and the last of them, which joins the sums over the
 // pieces of a prefix with those over a sequence's own positions.
 //
 // Mathematics: out = sum_k 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k over the pieces k and the
@@ -11,6 +11,8 @@
 // own positions, 256 sequences x 32 heads in 4 pieces took 22 us).
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "paged8_dev.cuh"
 #include "paged_dev.cuh"
 #include "paged_tma.cuh"
@@ -21,11 +23,11 @@ namespace {
 using namespace paged;
 
 constexpr int kWarps = 4;  // of a block
-constexpr int kAtOnce = 8; // pieces whose sums are in flight together
+constexpr int kAtOnce = 4; // pieces whose sums are in flight together
 
 // HD / 4 lanes a row, four values each.
 template <int HD, bool BF, bool F8>
-__global__ void __launch_bounds__(kWarps * 32) join_kernel(const __grid_constant__ PagedOwnArgs a,
+__global__ void __launch_bounds__(kWarps * 32, 8) join_kernel(const __grid_constant__ PagedOwnArgs a,
                                                            const __grid_constant__ PrefixParts p) {
   constexpr int kLanes = HD / 4, kRows = 32 / kLanes;
   const int lane = threadIdx.x & 31, d = 4 * (lane % kLanes);
@@ -34,50 +36,55 @@ __global__ void __launch_bounds__(kWarps * 32) join_kernel(const __grid_constant
   grid_dep_launch();
   const bool in = row < rows;
   const int32_t s = in ? (int32_t)(row / a.n_heads) : 0;
-  // (lengths and groups: earlier kernels' than the two that this one follows, and those
-  // waited for them before they let this one begin)
-  GroupAt at;
-  const Sight v = in ? sight_of<true>(a, s, __ldcg(a.b.kv_lens + s), at) : Sight{0, 0, 0};
   grid_dep_wait();
-  const int32_t chunk = __ldcg(p.chunk), pieces = v.pre > 0 ? (v.pre - 1) / chunk + 1 : 0;
+  // (look-ups that all warps share go through L1: thousands of warps at one line of L2 took 6 us)
+  PrefixSeq v = {0, 0, 0, 0};
+  if (in) v = p.seqs[s];
   float M = -INFINITY, L = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (v.len > v.own) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.own_ml) + row);
-    acc = __ldcg(reinterpret_cast<const float4*>(p.own + row * HD + d));
-    M = ml.x;
-    L = ml.y;
-    if (M == -INFINITY) acc = make_float4(0.f, 0.f, 0.f, 0.f), L = 0.0f;  // (saw nothing: what its sums hold counts for nothing)
-  }
-  for (int k0 = 0; k0 < pieces; k0 += kAtOnce) {
-    float2 ml[kAtOnce];
-    float4 o[kAtOnce];
-    float top = M;
+  // the sums of `count` pieces, piece k at row at(k) of o and ml
+  auto join = [&](int count, const float* o_rows, const float* ml_rows, auto at) {
+    for (int k0 = 0; k0 < count; k0 += kAtOnce) {
+      float2 ml[kAtOnce];
+      float4 o[kAtOnce];
+      float top = M;
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int64_t i = row + (k0 + k) * rows;
-      ml[k] = make_float2(-INFINITY, 0.0f);
-      if (k0 + k < pieces) {
-        ml[k] = __ldcg(reinterpret_cast<const float2*>(p.ml) + i);
-        o[k] = __ldcg(reinterpret_cast<const float4*>(p.part + i * HD + d));
+      for (int k = 0; k < kAtOnce; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        if (k0 + k < count) {
+          const int64_t i = at(k0 + k);
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(ml_rows) + i);
+          o[k] = __ldcg(reinterpret_cast<const float4*>(o_rows + i * HD + d));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, ml[k].x);
+      const float c = M == -INFINITY ? 0.0f : exp2_fast(M - top);
+      acc.x *= c, acc.y *= c, acc.z *= c, acc.w *= c;
+      L *= c;
+      M = top;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        if (ml[k].x == -INFINITY) continue;  // (saw nothing: what its sums hold counts for nothing)
+        const float c = exp2_fast(ml[k].x - top);
+        acc.x += c * o[k].x;
+        acc.y += c * o[k].y;
+        acc.z += c * o[k].z;
+        acc.w += c * o[k].w;
+        L += c * ml[k].y;
       }
     }
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, ml[k].x);
-    const float c = M == -INFINITY ? 0.0f : exp2_fast(M - top);
-    acc.x *= c, acc.y *= c, acc.z *= c, acc.w *= c;
-    L *= c;
-    M = top;
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      if (ml[k].x == -INFINITY) continue;
-      const float c = exp2_fast(ml[k].x - top);
-      acc.x += c * o[k].x;
-      acc.y += c * o[k].y;
-      acc.z += c * o[k].z;
-      acc.w += c * o[k].w;
-      L += c * ml[k].y;
-    }
+  };
+  const int32_t chunk = p.head->chunk * kPrefixKeys, pieces = v.pre > 0 ? (v.pre - 1) / chunk + 1 : 0;
+  join(pieces, p.part, p.ml, [&](int k) { return row + k * rows; });
+  if (v.len > v.own) {
+    const int G = a.n_heads / a.kv.n_kv, h = (int)(row - (int64_t)s * a.n_heads);
+    const uint32_t rec = (uint32_t)__ldcg(p.pieces + (int64_t)s * a.kv.n_kv + h / G);
+    const int slot = rec & 0xffffu;
+    if (rec == 0) join(1, p.own, p.own_ml, [&](int) { return row; });
+    else
+      join(min((int)(rec >> 16), 1024), p.slots, p.slots_ml,
+           [&](int k) { return (int64_t)min(k ? (slot & ~1) + 2 * k : slot, p.n_slots - 1) * G + h % G; });
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   if (in)
@@ -109,24 +116,56 @@ int pieces_of(int32_t n_seqs, int32_t n_heads) {
   return n < 1 ? 1 : n > kPieces ? kPieces : (int)n;
 }
 
-// The workspace: single-token attention's, the length of a piece, the pieces' sums, the
-// own positions', then all references and weights.
-int64_t front_bytes(int32_t n_heads, int32_t n_kv, int32_t hd) {
+// Slots of items that several CTAs share: two for each CTA of the kernel before.
+int64_t slot_count() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) cudaGetLastError();
+  return 2 * 4 * sm_count(dev);
+}
+
+// The workspace: single-token attention's (for calls without a group), then what the four
+// kernels hand on.
+struct Places {
+  PrefixParts parts;
+  int64_t bytes;
+};
+Places places(uint8_t* base, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd) {
   PagedView v{};
   v.n_kv = n_kv;
   v.hd = hd;
-  return (paged_decode_workspace(v, n_heads) + 255) / 256 * 256 + 256;
+  const int64_t rows = (int64_t)n_seqs * n_heads, pieces = pieces_of(n_seqs, n_heads), slots = slot_count() * (n_heads / n_kv);
+  int64_t at = paged_decode_workspace(v, n_heads);
+  Places p;
+  auto take = [&](auto** to, int64_t n) {
+    at += (256 - (int64_t)((reinterpret_cast<uintptr_t>(base) + (uintptr_t)at) & 255)) % 256;  // (the workspace may begin on any 16 bytes)
+    *to = reinterpret_cast<std::remove_reference_t<decltype(*to)>>(base + at);
+    at += n * (int64_t)sizeof(**to);
+  };
+  take(&p.parts.head, 1);
+  take(&p.parts.units, slot_count());
+  take(&p.parts.starts, slot_count());
+  take(&p.parts.seqs, n_seqs);
+  take(&p.parts.cum, (int64_t)n_seqs + 1);
+  take(&p.parts.pieces, (int64_t)n_seqs * n_kv);
+  take(&p.parts.ml, 2 * pieces * rows);
+  take(&p.parts.own_ml, 2 * rows);
+  take(&p.parts.slots_ml, 2 * slots);
+  take(&p.parts.part, pieces * rows * hd);
+  take(&p.parts.own, rows * hd);
+  take(&p.parts.slots, slots * hd);
+  p.parts.n_slots = (int32_t)slot_count();
+  p.bytes = at + 256;
+  return p;
 }
 
 }  // namespace
 
 int64_t paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd) {
-  return front_bytes(n_heads, n_kv, hd) + (int64_t)(pieces_of(n_seqs, n_heads) + 1) * n_seqs * n_heads * (hd + 2) * 4;
+  return places(nullptr, n_seqs, n_heads, n_kv, hd).bytes;
 }
 
 cudaError_t paged_prefix_decode_launch(const PagedOwnArgs& a, cudaStream_t s) {
   const int G = a.n_heads / a.kv.n_kv;
-  const int64_t rows = (int64_t)a.b.n_seqs * a.n_heads;
   int dev = 0;
   cudaGetDevice(&dev);
   PrefixShape shape;
@@ -136,14 +175,11 @@ cudaError_t paged_prefix_decode_launch(const PagedOwnArgs& a, cudaStream_t s) {
   const int64_t reach = (((int64_t)a.pre.max_pages << a.pre.kv.page_shift) + kPrefixKeys - 1) / kPrefixKeys,
                 most = (a.b.n_seqs / (2 * shape.T) + a.pre.n_groups) * a.kv.n_kv * (reach < shape.pieces ? reach : shape.pieces);
   shape.ctas = (int32_t)(most < sm_count(dev) ? most : sm_count(dev));
-  uint8_t* w = static_cast<uint8_t*>(a.workspace) + front_bytes(a.n_heads, a.kv.n_kv, a.kv.hd);
-  PrefixParts p;
-  p.chunk = reinterpret_cast<int32_t*>(w - 256);
-  p.part = reinterpret_cast<float*>(w);
-  p.own = p.part + shape.pieces * rows * a.kv.hd;
-  p.ml = p.own + rows * a.kv.hd;
-  p.own_ml = p.ml + 2 * shape.pieces * rows;
-  cudaError_t e = paged_prefix_launch(a, p, shape, s);
+  if (a.scales) paged8_decode_prefix_shape(a, &shape);
+  else paged_decode_prefix_shape(a, &shape);
+  const PrefixParts p = places(static_cast<uint8_t*>(a.workspace), a.b.n_seqs, a.n_heads, a.kv.n_kv, a.kv.hd).parts;
+  cudaError_t e = paged_plan_launch(a, p, shape, s);
+  if (e == cudaSuccess) e = paged_prefix_launch(a, p, shape, s);
   if (e == cudaSuccess) e = a.scales ? paged8_decode_prefix_launch(a, p, shape, s) : paged_decode_prefix_launch(a, p, shape, s);
   if (e != cudaSuccess) return e;
   if (a.kv.hd == 128) e = a.kv.bf16 ? join_go<128, true>(a, p, s) : join_go<128, false>(a, p, s);

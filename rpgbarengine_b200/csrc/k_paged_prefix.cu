@@ -16,9 +16,7 @@
 // to accumulator A and the odd ones to B, and their sums meet at the end.  Warps 0-3 / 4-7:
 // softmax of A / B, one row per thread; warp 8: MMAs; warp 9: TMA; warp 10: finds the units.
 //
-// Pieces: all groups' prefixes are cut into pieces of one length, the one whose units
-// finish first by a count of tiles (`plan`): short pieces fill the SMs, but each writes
-// its rows' sums, 4 HD bytes a row, which are read again.
+// The plan (k_paged_plan.cu) says how long a piece is and has each CTA's first unit.
 #include <cuda_runtime.h>
 
 #include "paged8_dev.cuh"
@@ -40,14 +38,7 @@ constexpr int kUnits = 2;  // units in flight between the finder and the other w
 constexpr int kPoly = 1, kPolyOf = 8;  // of every 8 pairs of a row, those on the FMA pipe
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct Unit {
-  int32_t seq;         // tile A's first sequence; < 0: no more work
-  int32_t kh, group;
-  int32_t rows[2];     // sequences of tiles A and B
-  int32_t tile, tiles; // its key tiles
-  int32_t end;         // positions of the prefix that exist
-  int32_t piece;
-};
+using Unit = PrefixUnit;
 
 template <int HD>
 struct Shape {
@@ -66,10 +57,7 @@ struct PrefixParams {
   int32_t T;       // sequences of a tile
   int32_t G;       // heads per kv head
   int32_t box;     // K/V rows of one TMA copy
-  PrefixShape shape;
-  int32_t* chunk;  // positions of a piece, for the kernel that joins them
-  float* part;     // [piece][sequence][head][HD]
-  float* ml;       // [piece][sequence][head][2]
+  PrefixParts parts;
 };
 
 template <int HD, bool BF>
@@ -151,48 +139,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 10) {
       // ---------------------------------------------------- finds the units
-      const PrefixPlan pl = prefix_plan(a, p.shape, lane);
-      const int32_t chunk = pl.chunk, U = 2 * p.T, kv = a.kv.n_kv;
-      if (blockIdx.x == 0 && lane == 0) *p.chunk = chunk * kKeys;
+      // the first is the plan's; where there are more than CTAs (or groups than the plan
+      // looks through), the groups' units in a row, every grid-th of them
+      Unit un = p.parts.units[blockIdx.x];
+      const PrefixHead head = *p.parts.head;
       int g0 = 0;          // the groups from g0 on are still to be looked through
       int32_t before = 0;  // units of those before them
-      Share s = pl.mine;
       for (int it = 0;; ++it) {
-        const int32_t u = it * (int32_t)gridDim.x + (int32_t)blockIdx.x;
         if (it >= kUnits) wait(u_empty + it % kUnits, (uint32_t)((it / kUnits) - 1) & 1u);
-        Unit un;
-        un.seq = -1;
-        while (g0 < a.pre.n_groups) {
-          const int32_t tiles = tiles_of(s);
-          const int32_t mine = ((s.n + U - 1) / U) * ((tiles + chunk - 1) / chunk) * kv;
-          int32_t sum = mine;
+        const int32_t u = it * (int32_t)gridDim.x + (int32_t)blockIdx.x;
+        if (it || un.seq == -2) {
+          un.seq = -1;
+          while (u < head.units && g0 < a.pre.n_groups) {
+            const Share s = share_of(a, g0 + lane);
+            const int32_t mine = units_of(s, 2 * p.T, head.chunk, a.kv.n_kv);
+            int32_t sum = mine;
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += x;
+            for (int o = 1; o < 32; o <<= 1) {
+              const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
+              if (lane >= o) sum += x;
+            }
+            const uint32_t in = __ballot_sync(0xffffffffu, u - before < sum);
+            if (in) {
+              const int src = __ffs(in) - 1;
+              const Share of = {__shfl_sync(0xffffffffu, s.seq, src), __shfl_sync(0xffffffffu, s.n, src), __shfl_sync(0xffffffffu, s.end, src)};
+              un = unit_of(of, g0 + src, u - before - __shfl_sync(0xffffffffu, sum - mine, src), p.T, head.chunk, a.kv.n_kv);
+              break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+            g0 += 32;
           }
-          const uint32_t in = __ballot_sync(0xffffffffu, u - before < sum);
-          if (in) {
-            const int src = __ffs(in) - 1;
-            int32_t w = u - before - __shfl_sync(0xffffffffu, sum - mine, src);
-            const int32_t n = __shfl_sync(0xffffffffu, s.n, src), nt = __shfl_sync(0xffffffffu, tiles, src);
-            const int32_t R = (n + U - 1) / U;
-            un.kh = w % kv;
-            w /= kv;
-            const int32_t r = w % R;
-            un.piece = w / R;
-            un.group = g0 + src;
-            un.seq = __shfl_sync(0xffffffffu, s.seq, src) + r * U;
-            un.rows[0] = min(p.T, n - r * U);
-            un.rows[1] = max(0, min(p.T, n - r * U - p.T));
-            un.tile = un.piece * chunk;
-            un.tiles = min(chunk, nt - un.tile);
-            un.end = __shfl_sync(0xffffffffu, s.end, src);
-            break;
-          }
-          before += __shfl_sync(0xffffffffu, sum, 31);
-          g0 += 32;
-          s = share_of(a, g0 + lane);
         }
         if (lane == 0) {
           units[it % kUnits] = un;
@@ -408,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       // a row sees the prefix as far as its sequence goes; one that sees nothing of this
       // piece (or is none) has nothing to wait for and is not written
       const bool in = tok < (dual && g ? un.rows[1] : un.rows[0]);
-      const int lim = in ? min(max(0, a.b.kv_lens[seq]), un.end) : 0;
+      const int lim = in ? p.parts.seqs[seq].pre : 0;
       const bool live = lim > un.tile * kKeys;
       const int whole = (int)(__reduce_min_sync(0xffffffffu, live ? (unsigned)lim : 0x7fffffffu) / kKeys);  // key tiles that every live row sees whole
       float m = live ? -INFINITY : 0.0f, l = 0.0f;
@@ -539,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       tc_fence_after();
       // with one tile of rows, each group has half the columns to write
       const int col0 = dual ? 0 : HD / 2 * g, cols = dual ? HD : HD / 2;
-      float* out = p.part + row * HD + col0;
+      float* out = p.parts.part + row * HD + col0;
       const uint64_t mine2 = pair(mine, mine), other2 = pair(other, other);
       const bool have = dual || g < un.tiles, two = !dual && (g ^ 1) < un.tiles;
 #pragma unroll 1
@@ -574,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       if (live && (dual || g == 0)) {
         // weights are 2^(score - reference); a score that is NaN or +inf makes the row NaN
         const bool fine = m < INFINITY;
-        *reinterpret_cast<float2*>(p.ml + row * 2) =
+        *reinterpret_cast<float2*>(p.parts.ml + row * 2) =
             make_float2(l == 0.0f ? -INFINITY : fine ? m - kLift : 0.0f, fine ? l : __int_as_float(0x7fffffff));
       }
       tc_fence_before();
@@ -589,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
 }
 
 template <int HD, bool BF>
-cudaError_t prefix_go(const PagedOwnArgs& a, const PrefixParams& given, cudaStream_t s) {
+cudaError_t prefix_go(const PagedOwnArgs& a, const PrefixParams& given, int ctas, cudaStream_t s) {
   PrefixParams p = given;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -615,7 +591,7 @@ cudaError_t prefix_go(const PagedOwnArgs& a, const PrefixParams& given, cudaStre
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const cudaError_t e = launch_pdl(prefix_kernel<HD, BF>, dim3((unsigned)p.shape.ctas), dim3(kThreads), smem, s, mq, mk, mv, p);
+  const cudaError_t e = launch_pdl(prefix_kernel<HD, BF>, dim3((unsigned)ctas), dim3(kThreads), smem, s, mq, mk, mv, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
@@ -629,12 +605,9 @@ cudaError_t paged_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts,
   p.a = a;
   p.G = a.n_heads / a.kv.n_kv;
   p.T = shape.T;
-  p.shape = shape;
-  p.chunk = parts.chunk;
-  p.part = parts.part;
-  p.ml = parts.ml;
-  if (a.kv.hd == 128) return a.kv.bf16 ? prefix_go<128, true>(a, p, s) : prefix_go<128, false>(a, p, s);
-  return a.kv.bf16 ? prefix_go<64, true>(a, p, s) : prefix_go<64, false>(a, p, s);
+  p.parts = parts;
+  if (a.kv.hd == 128) return a.kv.bf16 ? prefix_go<128, true>(a, p, shape.ctas, s) : prefix_go<128, false>(a, p, shape.ctas, s);
+  return a.kv.bf16 ? prefix_go<64, true>(a, p, shape.ctas, s) : prefix_go<64, false>(a, p, shape.ctas, s);
 }
 
 }  // namespace rpgc

@@ -411,28 +411,69 @@ cudaError_t paged_read_launch(const PagedReadArgs& a, cudaStream_t s);
 cudaError_t paged_read_status(int32_t* bits);
 cudaError_t paged8_decode_launch(const PagedOwnArgs& a, cudaStream_t s);  // no prefix
 cudaError_t paged8_decode_status(int32_t* bits);
-// With a prefix, three kernels: sums over the prefixes, sums over the sequences' own
-// positions, and the two joined.
+// The list of key tiles of single-token attention (paged_decode.cuh): weight of an item's
+// end, pieces of an item at most on average.
+constexpr int kItemEnd = 3, kItemPieces = 18;
+// With a prefix, four kernels: the plan, sums over the prefixes, sums over the sequences'
+// own positions, and all of them joined.
+struct PrefixHead {
+  int32_t chunk;  // key tiles of a piece of a prefix
+  int32_t units;  // of the prefix kernel
+};
+struct PrefixSeq {  // what a sequence's token sees: positions [0, pre) of its group's prefix, [own, len) of its own pages
+  int32_t len, own, pre, pad;
+};
+struct PrefixUnit {
+  int32_t seq;          // tile A's first sequence; -1: no more units, -2: look for it
+  int32_t kh, group;
+  int32_t rows[2];      // sequences of tiles A and B
+  int32_t tile, tiles;  // its key tiles
+  int32_t end;          // positions of the prefix that exist
+  int32_t piece;
+  int32_t pad[3];
+};
+struct PrefixStart {  // a CTA's range of the list of own tiles, and the item that it begins in
+  int64_t lo, hi, first;
+  int32_t seq, kh;
+  int32_t len, own;
+  int32_t tail;       // pieces of the item that goes on past hi, where this CTA has its first tile
+  int32_t pad;
+};
 struct PrefixParts {
-  int32_t* chunk;  // positions of a piece of a prefix
-  float* part;     // [piece][sequence][head][hd] sums of weights times values
-  float* ml;       // [piece][sequence][head][2] their reference and weight
-  float* own;      // [sequence][head][hd] the same over own positions
+  PrefixHead* head;
+  PrefixSeq* seqs;
+  PrefixUnit* units;    // [CTAs] the first unit of each
+  PrefixStart* starts;  // [CTAs]
+  int64_t* cum;         // [n_seqs + 1] (the plan's own)
+  float* part;          // [piece][sequence][head][hd] sums of weights times values over a prefix
+  float* ml;            // [piece][sequence][head][2] their reference and weight
+  float* own;           // [sequence][head][hd] the same over own positions
   float* own_ml;
+  // own positions that several CTAs share: piece 0's slot | pieces << 16 of each sequence and
+  // kv head (0: one piece, in own), the slots' sums [slot][head of the group]
+  int32_t* pieces;
+  float* slots;
+  float* slots_ml;
+  int32_t n_slots;
 };
 struct PrefixShape {
   int32_t T;       // sequences of a tile of rows
   int32_t ctas;    // of the prefix kernel
   int32_t pieces;  // of a prefix, at most
+  // of the kernel over own positions: keys of a tile (its logarithm) and its bytes, CTAs, CTAs on an SM
+  int32_t tile_log, stage, own_ctas, on_sm;
 };
 int64_t paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd);
-cudaError_t paged_prefix_decode_launch(const PagedOwnArgs& a, cudaStream_t s);  // all three
+cudaError_t paged_prefix_decode_launch(const PagedOwnArgs& a, cudaStream_t s);  // all four
+cudaError_t paged_plan_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged_prefix_status(int32_t* bits);
 cudaError_t paged_decode_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged_decode_prefix_status(int32_t* bits);
+void paged_decode_prefix_shape(const PagedOwnArgs& a, PrefixShape* shape);
 cudaError_t paged8_decode_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged8_decode_prefix_status(int32_t* bits);
+void paged8_decode_prefix_shape(const PagedOwnArgs& a, PrefixShape* shape);
 int64_t paged_decode_workspace(const PagedView& kv, int32_t n_heads);
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s);
 cudaError_t prompt_attn_launch(const PagedAttnArgs& a, cudaStream_t s);

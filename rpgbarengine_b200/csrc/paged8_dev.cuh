@@ -40,112 +40,69 @@ RPGC_DEV float2 float2_lo(uint32_t w) { return unpack2<false>(half2_lo(w)); }
 RPGC_DEV float2 float2_hi(uint32_t w) { return unpack2<false>(half2_hi(w)); }
 
 // ------------------------------------------------------- shared prefixes
-// First sequence of group g, kept inside [0, n_seqs] whatever cu holds.
-RPGC_DEV int32_t group_seq(const PagedPrefix& p, int32_t n_seqs, int g) {
-  return min(max(__ldcg(p.cu + g), 0), n_seqs);
-}
-// A group (or none, -1) and the sequences that it holds; look-ups of sequences beside one
-// another go to memory once for each group.
-struct GroupAt {
-  int32_t group = -1, lo = 0, hi = 0;  // sequences [lo, hi)
-  int32_t len = 0;                     // of the group's prefix
-  RPGC_DEV void find(const PagedPrefix& p, int32_t n_seqs, int32_t s) {
-    if (s >= lo && s < hi) return;
-    int32_t a = 0, b = p.n_groups;  // the last group that begins at s or before is a - 1
-    while (a < b) {
-      const int32_t mid = (a + b) >> 1;
-      if (group_seq(p, n_seqs, mid) <= s) a = mid + 1;
-      else b = mid;
-    }
-    group = -1;
-    lo = s;
-    len = 0;
-    hi = group_seq(p, n_seqs, a);  // (a <= n_groups)
-    if (a > 0 && s < hi) {
-      group = a - 1;
-      len = max(0, __ldcg(p.lens + group));
-    } else if (s >= hi) {
-      hi = 0x7fffffff;  // behind all groups
-    }
-  }
-};
+constexpr int kPrefixKeys = 128;  // keys of a tile of the prefix kernel
 
-// What the token of a sequence sees: positions [0, pre) of its group's prefix (those
-// past the prefix's table are not there), then [own, len) of its own pages.
-struct Sight {
-  int32_t pre, own, len;
-};
-template <bool SH>
-RPGC_DEV Sight sight_of(const PagedOwnArgs& a, int32_t s, int32_t kv_len, GroupAt& at) {
-  const int32_t n = max(0, kv_len);
-  Sight v{0, 0, (int32_t)min((int64_t)n, table_reach(a.kv, a.b))};
-  if (SH) {
-    at.find(a.pre, a.b.n_seqs, s);
-    if (at.group >= 0) {
-      v.own = min(n, at.len);
-      v.pre = (int32_t)min((int64_t)v.own, (int64_t)a.pre.max_pages << a.pre.kv.page_shift);
-      v.len = max(v.len, v.own);
-    }
+// First sequence of group g, kept inside [0, n_seqs] whatever cu holds.
+RPGC_DEV int32_t group_seq(const PagedPrefix& p, int32_t n_seqs, int g) { return min(max(p.cu[g], 0), n_seqs); }
+// Group of sequence s, or -1: the last g with group_seq(g) <= s, where s is before the
+// next one's.
+template <typename F>
+RPGC_DEV int32_t group_of(int32_t n_groups, int32_t s, F first) {
+  int32_t a = 0, b = n_groups;  // it is a - 1 in the end
+  while (a < b) {
+    const int32_t mid = (a + b) >> 1;
+    if (first(mid) <= s) a = mid + 1;
+    else b = mid;
   }
+  return a > 0 && s < first(a) ? a - 1 : -1;
+}
+// What the token of a sequence of kv_len positions sees; len: its group's prefix (0: none).
+RPGC_DEV PrefixSeq sight_of(const PagedOwnArgs& a, int32_t kv_len, int32_t len) {
+  const int32_t n = max(0, kv_len);
+  PrefixSeq v;
+  v.own = min(n, max(0, len));
+  v.pre = (int32_t)min((int64_t)v.own, (int64_t)a.pre.max_pages << a.pre.kv.page_shift);
+  v.len = max((int32_t)min((int64_t)n, table_reach(a.kv, a.b)), v.own);
+  v.pad = 0;
   return v;
 }
 
-// ------------------------------------------- how prefixes are cut into units
-constexpr int kPrefixKeys = 128;  // keys of a tile of the prefix kernel
 struct Share {
   int32_t seq, n;  // a group's sequences
-  int32_t end;     // positions that exist
+  int32_t end;     // positions that exist, if there is a sequence to see them
 };
 RPGC_DEV Share share_of(const PagedOwnArgs& a, int g) {
   Share s{0, 0, 0};
   if (g < a.pre.n_groups) {
-    const int32_t len = __ldcg(a.pre.lens + g);
+    const int32_t len = max(0, a.pre.lens[g]);
     s.seq = group_seq(a.pre, a.b.n_seqs, g);
     s.n = max(0, group_seq(a.pre, a.b.n_seqs, g + 1) - s.seq);
-    s.end = s.n ? (int32_t)min((int64_t)max(0, len), (int64_t)a.pre.max_pages << a.pre.kv.page_shift) : 0;
+    s.end = s.n ? (int32_t)min((int64_t)len, (int64_t)a.pre.max_pages << a.pre.kv.page_shift) : 0;
   }
   return s;
 }
 RPGC_DEV int32_t tiles_of(const Share& s) { return (int32_t)(((int64_t)s.end + kPrefixKeys - 1) / kPrefixKeys); }
-
-// The key tiles of a piece, one number for all groups.  Lane k weighs the length that cuts
-// the longest prefix into k + 1 pieces: rounds of units over the CTAs, each a piece's tiles
-// (two for each where a unit has two tiles of rows) and kUnitCost for its begin and end.
-constexpr int kUnitCost = 8;
-struct PrefixPlan {
-  int32_t chunk;   // key tiles of a piece
-  int32_t rounds;  // of units
-  int32_t busy;    // CTAs that have some
-  Share mine;      // of group `lane`
-};
-RPGC_DEV PrefixPlan prefix_plan(const PagedOwnArgs& a, const PrefixShape& shape, int lane) {
-  PrefixPlan p;
-  p.mine = share_of(a, lane);
-  const int32_t n_groups = a.pre.n_groups, U = 2 * shape.T;
-  int32_t most = 0, rows = 0;
-  for (int g0 = 0; g0 < n_groups; g0 += 32) {
-    const Share s = g0 ? share_of(a, g0 + lane) : p.mine;
-    most = max(most, tiles_of(s));
-    rows = max(rows, s.n);
-  }
-  most = __reduce_max_sync(0xffffffffu, most);
-  rows = __reduce_max_sync(0xffffffffu, rows);
-  const int32_t c = max(1, (most + lane) / (lane + 1));
-  int32_t units = 0;  // (n_seqs x kv heads is less than 2^31, and pieces are few where it is large)
-  for (int g0 = 0; g0 < n_groups; g0 += 32) {
-    const Share s = g0 ? share_of(a, g0 + lane) : p.mine;
-    const int32_t R = (s.n + U - 1) / U, nt = tiles_of(s);
-    for (int i = 0; i < min(32, n_groups - g0); ++i) units += __shfl_sync(0xffffffffu, R, i) * ((__shfl_sync(0xffffffffu, nt, i) + c - 1) / c);
-  }
-  units *= a.kv.n_kv;
-  const int32_t rounds = (units + shape.ctas - 1) / shape.ctas;
-  const float cost = lane < shape.pieces ? (float)rounds * (float)(c * (rows > shape.T ? 2 : 1) + kUnitCost) : INFINITY;
-  const uint32_t best = __reduce_min_sync(0xffffffffu, __float_as_uint(cost));  // (positive floats in order)
-  const int src = __ffs(__ballot_sync(0xffffffffu, __float_as_uint(cost) == best)) - 1;
-  p.chunk = __shfl_sync(0xffffffffu, c, src);
-  p.rounds = __shfl_sync(0xffffffffu, rounds, src);
-  p.busy = min(__shfl_sync(0xffffffffu, units, src), shape.ctas);
-  return p;
+// Units of a group: rows of two tiles x pieces x kv heads.  (n_seqs x kv heads is less
+// than 2^31, and pieces are few where it is large.)
+RPGC_DEV int32_t units_of(const Share& s, int32_t U, int32_t chunk, int32_t n_kv) {
+  return (s.n + U - 1) / U * ((tiles_of(s) + chunk - 1) / chunk) * n_kv;
+}
+// Unit w of a group.
+RPGC_DEV PrefixUnit unit_of(const Share& s, int32_t group, int32_t w, int32_t T, int32_t chunk, int32_t n_kv) {
+  PrefixUnit un;
+  const int32_t U = 2 * T, R = (s.n + U - 1) / U;
+  un.kh = w % n_kv;
+  w /= n_kv;
+  const int32_t r = w % R;
+  un.piece = w / R;
+  un.group = group;
+  un.seq = s.seq + r * U;
+  un.rows[0] = min(T, s.n - r * U);
+  un.rows[1] = max(0, min(T, s.n - r * U - T));
+  un.tile = un.piece * chunk;
+  un.tiles = min(chunk, tiles_of(s) - un.tile);
+  un.end = s.end;
+  return un;
 }
 
 // Attention of sequence s's token and query head h by one warp, 32 keys a step, lane
@@ -240,12 +197,12 @@ template <int HD, bool BF, bool F8, bool SH>
 RPGC_DEV void own_row(const PagedOwnArgs& a, int32_t s, int h, int lane) {
   constexpr int E = HD / 32;
   const int kh = h / (a.n_heads / a.kv.n_kv);
-  GroupAt at;
-  const Sight v = sight_of<SH>(a, s, a.b.kv_lens[s], at);
+  const int32_t g = SH ? group_of(a.pre.n_groups, s, [&](int i) { return group_seq(a.pre, a.b.n_seqs, i); }) : -1;
+  const PrefixSeq v = sight_of(a, a.b.kv_lens[s], g >= 0 ? a.pre.lens[g] : 0);
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + s * a.q_tok + h * a.q_head;
   RowState<HD, BF> r;
   if (SH && v.pre > 0)
-    r.template keys<false>(a.pre.kv, nullptr, 0, 0, a.pre.table + at.group * a.pre.table_stride, a.pre.max_pages, q, a.scale, kh, 0,
+    r.template keys<false>(a.pre.kv, nullptr, 0, 0, a.pre.table + g * a.pre.table_stride, a.pre.max_pages, q, a.scale, kh, 0,
                            v.pre, lane);
   r.template keys<F8>(a.kv, a.scales, a.sc_page, a.sc_head, a.b.table + s * a.b.table_stride, a.b.max_pages, q, a.scale, kh, v.own,
                       v.len, lane);

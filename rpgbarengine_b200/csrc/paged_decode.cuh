@@ -56,14 +56,19 @@ constexpr int kJoin = 8;   // pieces of a share whose sums are in flight at once
 constexpr int kAhead = 4;  // V operands loaded ahead of the probabilities
 constexpr float kLog2e = 1.4426950408889634f;
 
-// F8: K and V as codes, a byte each.
-template <int HD, int NT, bool F8 = false>
+// F8: K and V as codes, a byte each.  Many: four small CTAs on an SM.  What ends an item
+// and begins the next are chains of dependent steps (q, the first tile's scores, the warps'
+// sums: 2500 clocks beside 1200 a tile), so with many short items, as the positions behind
+// a prefix are, four chains at once do what two do in twice the time.
+template <int HD, int NT, bool F8 = false, bool Many = false>
 struct DShape {
-  static constexpr int kCtas = NT == 1 ? 2 : 1;       // CTAs on an SM (NT 2: over 240 registers a thread leave room for one)
-  static constexpr int kWarps = HD == 128 || NT == 1 ? 4 : 8;  // consumer warps
+  static constexpr bool kMany = Many && NT == 1;
+  static constexpr int kCtas = NT > 1 ? 1 : kMany ? 4 : 2;  // CTAs on an SM (NT 2: over 240 registers a thread leave room for one)
+  static constexpr int kWarps = kMany ? 2 : HD == 128 || NT == 1 ? 4 : 8;  // consumer warps
+  static constexpr int kLoaders = kMany ? 1 : 2;      // warps that copy K and V, or one K, one V
   static constexpr int kSub = F8 && NT == 1 ? 2 : 1;  // 16 keys of a tile each, or two times 16
   static constexpr int kTile = 16 * kSub * kWarps;    // keys
-  static constexpr int kThreads = (kWarps + 2) * 32;
+  static constexpr int kThreads = (kWarps + kLoaders) * 32;
   static constexpr int kPanels = F8 ? 1 : HD / 64;
   static constexpr int kPanel = F8 ? kTile * HD : kTile * 128;
   static constexpr int kHalf = kPanels * kPanel;  // K (or V) of a tile
@@ -100,7 +105,6 @@ struct DecodeParams {
   int32_t G;
   int32_t box;         // rows of one TMA copy
   PrefixParts pre;     // SH: own and own_ml are written
-  PrefixShape shape;
 };
 
 template <bool BF>
@@ -135,30 +139,21 @@ RPGC_DEV uint32_t transpose8(uint32_t x) {
 }
 
 // The list of key tiles: sequence by sequence, kv head by kv head.
-// Positions [own, len) are what the token of sequence s sees of its pages.
+// Positions [own, len) are what the token of sequence s sees of its pages (own: those
+// before are a prefix's, SH).
 struct Seen {
   int32_t len, own;
 };
-template <bool SH, typename Args>
-RPGC_DEV Seen seen(const Args& a, int s, int32_t kv_len, GroupAt& at) {
-  if constexpr (SH) {
-    const Sight v = sight_of<true>(a, s, kv_len, at);
-    return {v.len, v.own};
-  } else {
-    const int64_t n = min((int64_t)max(0, kv_len), table_reach(a.kv, a.b));
-    return {(int32_t)n, 0};
-  }
-}
 // What an item weighs in the list: its key tiles, and the end of an item (the
 // warps' sums, a share's join) as kEnd tiles more, at its front.  An item that sees
 // nothing weighs nothing.
-constexpr int kEnd = 3;
+constexpr int kEnd = kItemEnd;
 // Pieces of an item, at most on average: with 8 kv heads of 128, one sequence of 4200
 // positions takes 11.6 us in 37 pieces and 10.0 in 18.  Only few long items meet the
 // bound, and those of fewer kv heads than 8 lose by it: one sequence of 131072
 // positions takes 90 us with 8 kv heads (6.0 TB/s), 81 with 4 (3.3 TB/s) and 89 with one
 // (0.76 TB/s, 18 CTAs at work).
-constexpr int kPieces = 18;
+constexpr int kPieces = kItemPieces;
 template <int T>
 RPGC_DEV int64_t tiles_of(const Seen& v) {  // from the tile on that holds its first own position
   return v.len > v.own ? (v.len + (int64_t)T - 1) / T - v.own / T : 0;
@@ -174,7 +169,7 @@ struct Walk {
   int64_t total, lo, hi;  // weight of the list; this CTA's range
   int32_t seq, kh;        // the item
   Seen at;                // what it sees
-  GroupAt group;          // SH: of the sequence looked up last
+  Seen ahead;             // SH: of the next sequence
   int64_t i0, i1;         // its key tiles in the list
   int32_t t0, t1;         // those that are this CTA's, counted from at.own / T
   // where range b of n begins, and the range that holds place t
@@ -191,8 +186,8 @@ struct Walk {
     t1 = (int32_t)((hi < i1 ? hi : i1) - i0);
   }
   template <typename Args>
-  RPGC_DEV static int32_t length(const Args& a, int s) {
-    return s >= a.b.n_seqs ? 0 : SH ? __ldcg(a.b.kv_lens + s) : a.b.kv_lens[s];
+  RPGC_DEV static Seen seen(const Args& a, int s) {
+    return s < a.b.n_seqs ? Seen{(int32_t)min((int64_t)max(0, a.b.kv_lens[s]), table_reach(a.kv, a.b)), 0} : Seen{0, 0};
   }
   template <typename Args>
   RPGC_DEV bool start(const Args& a, int lane, int ctas, int cta, int* active) {
@@ -203,18 +198,11 @@ struct Walk {
     int64_t sum = 0;
     int32_t some = 0;
     Seen ln = {0, 0};
-    for (int i0 = 0; i0 < run; i0 += 4) {
-      int32_t n[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) n[i] = length(a, i0 + i < run ? lane * run + i0 + i : a.b.n_seqs);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int s = lane * run + i0 + i;
-        if (i0 + i >= run) break;
-        ln = s < a.b.n_seqs ? seen<SH>(a, s, n[i], group) : Seen{0, 0};
-        sum += weight_of<T>(ln);
-        some += ln.len > ln.own;
-      }
+#pragma unroll 4
+    for (int i = 0; i < run; ++i) {
+      ln = seen(a, lane * run + i);
+      sum += weight_of<T>(ln);
+      some += ln.len > 0;
     }
     sum *= kv;
     int64_t upto = scan(sum, lane);
@@ -230,8 +218,8 @@ struct Walk {
     int64_t before = __shfl_sync(0xffffffffu, upto - sum, src);  // weight of the sequences before s0
 #pragma unroll 1
     for (int s0 = src * run;; s0 += 32) {
-      if (run > 1) ln = s0 + lane < a.b.n_seqs ? seen<SH>(a, s0 + lane, length(a, s0 + lane), group) : Seen{0, 0};
-      else ln = from(ln, (src + lane) & 31);  // (only lane 0's counts: the run is one sequence)
+      if (run > 1) ln = seen(a, s0 + lane);
+      else ln.len = __shfl_sync(0xffffffffu, ln.len, (src + lane) & 31);  // (only lane 0's counts: the run is one sequence)
       const int64_t mine = weight_of<T>(ln) * kv;
       upto = scan(mine, lane);
       const uint32_t in = __ballot_sync(0xffffffffu, before + upto > lo);
@@ -239,7 +227,7 @@ struct Walk {
         const int i = __ffs(in) - 1;
         const int64_t first = before + __shfl_sync(0xffffffffu, upto - mine, i);
         seq = s0 + i;
-        at = from(ln, i);
+        at = {__shfl_sync(0xffffffffu, ln.len, i), 0};
         const int64_t w = weight_of<T>(at), in_seq = lo - first;
         kh = in_seq < (int64_t)0x7fffffff ? (int32_t)((uint32_t)in_seq / (uint32_t)w) : (int32_t)(in_seq / w);
         item(first + kh * w);
@@ -248,10 +236,28 @@ struct Walk {
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  RPGC_DEV static Seen from(const Seen& v, int lane) {
-    Seen r = {__shfl_sync(0xffffffffu, v.len, lane), 0};
-    if (SH) r.own = __shfl_sync(0xffffffffu, v.own, lane);
-    return r;
+  // SH: from the plan (through L2: the kernel has not waited for the one before, which
+  // waited for the plan)
+  RPGC_DEV static Seen planned(const PrefixParts& p, int s, int n_seqs) {
+    if (s >= n_seqs) return {0, 0};
+    const int2 v = __ldcg(reinterpret_cast<const int2*>(p.seqs + s));
+    return {v.x, v.y};
+  }
+  template <typename Args>
+  RPGC_DEV bool start_planned(const Args& a, const PrefixParts& p, int cta, int* tail) {
+    const PrefixStart* r = p.starts + cta;
+    const longlong2 x = __ldcg(reinterpret_cast<const longlong2*>(r));
+    const int4 y = __ldcg(reinterpret_cast<const int4*>(r) + 1), z = __ldcg(reinterpret_cast<const int4*>(r) + 2);
+    lo = x.x;
+    hi = x.y;
+    if (lo >= hi) return false;
+    seq = y.z;
+    kh = y.w;
+    at = {z.x, z.y};
+    *tail = z.z;
+    ahead = planned(p, seq + 1, a.b.n_seqs);
+    item((int64_t)(((uint64_t)(uint32_t)y.y << 32) | (uint32_t)y.x));
+    return true;
   }
   RPGC_DEV int64_t scan(int64_t v, int lane) const {  // inclusive sums over the lanes
 #pragma unroll
@@ -262,12 +268,15 @@ struct Walk {
     return v;
   }
   template <typename Args>
-  RPGC_DEV bool next(const Args& a) {
+  RPGC_DEV bool next(const Args& a, const PrefixParts& p) {
     if (i1 >= hi) return false;
     if (++kh == a.kv.n_kv) {
       kh = 0;
-      do ++seq, at = seen<SH>(a, seq, length(a, seq), group);
-      while (!weight_of<T>(at));  // (a later item exists: i1 < hi <= total)
+      do {
+        ++seq;
+        if (SH) at = ahead, ahead = planned(p, seq + 1, a.b.n_seqs);
+        else at = seen(a, seq);
+      } while (!weight_of<T>(at));  // (a later item exists: i1 < hi <= total)
     }
     item(i1);
     return true;
@@ -280,10 +289,10 @@ RPGC_DEV void bar_consumers() {
 }
 
 template <int HD, bool BF, int NT, bool F8, bool SH>
-__global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F8>::kCtas)
+__global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, NT, F8, SH>::kCtas)
     decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                   const __grid_constant__ std::conditional_t<F8 || SH, MoreMaps<F8>, NoMaps> tm, const __grid_constant__ DecodeParams<F8, SH> p) {
-  using S = DShape<HD, NT, F8>;
+  using S = DShape<HD, NT, F8, SH>;
   constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps, kTile = S::kTile;
   constexpr bool MB = BF && !F8;             // the MMAs' type: bf16, else fp16
   constexpr float kLift = MB ? 0.0f : 6.0f;  // fp16 probabilities carry 2^6: small ones keep their bits
@@ -303,7 +312,7 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(full + i, 2);
+      mbar_init(full + i, S::kLoaders);
       mbar_init(empty + i, kWarps);
     }
     *gave_up = 0;
@@ -321,11 +330,11 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
   if (!SH) grid_dep_wait();
   grid_dep_launch();
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, a.b.status); };
-  int active;
+  int active;  // CTAs that have a range (SH: pieces of the range's last item)
   Walk<kTile, SH> w;
-  const bool work = w.start(a, lane, gridDim.x, blockIdx.x, &active);
+  const bool work = SH ? w.start_planned(a, p.pre, blockIdx.x, &active) : w.start(a, lane, gridDim.x, blockIdx.x, &active);
 
-  if (warp >= kWarps) {  // one warp copies K, the other V
+  if (warp >= kWarps) {  // one warp copies K, the other V (or one both)
     // ---------------------------------------------------------------- loads
     if (!work) {
       if (SH) grid_dep_wait();  // (so that this kernel ends after the prefix's)
@@ -357,8 +366,9 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
         if (!ok) page = a.kv.n_pages;  // past the pool: TMA fills zeros
         const uint32_t have = __ballot_sync(0xffffffffu, lane < per && ok);
         const int at = (int)((base + (int64_t)(c + lane) * p.box) & ((1 << pshift) - 1));
-        const bool v = warp > kWarps;
-        uint8_t* dst = ring + st * S::kStage + (v ? S::kHalf : 0);
+        constexpr int kBoth = 3 - S::kLoaders;  // of K and V, this warp's: from v0 on
+        const int v0 = warp - kWarps;
+        uint8_t* dst = ring + st * S::kStage;
         if constexpr (F8 || SH) {
           // groups of 16 keys that the token sees; a tile that it does not see whole comes
           // in copies of 16 rows, those alone
@@ -373,17 +383,20 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
             if (*gave_up) break;
             if (lane == 0) {
               if (warp == kWarps) there[st] = groups;
-              mbar_arrive_expect_tx(full + st, (g1 - g0) * (S::kHalf * 16 / kTile) + S::kScales);
+              mbar_arrive_expect_tx(full + st, kBoth * ((g1 - g0) * (S::kHalf * 16 / kTile) + S::kScales));
             }
             __syncwarp();
-            if (in) {
-              const int at16 = (int)((tb + 16 * lane) & ((1 << pshift) - 1));
 #pragma unroll
-              for (int h = 0; h < S::kPanels; ++h)
-                tma_4d(dst + h * S::kPanel + lane * 16 * (F8 ? HD : 128), v ? &tm.v : &tm.k, 64 * h, w.kh, at16, fine, full + st);
+            for (int v = v0; v < v0 + kBoth; ++v) {
+              if (in) {
+                const int at16 = (int)((tb + 16 * lane) & ((1 << pshift) - 1));
+#pragma unroll
+                for (int h = 0; h < S::kPanels; ++h)
+                  tma_4d(dst + v * S::kHalf + h * S::kPanel + lane * 16 * (F8 ? HD : 128), v ? &tm.v : &tm.k, 64 * h, w.kh, at16, fine, full + st);
+              }
+              if constexpr (F8)
+                if (lane < per) tma_4d(scales + (2 * st + v) * (S::kScaleRoom / 4) + lane * max(p.box, 32), &tm.s, at, v, w.kh, page, full + st);
             }
-            if constexpr (F8)
-              if (lane < per) tma_4d(scales + (2 * st + v) * (S::kScaleRoom / 4) + lane * max(p.box, 32), &tm.s, at, v, w.kh, page, full + st);
             if (++st == kStages) st = 0, ph ^= 1u;
             continue;
           }
@@ -396,19 +409,21 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
           for (int i = 0; i < per; ++i)
             if (have >> i & 1u) groups |= ((1u << g) - 1u) << (i * g);
           if (warp == kWarps) there[st] = groups;
-          mbar_arrive_expect_tx(full + st, S::kHalf + S::kScales);
+          mbar_arrive_expect_tx(full + st, kBoth * (S::kHalf + S::kScales));
         }
         __syncwarp();
-        if (lane < per) {
+        if (lane < per)
 #pragma unroll
-          for (int h = 0; h < S::kPanels; ++h)
-            tma_4d(dst + h * S::kPanel + lane * p.box * (F8 ? HD : 128), v ? &tm_v : &tm_k, 64 * h, w.kh, at, page, full + st);
-          if constexpr (F8) tma_4d(scales + (2 * st + v) * (S::kScaleRoom / 4) + lane * max(p.box, 32), &tm.s, at, v, w.kh, page, full + st);
-        }
+          for (int v = v0; v < v0 + kBoth; ++v) {
+#pragma unroll
+            for (int h = 0; h < S::kPanels; ++h)
+              tma_4d(dst + v * S::kHalf + h * S::kPanel + lane * p.box * (F8 ? HD : 128), v ? &tm_v : &tm_k, 64 * h, w.kh, at, page, full + st);
+            if constexpr (F8) tma_4d(scales + (2 * st + v) * (S::kScaleRoom / 4) + lane * max(p.box, 32), &tm.s, at, v, w.kh, page, full + st);
+          }
         if (++st == kStages) st = 0, ph ^= 1u;
       }
       if (*gave_up) break;
-    } while (w.next(a));
+    } while (w.next(a, p.pre));
     if (*gave_up)  // copies in flight end before the CTA does
       for (int i = 0; i < kStages; ++i)
         for (int k = 0; k < 1 << 12; ++k)
@@ -420,7 +435,7 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
   // ----------------------------------------------------------- attention
   // sequences that see nothing: zeros, their rows dealt over the CTAs
   for (int s = blockIdx.x; !SH && s < a.b.n_seqs; s += gridDim.x)
-    if (min((int64_t)a.b.kv_lens[s], table_reach(a.kv, a.b)) <= 0)
+    if (w.seen(a, s).len == 0)
       for (int i = tid; i < a.n_heads * HD / 8; i += kWarps * 32)
         reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)s * a.n_heads * HD)[i] = make_uint4(0, 0, 0, 0);
   if (!work) {
@@ -441,7 +456,7 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
   int st = 0;
   uint32_t ph = 0;
   auto put = [&](int h, int d, float M, const float4& acc, float L) {  // four values of the item's row of head h
-    if constexpr (SH) {  // its sums, for the kernel that joins them with the prefix's (weights are 2^(score - reference))
+    if constexpr (SH) {  // its sums, for the kernel that joins all of them (weights are 2^(score - reference))
       const int64_t row = (int64_t)w.seq * a.n_heads + w.kh * G + h;
       __stcg(reinterpret_cast<float4*>(p.pre.own + row * HD + d), acc);
       if (d == 0) __stcg(reinterpret_cast<float2*>(p.pre.own_ml) + row, make_float2(L == L ? M - kLift : 0.0f, L));  // (NaN stays: a score was)
@@ -865,10 +880,16 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
         put(h, d, M, acc, L);
       } else {
         __stcg(reinterpret_cast<float4*>(p.part + ((int64_t)slot * G + h) * HD + d), acc);
-        if (d == 0) __stcg(reinterpret_cast<float2*>(p.part_ml) + (int64_t)slot * G + h, make_float2(M, L));
+        if (d == 0)
+          __stcg(reinterpret_cast<float2*>(p.part_ml) + (int64_t)slot * G + h,
+                 SH ? make_float2(L == L ? M - kLift : 0.0f, L) : make_float2(M, L));
       }
     }
-    if (!whole) {
+    if constexpr (SH) {  // where the item's pieces are: piece 0's slot, piece k in the first slot of the k-th CTA from its own
+      if (tid == 0 && w.i0 >= w.lo)
+        p.pre.pieces[(int64_t)w.seq * a.kv.n_kv + w.kh] = whole ? 0 : slot | active << 16;
+    }
+    if (!SH && !whole) {
       // ---- the last CTA to finish a shared item joins its pieces
       const int b0 = w.holder(w.i0, active), b1 = w.holder(w.i1 - 1, active);
       bar_consumers<kWarps * 32>();
@@ -934,7 +955,7 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8>::kThreads, DShape<HD, NT, F
       bar_consumers<kWarps * 32>();
       if (tid == 0) *again = 0;
     }
-  } while (w.next(a));
+  } while (w.next(a, p.pre));
   if (SH) grid_dep_wait();
 }
 
@@ -955,6 +976,22 @@ int decode_ctas(int G) {
   using S = DShape<HD, NT, F8>;
   const int n = device_sms() * S::kCtas, most = S::kMerge / (8 * G);
   return n < most ? n : most;
+}
+
+// What the plan has to know of the kernel behind a prefix.
+template <int HD, int NT, bool F8>
+void own_shape(PrefixShape* s) {
+  using S = DShape<HD, NT, F8, true>;
+  for (s->tile_log = 0; 1 << s->tile_log < S::kTile;) ++s->tile_log;
+  s->stage = S::kStage;
+  s->on_sm = S::kCtas;
+  s->own_ctas = device_sms() * S::kCtas;
+}
+template <bool F8>
+void own_shape_of(const PagedOwnArgs& a, PrefixShape* s) {
+  const bool one = a.n_heads / a.kv.n_kv <= 8;
+  if (a.kv.hd == 128) one ? own_shape<128, 1, F8>(s) : own_shape<128, 2, F8>(s);
+  else one ? own_shape<64, 1, F8>(s) : own_shape<64, 2, F8>(s);
 }
 
 // K or V as codes, and the scales: {position, K or V, kv head, page}.
@@ -981,19 +1018,22 @@ inline bool make_map_scales(CUtensorMap* m, const PagedOwnArgs& a, int box) {
 }
 
 template <int HD, bool BF, int NT, bool F8, bool SH, typename Args>
-cudaError_t decode_go(const Args& a, const PrefixParts& pre, const PrefixShape& shape, cudaStream_t s) {
-  using S = DShape<HD, NT, F8>;
-  const int ctas = decode_ctas<HD, NT, F8>(a.n_heads / a.kv.n_kv);
+cudaError_t decode_go(const Args& a, const PrefixParts& pre, int own_ctas, cudaStream_t s) {
+  using S = DShape<HD, NT, F8, SH>;
+  const int ctas = SH ? own_ctas : decode_ctas<HD, NT, F8>(a.n_heads / a.kv.n_kv);
   DecodeParams<F8, SH> p{};
   p.a = a;
   p.G = a.n_heads / a.kv.n_kv;
   p.box = (1 << a.kv.page_shift) < S::kTile ? 1 << a.kv.page_shift : S::kTile;
   p.pre = pre;
-  p.shape = shape;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.counters = reinterpret_cast<uint32_t*>(ws);
   p.part = reinterpret_cast<float*>(ws + counter_bytes());
   p.part_ml = p.part + (int64_t)2 * ctas * p.G * HD;
+  if (SH) {
+    p.part = pre.slots;
+    p.part_ml = pre.slots_ml;
+  }
   CUtensorMap mk, mv;
   std::conditional_t<F8 || SH, MoreMaps<F8>, NoMaps> more{};
   auto map = [&](CUtensorMap* m, bool v, int box) {
@@ -1021,10 +1061,10 @@ cudaError_t decode_go(const Args& a, const PrefixParts& pre, const PrefixShape& 
 }
 
 template <bool F8, bool SH, typename Args>
-cudaError_t decode_any(const Args& a, const PrefixParts& pre, const PrefixShape& shape, cudaStream_t s) {
+cudaError_t decode_any(const Args& a, const PrefixParts& pre, int own_ctas, cudaStream_t s) {
   auto heads = [&](auto hd, auto bf) {
-    return a.n_heads / a.kv.n_kv <= 8 ? decode_go<decltype(hd)::value, decltype(bf)::value, 1, F8, SH>(a, pre, shape, s)
-                                      : decode_go<decltype(hd)::value, decltype(bf)::value, 2, F8, SH>(a, pre, shape, s);
+    return a.n_heads / a.kv.n_kv <= 8 ? decode_go<decltype(hd)::value, decltype(bf)::value, 1, F8, SH>(a, pre, own_ctas, s)
+                                      : decode_go<decltype(hd)::value, decltype(bf)::value, 2, F8, SH>(a, pre, own_ctas, s);
   };
   using H64 = std::integral_constant<int, 64>;
   using H128 = std::integral_constant<int, 128>;
