@@ -23,7 +23,7 @@ namespace {
 using namespace paged;
 
 constexpr int kWarps = 4;  // of a block
-constexpr int kAtOnce = 4; // pieces whose sums are in flight together
+constexpr int kAtOnce = 5; // pieces whose sums are in flight together
 
 // HD / 4 lanes a row, four values each.
 template <int HD, bool BF, bool F8>
@@ -38,12 +38,17 @@ __global__ void __launch_bounds__(kWarps * 32, 8) join_kernel(const __grid_const
   const int32_t s = in ? (int32_t)(row / a.n_heads) : 0;
   grid_dep_wait();
   // (look-ups that all warps share go through L1: thousands of warps at one line of L2 took 6 us)
-  PrefixSeq v = {0, 0, 0, 0};
-  if (in) v = p.seqs[s];
+  PrefixSeq v = {0, 0, 0, 1};
+  uint32_t rec = 0;
+  const int G = a.n_heads / a.kv.n_kv, h = (int)(row - (int64_t)s * a.n_heads);
+  if (in) {
+    v = p.seqs[s];
+    rec = (uint32_t)p.pieces[(int64_t)s * a.kv.n_kv + h / G];
+  }
   float M = -INFINITY, L = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  // the sums of `count` pieces, piece k at row at(k) of o and ml
-  auto join = [&](int count, const float* o_rows, const float* ml_rows, auto at) {
+  // the sums of `count` pieces, piece k at row at(k) of the arrays that it names
+  auto join = [&](int count, auto at) {
     for (int k0 = 0; k0 < count; k0 += kAtOnce) {
       float2 ml[kAtOnce];
       float4 o[kAtOnce];
@@ -52,9 +57,10 @@ __global__ void __launch_bounds__(kWarps * 32, 8) join_kernel(const __grid_const
       for (int k = 0; k < kAtOnce; ++k) {
         ml[k] = make_float2(-INFINITY, 0.0f);
         if (k0 + k < count) {
-          const int64_t i = at(k0 + k);
-          ml[k] = __ldcg(reinterpret_cast<const float2*>(ml_rows) + i);
-          o[k] = __ldcg(reinterpret_cast<const float4*>(o_rows + i * HD + d));
+          const float *os, *mls;
+          const int64_t i = at(k0 + k, &os, &mls);
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(mls) + i);
+          o[k] = __ldcg(reinterpret_cast<const float4*>(os + i * HD + d));
         }
       }
 #pragma unroll
@@ -75,17 +81,15 @@ __global__ void __launch_bounds__(kWarps * 32, 8) join_kernel(const __grid_const
       }
     }
   };
-  const int32_t chunk = p.head->chunk * kPrefixKeys, pieces = v.pre > 0 ? (v.pre - 1) / chunk + 1 : 0;
-  join(pieces, p.part, p.ml, [&](int k) { return row + k * rows; });
-  if (v.len > v.own) {
-    const int G = a.n_heads / a.kv.n_kv, h = (int)(row - (int64_t)s * a.n_heads);
-    const uint32_t rec = (uint32_t)__ldcg(p.pieces + (int64_t)s * a.kv.n_kv + h / G);
-    const int slot = rec & 0xffffu;
-    if (rec == 0) join(1, p.own, p.own_ml, [&](int) { return row; });
-    else
-      join(min((int)(rec >> 16), 1024), p.slots, p.slots_ml,
-           [&](int k) { return (int64_t)min(k ? (slot & ~1) + 2 * k : slot, p.n_slots - 1) * G + h % G; });
-  }
+  // the prefix's pieces, then the own positions' (one, or those of an item that CTAs shared)
+  const int pieces = v.pre > 0 ? (v.pre - 1) / v.chunk + 1 : 0, slot = rec & 0xffffu;
+  const int own = v.len > v.own ? (rec ? min((int)(rec >> 16), 1024) : 1) : 0;
+  join(pieces + own, [&](int k, const float** os, const float** mls) {
+    const int j = k - pieces;
+    *os = j < 0 ? p.part : rec ? p.slots : p.own;
+    *mls = j < 0 ? p.ml : rec ? p.slots_ml : p.own_ml;
+    return j < 0 ? row + k * rows : rec ? (int64_t)min(j ? (slot & ~1) + 2 * j : slot, p.n_slots - 1) * G + h % G : row;
+  });
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   if (in)
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * HD + d) =
@@ -108,11 +112,14 @@ cudaError_t join_go(const PagedOwnArgs& a, const PrefixParts& p, cudaStream_t s)
                   : launch_pdl(join_kernel<HD, BF, false>, grid, block, 0, s, a, p);
 }
 
-// Pieces of a prefix that the workspace has room for: fewer for more rows, whose units
-// fill the SMs with longer ones (148 SMs, two tiles of 128 rows each, twice over).
-constexpr int kPieces = 32;  // (a lane of the plan for each)
-int pieces_of(int32_t n_seqs, int32_t n_heads) {
-  const int64_t rows = (int64_t)(n_seqs > 0 ? n_seqs : 1) * n_heads, n = 75776 / rows;
+// Pieces of a prefix: as many as fill the SMs once, a unit (two tiles of rows of a group
+// and kv head, a piece) each.  A group with few sequences has a unit of its own for the few.
+constexpr int kPieces = 32;  // at most (a piece's sums are written and read again)
+int pieces_of(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t n_groups) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) cudaGetLastError();
+  const int64_t U = 2 * (128 / (n_heads / n_kv)), rows = (n_seqs + U - 1) / U, units = (rows > n_groups ? rows : n_groups) * n_kv;
+  const int64_t n = sm_count(dev) / (units > 0 ? units : 1);
   return n < 1 ? 1 : n > kPieces ? kPieces : (int)n;
 }
 
@@ -129,11 +136,11 @@ struct Places {
   PrefixParts parts;
   int64_t bytes;
 };
-Places places(uint8_t* base, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd) {
+Places places(uint8_t* base, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd, int32_t n_groups) {
   PagedView v{};
   v.n_kv = n_kv;
   v.hd = hd;
-  const int64_t rows = (int64_t)n_seqs * n_heads, pieces = pieces_of(n_seqs, n_heads), slots = slot_count() * (n_heads / n_kv);
+  const int64_t rows = (int64_t)n_seqs * n_heads, pieces = pieces_of(n_seqs, n_heads, n_kv, n_groups), slots = slot_count() * (n_heads / n_kv);
   int64_t at = paged_decode_workspace(v, n_heads);
   Places p;
   auto take = [&](auto** to, int64_t n) {
@@ -141,8 +148,6 @@ Places places(uint8_t* base, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int3
     *to = reinterpret_cast<std::remove_reference_t<decltype(*to)>>(base + at);
     at += n * (int64_t)sizeof(**to);
   };
-  take(&p.parts.head, 1);
-  take(&p.parts.units, slot_count());
   take(&p.parts.starts, slot_count());
   take(&p.parts.seqs, n_seqs);
   take(&p.parts.cum, (int64_t)n_seqs + 1);
@@ -161,7 +166,7 @@ Places places(uint8_t* base, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int3
 }  // namespace
 
 int64_t paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t hd) {
-  return places(nullptr, n_seqs, n_heads, n_kv, hd).bytes;
+  return places(nullptr, n_seqs, n_heads, n_kv, hd, 0).bytes;  // (more groups, fewer pieces)
 }
 
 cudaError_t paged_prefix_decode_launch(const PagedOwnArgs& a, cudaStream_t s) {
@@ -170,14 +175,14 @@ cudaError_t paged_prefix_decode_launch(const PagedOwnArgs& a, cudaStream_t s) {
   cudaGetDevice(&dev);
   PrefixShape shape;
   shape.T = 128 / G;
-  shape.pieces = pieces_of(a.b.n_seqs, a.n_heads);
+  shape.pieces = pieces_of(a.b.n_seqs, a.n_heads, a.kv.n_kv, a.pre.n_groups);
   // as many CTAs as may have a unit: the others' SMs are free for the next kernel at once
   const int64_t reach = (((int64_t)a.pre.max_pages << a.pre.kv.page_shift) + kPrefixKeys - 1) / kPrefixKeys,
                 most = (a.b.n_seqs / (2 * shape.T) + a.pre.n_groups) * a.kv.n_kv * (reach < shape.pieces ? reach : shape.pieces);
   shape.ctas = (int32_t)(most < sm_count(dev) ? most : sm_count(dev));
   if (a.scales) paged8_decode_prefix_shape(a, &shape);
   else paged_decode_prefix_shape(a, &shape);
-  const PrefixParts p = places(static_cast<uint8_t*>(a.workspace), a.b.n_seqs, a.n_heads, a.kv.n_kv, a.kv.hd).parts;
+  const PrefixParts p = places(static_cast<uint8_t*>(a.workspace), a.b.n_seqs, a.n_heads, a.kv.n_kv, a.kv.hd, a.pre.n_groups).parts;
   cudaError_t e = paged_plan_launch(a, p, shape, s);
   if (e == cudaSuccess) e = paged_prefix_launch(a, p, shape, s);
   if (e == cudaSuccess) e = a.scales ? paged8_decode_prefix_launch(a, p, shape, s) : paged_decode_prefix_launch(a, p, shape, s);

@@ -16,7 +16,7 @@
 // to accumulator A and the odd ones to B, and their sums meet at the end.  Warps 0-3 / 4-7:
 // softmax of A / B, one row per thread; warp 8: MMAs; warp 9: TMA; warp 10: finds the units.
 //
-// The plan (k_paged_plan.cu) says how long a piece is and has each CTA's first unit.
+// A prefix is cut into as many pieces as fill the SMs once, by the host's count of rows.
 #include <cuda_runtime.h>
 
 #include "paged8_dev.cuh"
@@ -38,7 +38,14 @@ constexpr int kUnits = 2;  // units in flight between the finder and the other w
 constexpr int kPoly = 1, kPolyOf = 8;  // of every 8 pairs of a row, those on the FMA pipe
 constexpr float kLog2e = 1.4426950408889634f;
 
-using Unit = PrefixUnit;
+struct Unit {
+  int32_t seq;          // tile A's first sequence; < 0: no more work
+  int32_t kh, group;
+  int32_t rows[2];      // sequences of tiles A and B
+  int32_t tile, tiles;  // its key tiles
+  int32_t end;          // positions of the prefix that exist
+  int32_t piece;
+};
 
 template <int HD>
 struct Shape {
@@ -57,6 +64,7 @@ struct PrefixParams {
   int32_t T;       // sequences of a tile
   int32_t G;       // heads per kv head
   int32_t box;     // K/V rows of one TMA copy
+  int32_t pieces;  // of a prefix
   PrefixParts parts;
 };
 
@@ -126,10 +134,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // launched as a programmatic dependent; the kernel that joins the pieces relies on this
-  // one having waited here before it lets that one begin
-  grid_dep_wait();
-  grid_dep_launch();
+  // launched as a programmatic dependent of the plan, which it does not need itself and
+  // which let it begin when all that came earlier had ended: it waits for nothing, and what it
+  // reads comes from L2, by TMA or __ldcg
   const uint32_t tmem = *tslot;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, status); };
 
@@ -139,36 +146,44 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 10) {
       // ---------------------------------------------------- finds the units
-      // the first is the plan's; where there are more than CTAs (or groups than the plan
-      // looks through), the groups' units in a row, every grid-th of them
-      Unit un = p.parts.units[blockIdx.x];
-      const PrefixHead head = *p.parts.head;
       int g0 = 0;          // the groups from g0 on are still to be looked through
       int32_t before = 0;  // units of those before them
+      Share s = share_of<true>(a, lane);
       for (int it = 0;; ++it) {
         if (it >= kUnits) wait(u_empty + it % kUnits, (uint32_t)((it / kUnits) - 1) & 1u);
         const int32_t u = it * (int32_t)gridDim.x + (int32_t)blockIdx.x;
-        if (it || un.seq == -2) {
-          un.seq = -1;
-          while (u < head.units && g0 < a.pre.n_groups) {
-            const Share s = share_of(a, g0 + lane);
-            const int32_t mine = units_of(s, 2 * p.T, head.chunk, a.kv.n_kv);
-            int32_t sum = mine;
+        Unit un;
+        un.seq = -1;
+        while (g0 < a.pre.n_groups) {
+          const int32_t mine = units_of(s, p.T, p.pieces, a.kv.n_kv);
+          int32_t sum = mine;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
-              if (lane >= o) sum += x;
-            }
-            const uint32_t in = __ballot_sync(0xffffffffu, u - before < sum);
-            if (in) {
-              const int src = __ffs(in) - 1;
-              const Share of = {__shfl_sync(0xffffffffu, s.seq, src), __shfl_sync(0xffffffffu, s.n, src), __shfl_sync(0xffffffffu, s.end, src)};
-              un = unit_of(of, g0 + src, u - before - __shfl_sync(0xffffffffu, sum - mine, src), p.T, head.chunk, a.kv.n_kv);
-              break;
-            }
-            before += __shfl_sync(0xffffffffu, sum, 31);
-            g0 += 32;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int32_t x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
           }
+          const uint32_t in = __ballot_sync(0xffffffffu, u - before < sum);
+          if (in) {
+            const int src = __ffs(in) - 1;
+            const int32_t n = __shfl_sync(0xffffffffu, s.n, src), nt = __shfl_sync(0xffffffffu, tiles_of(s), src), R = (n + 2 * p.T - 1) / (2 * p.T),
+                          chunk = chunk_of(nt, p.pieces);
+            int32_t w = u - before - __shfl_sync(0xffffffffu, sum - mine, src);
+            un.kh = w % a.kv.n_kv;
+            w /= a.kv.n_kv;
+            const int32_t r = w % R;
+            un.piece = w / R;
+            un.group = g0 + src;
+            un.seq = __shfl_sync(0xffffffffu, s.seq, src) + r * 2 * p.T;
+            un.rows[0] = min(p.T, n - r * 2 * p.T);
+            un.rows[1] = max(0, min(p.T, n - r * 2 * p.T - p.T));
+            un.tile = un.piece * chunk;
+            un.tiles = min(chunk, nt - un.tile);
+            un.end = __shfl_sync(0xffffffffu, s.end, src);
+            break;
+          }
+          before += __shfl_sync(0xffffffffu, sum, 31);
+          g0 += 32;
+          s = share_of<true>(a, g0 + lane);
         }
         if (lane == 0) {
           units[it % kUnits] = un;
@@ -205,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
         // last, which TMA fills with zeros
         auto entry = [&](int j) {
           const int64_t t = (int64_t)j * kKeys + (int64_t)lane * p.box, e = t >> pshift;
-          return lane < per && e < a.pre.max_pages ? tab[e] : -1;
+          return lane < per && e < a.pre.max_pages ? __ldcg(tab + e) : -1;
         };
         int32_t page = entry(un.tile);
         for (int j = un.tile; j < un.tile + un.tiles; ++j) {
@@ -355,6 +370,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       __syncwarp();
       for (int k = 0; k < 1 << 14; ++k)
         if (mbar_try_wait(done, 0)) break;
+    } else {
+      // the kernel over own positions needs the plan and does not wait for this kernel: it
+      // may begin when this warp has seen the plan's end
+      grid_dep_wait();
+      grid_dep_launch();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -384,14 +404,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const __grid_consta
       // a row sees the prefix as far as its sequence goes; one that sees nothing of this
       // piece (or is none) has nothing to wait for and is not written
       const bool in = tok < (dual && g ? un.rows[1] : un.rows[0]);
-      const int lim = in ? p.parts.seqs[seq].pre : 0;
+      const int lim = in ? min(max(0, __ldcg(a.b.kv_lens + seq)), un.end) : 0;
       const bool live = lim > un.tile * kKeys;
       const int whole = (int)(__reduce_min_sync(0xffffffffu, live ? (unsigned)lim : 0x7fffffffu) / kKeys);  // key tiles that every live row sees whole
       float m = live ? -INFINITY : 0.0f, l = 0.0f;
       const int32_t* tab = a.pre.table + un.group * a.pre.table_stride;
       auto entry = [&](int j) {  // page of this lane's part of key tile j
         const int64_t e = (((int64_t)j * kKeys) >> pshift) + lane;
-        return lane < npg && e < a.pre.max_pages ? tab[e] : 0;
+        return lane < npg && e < a.pre.max_pages ? __ldcg(tab + e) : 0;
       };
       int32_t pg = j0 < j1 ? entry(j0) : 0;
       for (int j = j0; j < j1; j += step) {
@@ -606,6 +626,7 @@ cudaError_t paged_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts,
   p.G = a.n_heads / a.kv.n_kv;
   p.T = shape.T;
   p.parts = parts;
+  p.pieces = shape.pieces;
   if (a.kv.hd == 128) return a.kv.bf16 ? prefix_go<128, true>(a, p, shape.ctas, s) : prefix_go<128, false>(a, p, shape.ctas, s);
   return a.kv.bf16 ? prefix_go<64, true>(a, p, shape.ctas, s) : prefix_go<64, false>(a, p, shape.ctas, s);
 }

@@ -416,21 +416,9 @@ cudaError_t paged8_decode_status(int32_t* bits);
 constexpr int kItemEnd = 3, kItemPieces = 18;
 // With a prefix, four kernels: the plan, sums over the prefixes, sums over the sequences'
 // own positions, and all of them joined.
-struct PrefixHead {
-  int32_t chunk;  // key tiles of a piece of a prefix
-  int32_t units;  // of the prefix kernel
-};
 struct PrefixSeq {  // what a sequence's token sees: positions [0, pre) of its group's prefix, [own, len) of its own pages
-  int32_t len, own, pre, pad;
-};
-struct PrefixUnit {
-  int32_t seq;          // tile A's first sequence; -1: no more units, -2: look for it
-  int32_t kh, group;
-  int32_t rows[2];      // sequences of tiles A and B
-  int32_t tile, tiles;  // its key tiles
-  int32_t end;          // positions of the prefix that exist
-  int32_t piece;
-  int32_t pad[3];
+  int32_t len, own, pre;
+  int32_t chunk;  // positions of a piece of the prefix
 };
 struct PrefixStart {  // a CTA's range of the list of own tiles, and the item that it begins in
   int64_t lo, hi, first;
@@ -440,9 +428,7 @@ struct PrefixStart {  // a CTA's range of the list of own tiles, and the item th
   int32_t pad;
 };
 struct PrefixParts {
-  PrefixHead* head;
   PrefixSeq* seqs;
-  PrefixUnit* units;    // [CTAs] the first unit of each
   PrefixStart* starts;  // [CTAs]
   int64_t* cum;         // [n_seqs + 1] (the plan's own)
   float* part;          // [piece][sequence][head][hd] sums of weights times values over a prefix
@@ -459,7 +445,7 @@ struct PrefixParts {
 struct PrefixShape {
   int32_t T;       // sequences of a tile of rows
   int32_t ctas;    // of the prefix kernel
-  int32_t pieces;  // of a prefix, at most
+  int32_t pieces;  // of a prefix
   // of the kernel over own positions: keys of a tile (its logarithm) and its bytes, CTAs, CTAs on an SM
   int32_t tile_log, stage, own_ctas, on_sm;
 };

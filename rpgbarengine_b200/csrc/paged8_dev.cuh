@@ -42,10 +42,14 @@ RPGC_DEV float2 float2_hi(uint32_t w) { return unpack2<false>(half2_hi(w)); }
 // ------------------------------------------------------- shared prefixes
 constexpr int kPrefixKeys = 128;  // keys of a tile of the prefix kernel
 
-// First sequence of group g, kept inside [0, n_seqs] whatever cu holds.
-RPGC_DEV int32_t group_seq(const PagedPrefix& p, int32_t n_seqs, int g) { return min(max(p.cu[g], 0), n_seqs); }
-// Group of sequence s, or -1: the last g with group_seq(g) <= s, where s is before the
-// next one's.
+// First sequence of group g, kept inside [0, n_seqs] whatever cu holds.  L2: in kernels
+// that have not waited for the one before and rely on its wait.
+template <bool L2>
+RPGC_DEV int32_t group_seq(const PagedPrefix& p, int32_t n_seqs, int g) {
+  return min(max(L2 ? __ldcg(p.cu + g) : p.cu[g], 0), n_seqs);
+}
+// Group of sequence s, or -1: the last g with first(g) <= s, where s is before the next
+// one's.
 template <typename F>
 RPGC_DEV int32_t group_of(int32_t n_groups, int32_t s, F first) {
   int32_t a = 0, b = n_groups;  // it is a - 1 in the end
@@ -63,46 +67,34 @@ RPGC_DEV PrefixSeq sight_of(const PagedOwnArgs& a, int32_t kv_len, int32_t len) 
   v.own = min(n, max(0, len));
   v.pre = (int32_t)min((int64_t)v.own, (int64_t)a.pre.max_pages << a.pre.kv.page_shift);
   v.len = max((int32_t)min((int64_t)n, table_reach(a.kv, a.b)), v.own);
-  v.pad = 0;
+  v.chunk = 0;
   return v;
 }
 
+// A group as the prefix kernel sees it.
 struct Share {
-  int32_t seq, n;  // a group's sequences
+  int32_t seq, n;  // its sequences
   int32_t end;     // positions that exist, if there is a sequence to see them
 };
+template <bool L2>
 RPGC_DEV Share share_of(const PagedOwnArgs& a, int g) {
   Share s{0, 0, 0};
   if (g < a.pre.n_groups) {
-    const int32_t len = max(0, a.pre.lens[g]);
-    s.seq = group_seq(a.pre, a.b.n_seqs, g);
-    s.n = max(0, group_seq(a.pre, a.b.n_seqs, g + 1) - s.seq);
-    s.end = s.n ? (int32_t)min((int64_t)len, (int64_t)a.pre.max_pages << a.pre.kv.page_shift) : 0;
+    const int32_t len = L2 ? __ldcg(a.pre.lens + g) : a.pre.lens[g];
+    s.seq = group_seq<L2>(a.pre, a.b.n_seqs, g);
+    s.n = max(0, group_seq<L2>(a.pre, a.b.n_seqs, g + 1) - s.seq);
+    s.end = s.n ? (int32_t)min((int64_t)max(0, len), (int64_t)a.pre.max_pages << a.pre.kv.page_shift) : 0;
   }
   return s;
 }
 RPGC_DEV int32_t tiles_of(const Share& s) { return (int32_t)(((int64_t)s.end + kPrefixKeys - 1) / kPrefixKeys); }
+// Key tiles of a piece: a prefix is cut into `pieces`, or as many as it has tiles.
+RPGC_DEV int32_t chunk_of(int32_t tiles, int32_t pieces) { return max(1, (tiles + pieces - 1) / pieces); }
 // Units of a group: rows of two tiles x pieces x kv heads.  (n_seqs x kv heads is less
 // than 2^31, and pieces are few where it is large.)
-RPGC_DEV int32_t units_of(const Share& s, int32_t U, int32_t chunk, int32_t n_kv) {
-  return (s.n + U - 1) / U * ((tiles_of(s) + chunk - 1) / chunk) * n_kv;
-}
-// Unit w of a group.
-RPGC_DEV PrefixUnit unit_of(const Share& s, int32_t group, int32_t w, int32_t T, int32_t chunk, int32_t n_kv) {
-  PrefixUnit un;
-  const int32_t U = 2 * T, R = (s.n + U - 1) / U;
-  un.kh = w % n_kv;
-  w /= n_kv;
-  const int32_t r = w % R;
-  un.piece = w / R;
-  un.group = group;
-  un.seq = s.seq + r * U;
-  un.rows[0] = min(T, s.n - r * U);
-  un.rows[1] = max(0, min(T, s.n - r * U - T));
-  un.tile = un.piece * chunk;
-  un.tiles = min(chunk, tiles_of(s) - un.tile);
-  un.end = s.end;
-  return un;
+RPGC_DEV int32_t units_of(const Share& s, int32_t T, int32_t pieces, int32_t n_kv) {
+  const int32_t nt = tiles_of(s), chunk = chunk_of(nt, pieces);
+  return (s.n + 2 * T - 1) / (2 * T) * ((nt + chunk - 1) / chunk) * n_kv;
 }
 
 // Attention of sequence s's token and query head h by one warp, 32 keys a step, lane
@@ -197,7 +189,7 @@ template <int HD, bool BF, bool F8, bool SH>
 RPGC_DEV void own_row(const PagedOwnArgs& a, int32_t s, int h, int lane) {
   constexpr int E = HD / 32;
   const int kh = h / (a.n_heads / a.kv.n_kv);
-  const int32_t g = SH ? group_of(a.pre.n_groups, s, [&](int i) { return group_seq(a.pre, a.b.n_seqs, i); }) : -1;
+  const int32_t g = SH ? group_of(a.pre.n_groups, s, [&](int i) { return group_seq<false>(a.pre, a.b.n_seqs, i); }) : -1;
   const PrefixSeq v = sight_of(a, a.b.kv_lens[s], g >= 0 ? a.pre.lens[g] : 0);
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + s * a.q_tok + h * a.q_head;
   RowState<HD, BF> r;
