@@ -162,11 +162,11 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ Pag
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (h < heads && !isq && !drop) {
-          const float sc = scale_of(top), inv = 1.0f / sc;
+          const float sc = scale_of(top), inv = inverse_of(sc);
           const int kh = isk ? h - a.n_heads : h - nk;
           uint8_t* dst = isk ? kd + kh * a.kv.k_head : vd + kh * a.kv.v_head;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= inv;  // (within 1.5 ulp of the quotient)
+          for (int i = 0; i < 8; ++i) x[i] *= inv;  // (within 2 ulp of the quotient)
           *reinterpret_cast<uint32_t*>(dst) = pack_e4m3(x);
           *reinterpret_cast<uint32_t*>(dst + kHalf) = pack_e4m3(x + 4);
           if (d == 0) a.scales[page * a.sc_page + kh * a.sc_head + slot + (isk ? 0 : 1 << a.kv.page_shift)] = sc;

@@ -14,7 +14,13 @@ namespace paged {
 // Scale of a row whose largest absolute value is `top` (NaN where one was NaN).
 // 2^-126 at least, so that its inverse is finite.
 RPGC_DEV float scale_of(float top) {
-  return top < INFINITY ? fmaxf(top / 448.0f, 1.17549435e-38f) : __int_as_float(0x7fffffff);
+  return top < INFINITY ? fmaxf(top * (1.0f / 448.0f), 1.17549435e-38f) : __int_as_float(0x7fffffff);
+}
+// 1 / scale within an ulp.
+RPGC_DEV float inverse_of(float scale) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+  return r;
 }
 
 // Four values as codes, rounded to the nearest even (what rounds past 448 becomes 448).
