@@ -4,6 +4,8 @@
 
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "paged_dev.cuh"
@@ -104,14 +106,15 @@ RPGC_DEV int32_t units_of(const Share& s, int32_t T, int32_t pieces, int32_t n_k
 }
 
 // Attention of sequence s's token and query head h by one warp, 32 keys a step, lane
-// l scoring key l, then every lane adding the keys' values for its own dims; fp32
-// throughout.
+// l scoring key l, fp32 throughout: once over the keys for the largest score and the sum
+// of weights, once more with every lane adding the keys' values for its own dims by weights
+// that the sum has divided, so that no sum outgrows the values.
 template <int HD, bool BF>
 struct RowState {
   static constexpr int E = HD / 32;
-  float m = -INFINITY, l = 0.0f, o[E] = {};
-  // positions [t0, t1) through one row of a table; C8: codes and scales
-  template <bool C8>
+  float m = -INFINITY, l = 0.0f, inv = 0.0f, o[E] = {};
+  // positions [t0, t1) through one row of a table; C8: codes and scales; Values: the second time
+  template <bool C8, bool Values>
   RPGC_DEV void keys(const PagedView& kv, const float* scales, int64_t sc_page, int64_t sc_head, const int32_t* table,
                      int32_t max_pages, const uint16_t* q, float scale, int kh, int64_t t0, int64_t t1, int lane) {
     const int64_t mask = (1 << kv.page_shift) - 1;
@@ -158,12 +161,13 @@ struct RowState {
       }
       const uint32_t live = __ballot_sync(0xffffffffu, ok);
       if (!live) continue;
-      const float mn = fmaxf(m, warp_max(sc)), base = mn == -INFINITY ? 0.0f : mn;
-      const float corr = expf(m - base), p = ok ? expf(sc - base) : 0.0f;
-      m = mn;
-      l = l * corr + warp_sum(p);
-#pragma unroll
-      for (int i = 0; i < E; ++i) o[i] *= corr;
+      if (!Values) {
+        const float mn = fmaxf(m, warp_max(sc)), base = mn == -INFINITY ? 0.0f : mn;
+        l = l * expf(m - base) + warp_sum(ok ? expf(sc - base) : 0.0f);
+        m = mn;
+        continue;
+      }
+      const float p = ok ? expf(sc - (m == -INFINITY ? 0.0f : m)) * inv : 0.0f;
       const float pv = p * vs;
 #pragma unroll 8
       for (int k = 0; k < 32; ++k) {
@@ -199,15 +203,19 @@ RPGC_DEV void own_row(const PagedOwnArgs& a, int32_t s, int h, int lane) {
   const PrefixSeq v = sight_of(a, a.b.kv_lens[s], g >= 0 ? a.pre.lens[g] : 0);
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + s * a.q_tok + h * a.q_head;
   RowState<HD, BF> r;
-  if (SH && v.pre > 0)
-    r.template keys<false>(a.pre.kv, nullptr, 0, 0, a.pre.table + g * a.pre.table_stride, a.pre.max_pages, q, a.scale, kh, 0,
-                           v.pre, lane);
-  r.template keys<F8>(a.kv, a.scales, a.sc_page, a.sc_head, a.b.table + s * a.b.table_stride, a.b.max_pages, q, a.scale, kh, v.own,
-                      v.len, lane);
-  const float inv = r.l == 0.0f ? 0.0f : 1.0f / r.l;
+  auto all = [&](auto values) {
+    constexpr bool V = decltype(values)::value;
+    if (SH && v.pre > 0)
+      r.template keys<false, V>(a.pre.kv, nullptr, 0, 0, a.pre.table + g * a.pre.table_stride, a.pre.max_pages, q, a.scale, kh, 0, v.pre, lane);
+    r.template keys<F8, V>(a.kv, a.scales, a.sc_page, a.sc_head, a.b.table + s * a.b.table_stride, a.b.max_pages, q, a.scale, kh, v.own,
+                           v.len, lane);
+  };
+  all(std::false_type{});
+  r.inv = r.l == 0.0f ? 0.0f : 1.0f / r.l;
+  all(std::true_type{});
   uint16_t* op = static_cast<uint16_t*>(a.out) + ((int64_t)s * a.n_heads + h) * HD + E * lane;
 #pragma unroll
-  for (int i = 0; i < E; i += 2) *reinterpret_cast<uint32_t*>(op + i) = pack2<BF>(r.o[i] * inv, r.o[i + 1] * inv);
+  for (int i = 0; i < E; i += 2) *reinterpret_cast<uint32_t*>(op + i) = pack2<BF>(r.o[i], r.o[i + 1]);
 }
 
 }  // namespace paged
