@@ -553,6 +553,7 @@ def test_a_step_of_many_conversations():
     # decode over both; against the same calls on one 16-bit cache of the values held
     H, kv, hd, page, open_, own = 8, 2, 128, 16, 90, [5, 17, 33]
     g, S = gen(4), len(own)
+    rb.paged_status()  # (what earlier calls have reported)
     rope = rb.rope_table(256, hd)
     per = 10
     c8 = rb.PagedKV8.empty(S * per + 6, page, kv, hd, torch.bfloat16)
