@@ -894,10 +894,17 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
       const int b0 = w.holder(w.i0, active), b1 = w.holder(w.i1 - 1, active);
       bar_consumers<kWarps * 32>();
       if (tid == 0) {
-        __threadfence();  // (of all the warps' partial results: they are before this by the barrier)
+        // (of all the warps' partial results: they are before this by the barrier)
         // (only the last item of a range goes on past it: one counter per CTA, back at 0 after the join)
-        *last = atomicInc(p.counters + b0, (uint32_t)(b1 - b0)) == (uint32_t)(b1 - b0);
-        __threadfence();
+        if constexpr (F8) {
+          uint32_t before;
+          asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(before) : "l"(p.counters + b0), "r"((uint32_t)(b1 - b0)) : "memory");
+          *last = before == (uint32_t)(b1 - b0);
+        } else {
+          __threadfence();
+          *last = atomicInc(p.counters + b0, (uint32_t)(b1 - b0)) == (uint32_t)(b1 - b0);
+          __threadfence();
+        }
       }
       bar_consumers<kWarps * 32>();
       if (*last) {
