@@ -1010,7 +1010,7 @@ inline bool make_map8(CUtensorMap* m, const PagedOwnArgs& a, bool v, int box) {
                             (cuuint64_t)(v ? a.kv.v_page : a.kv.k_page)};
   const cuuint32_t b[4] = {(cuuint32_t)a.kv.hd, 1, (cuuint32_t)box, 1}, es[4] = {1, 1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(v ? a.kv.v : a.kv.k), d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             a.kv.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             a.kv.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, a.kv.hd == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 inline bool make_map_scales(CUtensorMap* m, const PagedOwnArgs& a, int box) {
