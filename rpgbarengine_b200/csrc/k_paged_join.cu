@@ -8,7 +8,8 @@
 //
 // Bound by the sums' bytes, 4 HD + 8 a row and piece, which come from L2; in a kernel of
 // its own all rows' chains of look-ups run at once (joined by the CTAs that end the items of
-// own positions, 256 sequences x 32 heads in 4 pieces took 22 us).
+// own positions, 256 sequences x 32 heads in 4 pieces took 22 us; here 6 us for 21 MB, and 4 us
+// for 64 sequences in two).
 #include <cuda_runtime.h>
 
 #include <type_traits>

@@ -16,7 +16,17 @@
 // to accumulator A and the odd ones to B, and their sums meet at the end.  Warps 0-3 / 4-7:
 // softmax of A / B, one row per thread; warp 8: MMAs; warp 9: TMA; warp 10: finds the units.
 //
-// A prefix is cut into as many pieces as fill the SMs once, by the host's count of rows.
+// A prefix is cut into as many pieces as fill the SMs once, by the host's count of rows: short
+// pieces fill the SMs, but each writes its rows' sums, 4 HD bytes a row, which are read again.
+//
+// Bound: a pair of tiles and 128 keys need 2048 clocks of the tensor core and as many of the
+// special-function unit; a row's scores, softmax and P V follow one another on two accumulators,
+// which takes 3050.  Few rows to a group: the prefixes' bytes.  Measured, 32 query and 8 kv heads of 128, bf16:
+// 256 sequences over 8192 positions, 128 units of 16 tiles, 41 us (0.84 PFLOP/s; 26 us of it the
+// tiles, 4 us from the launch to the first scores, 2 us for the sums out); 64 over 256 positions 12 us beside
+// the next kernel, its units' begin and end; six groups of 7 over 100-3000 positions (38 MB) 16 us.
+// Not kept: S in two halves of 64 keys, so that scores are there ahead (3970 clocks a pair:
+// twice the MMAs, each with as much of Q to read), P handed over in halves (3400).
 #include <cuda_runtime.h>
 
 #include "paged8_dev.cuh"

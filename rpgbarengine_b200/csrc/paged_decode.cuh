@@ -37,6 +37,20 @@
 // (3.7 TB/s), one of 4200 10.4 us, one of 33 (16 heads) 4.2 us; 48 sequences with
 // 12 heads of 64 in pages of 16, 167 MB, 39-41 us.  Groups of 16 (NT 2, one CTA per SM),
 // 64 of ~1090: 32 / 2 heads of 128 28 us (2.5 TB/s), 16 / 1 20.6 us (1.7 TB/s).
+//
+// 8-bit pages (F8): k_t = dk_t ck_t and v_t = dv_t cv_t, codes c (e4m3) and a scale d for
+// each row.  Codes become fp16 operands in registers (exact; two instructions a word), dk
+// goes onto the scores, dv onto the weights, q into fp16 by a power of two: scores, weights
+// and sums are as exact as over 16-bit pages.  Half the bytes leave half the time for the
+// steps of a tile, so a warp has two independent chains of 16 keys (with one: 128 sequences
+// of 1-8192 positions 220 us).  Measured, 32 / 8 heads of 128: those 128 sequences 191-211 us
+// (1.21 GB, 5.7-6.3 TB/s), one of 4200 10.6 us, one of 33 (16 heads) 4.9; 48 with 12 heads of 64 in
+// pages of 16, 92 MB, 37-40 us (2.4 TB/s): 5 us until the first tiles are there, 3 us for each of the
+// two shared items of a CTA, and in between 17 KB a tile at 1.6-1.8 k clocks.
+//
+// Behind a prefix (SH): an item's tiles begin with the one that holds its first own position,
+// ranges and items come from the plan, sums go to the kernel that joins them with the prefix's.
+// Tiles that are not seen whole come in copies of 16 rows (SH and F8).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -58,8 +72,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // F8: K and V as codes, a byte each.  Many: four small CTAs on an SM.  What ends an item
 // and begins the next are chains of dependent steps (q, the first tile's scores, the warps'
-// sums: 2500 clocks beside 1200 a tile), so with many short items, as the positions behind
-// a prefix are, four chains at once do what two do in twice the time.
+// sums: 2500 clocks beside 1200 a tile), and the positions behind a prefix are many short
+// items: four chains at once (256 sequences of 1-200 own positions behind 8192 shared ones
+// 67.2 us, with two CTAs of 4 warps 73.5; 64 of ~735 behind 256 47.7 both ways).
 template <int HD, int NT, bool F8 = false, bool Many = false>
 struct DShape {
   static constexpr bool kMany = Many && NT == 1;
@@ -896,7 +911,7 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
       if (tid == 0) {
         // (of all the warps' partial results: they are before this by the barrier)
         // (only the last item of a range goes on past it: one counter per CTA, back at 0 after the join)
-        if constexpr (F8) {
+        if constexpr (F8) {  // (one operation with both orders: one of 4200 positions 10.9 -> 10.6 us)
           uint32_t before;
           asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(before) : "l"(p.counters + b0), "r"((uint32_t)(b1 - b0)) : "memory");
           *last = before == (uint32_t)(b1 - b0);
