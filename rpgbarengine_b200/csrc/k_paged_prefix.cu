@@ -26,7 +26,7 @@
 // tiles, 4 us from the launch to the first scores, 2 us for the sums out); 64 over 256 positions 12 us beside
 // the next kernel, its units' begin and end; six groups of 7 over 100-3000 positions (38 MB) 16 us.
 // Not kept: S in two halves of 64 keys, so that scores are there ahead (3970 clocks a pair:
-// twice the MMAs, each with as much of Q to read), P handed over in halves (3400).
+// twice the MMAs, each with as much of Q to read), P handed over in halves (45 us).
 #include <cuda_runtime.h>
 
 #include "paged8_dev.cuh"
