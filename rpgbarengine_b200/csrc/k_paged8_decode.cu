@@ -8,7 +8,7 @@ cudaError_t paged8_decode_status(int32_t* bits) { return take_bits(bits); }
 
 cudaError_t paged8_decode_launch(const PagedOwnArgs& a, cudaStream_t s) {
   if (!a.b.n_tokens) return cudaSuccess;
-  return decode_any<true, false>(a, PrefixParts{}, 0, s);
+  return decode_any<true, 0>(a, PrefixParts{}, 0, s);
 }
 
 }  // namespace rpgc

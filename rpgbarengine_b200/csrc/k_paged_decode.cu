@@ -13,7 +13,7 @@ cudaError_t paged_decode_status(int32_t* bits) { return take_bits(bits); }
 
 cudaError_t paged_decode_launch(const PagedAttnArgs& a, cudaStream_t s) {
   if (!a.b.n_tokens) return cudaSuccess;
-  return decode_any<false, false>(a, PrefixParts{}, 0, s);
+  return decode_any<false, 0>(a, PrefixParts{}, 0, s);
 }
 
 }  // namespace rpgc

@@ -1,6 +1,7 @@
 // k_paged_join.cu -- single-token attention with a shared prefix: the workspace, the
-// launches of its four kernels, and the last of them, which joins the sums over the
-// pieces of a prefix with those over a sequence's own positions.
+// launches of its four kernels (or of the one that goes through a small prefix), and the
+// last of them, which joins the sums over the pieces of a prefix with those over a
+// sequence's own positions.
 //
 // Mathematics: out = sum_k 2^(m_k - M) o_k / sum_k 2^(m_k - M) l_k over the pieces k and the
 // own positions, M the largest of their references m_k, in fp32.  A row whose result is
@@ -131,7 +132,7 @@ int64_t slot_count() {
   return 2 * 4 * sm_count(dev);
 }
 
-// The workspace: single-token attention's (for calls without a group), then what the four
+// The workspace: single-token attention's (for calls of one kernel), then what the four
 // kernels hand on.
 struct Places {
   PrefixParts parts;
@@ -171,6 +172,7 @@ int64_t paged_prefix_workspace(int32_t n_seqs, int32_t n_heads, int32_t n_kv, in
 }
 
 cudaError_t paged_prefix_decode_launch(const PagedOwnArgs& a, cudaStream_t s) {
+  if (paged_decode_through_fits(a)) return paged_decode_through_launch(a, s);
   const int G = a.n_heads / a.kv.n_kv;
   int dev = 0;
   cudaGetDevice(&dev);

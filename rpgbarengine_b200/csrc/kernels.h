@@ -457,6 +457,9 @@ cudaError_t paged_prefix_status(int32_t* bits);
 cudaError_t paged_decode_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged_decode_prefix_status(int32_t* bits);
 void paged_decode_prefix_shape(const PagedOwnArgs& a, PrefixShape* shape);
+cudaError_t paged_decode_through_launch(const PagedOwnArgs& a, cudaStream_t s);
+cudaError_t paged_decode_through_status(int32_t* bits);
+bool paged_decode_through_fits(const PagedOwnArgs& a);
 cudaError_t paged8_decode_prefix_launch(const PagedOwnArgs& a, const PrefixParts& parts, const PrefixShape& shape, cudaStream_t s);
 cudaError_t paged8_decode_prefix_status(int32_t* bits);
 void paged8_decode_prefix_shape(const PagedOwnArgs& a, PrefixShape* shape);

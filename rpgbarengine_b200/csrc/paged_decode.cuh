@@ -1,7 +1,8 @@
 // paged_decode.cuh -- the kernel of attention of one new token per sequence over the
 // pages of the KV cache: 16-bit pages (k_paged_decode.cu), 8-bit ones (F8,
 // k_paged8_decode.cu), and either behind a shared prefix (SH, k_paged_decode_prefix.cu,
-// k_paged8_decode_prefix.cu), whose sums k_paged_prefix.cu has made.
+// k_paged8_decode_prefix.cu), whose sums k_paged_prefix.cu has made; or through a small prefix
+// and on through 16-bit pages (k_paged_decode_through.cu).
 //
 // Mathematics: out = sum_t p_t v_t / sum_t p_t with p_t = 2^(c s_t - m),
 // s_t = q . k_t, c = scale * log2(e): one pass over the keys with a reference m,
@@ -48,9 +49,12 @@
 // pages of 16, 92 MB, 37-40 us (2.4 TB/s): 5 us until the first tiles are there, 3 us for each of the
 // two shared items of a CTA, and in between 17 KB a tile at 1.6-1.8 k clocks.
 //
-// Behind a prefix (SH): an item's tiles begin with the one that holds its first own position,
-// ranges and items come from the plan, sums go to the kernel that joins them with the prefix's.
-// Tiles that are not seen whole come in copies of 16 rows (SH and F8).
+// Behind a prefix (SH): an item's tiles begin with the one that holds its first own position.
+// Planned: ranges and items come from the plan, sums go to the kernel that joins them with the
+// prefix's.  Through: the prefix's tiles come before them, by its own table and pool, and the
+// item ends as one without a prefix does (64 sequences of ~735 positions behind 256 shared ones
+// 41.8 us, where the same pages named by the sequences' own tables take 39.4).
+// Tiles that are not seen whole come in copies of 16 rows (planned, and F8).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -69,12 +73,16 @@ using namespace paged;
 constexpr int kJoin = 8;   // pieces of a share whose sums are in flight at once
 constexpr int kAhead = 4;  // V operands loaded ahead of the probabilities
 constexpr float kLog2e = 1.4426950408889634f;
+// SH: behind a prefix.  Planned: ranges by a plan, sums left to the kernel that joins them.
+// Through: an item's tiles are its prefix's, then its own, both of 16 bits.
+constexpr int kPlanned = 1, kThrough = 2;
+constexpr int kThroughGroups = 15;  // (a warp's lanes hold their first sequences and lengths)
 
 // F8: K and V as codes, a byte each.  Many: four small CTAs on an SM.  What ends an item
 // and begins the next are chains of dependent steps (q, the first tile's scores, the warps'
 // sums: 2500 clocks beside 1200 a tile), and the positions behind a prefix are many short
 // items: four chains at once (256 sequences of 1-200 own positions behind 8192 shared ones
-// 67.2 us, with two CTAs of 4 warps 73.5; 64 of ~735 behind 256 47.7 both ways).
+// 67.2 us, with two CTAs of 4 warps 73.5; 64 of ~735 behind 256 47.7 either way).
 template <int HD, int NT, bool F8 = false, bool Many = false>
 struct DShape {
   static constexpr bool kMany = Many && NT == 1;
@@ -111,7 +119,13 @@ struct MoreMaps<true> {
   CUtensorMap k, v, s;
 };
 struct NoMaps {};
-template <bool F8, bool SH>
+struct PrefixMaps {  // of the prefix's pool
+  CUtensorMap k, v;
+  int32_t box;  // rows of one copy
+};
+template <bool F8, int SH>
+using MapsOf = std::conditional_t<SH == kThrough, PrefixMaps, std::conditional_t<F8 || SH, MoreMaps<F8>, NoMaps>>;
+template <bool F8, int SH>
 struct DecodeParams {
   std::conditional_t<F8 || SH, PagedOwnArgs, PagedAttnArgs> a;
   uint32_t* counters;  // [CTAs] pieces that are done of the shared item that begins in a CTA's range
@@ -119,7 +133,7 @@ struct DecodeParams {
   float* part_ml;      // [2 * CTAs][G][2] their reference and weight
   int32_t G;
   int32_t box;         // rows of one TMA copy
-  PrefixParts pre;     // SH: own and own_ml are written
+  PrefixParts pre;     // kPlanned: own and own_ml are written
 };
 
 template <bool BF>
@@ -158,6 +172,7 @@ RPGC_DEV uint32_t transpose8(uint32_t x) {
 // before are a prefix's, SH).
 struct Seen {
   int32_t len, own;
+  int32_t pre;  // kThrough: positions of the prefix that it sees
 };
 // What an item weighs in the list: its key tiles, and the end of an item (the
 // warps' sums, a share's join) as kEnd tiles more, at its front.  An item that sees
@@ -171,20 +186,21 @@ constexpr int kEnd = kItemEnd;
 constexpr int kPieces = kItemPieces;
 template <int T>
 RPGC_DEV int64_t tiles_of(const Seen& v) {  // from the tile on that holds its first own position
-  return v.len > v.own ? (v.len + (int64_t)T - 1) / T - v.own / T : 0;
+  return (v.len > v.own ? (v.len + (int64_t)T - 1) / T - v.own / T : 0) + (v.pre + (int64_t)T - 1) / T;
 }
 template <int T>
 RPGC_DEV int64_t weight_of(const Seen& v) {
-  return v.len > v.own ? tiles_of<T>(v) + kEnd : 0;
+  return v.len > v.own || v.pre > 0 ? tiles_of<T>(v) + kEnd : 0;
 }
 
 // One CTA's range of the list, item by item; every warp walks it by itself.
-template <int T, bool SH>
+template <int T, int SH>
 struct Walk {
   int64_t total, lo, hi;  // weight of the list; this CTA's range
   int32_t seq, kh;        // the item
   Seen at;                // what it sees
-  Seen ahead;             // SH: of the next sequence
+  Seen ahead;             // kPlanned: of the next sequence
+  int32_t few;            // kThrough: lane i holds group i's first sequence, lane 16 + i its prefix's length
   int64_t i0, i1;         // its key tiles in the list
   int32_t t0, t1;         // those that are this CTA's, counted from at.own / T
   // where range b of n begins, and the range that holds place t
@@ -201,8 +217,32 @@ struct Walk {
     t1 = (int32_t)((hi < i1 ? hi : i1) - i0);
   }
   template <typename Args>
-  RPGC_DEV static Seen seen(const Args& a, int s) {
-    return s < a.b.n_seqs ? Seen{(int32_t)min((int64_t)max(0, a.b.kv_lens[s]), table_reach(a.kv, a.b)), 0} : Seen{0, 0};
+  RPGC_DEV void groups(const Args& a, int lane) {
+    const int i = lane & 15;
+    few = lane < 16 ? (i <= a.pre.n_groups ? group_seq<false>(a.pre, a.b.n_seqs, i) : 0x7fffffff)
+                    : (i < a.pre.n_groups ? a.pre.lens[i] : 0);
+  }
+  // (these two with kThrough: by all lanes of a warp together)
+  RPGC_DEV int last_group(int s) const {  // the last group that begins at s or before
+    int g = -1;
+#pragma unroll
+    for (int step = 8; step; step >>= 1) {
+      const int32_t first = __shfl_sync(0xffffffffu, few, g + step);
+      if (first <= s) g += step;
+    }
+    return g;
+  }
+  template <typename Args>
+  RPGC_DEV Seen seen(const Args& a, int s) const {
+    if constexpr (SH == kThrough) {
+      const int32_t n = s < a.b.n_seqs ? a.b.kv_lens[s] : 0;
+      const int g = last_group(s);
+      const int32_t first = __shfl_sync(0xffffffffu, few, 0), end = __shfl_sync(0xffffffffu, few, min(g + 1, 15)),
+                    len = __shfl_sync(0xffffffffu, few, 16 + max(g, 0));
+      const PrefixSeq v = sight_of(a, n, first <= s && s < end ? len : 0);
+      return {v.len, v.own, v.pre};
+    }
+    return s < a.b.n_seqs ? Seen{(int32_t)min((int64_t)max(0, a.b.kv_lens[s]), table_reach(a.kv, a.b)), 0, 0} : Seen{0, 0, 0};
   }
   template <typename Args>
   RPGC_DEV bool start(const Args& a, int lane, int ctas, int cta, int* active) {
@@ -212,7 +252,7 @@ struct Walk {
     const int run = (a.b.n_seqs + 31) / 32;
     int64_t sum = 0;
     int32_t some = 0;
-    Seen ln = {0, 0};
+    Seen ln = {0, 0, 0};
 #pragma unroll 4
     for (int i = 0; i < run; ++i) {
       ln = seen(a, lane * run + i);
@@ -233,7 +273,7 @@ struct Walk {
     int64_t before = __shfl_sync(0xffffffffu, upto - sum, src);  // weight of the sequences before s0
 #pragma unroll 1
     for (int s0 = src * run;; s0 += 32) {
-      if (run > 1) ln = seen(a, s0 + lane);
+      if (run > 1 || SH == kThrough) ln = seen(a, s0 + lane);
       else ln.len = __shfl_sync(0xffffffffu, ln.len, (src + lane) & 31);  // (only lane 0's counts: the run is one sequence)
       const int64_t mine = weight_of<T>(ln) * kv;
       upto = scan(mine, lane);
@@ -242,7 +282,8 @@ struct Walk {
         const int i = __ffs(in) - 1;
         const int64_t first = before + __shfl_sync(0xffffffffu, upto - mine, i);
         seq = s0 + i;
-        at = {__shfl_sync(0xffffffffu, ln.len, i), 0};
+        at = {__shfl_sync(0xffffffffu, ln.len, i), 0, 0};
+        if constexpr (SH == kThrough) at.own = __shfl_sync(0xffffffffu, ln.own, i), at.pre = __shfl_sync(0xffffffffu, ln.pre, i);
         const int64_t w = weight_of<T>(at), in_seq = lo - first;
         kh = in_seq < (int64_t)0x7fffffff ? (int32_t)((uint32_t)in_seq / (uint32_t)w) : (int32_t)(in_seq / w);
         item(first + kh * w);
@@ -251,12 +292,12 @@ struct Walk {
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  // SH: from the plan (through L2: the kernel has not waited for the one before, which
+  // kPlanned: from the plan (through L2: the kernel has not waited for the one before, which
   // waited for the plan)
   RPGC_DEV static Seen planned(const PrefixParts& p, int s, int n_seqs) {
-    if (s >= n_seqs) return {0, 0};
+    if (s >= n_seqs) return {0, 0, 0};
     const int2 v = __ldcg(reinterpret_cast<const int2*>(p.seqs + s));
-    return {v.x, v.y};
+    return {v.x, v.y, 0};
   }
   template <typename Args>
   RPGC_DEV bool start_planned(const Args& a, const PrefixParts& p, int cta, int* tail) {
@@ -268,7 +309,7 @@ struct Walk {
     if (lo >= hi) return false;
     seq = y.z;
     kh = y.w;
-    at = {z.x, z.y};
+    at = {z.x, z.y, 0};
     *tail = z.z;
     ahead = planned(p, seq + 1, a.b.n_seqs);
     item((int64_t)(((uint64_t)(uint32_t)y.y << 32) | (uint32_t)y.x));
@@ -289,7 +330,7 @@ struct Walk {
       kh = 0;
       do {
         ++seq;
-        if (SH) at = ahead, ahead = planned(p, seq + 1, a.b.n_seqs);
+        if (SH == kPlanned) at = ahead, ahead = planned(p, seq + 1, a.b.n_seqs);
         else at = seen(a, seq);
       } while (!weight_of<T>(at));  // (a later item exists: i1 < hi <= total)
     }
@@ -303,11 +344,11 @@ RPGC_DEV void bar_consumers() {
   asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
 }
 
-template <int HD, bool BF, int NT, bool F8, bool SH>
-__global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, NT, F8, SH>::kCtas)
+template <int HD, bool BF, int NT, bool F8, int SH>
+__global__ void __launch_bounds__(DShape<HD, NT, F8, SH == kPlanned>::kThreads, DShape<HD, NT, F8, SH == kPlanned>::kCtas)
     decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const __grid_constant__ std::conditional_t<F8 || SH, MoreMaps<F8>, NoMaps> tm, const __grid_constant__ DecodeParams<F8, SH> p) {
-  using S = DShape<HD, NT, F8, SH>;
+                  const __grid_constant__ MapsOf<F8, SH> tm, const __grid_constant__ DecodeParams<F8, SH> p) {
+  using S = DShape<HD, NT, F8, SH == kPlanned>;
   constexpr int kStages = S::kStages, kHeads = S::kHeads, kPad = S::kPad, kWarps = S::kWarps, kTile = S::kTile;
   constexpr bool MB = BF && !F8;             // the MMAs' type: bf16, else fp16
   constexpr float kLift = MB ? 0.0f : 6.0f;  // fp16 probabilities carry 2^6: small ones keep their bits
@@ -342,33 +383,79 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
   // this.  With a prefix the kernel before is the prefix's, whose results the next one
   // reads, not this, and which let this one begin when all that came earlier had ended: it
   // is waited for at the end, so that this kernel does not end before it.
-  if (!SH) grid_dep_wait();
+  if (SH != kPlanned) grid_dep_wait();
   grid_dep_launch();
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity, gave_up, a.b.status); };
-  int active;  // CTAs that have a range (SH: pieces of the range's last item)
+  int active;  // CTAs that have a range (kPlanned: pieces of the range's last item)
   Walk<kTile, SH> w;
-  const bool work = SH ? w.start_planned(a, p.pre, blockIdx.x, &active) : w.start(a, lane, gridDim.x, blockIdx.x, &active);
+  if constexpr (SH == kThrough) w.groups(a, lane);
+  const bool work = SH == kPlanned ? w.start_planned(a, p.pre, blockIdx.x, &active) : w.start(a, lane, gridDim.x, blockIdx.x, &active);
 
   if (warp >= kWarps) {  // one warp copies K, the other V (or one both)
     // ---------------------------------------------------------------- loads
     if (!work) {
-      if (SH) grid_dep_wait();  // (so that this kernel ends after the prefix's)
+      if (SH == kPlanned) grid_dep_wait();  // (so that this kernel ends after the prefix's)
       return;
     }
     int st = 0;
     uint32_t ph = 0;
     const int per = kTile / p.box;  // copies per panel
     const int pshift = a.kv.page_shift;
+    // kThrough: tiles [t0, t1) of a prefix
+    auto load_prefix = [&](const int32_t* tab, int t0, int t1) {
+      if constexpr (SH == kThrough) {
+        const int box = tm.box, per = kTile / box, shift = a.pre.kv.page_shift, copies = (t1 - t0) * per, v = warp - kWarps;
+        auto entry = [&](int c) {
+          const int64_t e = ((int64_t)t0 * kTile + (int64_t)c * box) >> shift;
+          return c < copies && e < a.pre.max_pages ? tab[e] : -1;
+        };
+        int32_t ids = entry(lane), ids_next = entry(32 + lane);
+        for (int c = 0; c < copies; c += per) {
+          if (c && !(c & 31)) {
+            ids = ids_next;
+            ids_next = entry(c + 32 + lane);
+          }
+          int32_t page = __shfl_sync(0xffffffffu, ids, (c + lane) & 31);
+          const bool ok = (uint32_t)page < (uint32_t)a.pre.kv.n_pages;
+          if (!ok) page = a.pre.kv.n_pages;
+          const uint32_t have = __ballot_sync(0xffffffffu, lane < per && ok);
+          const int at = (int)(((int64_t)t0 * kTile + (int64_t)(c + lane) * box) & ((1 << shift) - 1));
+          wait(empty + st, ph ^ 1u);
+          if (*gave_up) return;
+          if (lane == 0) {
+            const int g = box >> 4;
+            uint32_t groups = 0;
+            for (int i = 0; i < per; ++i)
+              if (have >> i & 1u) groups |= ((1u << g) - 1u) << (i * g);
+            if (v == 0) there[st] = groups;
+            mbar_arrive_expect_tx(full + st, S::kHalf);
+          }
+          __syncwarp();
+          if (lane < per)
+#pragma unroll
+            for (int h = 0; h < S::kPanels; ++h)
+              tma_4d(ring + st * S::kStage + v * S::kHalf + h * S::kPanel + lane * box * 128, v ? &tm.v : &tm.k, 64 * h, w.kh, at, page, full + st);
+          if (++st == kStages) st = 0, ph ^= 1u;
+        }
+      }
+    };
     do {
+      const int pt = SH == kThrough ? (int)(((uint32_t)w.at.pre + kTile - 1) / kTile) : 0;  // tiles of the prefix
       const int32_t* tab = a.b.table + (int64_t)w.seq * a.b.table_stride;
-      const int t0 = w.t0, t1 = w.t1;
-      if (t1 <= t0) continue;  // (the range ends in the item's front)
+      const int t0 = max(w.t0 - pt, 0), t1 = w.t1 - pt;
+      if constexpr (SH == kThrough)
+        if (w.t0 < pt) {
+          // (the sequence has a group whatever cu holds, for it sees a prefix)
+          load_prefix(a.pre.table + (int64_t)w.last_group(w.seq) * a.pre.table_stride, w.t0, min(w.t1, pt));
+          if (*gave_up) break;
+        }
+      if (t1 <= t0) continue;  // (the range ends in the item's front, or in the prefix)
       // page ids ahead of their use: lane l holds the one of copy l of the next 32
       const int copies = (t1 - t0) * per;
       const int64_t base = (int64_t)(t0 + (SH ? w.at.own / kTile : 0)) * kTile;
       auto entry = [&](int c) {
         const int64_t e = (base + (int64_t)c * p.box) >> pshift;
-        return c < copies && e < a.b.max_pages ? (SH ? __ldcg(tab + e) : tab[e]) : -1;
+        return c < copies && e < a.b.max_pages ? (SH == kPlanned ? __ldcg(tab + e) : tab[e]) : -1;
       };
       int32_t ids = entry(lane), ids_next = entry(32 + lane);
       for (int t = t0, c = 0; t < t1; ++t, c += per) {
@@ -384,7 +471,7 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
         constexpr int kBoth = 3 - S::kLoaders;  // of K and V, this warp's: from v0 on
         const int v0 = warp - kWarps;
         uint8_t* dst = ring + st * S::kStage;
-        if constexpr (F8 || SH) {
+        if constexpr (F8 || SH == kPlanned) {
           // groups of 16 keys that the token sees; a tile that it does not see whole comes
           // in copies of 16 rows, those alone
           const int64_t tb = base + (int64_t)(t - t0) * kTile;
@@ -443,18 +530,18 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
       for (int i = 0; i < kStages; ++i)
         for (int k = 0; k < 1 << 12; ++k)
           if (mbar_try_wait(full + i, ph ^ (i < st ? 0u : 1u))) break;
-    if (SH) grid_dep_wait();
+    if (SH == kPlanned) grid_dep_wait();
     return;
   }
 
   // ----------------------------------------------------------- attention
   // sequences that see nothing: zeros, their rows dealt over the CTAs
-  for (int s = blockIdx.x; !SH && s < a.b.n_seqs; s += gridDim.x)
+  for (int s = blockIdx.x; SH != kPlanned && s < a.b.n_seqs; s += gridDim.x)
     if (w.seen(a, s).len == 0)
       for (int i = tid; i < a.n_heads * HD / 8; i += kWarps * 32)
         reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)s * a.n_heads * HD)[i] = make_uint4(0, 0, 0, 0);
   if (!work) {
-    if (SH) grid_dep_wait();
+    if (SH == kPlanned) grid_dep_wait();
     return;
   }
   const int gr = lane >> 2, tq = lane & 3, G = p.G;
@@ -471,7 +558,7 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
   int st = 0;
   uint32_t ph = 0;
   auto put = [&](int h, int d, float M, const float4& acc, float L) {  // four values of the item's row of head h
-    if constexpr (SH) {  // its sums, for the kernel that joins all of them (weights are 2^(score - reference))
+    if constexpr (SH == kPlanned) {  // its sums, for the kernel that joins all of them (weights are 2^(score - reference))
       const int64_t row = (int64_t)w.seq * a.n_heads + w.kh * G + h;
       __stcg(reinterpret_cast<float4*>(p.pre.own + row * HD + d), acc);
       if (d == 0) __stcg(reinterpret_cast<float2*>(p.pre.own_ml) + row, make_float2(L == L ? M - kLift : 0.0f, L));  // (NaN stays: a score was)
@@ -523,8 +610,8 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
         const uint32_t *q0 = reinterpret_cast<const uint32_t*>(qp + 16 * k), *q1 = q0 + 4;
-        q[n][k][0] = h < G ? (SH ? __ldcg(q0) : *q0) : 0u;
-        q[n][k][1] = h < G ? (SH ? __ldcg(q1) : *q1) : 0u;
+        q[n][k][0] = h < G ? (SH == kPlanned ? __ldcg(q0) : *q0) : 0u;
+        q[n][k][1] = h < G ? (SH == kPlanned ? __ldcg(q1) : *q1) : 0u;
       }
     }
     float o[NT][HD / 16][4], m[NT][2], l[NT][2];
@@ -538,9 +625,12 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
     }
     for (int t = t0; t < t1; ++t) {
       wait(full + st, ph);
-      const int first = (t + (SH ? w.at.own / kTile : 0)) * kTile + 16 * S::kSub * warp;
-      const int left = w.at.len - first;          // keys of this warp's part
-      const int skip = SH ? w.at.own - first : 0;  // those before that the prefix has
+      // tile t is kTile positions of the prefix, or of the sequence's own pages from own / kTile on
+      const int pt = SH == kThrough ? (int)(((uint32_t)w.at.pre + kTile - 1) / kTile) : 0;
+      const bool shared = SH == kThrough && t < pt;
+      const int first = (shared ? t : t - pt + (SH ? w.at.own / kTile : 0)) * kTile + 16 * S::kSub * warp;
+      const int left = (shared ? w.at.pre : w.at.len) - first;  // keys of this warp's part
+      const int skip = SH && !shared ? w.at.own - first : 0;    // those before that the prefix has
       if constexpr (F8) {
         if (left > 0 && skip < 16 * S::kSub) {
           constexpr int kSub = S::kSub, kChains = 2 / kSub;  // two chains of MMAs, so that one's latency hides the other's
@@ -897,14 +987,14 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
         __stcg(reinterpret_cast<float4*>(p.part + ((int64_t)slot * G + h) * HD + d), acc);
         if (d == 0)
           __stcg(reinterpret_cast<float2*>(p.part_ml) + (int64_t)slot * G + h,
-                 SH ? make_float2(L == L ? M - kLift : 0.0f, L) : make_float2(M, L));
+                 SH == kPlanned ? make_float2(L == L ? M - kLift : 0.0f, L) : make_float2(M, L));
       }
     }
-    if constexpr (SH) {  // where the item's pieces are: piece 0's slot, piece k in the first slot of the k-th CTA from its own
+    if constexpr (SH == kPlanned) {  // where the item's pieces are: piece 0's slot, piece k in the first slot of the k-th CTA from its own
       if (tid == 0 && w.i0 >= w.lo)
         p.pre.pieces[(int64_t)w.seq * a.kv.n_kv + w.kh] = whole ? 0 : slot | active << 16;
     }
-    if (!SH && !whole) {
+    if (SH != kPlanned && !whole) {
       // ---- the last CTA to finish a shared item joins its pieces
       const int b0 = w.holder(w.i0, active), b1 = w.holder(w.i1 - 1, active);
       bar_consumers<kWarps * 32>();
@@ -967,18 +1057,18 @@ __global__ void __launch_bounds__(DShape<HD, NT, F8, SH>::kThreads, DShape<HD, N
     }
     bar_consumers<kWarps * 32>();  // the merge buffer is free again
     // (attn_row inlined: a kernel that calls takes 0.2 us longer to begin)
-    const uint32_t todo = SH ? 0u : *again;
+    const uint32_t todo = SH == kPlanned ? 0u : *again;
     if (__builtin_expect(todo != 0, 0)) {
       for (int h = warp; h < G; h += kWarps)
         if (todo >> h & 1u) {
-          if constexpr (F8) own_row<HD, BF, F8, false>(a, w.seq, w.kh * G + h, lane);
+          if constexpr (F8 || SH) own_row<HD, BF, F8, SH != 0>(a, w.seq, w.kh * G + h, lane);
           else attn_row<HD, BF>(a, w.seq, w.seq, w.kh * G + h, -1, lane);
         }
       bar_consumers<kWarps * 32>();
       if (tid == 0) *again = 0;
     }
   } while (w.next(a, p.pre));
-  if (SH) grid_dep_wait();
+  if (SH == kPlanned) grid_dep_wait();
 }
 
 int device_sms() {
@@ -1039,10 +1129,10 @@ inline bool make_map_scales(CUtensorMap* m, const PagedOwnArgs& a, int box) {
              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD, bool BF, int NT, bool F8, bool SH, typename Args>
+template <int HD, bool BF, int NT, bool F8, int SH, typename Args>
 cudaError_t decode_go(const Args& a, const PrefixParts& pre, int own_ctas, cudaStream_t s) {
-  using S = DShape<HD, NT, F8, SH>;
-  const int ctas = SH ? own_ctas : decode_ctas<HD, NT, F8>(a.n_heads / a.kv.n_kv);
+  using S = DShape<HD, NT, F8, SH == kPlanned>;
+  const int ctas = SH == kPlanned ? own_ctas : decode_ctas<HD, NT, F8>(a.n_heads / a.kv.n_kv);
   DecodeParams<F8, SH> p{};
   p.a = a;
   p.G = a.n_heads / a.kv.n_kv;
@@ -1052,19 +1142,26 @@ cudaError_t decode_go(const Args& a, const PrefixParts& pre, int own_ctas, cudaS
   p.counters = reinterpret_cast<uint32_t*>(ws);
   p.part = reinterpret_cast<float*>(ws + counter_bytes());
   p.part_ml = p.part + (int64_t)2 * ctas * p.G * HD;
-  if (SH) {
+  if (SH == kPlanned) {
     p.part = pre.slots;
     p.part_ml = pre.slots_ml;
   }
   CUtensorMap mk, mv;
-  std::conditional_t<F8 || SH, MoreMaps<F8>, NoMaps> more{};
+  MapsOf<F8, SH> more{};
   auto map = [&](CUtensorMap* m, bool v, int box) {
     if constexpr (F8) return make_map8(m, a, v, box);
     else return make_kv_map(m, a, v, box);
   };
   bool made = map(&mk, false, p.box) && map(&mv, true, p.box);
   if constexpr (F8) made = made && make_map_scales(&more.s, a, p.box);
-  if constexpr (F8 || SH) made = made && map(&more.k, false, 16) && map(&more.v, true, 16);
+  if constexpr (SH == kThrough) {
+    PagedAttnArgs x = a;
+    x.kv = a.pre.kv;
+    more.box = (1 << x.kv.page_shift) < S::kTile ? 1 << x.kv.page_shift : S::kTile;
+    made = made && make_kv_map(&more.k, x, false, more.box) && make_kv_map(&more.v, x, true, more.box);
+  } else if constexpr (F8 || SH) {
+    made = made && map(&more.k, false, 16) && map(&more.v, true, 16);
+  }
   if (!made) return cudaErrorInvalidValue;
   constexpr int smem = S::kSmem;
   static_assert(smem <= 233472 / S::kCtas - 1024, "shared memory of one CTA");
@@ -1082,7 +1179,7 @@ cudaError_t decode_go(const Args& a, const PrefixParts& pre, int own_ctas, cudaS
   return e;
 }
 
-template <bool F8, bool SH, typename Args>
+template <bool F8, int SH, typename Args>
 cudaError_t decode_any(const Args& a, const PrefixParts& pre, int own_ctas, cudaStream_t s) {
   auto heads = [&](auto hd, auto bf) {
     return a.n_heads / a.kv.n_kv <= 8 ? decode_go<decltype(hd)::value, decltype(bf)::value, 1, F8, SH>(a, pre, own_ctas, s)

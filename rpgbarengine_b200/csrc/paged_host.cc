@@ -303,6 +303,7 @@ int rpgc_paged_status(int32_t* bits) {
     check(rpgc::paged8_decode_status(bits), "single-token attention's status");
     check(rpgc::paged_decode_prefix_status(bits), "single-token attention's status");
     check(rpgc::paged8_decode_prefix_status(bits), "single-token attention's status");
+    check(rpgc::paged_decode_through_status(bits), "single-token attention's status");
     check(rpgc::paged_prefix_status(bits), "the prefix's status");
     check(rpgc::paged_read_status(bits), "read's status");
     return RPGC_OK;

@@ -94,6 +94,67 @@ def test_with_and_without_a_prefix(c):
     check(*case(**c, seed=c["n_seqs"] + c["groups"]))
 
 
+FEW = [
+    dict(n_seqs=1, groups=1, plen=(16, 16), own=(0, 0), H=1, kv=1, hd=64, page=16, io="f16"),  # half a warp of output
+    dict(n_seqs=7, groups=2, plen=(16, 700), own=(0, 1), H=3, kv=3, hd=64, page=16, io="bf16", empty=3),
+    dict(n_seqs=64, groups=1, plen=(256, 256), own=(0, 900), H=32, kv=8, hd=128, page=64, io="bf16", loose=3),
+    dict(n_seqs=5, groups=4, plen=(32, 1000), own=(1, 9000), H=8, kv=2, hd=128, page=32, io="f16", loose=1),
+    dict(n_seqs=512, groups=3, plen=(128, 128), own=(0, 70), H=2, kv=2, hd=64, page=128, io="bf16", empty=5),
+    dict(n_seqs=40, groups=2, plen=(64, 1200), own=(0, 500), H=32, kv=2, hd=128, page=64, io="f16", empty=9),
+    dict(n_seqs=33, groups=3, plen=(0, 400), own=(3, 300), H=16, kv=1, hd=64, page=16, io="bf16", loose=2),
+]
+
+
+@pytest.mark.parametrize("c", FEW, ids=lambda c: f"{c['n_seqs']}x{c['groups']}-{c['H']}-{c['kv']}-{c['hd']}")
+def test_few_groups_and_the_same_beside_groups_of_none(c):
+    # groups without a sequence change no result, though the work may be cut another way with them;
+    # over pages of 16 bits, and with the own positions in 8
+    k, v, q, table, lens, ptable, plens, cu = case(**c, seed=c["n_seqs"])
+    none = (torch.cat([ptable, ptable.new_full((5, ptable.shape[1]), -1)]), torch.cat([plens, plens[:1].expand(5) * 0 + 32]),
+            torch.cat([cu, cu[-1:].expand(5)]))
+    check(k, v, q, table, lens, ptable, plens, cu)
+    cache, batch, _, _ = check(k, v, q, table, lens, *none)
+    ones = torch.ones(k.shape[0], c["kv"], 2, c["page"], device="cuda")
+    kc, vc = k.float().to(torch.float8_e4m3fn), v.float().to(torch.float8_e4m3fn)
+    c8, mags = (rb.PagedKV8(kc, x, ones, dtype=k.dtype) for x in (vc, vc.float().abs().to(torch.float8_e4m3fn)))
+    few, many = (rb.PagedPrefix(cache, *x) for x in ((ptable, plens, cu), none))
+    a, b = (rb.paged_attention_decode(c8, batch, q, prefix=x) for x in (few, many))
+    mag = rb.paged_attention_decode(mags, batch, q, prefix=rb.PagedPrefix(rb.PagedKV(k, v.abs()), *none)).double()
+    assert torch.isfinite(a).all()
+    assert float(((a.double() - b.double()).abs() - 2.5 * U[q.dtype] * (b.double().abs() + 1.02 * mag)).max()) <= 0
+    for _ in range(3):
+        assert torch.equal(rb.paged_attention_decode(c8, batch, q, prefix=few), a)
+
+
+@pytest.mark.parametrize("groups", [1, 20])
+def test_a_prefix_longer_than_its_table(groups):
+    # positions without a page are left out
+    k, v, q, table, lens, ptable, plens, cu = case(40, groups, (64, 64), (0, 1), 4, 2, 64, 16, "bf16", seed=2)
+    cache, out = rb.PagedKV(k, v), torch.full((40, 4, 64), 9.0, device="cuda", dtype=torch.bfloat16)
+    for width in (1, 3):
+        rb.paged_attention_decode(cache, rb.PagedBatch(table, lens), q, out=out, prefix=rb.PagedPrefix(cache, ptable[:, :width].contiguous(), plens, cu))
+        t = table.clone()
+        t[:, width:4] = -1
+        want = rb.paged_attention_decode(cache, rb.PagedBatch(t, lens), q).double()
+        mag = rb.paged_attention_decode(rb.PagedKV(k, v.abs()), rb.PagedBatch(t, lens), q).double()
+        assert float(((out.double() - want).abs() - 2.5 * 2.0 ** -8 * (want.abs() + 1.02 * mag)).max()) <= 0
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+def test_huge_values_in_a_prefix_that_is_all(io):
+    # three heads of 64: the last warp has half its rows
+    k, v, q, table, lens, ptable, plens, cu = case(5, 2, (64, 320), (0, 0), 3, 1, 64, 32, io, seed=4)
+    for g in range(2):
+        v[int(ptable[g, 0]), 5, 0, 7] = HUGE[io]
+        k[int(ptable[g, 0]), 5, 0] *= 3
+    got = rb.paged_attention_decode(rb.PagedKV(k, v), rb.PagedBatch(table, lens), q, prefix=rb.PagedPrefix(rb.PagedKV(k, v), ptable, plens, cu))
+    assert torch.isfinite(got).all()
+    for s, n in enumerate(lens.tolist()):
+        K, V = (x[table[s, : n // 32].long()].reshape(-1, 64)[:n].double() for x in (k, v))
+        p = torch.softmax(q[s].double() @ K.T / 8, -1)
+        assert float(((got[s].double() - p @ V).abs() - 1.25 * U[DT[io]] * ((p @ V).abs() + p @ V.abs())).max()) <= 0
+
+
 HUGE = {"bf16": 3.0e38, "f16": 65504.0}
 
 
