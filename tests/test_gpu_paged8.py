@@ -367,17 +367,25 @@ SHARED = [  # own lengths (None: no positions at all), prefixes, cu, heads, kv, 
 ]
 
 
+NONE = 16  # groups without a sequence, after those of "many"
+KINDS = pytest.mark.parametrize("kind", ["same", "other", "many", "e4m3"])
+
+
 def shared_case(own, plens, cu, H, kv, hd, page, io, hnd, kind, seed=0):
-    """kind: "same" (16 bits, the prefix in the sequences' own pool) or "e4m3"."""
+    """kind: "same" (16 bits, the prefix in the sequences' own pool), "other" (16 bits, the prefix
+    in a pool of other pages), "many" (as "same", among so many groups that a plan is made) or "e4m3"."""
+    if kind == "many" and plens:
+        plens, cu = plens + [0] * NONE, cu + [cu[-1]] * NONE
+    ppage = (16 if page > 16 else 64) if kind == "other" else page
     g = gen(len(own) * hd + sum(plens) + seed)
     group = [next((j for j in range(len(plens)) if cu[j] <= s < cu[j + 1]), -1) for s in range(len(own))]
     lens = [0 if n is None else n + (plens[j] if j >= 0 else 0) for n, j in zip(own, group)]
     held = [plens[j] // page if j >= 0 else 0 for j in group]
     need = [max(0, -(-n // page) - h) for n, h in zip(lens, held)]
-    rows, pages = ids_of(g, [-(-p // page) for p in plens] + need)
+    rows, pages = ids_of(g, [-(-p // ppage) for p in plens] + need)
     first, mine = rows[:len(plens)], rows[len(plens):]
-    cache = own_cache(g, "16" if kind == "same" else "e4m3", pages, page, kv, hd, io, hnd)
-    pre = cache if kind == "same" else own_cache(g, "16", pages, page, kv, hd, io, hnd)
+    cache = own_cache(g, "e4m3" if kind == "e4m3" else "16", pages, page, kv, hd, io, hnd)
+    pre = cache if kind in ("same", "many") else own_cache(g, "16", pages, ppage, kv, hd, io, hnd != (kind == "other"))
     # (their own tables do not have the prefix's positions at all)
     table = [[-1] * h + r for h, r in zip(held, mine)]
     q = randn(g, len(own), H, hd, dtype=DT[io])
@@ -386,7 +394,7 @@ def shared_case(own, plens, cu, H, kv, hd, page, io, hnd, kind, seed=0):
     return cache, batch, prefix, q, table, lens, (pre, first, plens, cu)
 
 
-@pytest.mark.parametrize("kind", ["same", "e4m3"])
+@KINDS
 @pytest.mark.parametrize("own,plens,cu,H,kv,hd,page,io,hnd", SHARED)
 def test_decode_with_a_shared_prefix(own, plens, cu, H, kv, hd, page, io, hnd, kind):
     cache, batch, prefix, q, table, lens, pre = shared_case(own, plens, cu, H, kv, hd, page, io, hnd, kind)
@@ -396,7 +404,7 @@ def test_decode_with_a_shared_prefix(own, plens, cu, H, kv, hd, page, io, hnd, k
         assert torch.equal(rb.paged_attention_decode(cache, batch, q, prefix=prefix), got)
 
 
-@pytest.mark.parametrize("kind", ["same", "e4m3"])
+@pytest.mark.parametrize("kind", ["same", "many", "e4m3"])
 def test_sequences_shorter_than_their_prefix(kind):
     # they see as much of it as they have positions; pages that are not there, in the
     # prefix and behind it; a prefix longer than its table, a length below zero
@@ -413,7 +421,8 @@ def test_sequences_shorter_than_their_prefix(kind):
     width = max(len(r) for r in first)
     first[1] += [-1] * (width - 5)
     batch = rb.PagedBatch(i32(padded(table)), i32(lens))
-    prefix = rb.PagedPrefix(pre[0], i32(first), i32(plens), i32(cu))
+    plens, cu = plens + pre[2][2:], pre[3]
+    prefix = rb.PagedPrefix(pre[0], i32(padded(first)), i32(plens), i32(cu))
     got = rb.paged_attention_decode(cache, batch, q, prefix=prefix)
     close(got, *definition(cache, table, lens, q, 128 ** -0.5, (pre[0], first, plens, cu)))
 
@@ -426,7 +435,7 @@ def test_a_prefix_without_groups_is_none():
     close(got, *definition(cache, table, lens, q, 64 ** -0.5))
 
 
-@pytest.mark.parametrize("kind", ["same", "e4m3"])
+@KINDS
 @pytest.mark.parametrize("hd", [64, 128])
 def test_what_nobody_sees_is_never_used(kind, hd):
     # every slot that no sequence sees: NaN, infinities, codes and scales that are NaN
@@ -434,24 +443,27 @@ def test_what_nobody_sees_is_never_used(kind, hd):
     cache, batch, prefix, q, table, lens, pre = shared_case(own, plens, cu, 8, 2, hd, 32, "bf16", False, kind)
     want = rb.paged_attention_decode(cache, batch, q, prefix=prefix)
     used = torch.zeros(cache.k.shape[:2], dtype=torch.bool, device="cuda")
-    pused = used if kind == "same" else torch.zeros_like(used)
+    pused = used if kind in ("same", "many") else torch.zeros(pre[0].k.shape[:2], dtype=torch.bool, device="cuda")
+    size = pused.shape[1]
     group = [0, 0, 0, 1, -1]
     for s, n in enumerate(lens):
         for t in range(plens[group[s]] if group[s] >= 0 else 0, n):
             used[table[s][t // 32], t % 32] = True
     for j, p in enumerate(plens):
         for t in range(p):
-            pused[pre[1][j][t // 32], t % 32] = True
+            pused[pre[1][j][t // size], t % size] = True
     for bad in (float("nan"), float("inf"), -3e38):
         pre[0].k[~pused], pre[0].v[~pused] = bad, bad
         if kind == "e4m3":
             for t in (cache.k, cache.v):
                 t.view(torch.uint8)[~used] = 0x7F if bad != bad else 0x7E
             cache.scales.permute(0, 3, 1, 2)[~used] = bad
+        elif kind == "other":
+            cache.k[~used], cache.v[~used] = bad, bad
         assert torch.equal(rb.paged_attention_decode(cache, batch, q, prefix=prefix), want)
 
 
-@pytest.mark.parametrize("kind", ["same", "e4m3"])
+@KINDS
 def test_values_that_are_not_finite_show(kind):
     own, plens, cu = [40, 40, 40, 40], [100], [0, 2]
     cache, batch, prefix, q, table, lens, pre = shared_case(own, plens, cu, 4, 2, 64, 16, "bf16", False, kind)
@@ -459,19 +471,19 @@ def test_values_that_are_not_finite_show(kind):
     # an own position of sequence 0, kv head 1
     t = 105
     at = table[0][t // 16], t % 16
-    if kind == "same":
+    if kind != "e4m3":
         cache.v[at[0], at[1], 1, 3] = float("inf")
     else:
         cache.scales[at[0], 1, 1, at[1]] = float("nan")
     got = rb.paged_attention_decode(cache, batch, q, prefix=prefix)
-    if kind == "same":
+    if kind != "e4m3":
         assert bool((got[0, 2:, 3] == float("inf")).all())
         assert torch.isfinite(got[0, 2:, :3]).all() and torch.isfinite(got[0, 2:, 4:]).all()
     else:
         assert bool(got[0, 2:].isnan().all())
     assert torch.equal(got[0, :2], want[0, :2]) and torch.equal(got[1:], want[1:])
     # a position of the prefix, kv head 0: all of its group
-    pre[0].v[pre[1][0][2], 7, 0, 5] = float("-inf")
+    pre[0].v[pre[1][0][1 if kind == "other" else 2], 7, 0, 5] = float("-inf")
     got2 = rb.paged_attention_decode(cache, batch, q, prefix=prefix)
     assert bool((got2[:2, :2, 5] == float("-inf")).all()) and torch.isfinite(got2[:2, :2, :5]).all()
     assert torch.equal(got2[2:], want[2:]) and torch.equal(got2[1, 2:], want[1, 2:])
@@ -481,7 +493,7 @@ def test_values_that_are_not_finite_show(kind):
     assert bool(got3[3, 1].isnan().all()) and torch.equal(got3[3, 0], got2[3, 0]) and torch.equal(got3[2], got2[2])
 
 
-@pytest.mark.parametrize("kind", ["same", "e4m3"])
+@KINDS
 @pytest.mark.parametrize("io", ["bf16", "f16"])
 def test_scores_and_values_over_a_wide_range(kind, io):
     # scores that grow along the sequence, scales over many powers of two, large q
@@ -515,7 +527,7 @@ def test_strides_scale_and_out():
     close(got, *definition(cache, rows, lens, q, 0.3))
 
 
-@pytest.mark.parametrize("kind", ["same", "e4m3"])
+@KINDS
 def test_captured_calls_follow_lengths_and_tables(kind):
     own, plens, cu = [30, 5, 0, 99], [150], [0, 3]
     cache, batch, prefix, q, table, lens, pre = shared_case(own, plens, cu, 8, 2, 128, 16, "bf16", False, kind)
@@ -524,17 +536,19 @@ def test_captured_calls_follow_lengths_and_tables(kind):
     with torch.cuda.graph(graph):
         got = rb.paged_attention_decode(cache, batch, q, prefix=prefix)
     for plen, n, c in ((150, [180, 155, 150, 99], [0, 3]), (64, [170, 64, 1, 50], [1, 2]), (0, [4, 5, 6, 7], [0, 4]), (150, [0, 0, 0, 0], [0, 4])):
+        plens, c = [plen] + pre[2][1:], c + c[-1:] * (len(pre[3]) - 2)
         batch.keep[1].copy_(i32(n))
-        prefix.keep[1].copy_(i32([plen]))
+        prefix.keep[1].copy_(i32(plens))
         prefix.keep[2].copy_(i32(c))
         graph.replay()
         tab = [[x if x >= 0 else -1 for x in r] for r in table]
-        close(got, *definition(cache, tab, n, q, 128 ** -0.5, (pre[0], pre[1], [plen], c)))
+        close(got, *definition(cache, tab, n, q, 128 ** -0.5, (pre[0], pre[1], plens, c)))
 
 
-def test_two_streams_at_once():
+@pytest.mark.parametrize("kind", ["same", "many"])
+def test_two_streams_at_once(kind):
     own, plens, cu = [300 + i for i in range(6)], [2000], [0, 6]
-    cache, batch, prefix, q, *_ = shared_case(own, plens, cu, 32, 8, 128, 64, "bf16", False, "same")
+    cache, batch, prefix, q, *_ = shared_case(own, plens, cu, 32, 8, 128, 64, "bf16", False, kind)
     want = rb.paged_attention_decode(cache, batch, q, prefix=prefix)
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()

@@ -101,17 +101,19 @@ FEW = [
     dict(n_seqs=5, groups=4, plen=(32, 1000), own=(1, 9000), H=8, kv=2, hd=128, page=32, io="f16", loose=1),
     dict(n_seqs=512, groups=3, plen=(128, 128), own=(0, 70), H=2, kv=2, hd=64, page=128, io="bf16", empty=5),
     dict(n_seqs=40, groups=2, plen=(64, 1200), own=(0, 500), H=32, kv=2, hd=128, page=64, io="f16", empty=9),
+    dict(n_seqs=60, groups=15, plen=(0, 90), own=(0, 200), H=8, kv=4, hd=64, page=16, io="f16", loose=4),
+    dict(n_seqs=60, groups=16, plen=(0, 90), own=(0, 200), H=8, kv=4, hd=64, page=16, io="f16", loose=4),
     dict(n_seqs=33, groups=3, plen=(0, 400), own=(3, 300), H=16, kv=1, hd=64, page=16, io="bf16", loose=2),
 ]
 
 
 @pytest.mark.parametrize("c", FEW, ids=lambda c: f"{c['n_seqs']}x{c['groups']}-{c['H']}-{c['kv']}-{c['hd']}")
 def test_few_groups_and_the_same_beside_groups_of_none(c):
-    # groups without a sequence change no result, though the work may be cut another way with them;
-    # over pages of 16 bits, and with the own positions in 8
+    # groups without a sequence change no result, though the call takes other kernels with them
+    # (16 bits) or cuts the work another way (own positions in 8)
     k, v, q, table, lens, ptable, plens, cu = case(**c, seed=c["n_seqs"])
-    none = (torch.cat([ptable, ptable.new_full((5, ptable.shape[1]), -1)]), torch.cat([plens, plens[:1].expand(5) * 0 + 32]),
-            torch.cat([cu, cu[-1:].expand(5)]))
+    none = (torch.cat([ptable, ptable.new_full((16, ptable.shape[1]), -1)]), torch.cat([plens, plens[:1].expand(16) * 0 + 32]),
+            torch.cat([cu, cu[-1:].expand(16)]))
     check(k, v, q, table, lens, ptable, plens, cu)
     cache, batch, _, _ = check(k, v, q, table, lens, *none)
     ones = torch.ones(k.shape[0], c["kv"], 2, c["page"], device="cuda")
